@@ -251,6 +251,124 @@ int slm_causal_attention_rows(const float *q_dev, const float *k_cache_dev,
 /* sample_argmax (transformer.rs:654-667): first maximum wins. */
 int slm_sample_argmax(const float *logits_dev, uint64_t n, int32_t *out_dev, void *stream);
 
+/* -------------------------------------------------- paged key/value cache
+ * No reference counterpart (its LayerKvCache, transformer.rs:323-338, holds
+ * one sequence of max_seq_len positions).  Sequences of unlike and changing
+ * lengths share one pool of pages; a table says which pages hold a sequence's
+ * positions.  Activations are f32 as everywhere in this library, the pages
+ * f32, f16 or bf16.  All pointers are the caller's device memory; the calls
+ * allocate nothing, copy nothing to the host and are stream-ordered, so they
+ * can be captured in a CUDA graph. */
+enum {
+    SLM_KV_F32 = 0,
+    SLM_KV_F16 = 1, /* rounded to nearest even; past 65504 to infinity */
+    SLM_KV_BF16 = 2
+};
+/* Pair layout of the rotation: neighbours (v[2j], v[2j+1]) as
+ * apply_rope_cached, or halves (v[j], v[j + rotary_dim/2]). */
+enum { SLM_ROPE_PAIRS = 0, SLM_ROPE_HALVES = 1 };
+/* Bits of the status word (slm_kv_pages.status). */
+enum {
+    SLM_PAGED_BAD_PAGE = 1,     /* a page id >= num_pages, or none where a key is written */
+    SLM_PAGED_BAD_POSITION = 2, /* a position past the page table or the rope table */
+    SLM_PAGED_WAIT_GAVE_UP = 4  /* a bounded device wait gave up */
+};
+
+/* One layer's pages.  K and V of (page, KV head, slot) are head_dim elements
+ * at page*page_stride + (head*page_size + slot)*head_dim; page_stride 0 means
+ * num_kv_heads*page_size*head_dim, a larger one lets layers or K and V share
+ * an allocation.  k, v and page_stride (in bytes) are multiples of 16.
+ * head_dim is a multiple of 8, at most 128; page_size is any positive number.
+ * `status` (optional) is one zeroed device word that the kernels set bits in
+ * (SLM_PAGED_*); slm_paged_check reads it. */
+typedef struct {
+    void *k, *v;
+    uint64_t page_stride;
+    uint32_t num_pages, page_size, num_kv_heads, head_dim;
+    int32_t dtype;
+    int32_t *status;
+} slm_kv_pages;
+
+/* The rows of one call.  Sequence s owns rows row_start[s]..row_start[s+1]-1
+ * of the activations (any number, zero included), which are its last
+ * positions: row i of them sits at position kv_len[s] - rows + i, kv_len
+ * counting them.  row_start NULL means one new row per sequence
+ * (num_rows = num_seqs).  Key j of sequence s is in page
+ * page_table[s*table_stride + j/page_size], slot j%page_size; a negative id
+ * is a page that is not held (given back, or not needed yet): its keys are
+ * not seen.  kv_len 0 marks an unused place of a padded batch.  max_kv_len is
+ * the host's upper bound of kv_len: it sizes grids and scratch, never results.
+ * Arrays are device memory (int32). */
+typedef struct {
+    const int32_t *row_start;  /* [num_seqs + 1], or NULL */
+    const int32_t *kv_len;     /* [num_seqs] */
+    const int32_t *page_table; /* [num_seqs][table_stride] */
+    uint32_t table_stride, num_seqs, num_rows, max_kv_len;
+} slm_paged_batch;
+
+/* New rows into the cache.  For every row: q and k per head through RMSNorm
+ * (q_norm, k_norm [head_dim], each optional: x / sqrt(mean(x^2) + norm_eps)
+ * * w), then the rotation of their first rotary_dim elements (rope_cos and
+ * rope_sin [rope_rows][rotary_dim/2], indexed by position; NULL with
+ * rotary_dim 0: none; slm_rope_tables makes them for rotary_dim = head_dim),
+ * then k and v into the row's slot and q into q_out.  q, k, v and q_out are
+ * rows of heads, ld* floats apart (>= heads*head_dim; they may be parts of
+ * one projection's output).  q_out may be q itself (with ldq_out = ldq), else
+ * it is apart from q, k and v.  q NULL (with num_heads 0) appends k and v
+ * alone.  rotary_dim is a multiple of 8, at most head_dim.  A row outside
+ * every sequence or before position 0 stores nothing and gets a zero q_out;
+ * so does one past the rope table (SLM_PAGED_BAD_POSITION).  A page id that
+ * is not a page of the pool stores nothing (SLM_PAGED_BAD_PAGE).  Two rows at
+ * one slot of one page leave either's values.  Pairs without a norm into f32
+ * pages give the bits of slm_apply_rope_cached. */
+typedef struct {
+    const float *q, *k, *v;
+    float *q_out;
+    uint64_t ldq, ldk, ldv, ldq_out;
+    uint32_t num_heads;
+    const float *q_norm, *k_norm;
+    float norm_eps;
+    const float *rope_cos, *rope_sin;
+    uint32_t rope_rows, rotary_dim;
+    int32_t rope_style;
+} slm_paged_append_args;
+int slm_paged_append(const slm_kv_pages *pages, const slm_paged_batch *batch,
+                     const slm_paged_append_args *args, void *stream);
+
+/* Attention of every row over its sequence's pages:
+ *   out = sum_j softmax_j(scale * q.k_j) v_j
+ * over the keys j <= p the row at position p sees; with window > 0 those with
+ * p - j < window or j < sinks.  num_heads is a multiple of num_kv_heads;
+ * query head h reads KV head h / (num_heads / num_kv_heads).  scale 0 means
+ * 1/sqrt(head_dim).  A row that sees no key (outside every sequence, before
+ * position 0, no page held), or whose every score is -infinity, is zero.
+ * What is in slots a row does not see (stale, infinite, NaN) does not reach
+ * it.  Sums and the softmax are f32.  out is apart from q.
+ * `scratch` holds slm_paged_attention_scratch_bytes bytes, 16-byte aligned,
+ * contents of no account before and after; calls that may overlap on the GPU
+ * need scratches of their own.  Rows far outnumbering sequences (prompts) and
+ * single new rows take different kernels; see slm_paged_batch.row_start. */
+typedef struct {
+    const float *q;
+    float *out;
+    uint64_t ldq, ldo;
+    uint32_t num_heads;
+    float scale;
+    uint32_t window, sinks;
+} slm_paged_attention_args;
+int slm_paged_attention(const slm_kv_pages *pages, const slm_paged_batch *batch,
+                        const slm_paged_attention_args *args, void *scratch, uint64_t scratch_bytes,
+                        void *stream);
+/* Bytes of scratch for such a call (0 may be returned; then scratch may be
+ * NULL).  It grows with num_rows, num_seqs and max_kv_len: the size for the
+ * largest values of a serving loop serves every smaller call of it. */
+uint64_t slm_paged_attention_scratch_bytes(const slm_kv_pages *pages, const slm_paged_batch *batch,
+                                           const slm_paged_attention_args *args);
+
+/* Wait for `stream`, read the pages' status word and zero it: SLM_OK, or
+ * SLM_ERR_DEVICE_INPUT with what the kernels of earlier calls met. */
+int slm_paged_check(const slm_kv_pages *pages, void *stream);
+
 /* ------------------------------------------------------------------- model
  * TransformerModel (transformer.rs:698-949) for up to `max_sequences`
  * independent sequences, each with its own KV cache, in one device arena.

@@ -9,6 +9,7 @@
 #include <utility>
 
 #include "common.cuh"
+#include "paged.cuh"
 
 namespace slm {
 
@@ -306,5 +307,30 @@ void launch_shard_pack(const float *x, size_t ldx, float *send, int units_per_ra
                        int rank, int kvh, int kd, int n, cudaStream_t s);
 void launch_shard_unpack(const float *recv, float *x, size_t ldx, int units_per_rank, int nranks,
                          int kvh, int kd, int n, cudaStream_t s);
+
+// ---- paged key/value cache (kernels_paged.cu)
+struct AppendView {
+    const float *q, *k, *v;  // rows of heads; q null with num_heads 0
+    float *q_out;
+    size_t ldq, ldk, ldv, ldq_out;
+    int num_heads;
+    const float *q_norm, *k_norm;  // [head_dim] or null
+    float eps;
+    const float *cos, *sin;  // [rope_rows][rotary_dim / 2]
+    int rope_rows, rotary_dim;  // rotary_dim 0: no rotation
+    bool halves;
+    bool vec;  // every f32 pointer 16-byte aligned, every stride a multiple of 4
+};
+void launch_paged_append(const KvView &kv, const BatchView &b, const AppendView &a, cudaStream_t s);
+
+struct PagedAttnView {
+    const float *q;
+    float *out;
+    size_t ldq, ldo;
+    int num_heads;
+    float scale;
+    unsigned window, sinks;
+};
+void launch_paged_attention(const KvView &kv, const BatchView &b, const PagedAttnView &a, cudaStream_t s);
 
 }  // namespace slm

@@ -812,6 +812,191 @@ SLM_EXPORT int slm_sample_argmax(const float *logits, uint64_t n, int32_t *out, 
     return launch_check("argmax kernel");
 }
 
+// ======================================================= paged KV cache
+
+namespace {
+
+bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+int check_pages(const slm_kv_pages *p, KvView *kv) {
+    if (!p) return fail(SLM_ERR_INVALID_ARG, "pages are null");
+    if (!p->k || !p->v) return fail(SLM_ERR_INVALID_ARG, "null page pool");
+    if (p->dtype != SLM_KV_F32 && p->dtype != SLM_KV_F16 && p->dtype != SLM_KV_BF16)
+        return fail(SLM_ERR_INVALID_ARG, "unknown page type");
+    if (p->num_pages == 0 || p->page_size == 0 || p->num_kv_heads == 0)
+        return fail(SLM_ERR_SHAPE, "page counts and sizes must be positive");
+    if (p->head_dim == 0 || p->head_dim % 8 || p->head_dim > 128)
+        return fail(SLM_ERR_SHAPE, "head_dim must be a multiple of 8, at most 128");
+    if (p->num_pages > (uint32_t)INT32_MAX || p->page_size > (1u << 24) || p->num_kv_heads > (1u << 16))
+        return fail(SLM_ERR_SHAPE, "page pool too large");
+    const uint64_t dense = (uint64_t)p->num_kv_heads * p->page_size * p->head_dim;
+    const uint64_t stride = p->page_stride ? p->page_stride : dense;
+    if (stride < dense) return fail(SLM_ERR_SHAPE, "page_stride below one page");
+    if (stride > (uint64_t)1 << 40) return fail(SLM_ERR_SHAPE, "page_stride too large");
+    const uint64_t bytes = stride * (p->dtype == SLM_KV_F32 ? 4 : 2);
+    if (!aligned16(p->k) || !aligned16(p->v) || bytes % 16)
+        return fail(SLM_ERR_INVALID_ARG, "pages must be 16-byte aligned");
+    if ((uintptr_t)p->status & 3) return fail(SLM_ERR_INVALID_ARG, "status word is misaligned");
+    kv->k = p->k;
+    kv->v = p->v;
+    kv->page_stride = stride;
+    kv->num_pages = (int)p->num_pages;
+    kv->page_size = (int)p->page_size;
+    kv->page_shift = -1;
+    for (int s = 0; s < 25; s++)
+        if (p->page_size == 1u << s) kv->page_shift = s;
+    kv->kv_heads = (int)p->num_kv_heads;
+    kv->hd = (int)p->head_dim;
+    kv->type = p->dtype;
+    kv->status = p->status;
+    return SLM_OK;
+}
+
+int check_batch(const slm_paged_batch *b, const KvView &kv, BatchView *v) {
+    if (!b) return fail(SLM_ERR_INVALID_ARG, "batch is null");
+    if (b->num_rows > (uint32_t)INT32_MAX || b->num_seqs >= (uint32_t)INT32_MAX)
+        return fail(SLM_ERR_SHAPE, "too many rows or sequences");
+    if (!b->row_start && b->num_rows != b->num_seqs)
+        return fail(SLM_ERR_SHAPE, "without row_start, num_rows must equal num_seqs");
+    if (b->num_rows && b->num_seqs == 0) return fail(SLM_ERR_SHAPE, "rows without a sequence");
+    if (b->num_rows && (!b->kv_len || !b->page_table)) return fail(SLM_ERR_INVALID_ARG, "null device pointer");
+    if (b->num_rows && b->table_stride == 0) return fail(SLM_ERR_SHAPE, "table_stride must be positive");
+    if ((uint64_t)b->table_stride * (uint64_t)kv.page_size > (uint64_t)INT32_MAX)
+        return fail(SLM_ERR_SHAPE, "page table covers too many positions");
+    if (b->max_kv_len > (uint32_t)INT32_MAX) return fail(SLM_ERR_SHAPE, "max_kv_len too large");
+    v->row_start = b->row_start;
+    v->kv_len = b->kv_len;
+    v->table = b->page_table;
+    v->table_stride = b->table_stride;
+    v->num_seqs = (int)b->num_seqs;
+    v->num_rows = (int)b->num_rows;
+    return SLM_OK;
+}
+
+int check_heads(uint32_t num_heads, const KvView &kv) {
+    if (num_heads == 0 || num_heads % (uint32_t)kv.kv_heads)
+        return fail(SLM_ERR_SHAPE, "num_heads must be a positive multiple of num_kv_heads");
+    if (num_heads > (1u << 16)) return fail(SLM_ERR_SHAPE, "too many heads");
+    return SLM_OK;
+}
+
+int check_attention(const slm_kv_pages *pages, const slm_paged_batch *batch, const slm_paged_attention_args *args,
+                    KvView *kv, BatchView *b, PagedAttnView *a) {
+    TRY(check_pages(pages, kv));
+    TRY(check_batch(batch, *kv, b));
+    if (!args) return fail(SLM_ERR_INVALID_ARG, "arguments are null");
+    TRY(check_heads(args->num_heads, *kv));
+    const uint64_t width = (uint64_t)args->num_heads * kv->hd;
+    if (args->ldq < width || args->ldo < width) return fail(SLM_ERR_SHAPE, "row stride below one row");
+    if (!std::isfinite(args->scale) || args->scale < 0.0f)
+        return fail(SLM_ERR_INVALID_ARG, "scale must be finite and not negative");
+    a->q = args->q;
+    a->out = args->out;
+    a->ldq = args->ldq;
+    a->ldo = args->ldo;
+    a->num_heads = (int)args->num_heads;
+    a->scale = args->scale == 0.0f ? 1.0f / std::sqrt((float)kv->hd) : args->scale;
+    a->window = args->window;
+    a->sinks = args->sinks;
+    return SLM_OK;
+}
+
+}  // namespace
+
+SLM_EXPORT int slm_paged_append(const slm_kv_pages *pages, const slm_paged_batch *batch,
+                                const slm_paged_append_args *args, void *stream) {
+    KvView kv{};
+    BatchView b{};
+    TRY(check_pages(pages, &kv));
+    TRY(check_batch(batch, kv, &b));
+    if (!args) return fail(SLM_ERR_INVALID_ARG, "arguments are null");
+    const uint64_t hd = kv.hd, kw = kv.kv_heads * hd;
+    if (args->q || args->num_heads) {
+        TRY(check_heads(args->num_heads, kv));
+        if (args->ldq < args->num_heads * hd || args->ldq_out < args->num_heads * hd)
+            return fail(SLM_ERR_SHAPE, "row stride below one row");
+    }
+    if (args->ldk < kw || args->ldv < kw) return fail(SLM_ERR_SHAPE, "row stride below one row");
+    if (args->rope_style != SLM_ROPE_PAIRS && args->rope_style != SLM_ROPE_HALVES)
+        return fail(SLM_ERR_INVALID_ARG, "unknown rope style");
+    if (args->rotary_dim % 8 || args->rotary_dim > hd)
+        return fail(SLM_ERR_SHAPE, "rotary_dim must be a multiple of 8, at most head_dim");
+    if (args->rotary_dim && (!args->rope_cos || !args->rope_sin))
+        return fail(SLM_ERR_INVALID_ARG, "null rope table");
+    if ((args->q_norm || args->k_norm) && !(args->norm_eps >= 0.0f && std::isfinite(args->norm_eps)))
+        return fail(SLM_ERR_INVALID_ARG, "norm_eps must be finite and not negative");
+    if (b.num_rows == 0) return SLM_OK;
+    if (!args->k || !args->v || (args->num_heads && (!args->q || !args->q_out)))
+        return fail(SLM_ERR_INVALID_ARG, "null device pointer");
+    if (args->num_heads && args->q_out == args->q && args->ldq_out != args->ldq)
+        return fail(SLM_ERR_OVERLAP, "q_out is q with another row stride");
+    AppendView a{};
+    a.q = args->q;
+    a.k = args->k;
+    a.v = args->v;
+    a.q_out = args->q_out;
+    a.ldq = args->ldq;
+    a.ldk = args->ldk;
+    a.ldv = args->ldv;
+    a.ldq_out = args->ldq_out;
+    a.num_heads = (int)args->num_heads;
+    a.q_norm = args->q_norm;
+    a.k_norm = args->k_norm;
+    a.eps = args->norm_eps;
+    a.cos = args->rope_cos;
+    a.sin = args->rope_sin;
+    a.rope_rows = (int)std::min<uint32_t>(args->rope_rows, (uint32_t)INT32_MAX);
+    a.rotary_dim = (int)args->rotary_dim;
+    a.halves = args->rope_style == SLM_ROPE_HALVES;
+    a.vec = aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.q_out) && aligned16(a.q_norm) &&
+            aligned16(a.k_norm) && aligned16(a.cos) && aligned16(a.sin) &&
+            ((a.ldq | a.ldk | a.ldv | a.ldq_out) & 3) == 0;
+    launch_paged_append(kv, b, a, (cudaStream_t)stream);
+    return launch_check("paged append kernel");
+}
+
+SLM_EXPORT uint64_t slm_paged_attention_scratch_bytes(const slm_kv_pages *pages, const slm_paged_batch *batch,
+                                                      const slm_paged_attention_args *args) {
+    KvView kv{};
+    BatchView b{};
+    PagedAttnView a{};
+    if (check_attention(pages, batch, args, &kv, &b, &a) != SLM_OK) return 0;
+    return 0;
+}
+
+SLM_EXPORT int slm_paged_attention(const slm_kv_pages *pages, const slm_paged_batch *batch,
+                                   const slm_paged_attention_args *args, void *scratch, uint64_t scratch_bytes,
+                                   void *stream) {
+    KvView kv{};
+    BatchView b{};
+    PagedAttnView a{};
+    TRY(check_attention(pages, batch, args, &kv, &b, &a));
+    (void)scratch;
+    (void)scratch_bytes;
+    if (b.num_rows == 0) return SLM_OK;
+    if (!a.q || !a.out) return fail(SLM_ERR_INVALID_ARG, "null device pointer");
+    if (a.q == a.out) return fail(SLM_ERR_OVERLAP, "out is q");
+    launch_paged_attention(kv, b, a, (cudaStream_t)stream);
+    return launch_check("paged attention kernel");
+}
+
+SLM_EXPORT int slm_paged_check(const slm_kv_pages *pages, void *stream) {
+    KvView kv{};
+    TRY(check_pages(pages, &kv));
+    if (!kv.status) return fail(SLM_ERR_INVALID_ARG, "the pages have no status word");
+    cudaStream_t st = (cudaStream_t)stream;
+    int32_t bits = 0;
+    CUDA_TRY(cudaMemcpyAsync(&bits, kv.status, sizeof bits, cudaMemcpyDeviceToHost, st));
+    CUDA_TRY(cudaMemsetAsync(kv.status, 0, sizeof bits, st));
+    CUDA_TRY(cudaStreamSynchronize(st));
+    if (bits == 0) return SLM_OK;
+    std::string what;
+    if (bits & SLM_PAGED_BAD_PAGE) what += "a page id is not a page of the pool; ";
+    if (bits & SLM_PAGED_BAD_POSITION) what += "a position is past the page table or the rope table; ";
+    if (bits & SLM_PAGED_WAIT_GAVE_UP) what += "a device wait timed out; ";
+    return fail(SLM_ERR_DEVICE_INPUT, what.substr(0, what.size() - 2));
+}
+
 // ============================================================== model
 
 namespace {

@@ -15,10 +15,14 @@ import ctypes as C
 
 import numpy as np
 
-from ._lib import JIT_KERNEL_FN, JIT_OPS, PHASES, Config, LayerWeights, ModelWeights, SlmError, Slice, lib
+from ._lib import (JIT_KERNEL_FN, JIT_OPS, KV_BF16, KV_DTYPES, KV_F16, KV_F32, PHASES, ROPE_HALVES, ROPE_PAIRS,
+                   Config, KvPages, LayerWeights, ModelWeights, PagedAppendArgs, PagedAttentionArgs, PagedBatch,
+                   SlmError, Slice, lib)
 
 __all__ = ["Config", "Slice", "SlmError", "Arena", "QMatrix", "Model", "JitEngine", "lib",
-           "gemv_q4_0_arena", "gemm_q4_0_arena", "rope_tables"]
+           "gemv_q4_0_arena", "gemm_q4_0_arena", "rope_tables", "KvPages", "PagedBatch", "PagedAppendArgs",
+           "PagedAttentionArgs", "KV_F32", "KV_F16", "KV_BF16", "KV_DTYPES", "ROPE_PAIRS", "ROPE_HALVES",
+           "paged_append", "paged_attention", "paged_attention_scratch_bytes", "paged_check"]
 
 Q4_BLOCK_BYTES = 18
 Q8_BLOCK_BYTES = 34
@@ -123,6 +127,30 @@ def gemv_q4_0_arena(arena: Arena, w: QMatrix, inp: Slice, q8: Slice, out: Slice,
 def gemm_q4_0_arena(arena: Arena, w: QMatrix, inp: Slice, q8: Slice, out: Slice, batch: int,
                     rows: int, cols: int, stream: int = 0) -> None:
     lib().slm_gemm_q4_0_arena(arena.h, w.h, inp, q8, out, batch, rows, cols, stream)
+
+
+def paged_append(pages: KvPages, batch: PagedBatch, args: PagedAppendArgs, stream: int = 0) -> None:
+    """New rows into the paged cache: per-head RMSNorm of q and k (optional),
+    rotation, K and V into their slots, q into q_out (slm_paged_append)."""
+    lib().slm_paged_append(pages, batch, args, stream)
+
+
+def paged_attention(pages: KvPages, batch: PagedBatch, args: PagedAttentionArgs, scratch: int = 0,
+                    scratch_bytes: int = 0, stream: int = 0) -> None:
+    """Causal attention of every row over its sequence's pages, with an optional
+    window and sinks (slm_paged_attention)."""
+    lib().slm_paged_attention(pages, batch, args, scratch, scratch_bytes, stream)
+
+
+def paged_attention_scratch_bytes(pages: KvPages, batch: PagedBatch, args: PagedAttentionArgs) -> int:
+    """Bytes of device scratch paged_attention needs for such a call."""
+    return int(lib().slm_paged_attention_scratch_bytes(pages, batch, args))
+
+
+def paged_check(pages: KvPages, stream: int = 0) -> None:
+    """Wait for `stream` and raise SlmError when the pages' status word was set
+    (slm_paged_check)."""
+    lib().slm_paged_check(pages, stream)
 
 
 def rope_tables(max_seq: int, head_dim: int):

@@ -54,6 +54,40 @@ class ModelWeights(C.Structure):
                 ("vocab_size", C.c_uint32)]
 
 
+class KvPages(C.Structure):
+    """slm_kv_pages: one layer's page pool (device addresses)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_uint64), ("num_pages", C.c_uint32),
+                ("page_size", C.c_uint32), ("num_kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("dtype", C.c_int32), ("status", C.c_void_p)]
+
+
+class PagedBatch(C.Structure):
+    """slm_paged_batch: the rows of one call and the pages of their sequences."""
+    _fields_ = [("row_start", C.c_void_p), ("kv_len", C.c_void_p), ("page_table", C.c_void_p),
+                ("table_stride", C.c_uint32), ("num_seqs", C.c_uint32), ("num_rows", C.c_uint32),
+                ("max_kv_len", C.c_uint32)]
+
+
+class PagedAppendArgs(C.Structure):
+    """slm_paged_append_args."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_out", C.c_void_p),
+                ("ldq", C.c_uint64), ("ldk", C.c_uint64), ("ldv", C.c_uint64), ("ldq_out", C.c_uint64),
+                ("num_heads", C.c_uint32), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p),
+                ("norm_eps", C.c_float), ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p),
+                ("rope_rows", C.c_uint32), ("rotary_dim", C.c_uint32), ("rope_style", C.c_int32)]
+
+
+class PagedAttentionArgs(C.Structure):
+    """slm_paged_attention_args."""
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("ldq", C.c_uint64), ("ldo", C.c_uint64),
+                ("num_heads", C.c_uint32), ("scale", C.c_float), ("window", C.c_uint32),
+                ("sinks", C.c_uint32)]
+
+
+KV_F32, KV_F16, KV_BF16 = 0, 1, 2
+KV_DTYPES = {"f32": KV_F32, "f16": KV_F16, "bf16": KV_BF16}
+ROPE_PAIRS, ROPE_HALVES = 0, 1
+
 _V = C.c_void_p
 _U64 = C.c_uint64
 _U32 = C.c_uint32
@@ -97,6 +131,13 @@ SIGNATURES = {
     "slm_causal_attention_rows": (C.c_int, [_V, _V, _V, _V, _V, C.POINTER(Config), _U32, _U32, C.c_int, _V],
                                   True),
     "slm_sample_argmax": (C.c_int, [_V, _U64, _V, _V], True),
+    "slm_paged_append": (C.c_int, [C.POINTER(KvPages), C.POINTER(PagedBatch), C.POINTER(PagedAppendArgs), _V],
+                         True),
+    "slm_paged_attention": (C.c_int, [C.POINTER(KvPages), C.POINTER(PagedBatch), C.POINTER(PagedAttentionArgs),
+                                      _V, _U64, _V], True),
+    "slm_paged_attention_scratch_bytes": (_U64, [C.POINTER(KvPages), C.POINTER(PagedBatch),
+                                                 C.POINTER(PagedAttentionArgs)], False),
+    "slm_paged_check": (C.c_int, [C.POINTER(KvPages), _V], True),
     "slm_model_create": (C.c_int, [C.c_int, C.POINTER(Config), C.POINTER(ModelWeights), _U32, _U32,
                                    C.POINTER(_V)], True),
     "slm_model_destroy": (None, [_V], False),
