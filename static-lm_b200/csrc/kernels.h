@@ -6,6 +6,9 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
 #include <utility>
 
 #include "common.cuh"
@@ -52,6 +55,21 @@ inline void launch_kernel_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 bloc
     cfg.numAttrs = pdl ? 2 : 1;
     cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
+
+// Opts one kernel into more than 48 KB of dynamic shared memory, once per
+// device (a static of the launcher; devices past 63 set it every time).
+struct SmemOptIn {
+    std::atomic<uint64_t> done{0};
+    template <typename K>
+    void operator()(K *kernel, int bytes) {
+        int dev = 0;
+        cudaGetDevice(&dev);
+        const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+        if (done.load(std::memory_order_relaxed) & bit) return;
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        done.fetch_or(bit, std::memory_order_relaxed);
+    }
+};
 
 // ---- vector ops / quantization (kernels_vec.cu)
 // RMSNorm of `rows` rows (graph.rs:141-155) fused with Q8_0 quantization of the
@@ -332,5 +350,18 @@ struct PagedAttnView {
     unsigned window, sinks;
 };
 void launch_paged_attention(const KvView &kv, const BatchView &b, const PagedAttnView &a, cudaStream_t s);
+
+// One new row per sequence (kernels_paged_decode.cu): how its keys are split
+// over CTAs, and where the partial results go.
+struct DecodePlan {
+    int heads, head_groups;  // query heads of a KV head per CTA, CTAs per KV head
+    int chunk, splits;       // keys per split; the last split takes what is left
+    float2 *part_ml;         // [row][query head][split] running maximum and sum
+    float *part_o;           // [row][query head][split][head_dim]
+    uint64_t ml_bytes, scratch_bytes;
+};
+DecodePlan plan_paged_decode(const KvView &kv, const BatchView &b, const PagedAttnView &a, uint32_t max_kv_len);
+void launch_paged_decode(const KvView &kv, const BatchView &b, const PagedAttnView &a, const DecodePlan &plan,
+                         cudaStream_t s);
 
 }  // namespace slm

@@ -901,6 +901,14 @@ int check_attention(const slm_kv_pages *pages, const slm_paged_batch *batch, con
     return SLM_OK;
 }
 
+int check_scratch(const void *scratch, uint64_t have, uint64_t need) {
+    if (need == 0) return SLM_OK;
+    if (!scratch) return fail(SLM_ERR_INVALID_ARG, "scratch is null");
+    if (!aligned16(scratch)) return fail(SLM_ERR_INVALID_ARG, "scratch must be 16-byte aligned");
+    if (have < need) return fail(SLM_ERR_CAPACITY, "scratch too small");
+    return SLM_OK;
+}
+
 }  // namespace
 
 SLM_EXPORT int slm_paged_append(const slm_kv_pages *pages, const slm_paged_batch *batch,
@@ -961,7 +969,7 @@ SLM_EXPORT uint64_t slm_paged_attention_scratch_bytes(const slm_kv_pages *pages,
     BatchView b{};
     PagedAttnView a{};
     if (check_attention(pages, batch, args, &kv, &b, &a) != SLM_OK) return 0;
-    return 0;
+    return b.row_start ? 0 : plan_paged_decode(kv, b, a, batch->max_kv_len).scratch_bytes;
 }
 
 SLM_EXPORT int slm_paged_attention(const slm_kv_pages *pages, const slm_paged_batch *batch,
@@ -971,11 +979,17 @@ SLM_EXPORT int slm_paged_attention(const slm_kv_pages *pages, const slm_paged_ba
     BatchView b{};
     PagedAttnView a{};
     TRY(check_attention(pages, batch, args, &kv, &b, &a));
-    (void)scratch;
-    (void)scratch_bytes;
     if (b.num_rows == 0) return SLM_OK;
     if (!a.q || !a.out) return fail(SLM_ERR_INVALID_ARG, "null device pointer");
     if (a.q == a.out) return fail(SLM_ERR_OVERLAP, "out is q");
+    if (!b.row_start) {
+        DecodePlan plan = plan_paged_decode(kv, b, a, batch->max_kv_len);
+        TRY(check_scratch(scratch, scratch_bytes, plan.scratch_bytes));
+        plan.part_ml = (float2 *)scratch;
+        plan.part_o = (float *)((char *)scratch + plan.ml_bytes);
+        launch_paged_decode(kv, b, a, plan, (cudaStream_t)stream);
+        return launch_check("paged decode kernels");
+    }
     launch_paged_attention(kv, b, a, (cudaStream_t)stream);
     return launch_check("paged attention kernel");
 }

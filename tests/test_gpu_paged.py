@@ -556,6 +556,21 @@ def test_another_stream_and_graph_replay(cuda, rows):
     near(out, reference(c, q, n, 8))
 
 
+def test_scratch_too_small_is_refused(cuda):
+    c = Cache(cuda, "f16", [8192], 1, 128, 16, seed=20)
+    q = queries(cuda, 1, 8, 128, 5)
+    out = cuda.zeros_like(q)
+    batch = c.batch(None)
+    args = S.PagedAttentionArgs(q=q.data_ptr(), out=out.data_ptr(), ldq=1024, ldo=1024, num_heads=8)
+    size = S.paged_attention_scratch_bytes(c.pages, batch, args)
+    assert size > 0
+    scratch = cuda.empty(size, dtype=cuda.uint8, device="cuda")
+    for ptr, n in ((scratch.data_ptr(), size - 1), (0, size), (scratch.data_ptr() + 8, size)):
+        with pytest.raises(SlmError) as e:
+            S.paged_attention(c.pages, batch, args, ptr, n)
+        assert e.value.code in (1, 5)
+
+
 def test_wrong_length_hint_changes_nothing(cuda):
     """max_kv_len sizes the grid and the scratch; the lengths on the device decide."""
     for rows in (None, [50, 3]):
