@@ -349,8 +349,6 @@ struct PagedAttnView {
     float scale;
     unsigned window, sinks;
 };
-void launch_paged_attention(const KvView &kv, const BatchView &b, const PagedAttnView &a, cudaStream_t s);
-
 // One new row per sequence (kernels_paged_decode.cu): how its keys are split
 // over CTAs, and where the partial results go.
 struct DecodePlan {
@@ -363,5 +361,21 @@ struct DecodePlan {
 DecodePlan plan_paged_decode(const KvView &kv, const BatchView &b, const PagedAttnView &a, uint32_t max_kv_len);
 void launch_paged_decode(const KvView &kv, const BatchView &b, const PagedAttnView &a, const DecodePlan &plan,
                          cudaStream_t s);
+// Joins the partial results of a row's splits into out.  chunk > 0: splits of
+// `chunk` seen keys, of which only those that have a key were written;
+// chunk 0: every split was written.
+void launch_paged_join(const KvView &kv, const BatchView &b, const PagedAttnView &a, const float2 *part_ml,
+                       const float *part_o, int chunk, int splits, cudaStream_t s);
+
+// Several new rows per sequence (kernels_paged_rows.cu).
+struct RowsPlan {
+    uint64_t tiles;  // row tiles, an upper bound
+    int splits;      // CTAs that share a tile's keys
+    float2 *part_ml;
+    float *part_o;
+    uint64_t ml_bytes, scratch_bytes;
+};
+RowsPlan plan_paged_rows(const KvView &kv, const BatchView &b, const PagedAttnView &a, uint32_t max_kv_len);
+void launch_paged_rows(const KvView &kv, const BatchView &b, const PagedAttnView &a, const RowsPlan &plan, cudaStream_t s);
 
 }  // namespace slm

@@ -1,6 +1,6 @@
 // kernels_paged.cu -- the paged key/value cache: new keys and values into
 // their pages with the per-head RMSNorm and the position rotation applied on
-// the way, and attention over the pages.
+// the way.
 #include "kernels.h"
 
 namespace slm {
@@ -130,66 +130,6 @@ __global__ void __launch_bounds__(AP_THREADS) paged_append_kernel(KvView kv, Bat
     KvElem<TYPE>::store4(pool + i1, y);
 }
 
-// ------------------------------------------------------------- attention
-// One warp per (row, query head): 32 keys at a time, a key per lane for the
-// scores, head_dim over the lanes for the values, with the running maximum
-// and sum of the softmax in f32.
-constexpr int SA_WARPS = 4;
-
-template <int TYPE>
-__global__ void __launch_bounds__(SA_WARPS * 32) paged_attn_kernel(KvView kv, BatchView b, PagedAttnView a) {
-    using T = typename KvElem<TYPE>::T;
-    __shared__ float s_q[SA_WARPS][128];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hd = kv.hd;
-    const uint64_t item = (uint64_t)blockIdx.x * SA_WARPS + warp;
-    if (item >= (uint64_t)b.num_rows * (unsigned)a.num_heads) return;
-    const int row = (int)(item / (unsigned)a.num_heads), h = (int)(item % (unsigned)a.num_heads);
-    const int head = h / (a.num_heads / kv.kv_heads);
-    for (int d = lane; d < hd; d += 32) s_q[warp][d] = a.q[(size_t)row * a.ldq + (size_t)h * hd + d];
-    __syncwarp();
-    int seq, pos;
-    row_place(b, row, seq, pos);
-    const SeenKeys keys = seen_keys(pos, pos, a.window, a.sinks);
-    float m = -INFINITY, sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int i0 = 0; i0 < keys.n; i0 += 32) {
-        long long off = -1;
-        if (i0 + lane < keys.n) off = key_offset(kv, b, seq, (unsigned)keys.key(i0 + lane), head);
-        float s = -INFINITY;
-        if (off >= 0) {
-            const T *k = reinterpret_cast<const T *>(kv.k) + off;
-            float dot = 0.f;
-            for (int d = 0; d < hd; d++) dot = __fmaf_rn(s_q[warp][d], KvElem<TYPE>::get(k + d), dot);
-            s = __fmul_rn(dot, a.scale);
-        }
-        float top = s;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float m_new = fmaxf(m, top);
-        const float base = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = __expf(__fsub_rn(m, base)), p = off >= 0 ? __expf(__fsub_rn(s, base)) : 0.f;
-        m = m_new;
-        float total = p;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) total = __fadd_rn(total, __shfl_xor_sync(0xffffffffu, total, o));
-        sum = __fmaf_rn(sum, alpha, total);
-#pragma unroll
-        for (int c = 0; c < 4; c++) acc[c] = __fmul_rn(acc[c], alpha);
-        for (int j = 0; j < 32; j++) {
-            const long long o = __shfl_sync(0xffffffffu, off, j);
-            const float pj = __shfl_sync(0xffffffffu, p, j);
-            if (o < 0) continue;
-            const T *v = reinterpret_cast<const T *>(kv.v) + o;
-#pragma unroll
-            for (int c = 0; c < 4; c++)
-                if (lane + 32 * c < hd) acc[c] = __fmaf_rn(pj, KvElem<TYPE>::get(v + lane + 32 * c), acc[c]);
-        }
-    }
-    const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.0f, sum);
-#pragma unroll
-    for (int c = 0; c < 4; c++)
-        if (lane + 32 * c < hd) a.out[(size_t)row * a.ldo + (size_t)h * hd + lane + 32 * c] = __fmul_rn(acc[c], inv);
-}
-
 template <int TYPE>
 void append_typed(const KvView &kv, const BatchView &b, const AppendView &a, cudaStream_t s) {
     const uint64_t items = (uint64_t)b.num_rows * (unsigned)(a.num_heads + 2 * kv.kv_heads);
@@ -214,17 +154,6 @@ void launch_paged_append(const KvView &kv, const BatchView &b, const AppendView 
         append_typed<KV_F16>(kv, b, a, s);
     else
         append_typed<KV_BF16>(kv, b, a, s);
-}
-
-void launch_paged_attention(const KvView &kv, const BatchView &b, const PagedAttnView &a, cudaStream_t s) {
-    const uint64_t items = (uint64_t)b.num_rows * (unsigned)a.num_heads;
-    const unsigned grid = (unsigned)((items + SA_WARPS - 1) / SA_WARPS);
-    if (kv.type == KV_F32)
-        paged_attn_kernel<KV_F32><<<grid, SA_WARPS * 32, 0, s>>>(kv, b, a);
-    else if (kv.type == KV_F16)
-        paged_attn_kernel<KV_F16><<<grid, SA_WARPS * 32, 0, s>>>(kv, b, a);
-    else
-        paged_attn_kernel<KV_BF16><<<grid, SA_WARPS * 32, 0, s>>>(kv, b, a);
 }
 
 }  // namespace slm

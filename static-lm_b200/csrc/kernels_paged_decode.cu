@@ -315,45 +315,65 @@ __global__ void __launch_bounds__(PD_THREADS, 2)
     }
 }
 
-// Joins the splits of one (row, query head): a warp per pair.
+// Joins the splits of one (row, query head): warp w takes splits w, w + 4, ..
+// (four loads in flight), a lane four elements of head_dim, and the warps'
+// sums meet in shared memory.
 constexpr int PJ_WARPS = 4;
-__global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(KvView kv, BatchView b, PagedAttnView a, DecodePlan plan) {
-    pdl_wait();
-    const int lane = threadIdx.x & 31;
-    const uint64_t item = (uint64_t)blockIdx.x * PJ_WARPS + (threadIdx.x >> 5);
-    if (item >= (uint64_t)b.num_rows * (unsigned)a.num_heads) return;
+__global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(KvView kv, BatchView b, PagedAttnView a, const float2 *part_ml,
+                                                                       const float *part_o, int chunk, int splits) {
+    __shared__ float4 s_o[PJ_WARPS][32];
+    __shared__ float s_l[PJ_WARPS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint64_t item = blockIdx.x;
     const int row = (int)(item / (unsigned)a.num_heads), h = (int)(item % (unsigned)a.num_heads);
-    const int pos = b.kv_len[row] - 1;
-    const SeenKeys keys = seen_keys(pos, pos, a.window, a.sinks);
-    int live = (keys.n + plan.chunk - 1) / plan.chunk;
-    live = live < 1 ? 1 : live > plan.splits ? plan.splits : live;
-    const float2 *ml = plan.part_ml + item * plan.splits;
-    const float *po = plan.part_o + item * plan.splits * (uint64_t)kv.hd;
+    int live = splits;
+    if (chunk > 0) {
+        const int pos = b.kv_len[row] - 1;  // not written by the kernel waited for
+        const SeenKeys keys = seen_keys(pos, pos, a.window, a.sinks);
+        live = (keys.n + chunk - 1) / chunk;
+        live = live < 1 ? 1 : live > splits ? splits : live;
+    } else if (row >= b.row_start[b.num_seqs]) {
+        return;  // no sequence's: zeroed already
+    }
+    pdl_wait();
+    const float2 *ml = part_ml + item * splits;
+    const float *po = part_o + item * splits * (uint64_t)kv.hd + 4 * lane;
+    const bool mine = 4 * lane < kv.hd;
     float top = PD_NO_MAX;
     for (int s = lane; s < live; s += 32) top = fmaxf(top, ml[s].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; s0 < live; s0 += 32) {
-        float f = 0.f, lf = 0.f;
-        if (s0 + lane < live) {
-            const float2 x = ml[s0 + lane];
-            f = exp2_approx(__fsub_rn(x.x, top));
-            lf = __fmul_rn(f, x.y);
-        }
-        const int n = live - s0 < 32 ? live - s0 : 32;
-        for (int s = 0; s < n; s++) {
-            const float fs = __shfl_sync(0xffffffffu, f, s);
-            sum = __fadd_rn(sum, __shfl_sync(0xffffffffu, lf, s));
+    float sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = warp; s0 < live; s0 += 4 * PJ_WARPS) {
+        float2 x[4];
+        float4 v[4];
 #pragma unroll
-            for (int c = 0; c < 4; c++)
-                if (lane + 32 * c < kv.hd) acc[c] = __fmaf_rn(fs, po[(size_t)(s0 + s) * kv.hd + lane + 32 * c], acc[c]);
+        for (int u = 0; u < 4; u++) {
+            const int s = s0 + u * PJ_WARPS;
+            x[u] = s < live ? ml[s] : make_float2(PD_NO_MAX, 0.f);
+            v[u] = s < live && mine ? *reinterpret_cast<const float4 *>(po + (size_t)s * kv.hd) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const float f = exp2_approx(__fsub_rn(x[u].x, top));
+            sum = __fmaf_rn(f, x[u].y, sum);
+            acc.x = __fmaf_rn(f, v[u].x, acc.x);
+            acc.y = __fmaf_rn(f, v[u].y, acc.y);
+            acc.z = __fmaf_rn(f, v[u].z, acc.z);
+            acc.w = __fmaf_rn(f, v[u].w, acc.w);
         }
     }
-    const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.0f, sum);
-#pragma unroll
-    for (int c = 0; c < 4; c++)
-        if (lane + 32 * c < kv.hd) a.out[(size_t)row * a.ldo + (size_t)h * kv.hd + lane + 32 * c] = __fmul_rn(acc[c], inv);
+    s_o[warp][lane] = acc;
+    if (lane == 0) s_l[warp] = sum;
+    __syncthreads();
+    const float total = __fadd_rn(__fadd_rn(s_l[0], s_l[1]), __fadd_rn(s_l[2], s_l[3]));
+    const float *f = reinterpret_cast<const float *>(s_o);
+    const int d = threadIdx.x;
+    if (d < kv.hd) {
+        const float o = __fadd_rn(__fadd_rn(f[d], f[128 + d]), __fadd_rn(f[256 + d], f[384 + d]));
+        a.out[(size_t)row * a.ldo + (size_t)h * kv.hd + d] = total == 0.f ? 0.f : __fdiv_rn(o, total);
+    }
 }
 
 constexpr size_t PD_SMEM = (size_t)PD_WARPS * PD_STAGES * 2 * PD_TILE;
@@ -430,11 +450,14 @@ void launch_paged_decode(const KvView &kv, const BatchView &b, const PagedAttnVi
     for_rows(kv.type, kv.hd, [&](auto type, auto lpr) {
         for_heads(plan.heads, [&](auto g) { go<decltype(type)::value, decltype(lpr)::value, decltype(g)::value>(kv, b, a, plan, s); });
     });
-    if (plan.splits > 1) {
-        const uint64_t items = (uint64_t)b.num_rows * a.num_heads;
-        launch_kernel(paged_join_kernel, dim3((unsigned)((items + PJ_WARPS - 1) / PJ_WARPS)), dim3(PJ_WARPS * 32), 0, s, true,
-                      kv, b, a, plan);
-    }
+    if (plan.splits > 1) launch_paged_join(kv, b, a, plan.part_ml, plan.part_o, plan.chunk, plan.splits, s);
+}
+
+void launch_paged_join(const KvView &kv, const BatchView &b, const PagedAttnView &a, const float2 *part_ml,
+                       const float *part_o, int chunk, int splits, cudaStream_t s) {
+    const uint64_t items = (uint64_t)b.num_rows * a.num_heads;
+    launch_kernel(paged_join_kernel, dim3((unsigned)items), dim3(PJ_WARPS * 32), 0, s, true, kv, b, a, part_ml, part_o,
+                  chunk, splits);
 }
 
 }  // namespace slm

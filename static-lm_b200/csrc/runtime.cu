@@ -969,7 +969,8 @@ SLM_EXPORT uint64_t slm_paged_attention_scratch_bytes(const slm_kv_pages *pages,
     BatchView b{};
     PagedAttnView a{};
     if (check_attention(pages, batch, args, &kv, &b, &a) != SLM_OK) return 0;
-    return b.row_start ? 0 : plan_paged_decode(kv, b, a, batch->max_kv_len).scratch_bytes;
+    return b.row_start ? plan_paged_rows(kv, b, a, batch->max_kv_len).scratch_bytes
+                       : plan_paged_decode(kv, b, a, batch->max_kv_len).scratch_bytes;
 }
 
 SLM_EXPORT int slm_paged_attention(const slm_kv_pages *pages, const slm_paged_batch *batch,
@@ -990,8 +991,12 @@ SLM_EXPORT int slm_paged_attention(const slm_kv_pages *pages, const slm_paged_ba
         launch_paged_decode(kv, b, a, plan, (cudaStream_t)stream);
         return launch_check("paged decode kernels");
     }
-    launch_paged_attention(kv, b, a, (cudaStream_t)stream);
-    return launch_check("paged attention kernel");
+    RowsPlan plan = plan_paged_rows(kv, b, a, batch->max_kv_len);
+    TRY(check_scratch(scratch, scratch_bytes, plan.scratch_bytes));
+    plan.part_ml = (float2 *)scratch;
+    plan.part_o = (float *)((char *)scratch + plan.ml_bytes);
+    launch_paged_rows(kv, b, a, plan, (cudaStream_t)stream);
+    return launch_check("paged rows kernels");
 }
 
 SLM_EXPORT int slm_paged_check(const slm_kv_pages *pages, void *stream) {
