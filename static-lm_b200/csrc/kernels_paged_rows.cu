@@ -610,12 +610,14 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
                 n_take++;
                 return slot;
             };
-            auto parts = [&](auto f) {  // the products of parts that count
+            // the products of parts that count, the smallest first: each MMA
+            // cuts its sum at the last bit of the largest addend
+            auto parts = [&](auto f) {
                 if constexpr (NC == 1) {
 #pragma unroll
-                    for (int i = 0; i < NQ; i++) f(i, 0, i == 0);
+                    for (int i = NQ - 1; i >= 0; i--) f(i, 0, i == NQ - 1);
                 } else {
-                    f(0, 0, true), f(0, 1, false), f(1, 0, false), f(1, 1, false), f(0, 2, false), f(2, 0, false);
+                    f(2, 0, true), f(0, 2, false), f(1, 1, false), f(1, 0, false), f(0, 1, false), f(0, 0, false);
                 }
             };
             auto scores = [&](int x, int slot) {
