@@ -12,14 +12,19 @@
 //   f32 pages:  three bf16 parts of q, w, k and v; the 6 products whose size
 //               is above 2^-24 of the leading one.
 //
-// A CTA takes one (sequence, KV head) and a run of its rows, the query heads
-// of the KV head side by side (row = token * group + head in group), so every
-// key read serves all of them.  Two streams of work keep the tensor core busy
-// while the other's softmax runs: with f16 pages two tiles of 128 rows over
-// the same keys, else one tile of 128 rows over the even and the odd key tiles
-// (their sums are joined at the end).  Warps 0-3 and 4-7 run the streams'
-// softmax, a row per thread; warp 8 issues the MMAs; warps 9-11 bring keys and
-// values from the pages into a ring of shared-memory slots.
+// The tensor core cuts each sum at the last bit of its largest addend, always
+// towards zero: about 2e-8 of the sum per MMA, which over the hundreds of MMAs
+// of a long row adds up.  So no chain of MMAs is longer than one key tile (at
+// most 24, the smallest products first): every tile's w.v goes to TMEM afresh
+// and is added to the row's sums in registers.
+//
+// A CTA takes 128 rows of one (sequence, KV head), the query heads of the KV
+// head side by side (row = token * group + head in group), so every key read
+// serves all of them.  Warps 0-7 run the softmax: thread r and r + 128 hold
+// the two halves of row r's keys of a tile, and of its head_dim.  Warp 8
+// issues the MMAs, warps 9-11 bring keys and values from the pages into a
+// ring of shared-memory slots.  Scores and tile results are double-buffered in
+// TMEM: q.k of tile j + 1 and w.v of tile j - 1 run under the softmax of j.
 #include "async.cuh"
 #include "kernels.h"
 #include "tc.cuh"
@@ -37,32 +42,31 @@ constexpr unsigned PR_TMEM_COLS = 512;
 template <int TYPE, int HDP>
 struct RowsCfg {
     static constexpr bool F16 = TYPE == KV_F16;
-    static constexpr int T = F16 ? 2 : 1;        // row tiles per CTA
     static constexpr int KT = F16 ? 128 : 64;    // keys per tile
     static constexpr int NQ = F16 ? 2 : 3;       // parts of q and of the weights
     static constexpr int NC = TYPE == KV_F32 ? 3 : 1;  // parts of k and v
-    static constexpr int RT = T * 128;
     static constexpr int PART = KT * HDP * 2;    // bytes of one part of a key tile
     static constexpr int SLOT = PART * NC;
     static constexpr int QPART = 128 * HDP * 2;
-    static constexpr int QBYTES = T * NQ * QPART;
-    static constexpr int NSLOT = F16 ? (HDP == 128 ? 3 : 6) : TYPE == KV_BF16 ? (HDP == 128 ? 6 : 8) : (HDP == 128 ? 2 : 4);
-    static constexpr int SP = F16 ? 128 : 96;    // TMEM columns of scores / weights
-    static constexpr int STREAM = SP + HDP;      // TMEM columns of a stream
+    static constexpr int QBYTES = NQ * QPART;
+    static constexpr int NSLOT = F16 ? (HDP == 128 ? 5 : 8) : TYPE == KV_BF16 ? 8 : (HDP == 128 ? 2 : 6);
+    // TMEM columns: score / weight buffers (128 or 3 x 32 used) at 0 and 128,
+    // results at 256 and 256 + HDP: each buffer at a multiple of its width, as
+    // an accumulator laid across column 256 faulted
+    static constexpr int T_S = 128, T_O = 256;
     static constexpr int BIG = QBYTES + NSLOT * SLOT;
     // at least 120 KB: one CTA per SM, whose TMEM it takes whole
     static constexpr int SMEM = (BIG > 120 * 1024 ? BIG : 120 * 1024) + 3072;
     static_assert(SMEM <= 227 * 1024, "shared memory");
-    static_assert(2 * STREAM <= (int)PR_TMEM_COLS, "TMEM");
-    static_assert(QBYTES >= 128 * HDP * 4, "the odd stream's sums fit the q tiles");
+    static_assert(T_O + 2 * HDP <= (int)PR_TMEM_COLS && KT <= T_S && NQ * KT / 2 <= T_S, "TMEM");
 };
 
 // The small shared data, after the tiles.
 struct RowsShared {
     uint64_t full[8], empty[8], s_full[2], p_full[2], o_full[2], q_full, drain;
-    long long off[128];       // element offsets of the keys of the newest tiles
-    float ml[2][128];         // the odd stream's maxima and sums
+    long long off[128];       // element offsets of the newest tile's keys
     unsigned valid[8][4];     // held keys of the newest 8 tiles
+    float row[2][128];        // exchanged between the halves of a row; 2^-e of q's rows before
     unsigned taddr;
     int abort;
     // the CTA's work
@@ -93,19 +97,30 @@ __device__ __forceinline__ unsigned umma_idesc_f16(bool bf16, int M, int N, bool
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn ? 1u : 0u) << 16) |
            ((unsigned)(N >> 3) << 17) | ((unsigned)(M >> 4) << 24);
 }
-// D[128 x N] (+)= A[128 x 16] B[N x 16]^T; A in shared memory or in TMEM.
-__device__ __forceinline__ void tc_mma_f16(unsigned d, uint64_t adesc, uint64_t bdesc, unsigned idesc, bool acc) {
+// D[128 x N] (+)= A[128 x 16] B[N x 16]^T, A in shared memory or in TMEM, and
+// the commit of what a lane issued: the whole warp comes here with the same
+// operands and the lane with `me` issues.  (The operands are the warp's
+// uniform registers; issued from a branch of one lane, unrolled MMAs were
+// given each other's.)
+__device__ __forceinline__ void tc_mma_f16(bool me, unsigned d, uint64_t adesc, uint64_t bdesc, unsigned idesc, bool acc) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n}\n" ::"r"(d),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"((unsigned)acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %9, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n}\n" ::"r"(d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"((unsigned)acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u), "r"((unsigned)me)
         : "memory");
 }
-__device__ __forceinline__ void tc_mma_f16_ta(unsigned d, unsigned a, uint64_t bdesc, unsigned idesc, bool acc) {
+__device__ __forceinline__ void tc_mma_f16_ta(bool me, unsigned d, unsigned a, uint64_t bdesc, unsigned idesc, bool acc) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n}\n" ::"r"(d),
-        "r"(a), "l"(bdesc), "r"(idesc), "r"((unsigned)acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %9, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(bdesc), "r"(idesc), "r"((unsigned)acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u), "r"((unsigned)me)
+        : "memory");
+}
+__device__ __forceinline__ void tc_commit_by(bool me, uint64_t *bar) {
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_addr(bar)),
+        "r"((unsigned)me)
         : "memory");
 }
 
@@ -140,22 +155,6 @@ __device__ __forceinline__ void tmem_st16(unsigned taddr, const unsigned *r) {
         : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
-
-// 8 columns of this thread's lane times f.
-__device__ __forceinline__ void tmem_scale8(unsigned taddr, float f) {
-    float v[8];
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
-                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
-                 : "r"(taddr)
-                 : "memory");
-    tmem_wait_ld();
-    asm volatile("" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7])::"memory");
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = __fmul_rn(v[i], f);
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"r"(taddr), "f"(v[0]),
-                 "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
-                 : "memory");
-}
 
 __device__ __forceinline__ float ex2(float x) {
     float r;
@@ -281,9 +280,10 @@ template <int TYPE, int HDP>
 __global__ void __launch_bounds__(PR_THREADS, 1)
     paged_rows_kernel(KvView kv, BatchView b, PagedAttnView a, RowsPlan plan) {
     using Cfg = RowsCfg<TYPE, HDP>;
-    constexpr int KT = Cfg::KT, NQ = Cfg::NQ, NC = Cfg::NC, T = Cfg::T, RT = Cfg::RT;
+    constexpr int KT = Cfg::KT, NQ = Cfg::NQ, NC = Cfg::NC;
+    constexpr int CT = KT / 2, OC = HDP / 2;        // a thread's keys of a tile, and its part of head_dim
     extern __shared__ __align__(1024) unsigned char pr_smem[];
-    unsigned char *s_q = pr_smem;                   // [tile][part] operands of 128 rows
+    unsigned char *s_q = pr_smem;                   // [part] operands of 128 rows
     unsigned char *s_kv = pr_smem + Cfg::QBYTES;    // ring of key / value tiles
     RowsShared *sh = reinterpret_cast<RowsShared *>(pr_smem + Cfg::SMEM - 3072);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
                 rows = b.row_start[s + 1] - start;
                 if (start < 0 || rows < 0 || rows > b.num_rows - start) rows = 0;
             }
-            const int n = (int)(((long long)rows * group + RT - 1) / RT);
+            const int n = (int)(((long long)rows * group + 127) / 128);
             int sum = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
         }
         for (int x = 0; x < 2; x++) {
             mbar_init(&sh->s_full[x], 1);
-            mbar_init(&sh->p_full[x], 128);
+            mbar_init(&sh->p_full[x], 256);
             mbar_init(&sh->o_full[x], 1);
         }
         mbar_init(&sh->q_full, 256);
@@ -356,9 +356,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
     const int seq = sh->seq, row0 = sh->row0, rows = sh->rows, tile = sh->tile;
     const int pos0 = b.kv_len[seq] - rows;  // position of the sequence's first row
     // tokens of this tile, and the list of keys any of them sees
-    const int tok0 = (int)((long long)tile * RT / group);
-    const long long last_flat = (long long)tile * RT + RT - 1;
-    const int tok1 = last_flat / group < rows ? (int)(last_flat / group) : rows - 1;
+    const long long flat0 = (long long)tile * 128;
+    const int tok0 = (int)(flat0 / group);
+    const int tok1 = (flat0 + 127) / group < rows ? (int)((flat0 + 127) / group) : rows - 1;
     const SeenKeys keys = seen_keys(pos0 + tok0, pos0 + tok1, a.window, a.sinks);
     const int all_tiles = (keys.n + KT - 1) / KT;
     const int per_split = (all_tiles + plan.splits - 1) / plan.splits;
@@ -373,9 +373,60 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
 
     if (warp < 8) {
         // ------------------------------------------------ q, softmax, output
-        const int x = warp >> 2, r = tid & 127;      // stream, row of its tile
-        const long long flat = (long long)tile * RT + (T == 2 ? x * 128 : 0) + r;
-        const int tok = (int)(flat / group), h = head * group + (int)(flat % group);
+        const float sl2_all = __fmul_rn(a.scale, 1.44269504088896340736f);
+        {  // a warp per row, four rows at a time
+            const bool vec = (((uintptr_t)a.q | (a.ldq * 4)) & 15) == 0;
+            const int c4 = lane * 4;
+            for (int r0 = warp * 16; r0 < warp * 16 + 16; r0 += 4) {
+                float f[4][4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const long long flat = flat0 + r0 + u;
+                    const int tok = (int)(flat / group);
+                    const float *src = a.q + (size_t)(row0 + tok) * a.ldq + (size_t)(head * group + (int)(flat - (long long)tok * group)) * hd + c4;
+                    const bool in = tok < rows && c4 < hd;
+                    if (in && vec) {
+                        const float4 t = *reinterpret_cast<const float4 *>(src);
+                        f[u][0] = t.x, f[u][1] = t.y, f[u][2] = t.z, f[u][3] = t.w;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) f[u][i] = in ? src[i] : 0.f;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    if constexpr (Cfg::F16) {
+                        float top = fmaxf(fmaxf(fabsf(f[u][0]), fabsf(f[u][1])), fmaxf(fabsf(f[u][2]), fabsf(f[u][3])));
+#pragma unroll
+                        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                        int e = 0;
+                        if (top > 0.f && top < INFINITY) {
+                            frexpf(top, &e);  // top = f 2^e, 0.5 <= f < 1
+                            e = 15 - e;
+                            e = e > 120 ? 120 : e < -120 ? -120 : e;
+                        }
+                        const float up = __uint_as_float((unsigned)(127 + e) << 23);
+                        if (lane == 0) sh->row[0][r0 + u] = __uint_as_float((unsigned)(127 - e) << 23);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) f[u][i] = __fmul_rn(f[u][i], up);
+                    }
+                    if (c4 < HDP) {
+                        unsigned p[NQ], q[NQ];
+                        split2<TYPE, NQ>(f[u][0], f[u][1], p);
+                        split2<TYPE, NQ>(f[u][2], f[u][3], q);
+                        const unsigned o = sw16_off(r0 + u, lane >> 1, 128) + (lane & 1) * 8;
+#pragma unroll
+                        for (int i = 0; i < NQ; i++)
+                            *reinterpret_cast<uint2 *>(s_q + i * Cfg::QPART + o) = make_uint2(p[i], q[i]);
+                    }
+                }
+            }
+            fence_async_smem();
+            mbar_arrive(&sh->q_full);
+            if constexpr (Cfg::F16) named_bar_sync(2, 256);  // the rows' 2^-e
+        }
+        const int x = warp >> 2, r = tid & 127;  // half, row of the tile
+        const int tok = (int)((flat0 + r) / group), h = head * group + (int)((flat0 + r) % group);
         const bool row_ok = tok < rows;
         const int row = row0 + (row_ok ? tok : 0);
         const int pos = row_ok ? pos0 + tok : -1;
@@ -384,102 +435,84 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
         const int sink_end = a.sinks < 0x7fffffffu ? (int)a.sinks : 0x7fffffff;
         int from = 0;
         if (a.window != 0 && pos >= 0 && (unsigned)pos >= a.window) from = pos - (int)a.window + 1 - keys.low + keys.sinks;
-        float sl2 = __fmul_rn(a.scale, 1.44269504088896340736f);
-        {
-            const float *src = a.q + (size_t)row * a.ldq + (size_t)h * hd;
-            const bool vec = (((uintptr_t)a.q | (a.ldq * 4)) & 15) == 0;
-            float up = 1.0f;
-            if constexpr (Cfg::F16) {
-                float top = 0.f;
-                if (row_ok)
-                    for (int d = 0; d < hd; d++) top = fmaxf(top, fabsf(src[d]));
-                if (top > 0.f && top < INFINITY) {
-                    int e;
-                    frexpf(top, &e);  // top = f 2^e, 0.5 <= f < 1
-                    e = 15 - e;
-                    e = e > 120 ? 120 : e < -120 ? -120 : e;
-                    up = __uint_as_float((unsigned)(127 + e) << 23);
-                    sl2 = __fmul_rn(sl2, __uint_as_float((unsigned)(127 - e) << 23));
-                }
-            }
-            unsigned char *tq = s_q + (T == 2 ? x * NQ * Cfg::QPART : 0);
-            // with one tile the two warpgroups take alternate chunks of it
-            for (int c = T == 2 ? 0 : x; c < HDP / 8; c += T == 2 ? 1 : 2) {
-                float f[8];
-                const bool in = row_ok && c * 8 < hd;
-                if (in && vec) {
-                    const float4 u = *reinterpret_cast<const float4 *>(src + c * 8);
-                    const float4 w = *reinterpret_cast<const float4 *>(src + c * 8 + 4);
-                    f[0] = u.x, f[1] = u.y, f[2] = u.z, f[3] = u.w, f[4] = w.x, f[5] = w.y, f[6] = w.z, f[7] = w.w;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) f[i] = in ? src[c * 8 + i] : 0.f;
-                }
-                unsigned part[4][NQ];
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    split2<TYPE, NQ>(__fmul_rn(f[2 * i], up), __fmul_rn(f[2 * i + 1], up), part[i]);
-                const unsigned o = sw16_off(r, c, 128);
-#pragma unroll
-                for (int p = 0; p < NQ; p++)
-                    *reinterpret_cast<uint4 *>(tq + p * Cfg::QPART + o) =
-                        make_uint4(part[0][p], part[1][p], part[2][p], part[3][p]);
-            }
-            fence_async_smem();
-            mbar_arrive(&sh->q_full);
-        }
-        const unsigned t_s = taddr + ((unsigned)((warp & 3) * 32) << 16) + (unsigned)(x * Cfg::STREAM);
-        const unsigned t_o = t_s + Cfg::SP;
+        const float sl2 = Cfg::F16 ? __fmul_rn(sl2_all, sh->row[0][r]) : sl2_all;
+        const unsigned t_lane = taddr + ((unsigned)((warp & 3) * 32) << 16);
         float m = PR_NO_MAX, l = 0.f;
-        bool ok = true, any = false;
-        unsigned phase = 0;
-        for (int j = T == 2 ? 0 : x; j < ntile; j += T == 2 ? 1 : 2) {
-            ok = __all_sync(0xffffffffu, pr_wait(&sh->s_full[x], phase, sh, kv));  // TMEM loads are warp-wide
-            if (!ok) break;
-            phase ^= 1;
+        float acc[OC];
+#pragma unroll
+        for (int i = 0; i < OC; i++) acc[i] = 0.f;
+        bool ok = true;
+        // adds this half of tile j's w.v to the row's sums
+        auto gather = [&](int j) {
+            ok = __all_sync(0xffffffffu, ok && pr_wait(&sh->o_full[j & 1], (j >> 1) & 1u, sh, kv));
+            if (!ok) return;
             tc_fence_after();
-            float v[KT];
 #pragma unroll
-            for (int c = 0; c < KT; c += 32) tmem_ld32(t_s + c, v + c);
-            tmem_wait_ld();
+            for (int c = 0; c < OC; c += 32) {
+                float o[32];
+                tmem_ld32(t_lane + Cfg::T_O + (j & 1) * HDP + x * OC + c, o);
+                tmem_wait_ld();
+                pin32(o);
 #pragma unroll
-            for (int c = 0; c < KT; c += 32) pin32(v + c);
-            const int i0 = lo + j * KT;
-            bool whole = i0 + KT <= to && i0 + KT <= hi && (i0 + KT <= sink_end || i0 >= from);
+                for (int i = 0; i < 32; i++) acc[c + i] = __fadd_rn(acc[c + i], o[i]);
+            }
+        };
+        for (int j = 0; j < ntile; j++) {
+            const unsigned t_s = t_lane + (j & 1) * Cfg::T_S;
+            ok = __all_sync(0xffffffffu, ok && pr_wait(&sh->s_full[j & 1], (j >> 1) & 1u, sh, kv));  // TMEM loads are warp-wide
+            float v[CT];
+            float top = -INFINITY;
+            if (ok) {
+                tc_fence_after();
 #pragma unroll
-            for (int c = 0; c < KT / 32; c++) whole = whole && sh->valid[j & 7][c] == 0xffffffffu;
-            if (!__all_sync(0xffffffffu, whole)) {
+                for (int c = 0; c < CT; c += 32) tmem_ld32(t_s + x * CT + c, v + c);
+                tmem_wait_ld();
 #pragma unroll
-                for (int c = 0; c < KT; c++) {
-                    const int i = i0 + c;
-                    const bool seen = i < to && (i < sink_end || i >= from) && ((sh->valid[j & 7][c >> 5] >> (c & 31)) & 1u);
-                    v[c] = seen ? v[c] : -INFINITY;
+                for (int c = 0; c < CT; c += 32) pin32(v + c);
+                const int i0 = lo + j * KT + x * CT;
+                const unsigned *valid = &sh->valid[j & 7][x * CT / 32];
+                bool whole = i0 + CT <= to && i0 + CT <= hi && (i0 + CT <= sink_end || i0 >= from);
+#pragma unroll
+                for (int c = 0; c < CT / 32; c++) whole = whole && valid[c] == 0xffffffffu;
+                if (!__all_sync(0xffffffffu, whole)) {
+#pragma unroll
+                    for (int c = 0; c < CT; c++) {
+                        const int i = i0 + c;
+                        const bool seen = i < to && (i < sink_end || i >= from) && ((valid[c >> 5] >> (c & 31)) & 1u);
+                        v[c] = seen ? v[c] : -INFINITY;
+                    }
                 }
-            }
-            float t0 = v[0], t1 = v[1], t2 = v[2], t3 = v[3];
+                float t0 = v[0], t1 = v[1], t2 = v[2], t3 = v[3];
 #pragma unroll
-            for (int c = 4; c < KT; c += 4) {
-                t0 = fmaxf(t0, v[c]);
-                t1 = fmaxf(t1, v[c + 1]);
-                t2 = fmaxf(t2, v[c + 2]);
-                t3 = fmaxf(t3, v[c + 3]);
-            }
-            const float top = __fmul_rn(fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)), sl2);
-            const bool move = top > m + PR_RESCALE;
-            if (__any_sync(0xffffffffu, move)) {
-                const float f = move ? ex2(__fsub_rn(m, top)) : 1.0f;
-                m = move ? top : m;
-                l = __fmul_rn(l, f);
-                if (any) {  // the stream's earlier products are complete: so are its scores
-#pragma unroll 1
-                    for (int c = 0; c < HDP; c += 8) tmem_scale8(t_o + c, f);  // few registers: the scores are live
+                for (int c = 4; c < CT; c += 4) {
+                    t0 = fmaxf(t0, v[c]);
+                    t1 = fmaxf(t1, v[c + 1]);
+                    t2 = fmaxf(t2, v[c + 2]);
+                    t3 = fmaxf(t3, v[c + 3]);
                 }
+                top = __fmul_rn(fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)), sl2);
             }
-            any = true;
+            // every score of the tile is in registers after this barrier, and
+            // the halves of each row move their reference together
+            float f = 1.0f;
+            const bool moved = named_bar_or(2, 256, top > m + PR_RESCALE || !ok);
+            if (moved) {
+                sh->row[x][r] = top;
+                if (named_bar_or(2, 256, !ok)) {
+                    ok = false;
+                    break;
+                }
+                const float both = fmaxf(top, sh->row[x ^ 1][r]);
+                if (both > m + PR_RESCALE) {
+                    f = ex2(__fsub_rn(m, both));
+                    m = both;
+                    l = __fmul_rn(l, f);
+                }
+                named_bar_sync(2, 256);  // read before the next tile's
+            }
             float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;
-            // the scores are all in registers: the weights' parts take their place
 #pragma unroll
-            for (int c = 0; c < KT; c += 32) {
+            for (int c = 0; c < CT; c += 32) {
                 unsigned w[NQ][16];
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {
@@ -495,123 +528,85 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
 #pragma unroll
                     for (int n = 0; n < NQ; n++) w[n][i / 2] = p[n], w[n][i / 2 + 1] = q[n];
                 }
+                // the weights' parts take the scores' place
 #pragma unroll
-                for (int n = 0; n < NQ; n++) tmem_st16(t_s + n * (KT / 2) + c / 2, w[n]);
+                for (int n = 0; n < NQ; n++) tmem_st16(t_s + n * (KT / 2) + (x * CT + c) / 2, w[n]);
             }
             l = __fadd_rn(l, __fadd_rn(__fadd_rn(l0, l1), __fadd_rn(l2, l3)));
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(&sh->p_full[x]);
-        }
-        if (ok && any) ok = __all_sync(0xffffffffu, pr_wait(&sh->o_full[x], 0, sh, kv));
-        tc_fence_after();
-        float *s_o = reinterpret_cast<float *>(s_q);  // [head_dim][128]: the odd stream's sums
-        if constexpr (T == 1) {
-            // the q tiles are free: every q.k product is complete once o_full[1]
-            // is, and with fewer than two key tiles there is no odd stream
-            if (x == 1) {
-                if (ok && any) {
-#pragma unroll 1
-                    for (int c = 0; c < HDP; c += 32) {
-                        float o[32];
-                        tmem_ld32(t_o + c, o);
-                        tmem_wait_ld();
-                        pin32(o);
+            mbar_arrive(&sh->p_full[j & 1]);
+            if (j > 0) gather(j - 1);  // under w.v of this tile
+            if (moved) {
 #pragma unroll
-                        for (int i = 0; i < 32; i++)
-                            if (c + i < hd) s_o[(c + i) * 128 + r] = o[i];
-                    }
-                }
-                sh->ml[0][r] = m;
-                sh->ml[1][r] = l;
+                for (int i = 0; i < OC; i++) acc[i] = __fmul_rn(acc[i], f);
             }
-            if (named_bar_or(2, 256, !ok)) ok = false;
         }
-        if (ok && (T == 2 || x == 0)) {
-            float mine = 1.0f, other = 0.f;
-            if constexpr (T == 1) {
-                const float m1 = sh->ml[0][r], l1 = sh->ml[1][r];
-                const float top = fmaxf(m, m1);
-                mine = ex2(__fsub_rn(m, top));
-                other = ex2(__fsub_rn(m1, top));
-                l = __fadd_rn(__fmul_rn(l, mine), __fmul_rn(l1, other));
-                m = top;
-            }
-            const bool two = T == 1 && ntile > 1;
+        if (ok && ntile > 0) gather(ntile - 1);
+        sh->row[x][r] = l;
+        if (!named_bar_or(2, 256, !ok)) {
+            l = __fadd_rn(sh->row[0][r], sh->row[1][r]);
             const bool whole = plan.splits == 1;
             const float inv = !whole ? 1.0f : l == 0.f ? 0.f : __fdiv_rn(1.0f, l);
             const size_t part = ((size_t)row * a.num_heads + h) * plan.splits + split;
-            float *dst = whole ? a.out + (size_t)row * a.ldo + (size_t)h * hd : plan.part_o + part * hd;
+            float *dst = (whole ? a.out + (size_t)row * a.ldo + (size_t)h * hd : plan.part_o + part * hd) + x * OC;
             const bool vec = !whole || (((uintptr_t)a.out | (a.ldo * 4)) & 15) == 0;
             bool finite = fabsf(l) < INFINITY;
-#pragma unroll 1
-            for (int c = 0; c < HDP; c += 32) {
-                float o[32];
-                if (any) {
-                    tmem_ld32(t_o + c, o);
-                    tmem_wait_ld();
-                    pin32(o);
-                }
 #pragma unroll
-                for (int i = 0; i < 32; i++) {
-                    float y = any ? o[i] : 0.f;
-                    if constexpr (T == 1) {
-                        y = __fmul_rn(y, mine);
-                        if (two && c + i < hd) y = __fmaf_rn(s_o[(c + i) * 128 + r], other, y);
-                    }
-                    y = __fmul_rn(y, inv);
-                    if (c + i < hd) finite = finite && fabsf(y) < INFINITY;
-                    o[i] = y;
-                }
-                if (row_ok) {
-#pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        if (c + i >= hd) continue;
-                        if (vec)
-                            *reinterpret_cast<float4 *>(dst + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                        else
-#pragma unroll
-                            for (int u = 0; u < 4; u++) dst[c + i + u] = o[i + u];
-                    }
-                }
+            for (int i = 0; i < OC; i++) {
+                acc[i] = __fmul_rn(acc[i], inv);
+                if (x * OC + i < hd) finite = finite && fabsf(acc[i]) < INFINITY;
             }
-            if (!whole && row_ok) plan.part_ml[part] = make_float2(m, l);
-            unsigned redo = __ballot_sync(0xffffffffu, row_ok && !finite);
-            __syncwarp();
-            while (redo) {
-                const int who = __ffs(redo) - 1;
-                redo &= redo - 1;
-                const int rrow = __shfl_sync(0xffffffffu, row, who), rh = __shfl_sync(0xffffffffu, h, who);
-                const int rfrom = __shfl_sync(0xffffffffu, from, who), rto = __shfl_sync(0xffffffffu, to, who);
-                const RowState st = attend_row<TYPE>(kv, b, seq, head, a.q + (size_t)rrow * a.ldq + (size_t)rh * hd,
-                                                     __fmul_rn(a.scale, 1.44269504088896340736f), keys, lo, hi, rfrom,
-                                                     sink_end, rto);
-                const size_t at = ((size_t)rrow * a.num_heads + rh) * plan.splits + split;
-                float *d = whole ? a.out + (size_t)rrow * a.ldo + (size_t)rh * hd : plan.part_o + at * hd;
-                const float div = whole ? st.l : 1.0f;
+            if (row_ok) {
 #pragma unroll
-                for (int c = 0; c < 4; c++)
-                    if (lane + 32 * c < hd) d[lane + 32 * c] = div == 0.f ? 0.f : __fdiv_rn(st.acc[c], div);
-                if (!whole && lane == 0) plan.part_ml[at] = make_float2(st.m, st.l);
+                for (int i = 0; i < OC; i += 4) {
+                    if (x * OC + i >= hd) continue;
+                    if (vec)
+                        *reinterpret_cast<float4 *>(dst + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+                    else
+#pragma unroll
+                        for (int u = 0; u < 4; u++) dst[i + u] = acc[i + u];
+                }
+                if (!whole && x == 0) plan.part_ml[part] = make_float2(m, l);
+            }
+            // rows that met a value that is not finite, once their first
+            // results are written (the barrier orders the two halves' stores)
+            if (named_bar_or(2, 256, row_ok && !finite)) {
+                sh->row[x][r] = finite ? 0.f : 1.f;
+                named_bar_sync(2, 256);
+                unsigned redo = __ballot_sync(0xffffffffu, x == 0 && row_ok && (sh->row[0][r] != 0.f || sh->row[1][r] != 0.f));
+                while (redo) {
+                    const int who = __ffs(redo) - 1;
+                    redo &= redo - 1;
+                    const int rrow = __shfl_sync(0xffffffffu, row, who), rh = __shfl_sync(0xffffffffu, h, who);
+                    const int rfrom = __shfl_sync(0xffffffffu, from, who), rto = __shfl_sync(0xffffffffu, to, who);
+                    const RowState st = attend_row<TYPE>(kv, b, seq, head, a.q + (size_t)rrow * a.ldq + (size_t)rh * hd,
+                                                         sl2_all, keys, lo, hi, rfrom, sink_end, rto);
+                    const size_t at = ((size_t)rrow * a.num_heads + rh) * plan.splits + split;
+                    float *d = whole ? a.out + (size_t)rrow * a.ldo + (size_t)rh * hd : plan.part_o + at * hd;
+                    const float div = whole ? st.l : 1.0f;
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        if (lane + 32 * c < hd) d[lane + 32 * c] = div == 0.f ? 0.f : __fdiv_rn(st.acc[c], div);
+                    if (!whole && lane == 0) plan.part_ml[at] = make_float2(st.m, st.l);
+                }
             }
         }
     } else if (warp == 8) {
         // --------------------------------------------------------- the MMAs
-        if (lane == 0 && ntile > 0) {
+        if (ntile > 0) {
+            const bool me = lane == 0;
             const unsigned idesc_s = umma_idesc_f16(TYPE != KV_F16, 128, KT, false);
             const unsigned idesc_o = umma_idesc_f16(TYPE != KV_F16, 128, (hd + 15) / 16 * 16, true);
             const int qk_steps = (hd + 15) / 16;
-            const unsigned a_q = smem_addr(s_q), a_kv = smem_addr(s_kv);
-            unsigned n_take = 0;  // slots taken so far
-            bool ok = pr_wait(&sh->q_full, 0, sh, kv);
-            auto take = [&]() -> int {  // the next slot, filled
-                const int slot = (int)(n_take % Cfg::NSLOT);
-                ok = ok && pr_wait(&sh->full[slot], (n_take / Cfg::NSLOT) & 1u, sh, kv);
-                n_take++;
-                return slot;
+            const uint64_t dq = umma_desc_sw128(smem_addr(s_q));
+            const uint64_t dk0 = umma_desc_sw128(smem_addr(s_kv)), dv0 = umma_desc_sw128_mn(smem_addr(s_kv), KT * 128);
+            bool ok = true;
+            auto wait = [&](uint64_t *bar, int phase) {  // the warp goes on together
+                ok = __all_sync(0xffffffffu, ok && pr_wait(bar, (unsigned)phase & 1u, sh, kv));
+                tc_fence_after();
             };
-            // the products of parts that count, the smallest first: each MMA
-            // cuts its sum at the last bit of the largest addend
+            // the products of parts that count, the smallest first
             auto parts = [&](auto f) {
                 if constexpr (NC == 1) {
 #pragma unroll
@@ -620,99 +615,64 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
                     f(2, 0, true), f(0, 2, false), f(1, 1, false), f(1, 0, false), f(0, 1, false), f(0, 0, false);
                 }
             };
-            auto scores = [&](int x, int slot) {
-                const uint64_t dq = umma_desc_sw128(a_q + (T == 2 ? x * NQ * Cfg::QPART : 0));
-                const uint64_t dk = umma_desc_sw128(a_kv + slot * Cfg::SLOT);
+            // tile n of the ring: the keys of tile n / 2, or its values
+            auto scores = [&](int j) {
+                const int n = 2 * j, s = n % Cfg::NSLOT;
+                wait(&sh->full[s], n / Cfg::NSLOT);
+                if (!ok) return;
+                const uint64_t dk = dk0 + (uint64_t)(s * (Cfg::SLOT >> 4));
+                const unsigned d = taddr + (j & 1) * Cfg::T_S;
                 parts([&](int i, int c, bool first) {
-                    for (int ks = 0; ks < qk_steps; ks++) {
+#pragma unroll
+                    for (int ks = 0; ks < HDP / 16; ks++) {
                         const unsigned ao = i * Cfg::QPART + (ks >> 2) * 128 * 128 + (ks & 3) * 32;
                         const unsigned bo = c * Cfg::PART + (ks >> 2) * KT * 128 + (ks & 3) * 32;
-                        tc_mma_f16(taddr + x * Cfg::STREAM, dq + (ao >> 4), dk + (bo >> 4), idesc_s, !first || ks > 0);
+                        if (ks < qk_steps) tc_mma_f16(me, d, dq + (ao >> 4), dk + (bo >> 4), idesc_s, !first || ks > 0);
                     }
                 });
+                tc_commit_by(me, &sh->s_full[j & 1]);
+                tc_commit_by(me, &sh->empty[s]);
             };
-            auto values = [&](int x, int slot, bool acc) {
-                const uint64_t dv = umma_desc_sw128_mn(a_kv + slot * Cfg::SLOT, KT * 128);
+            wait(&sh->q_full, 0);
+            scores(0);
+            for (int j = 0; j < ntile && ok; j++) {
+                // over the weights of tile j - 1, which its w.v has read by then
+                if (j + 1 < ntile) scores(j + 1);
+                const int n = 2 * j + 1, s = n % Cfg::NSLOT;
+                wait(&sh->full[s], n / Cfg::NSLOT);
+                wait(&sh->p_full[j & 1], j >> 1);
+                if (!ok) break;
+                const uint64_t dv = dv0 + (uint64_t)(s * (Cfg::SLOT >> 4));
+                const unsigned d = taddr + Cfg::T_O + (j & 1) * HDP, w = taddr + (j & 1) * Cfg::T_S;
                 parts([&](int i, int c, bool first) {
 #pragma unroll
                     for (int ks = 0; ks < KT / 16; ks++)
-                        tc_mma_f16_ta(taddr + x * Cfg::STREAM + Cfg::SP, taddr + x * Cfg::STREAM + i * (KT / 2) + ks * 8,
-                                      dv + ((c * Cfg::PART + ks * 2048) >> 4), idesc_o, acc || !first || ks > 0);
+                        tc_mma_f16_ta(me, d, w + i * (KT / 2) + ks * 8, dv + ((c * Cfg::PART + ks * 2048) >> 4), idesc_o,
+                                      !first || ks > 0);
                 });
-            };
-            if constexpr (T == 2) {
-                int k = take();
-                if (ok) {
-                    tc_fence_after();
-                    scores(0, k);
-                    tc_commit(&sh->s_full[0]);
-                    scores(1, k);
-                    tc_commit(&sh->s_full[1]);
-                    tc_commit(&sh->empty[k]);
-                }
-                for (int j = 0; j < ntile && ok; j++) {
-                    const int v = take();
-                    k = -1;
-                    for (int x = 0; x < 2 && ok; x++) {
-                        ok = ok && pr_wait(&sh->p_full[x], j & 1u, sh, kv);
-                        if (!ok) break;
-                        tc_fence_after();
-                        values(x, v, j > 0);
-                        if (j + 1 < ntile) {
-                            if (x == 0) k = take();
-                            if (!ok) break;
-                            tc_fence_after();
-                            scores(x, k);
-                            tc_commit(&sh->s_full[x]);
-                        } else {
-                            tc_commit(&sh->o_full[x]);
-                        }
-                    }
-                    if (!ok) break;
-                    tc_commit(&sh->empty[v]);
-                    if (k >= 0) tc_commit(&sh->empty[k]);
-                }
-            } else {
-                for (int j = 0; j < 2 && j < ntile && ok; j++) {
-                    const int k = take();
-                    if (!ok) break;
-                    tc_fence_after();
-                    scores(j, k);
-                    tc_commit(&sh->s_full[j]);
-                    tc_commit(&sh->empty[k]);
-                }
-                for (int j = 0; j < ntile && ok; j++) {
-                    const int x = j & 1, v = take();
-                    ok = ok && pr_wait(&sh->p_full[x], (j >> 1) & 1u, sh, kv);
-                    if (!ok) break;
-                    tc_fence_after();
-                    values(x, v, j > 1);
-                    tc_commit(&sh->empty[v]);
-                    if (j + 2 < ntile) {
-                        const int k = take();
-                        if (!ok) break;
-                        tc_fence_after();
-                        scores(x, k);
-                        tc_commit(&sh->s_full[x]);
-                        tc_commit(&sh->empty[k]);
-                    } else {
-                        tc_commit(&sh->o_full[x]);
-                    }
-                }
+                tc_commit_by(me, &sh->o_full[j & 1]);
+                tc_commit_by(me, &sh->empty[s]);
             }
             // what was issued has to end before the TMEM is freed
-            tc_commit(&sh->drain);
+            tc_commit_by(me, &sh->drain);
             const long long t0 = clock64();
             while (!mbar_test(&sh->drain, 0) && clock64() - t0 < WAIT_LIMIT) {
             }
+            __syncwarp();
         }
     } else {
         // ------------------------------------------- keys and values to slots
         const int p = tid - 9 * 32;
-        constexpr int NOFF = 128 / KT;  // tiles whose offsets are kept
-        constexpr int CH = HDP / 8;     // 16-byte chunks of a row's part
-        const int in_chunks = (hd + 15) / 16 * 2;  // chunks a product reads
-        unsigned n_put = 0;
+        constexpr int CH = HDP / 8;               // 16-byte chunks of a row's part
+        constexpr int RSTEP = PR_PRODUCERS / CH;  // rows a pass
+        constexpr int PASSES = (KT + RSTEP - 1) / RSTEP;
+        static_assert(PR_PRODUCERS % CH == 0, "a thread keeps its chunk");
+        const int c = p % CH, r_first = p / CH;
+        const bool read = c < (hd + 15) / 16 * 2;  // a chunk some product reads
+        const bool in_row = c * 8 < hd;
+        int slot = 0;
+        unsigned turn = 1;  // phase of an empty slot: none is waited for in the first round
+        bool first_round = true;
         int pending = -1;  // slot whose copies are under way
         bool ok = true;
         auto land = [&]() {
@@ -726,37 +686,39 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
         auto lookup = [&](int j) {
             for (int i = p; i < KT; i += PR_PRODUCERS) {
                 const int at = lo + j * KT + i;
-                sh->off[(j % NOFF) * KT + i] = at < hi ? key_offset(kv, b, seq, (unsigned)keys.key(at), head) : -1;
+                sh->off[i] = at < hi ? key_offset(kv, b, seq, (unsigned)keys.key(at), head) : -1;
             }
             named_bar_sync(1, PR_PRODUCERS);
             if (p < KT / 32) {
                 unsigned bits = 0;
-                for (int i = 0; i < 32; i++) bits |= (sh->off[(j % NOFF) * KT + p * 32 + i] >= 0 ? 1u : 0u) << i;
+                for (int i = 0; i < 32; i++) bits |= (sh->off[p * 32 + i] >= 0 ? 1u : 0u) << i;
                 sh->valid[j & 7][p] = bits;
             }
         };
-        auto put = [&](int j, const void *pool) {
-            const int slot = (int)(n_put % Cfg::NSLOT);
-            if (n_put >= (unsigned)Cfg::NSLOT) {
-                const unsigned par = (n_put / Cfg::NSLOT - 1) & 1u;
-                if (!mbar_test(&sh->empty[slot], par)) {
-                    land();
-                    ok = pr_wait(&sh->empty[slot], par, sh, kv);
-                }
+        auto put = [&](const void *pool) {
+            const int s = slot;
+            if (!first_round && !mbar_test(&sh->empty[s], turn)) {
+                land();
+                ok = pr_wait(&sh->empty[s], turn, sh, kv);
             }
-            n_put++;
+            if (++slot == Cfg::NSLOT) slot = 0, turn ^= 1u, first_round = false;
             if (!ok) return;
-            const long long *off = sh->off + (j % NOFF) * KT;
-            unsigned char *dst = s_kv + slot * Cfg::SLOT;
+            const long long *off = sh->off;
+            unsigned char *dst = s_kv + s * Cfg::SLOT;
             if constexpr (TYPE != KV_F32) {
-                for (int e = p; e < KT * CH; e += PR_PRODUCERS) {
-                    const int r = e / CH, c = e % CH;
-                    if (c >= in_chunks) continue;
-                    const long long o = off[r];
-                    const bool in = o >= 0 && c * 8 < hd;
-                    const char *src = reinterpret_cast<const char *>(pool) + (in ? (size_t)o * 2 + c * 16 : 0);
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_addr(dst) + sw16_off(r, c, KT)),
-                                 "l"(src), "r"(in ? 16u : 0u));
+                const unsigned d0 = smem_addr(dst);
+                const char *base = reinterpret_cast<const char *>(pool) + c * 16;
+                if (read) {
+#pragma unroll 4
+                    for (int n = 0; n < PASSES; n++) {
+                        const int r = r_first + n * RSTEP;
+                        if (r >= KT) break;
+                        const long long o = off[r];
+                        const bool in = o >= 0 && in_row;
+                        const char *src = in ? base + o * 2 : reinterpret_cast<const char *>(pool);
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(d0 + sw16_off(r, c, KT)),
+                                     "l"(src), "r"(in ? 16u : 0u));
+                    }
                 }
                 cp_async_commit();
                 if (pending >= 0) {
@@ -764,15 +726,14 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
                     fence_async_smem();
                     mbar_arrive(&sh->full[pending]);
                 }
-                pending = slot;
+                pending = s;
             } else {
-                constexpr int PER = (KT * CH + PR_PRODUCERS - 1) / PR_PRODUCERS;
-                float4 u[PER][2];
+                float4 u[PASSES][2];
 #pragma unroll
-                for (int n = 0; n < PER; n++) {
-                    const int e = p + n * PR_PRODUCERS, r = e / CH, c = e % CH;
-                    const long long o = e < KT * CH ? off[r] : -1;
-                    if (o >= 0 && c * 8 < hd) {
+                for (int n = 0; n < PASSES; n++) {
+                    const int r = r_first + n * RSTEP;
+                    const long long o = r < KT ? off[r] : -1;
+                    if (o >= 0 && in_row) {
                         const float4 *src = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(pool) + o + c * 8);
                         u[n][0] = src[0];
                         u[n][1] = src[1];
@@ -781,9 +742,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
                     }
                 }
 #pragma unroll
-                for (int n = 0; n < PER; n++) {
-                    const int e = p + n * PR_PRODUCERS, r = e / CH, c = e % CH;
-                    if (e >= KT * CH || c >= in_chunks) continue;
+                for (int n = 0; n < PASSES; n++) {
+                    const int r = r_first + n * RSTEP;
+                    if (r >= KT || !read) continue;
                     unsigned part[4][3];
                     split2<KV_BF16, 3>(u[n][0].x, u[n][0].y, part[0]);
                     split2<KV_BF16, 3>(u[n][0].z, u[n][0].w, part[1]);
@@ -796,27 +757,15 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
                             make_uint4(part[0][i], part[1][i], part[2][i], part[3][i]);
                 }
                 fence_async_smem();
-                mbar_arrive(&sh->full[slot]);
+                mbar_arrive(&sh->full[s]);
             }
         };
-        if constexpr (T == 2) {
-            for (int j = 0; j < ntile && ok; j++) {
-                lookup(j);
-                named_bar_sync(1, PR_PRODUCERS);
-                put(j, kv.k);
-                if (ok) put(j, kv.v);
-                ok = !named_bar_or(1, PR_PRODUCERS, !ok);
-            }
-        } else {
-            for (int j = 0; j <= ntile && ok && ntile > 0; j++) {
-                if (j < ntile) {
-                    lookup(j);
-                    named_bar_sync(1, PR_PRODUCERS);
-                    put(j, kv.k);
-                }
-                if (j > 0 && ok) put(j - 1, kv.v);
-                ok = !named_bar_or(1, PR_PRODUCERS, !ok);
-            }
+        for (int j = 0; j < ntile && ok; j++) {
+            lookup(j);
+            named_bar_sync(1, PR_PRODUCERS);
+            put(kv.k);
+            if (ok) put(kv.v);
+            ok = !named_bar_or(1, PR_PRODUCERS, !ok);
         }
         land();
         cp_async_wait<0>();
@@ -841,7 +790,7 @@ void go(const KvView &kv, const BatchView &b, const PagedAttnView &a, const Rows
 RowsPlan plan_paged_rows(const KvView &kv, const BatchView &b, const PagedAttnView &a, uint32_t max_kv_len) {
     RowsPlan p{};
     const uint64_t group = a.num_heads / kv.kv_heads;
-    const uint64_t rt = kv.type == KV_F16 ? 256 : 128, kt = kv.type == KV_F16 ? 128 : 64;
+    const uint64_t rt = 128, kt = kv.type == KV_F16 ? 128 : 64;
     // a tile may end inside each sequence: an upper bound of their number
     p.tiles = (uint64_t)b.num_rows * group / rt + (uint64_t)std::min(b.num_seqs, b.num_rows);
     const uint64_t units = std::max<uint64_t>(p.tiles * kv.kv_heads, 1);
