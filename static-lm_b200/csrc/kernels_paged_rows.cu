@@ -63,10 +63,11 @@ struct RowsCfg {
 
 // The small shared data, after the tiles.
 struct RowsShared {
-    uint64_t full[8], empty[8], s_full[2], p_full[2], o_full[2], q_full, drain;
+    uint64_t full[8], empty[8], s_full[2], p_full[2], o_full[2], q_full, seen_all, swapped, drain;
     long long off[128];       // element offsets of the newest tile's keys
     unsigned valid[8][4];     // held keys of the newest 8 tiles
     float row[2][128];        // exchanged between the halves of a row; 2^-e of q's rows before
+    int move[4];              // some row's reference has to move, by tile
     unsigned taddr;
     int abort;
     // the CTA's work
@@ -156,12 +157,6 @@ __device__ __forceinline__ void tmem_st16(unsigned taddr, const unsigned *r) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 
-__device__ __forceinline__ float ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-
 // A bounded wait; false once any wait of the CTA gave up.
 __device__ __forceinline__ bool pr_wait(uint64_t *bar, unsigned parity, RowsShared *sh, const KvView &kv) {
     if (mbar_test(bar, parity)) return true;
@@ -202,22 +197,23 @@ __device__ __forceinline__ void split2(float a, float b, unsigned (&part)[N]) {
 }
 // The same of two softmax weights (finite, or NaN: then the row is redone).
 template <int TYPE, int N>
-__device__ __forceinline__ void split2_weights(float a, float b, unsigned (&part)[N]) {
+__device__ __forceinline__ void split2_weights(uint64_t e, unsigned (&part)[N]) {
+    const uint64_t minus = 0xbf800000bf800000ull;  // (-1, -1)
+    float a, b;
     if constexpr (TYPE == KV_F16) {
+        unpack2(e, a, b);
         const __half2 h = __floats2half2_rn(a, b);
         const float2 f = __half22float2(h);
-        const __half2 r = __floats2half2_rn(__fsub_rn(a, f.x), __fsub_rn(b, f.y));
+        unpack2(fma2(pack2(f.x, f.y), minus, e), a, b);
+        const __half2 r = __floats2half2_rn(a, b);
         part[0] = *reinterpret_cast<const unsigned *>(&h);
         part[1] = *reinterpret_cast<const unsigned *>(&r);
     } else {
 #pragma unroll
         for (int i = 0; i < N; i++) {  // cut, not rounded: 8 bits each
-            const unsigned ua = __float_as_uint(a), ub = __float_as_uint(b);
-            part[i] = __byte_perm(ua, ub, 0x7632);
-            if (i + 1 < N) {
-                a = __fsub_rn(a, __uint_as_float(ua & 0xffff0000u));
-                b = __fsub_rn(b, __uint_as_float(ub & 0xffff0000u));
-            }
+            const uint64_t hi = e & 0xffff0000ffff0000ull;
+            part[i] = __byte_perm((unsigned)e, (unsigned)(e >> 32), 0x7632);
+            if (i + 1 < N) e = fma2(hi, minus, e);
         }
     }
 }
@@ -255,7 +251,7 @@ __device__ __noinline__ RowState attend_row(const KvView &kv, const BatchView &b
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         top = fmaxf(top, r.m);
-        const float f = ex2(__fsub_rn(r.m, top)), w = ex2(__fsub_rn(x, top));
+        const float f = exp2_approx(__fsub_rn(r.m, top)), w = exp2_approx(__fsub_rn(x, top));
         r.m = top;
         float total = w;
 #pragma unroll
@@ -315,7 +311,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
                 rows = b.row_start[s + 1] - start;
                 if (start < 0 || rows < 0 || rows > b.num_rows - start) rows = 0;
             }
-            const int n = (int)(((long long)rows * group + 127) / 128);
+            const int n = (int)(((long long)rows * group + 127) >> 7);
             int sum = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -349,6 +345,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             mbar_init(&sh->o_full[x], 1);
         }
         mbar_init(&sh->q_full, 256);
+        mbar_init(&sh->seen_all, 256);
+        mbar_init(&sh->swapped, 256);
+        for (int i = 0; i < 4; i++) sh->move[i] = 0;
         mbar_init(&sh->drain, 1);
         sh->abort = 0;
         mbar_fence_init();
@@ -356,9 +355,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
     const int seq = sh->seq, row0 = sh->row0, rows = sh->rows, tile = sh->tile;
     const int pos0 = b.kv_len[seq] - rows;  // position of the sequence's first row
     // tokens of this tile, and the list of keys any of them sees
-    const long long flat0 = (long long)tile * 128;
-    const int tok0 = (int)(flat0 / group);
-    const int tok1 = (flat0 + 127) / group < rows ? (int)((flat0 + 127) / group) : rows - 1;
+    const unsigned flat0 = (unsigned)tile * 128u;
+    const int tok0 = (int)(flat0 / (unsigned)group);
+    int tok1 = (int)((flat0 + 127u) / (unsigned)group);
+    tok1 = tok1 < rows ? tok1 : rows - 1;
     const SeenKeys keys = seen_keys(pos0 + tok0, pos0 + tok1, a.window, a.sinks);
     const int all_tiles = (keys.n + KT - 1) / KT;
     const int per_split = (all_tiles + plan.splits - 1) / plan.splits;
@@ -371,20 +371,26 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
     tc_fence_after();
     const unsigned taddr = sh->taddr;
 
+    // the softmax threads keep a tile's scores and the row's sums in registers:
+    // they take some of the others' (256 x A + 128 x B = 384 x 168)
+    constexpr int R_SOFTMAX = Cfg::F16 ? 200 : 184, R_OTHER = Cfg::F16 ? 104 : 136;
+    static_assert(256 * R_SOFTMAX + 128 * R_OTHER == 384 * 168, "registers");
     if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(R_SOFTMAX));
         // ------------------------------------------------ q, softmax, output
         const float sl2_all = __fmul_rn(a.scale, 1.44269504088896340736f);
-        {  // a warp per row, four rows at a time
+        {  // a warp per row, eight rows at a time
             const bool vec = (((uintptr_t)a.q | (a.ldq * 4)) & 15) == 0;
             const int c4 = lane * 4;
-            for (int r0 = warp * 16; r0 < warp * 16 + 16; r0 += 4) {
-                float f[4][4];
 #pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    const long long flat = flat0 + r0 + u;
-                    const int tok = (int)(flat / group);
-                    const float *src = a.q + (size_t)(row0 + tok) * a.ldq + (size_t)(head * group + (int)(flat - (long long)tok * group)) * hd + c4;
-                    const bool in = tok < rows && c4 < hd;
+            for (int r0 = 0; r0 < 16; r0 += 8) {
+                float f[8][4];
+#pragma unroll
+                for (int u = 0; u < 8; u++) {
+                    const unsigned flat = flat0 + (unsigned)(warp * 16 + r0 + u), tok = flat / (unsigned)group;
+                    const float *src = a.q + (size_t)(row0 + (int)tok) * a.ldq +
+                                       (size_t)(head * group + (int)(flat - tok * (unsigned)group)) * hd + c4;
+                    const bool in = (int)tok < rows && c4 < hd;
                     if (in && vec) {
                         const float4 t = *reinterpret_cast<const float4 *>(src);
                         f[u][0] = t.x, f[u][1] = t.y, f[u][2] = t.z, f[u][3] = t.w;
@@ -394,19 +400,18 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
                     }
                 }
 #pragma unroll
-                for (int u = 0; u < 4; u++) {
+                for (int u = 0; u < 8; u++) {
+                    const int r = warp * 16 + r0 + u;
                     if constexpr (Cfg::F16) {
-                        float top = fmaxf(fmaxf(fabsf(f[u][0]), fabsf(f[u][1])), fmaxf(fabsf(f[u][2]), fabsf(f[u][3])));
+                        // the bits of non-negative floats order as they do
+                        unsigned top = __float_as_uint(fabsf(f[u][0]));
 #pragma unroll
-                        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                        int e = 0;
-                        if (top > 0.f && top < INFINITY) {
-                            frexpf(top, &e);  // top = f 2^e, 0.5 <= f < 1
-                            e = 15 - e;
-                            e = e > 120 ? 120 : e < -120 ? -120 : e;
-                        }
+                        for (int i = 1; i < 4; i++) top = max(top, __float_as_uint(fabsf(f[u][i])));
+                        top = __reduce_max_sync(0xffffffffu, top);
+                        int e = 141 - (int)(top >> 23);  // 2^14 <= top 2^e < 2^15
+                        e = top == 0 || top >= 0x7f800000u ? 0 : e > 120 ? 120 : e;
                         const float up = __uint_as_float((unsigned)(127 + e) << 23);
-                        if (lane == 0) sh->row[0][r0 + u] = __uint_as_float((unsigned)(127 - e) << 23);
+                        if (lane == 0) sh->row[0][r] = __uint_as_float((unsigned)(127 - e) << 23);
 #pragma unroll
                         for (int i = 0; i < 4; i++) f[u][i] = __fmul_rn(f[u][i], up);
                     }
@@ -414,7 +419,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
                         unsigned p[NQ], q[NQ];
                         split2<TYPE, NQ>(f[u][0], f[u][1], p);
                         split2<TYPE, NQ>(f[u][2], f[u][3], q);
-                        const unsigned o = sw16_off(r0 + u, lane >> 1, 128) + (lane & 1) * 8;
+                        const unsigned o = sw16_off(r, lane >> 1, 128) + (lane & 1) * 8;
 #pragma unroll
                         for (int i = 0; i < NQ; i++)
                             *reinterpret_cast<uint2 *>(s_q + i * Cfg::QPART + o) = make_uint2(p[i], q[i]);
@@ -426,7 +431,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             if constexpr (Cfg::F16) named_bar_sync(2, 256);  // the rows' 2^-e
         }
         const int x = warp >> 2, r = tid & 127;  // half, row of the tile
-        const int tok = (int)((flat0 + r) / group), h = head * group + (int)((flat0 + r) % group);
+        const unsigned flat = flat0 + (unsigned)r;
+        const int tok = (int)(flat / (unsigned)group), h = head * group + (int)(flat % (unsigned)group);
         const bool row_ok = tok < rows;
         const int row = row0 + (row_ok ? tok : 0);
         const int pos = row_ok ? pos0 + tok : -1;
@@ -438,13 +444,16 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
         const float sl2 = Cfg::F16 ? __fmul_rn(sl2_all, sh->row[0][r]) : sl2_all;
         const unsigned t_lane = taddr + ((unsigned)((warp & 3) * 32) << 16);
         float m = PR_NO_MAX, l = 0.f;
-        float acc[OC];
+        uint64_t acc[OC / 2];
 #pragma unroll
-        for (int i = 0; i < OC; i++) acc[i] = 0.f;
+        for (int i = 0; i < OC / 2; i++) acc[i] = 0ull;
         bool ok = true;
+        auto wait = [&](uint64_t *bar, int phase) {  // a warp goes on together: TMEM accesses are warp-wide
+            ok = __all_sync(0xffffffffu, ok && pr_wait(bar, (unsigned)phase & 1u, sh, kv));
+        };
         // adds this half of tile j's w.v to the row's sums
         auto gather = [&](int j) {
-            ok = __all_sync(0xffffffffu, ok && pr_wait(&sh->o_full[j & 1], (j >> 1) & 1u, sh, kv));
+            wait(&sh->o_full[j & 1], j >> 1);
             if (!ok) return;
             tc_fence_after();
 #pragma unroll
@@ -454,123 +463,159 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
                 tmem_wait_ld();
                 pin32(o);
 #pragma unroll
-                for (int i = 0; i < 32; i++) acc[c + i] = __fadd_rn(acc[c + i], o[i]);
+                for (int i = 0; i < 32; i += 2) acc[(c + i) / 2] = add2(acc[(c + i) / 2], pack2(o[i], o[i + 1]));
             }
         };
+        const uint64_t sl22 = pack2(sl2, sl2);
         for (int j = 0; j < ntile; j++) {
             const unsigned t_s = t_lane + (j & 1) * Cfg::T_S;
-            ok = __all_sync(0xffffffffu, ok && pr_wait(&sh->s_full[j & 1], (j >> 1) & 1u, sh, kv));  // TMEM loads are warp-wide
+            wait(&sh->s_full[j & 1], j >> 1);
+            if (!ok) break;
+            tc_fence_after();
             float v[CT];
-            float top = -INFINITY;
-            if (ok) {
-                tc_fence_after();
 #pragma unroll
-                for (int c = 0; c < CT; c += 32) tmem_ld32(t_s + x * CT + c, v + c);
-                tmem_wait_ld();
+            for (int c = 0; c < CT; c += 32) tmem_ld32(t_s + x * CT + c, v + c);
+            tmem_wait_ld();
 #pragma unroll
-                for (int c = 0; c < CT; c += 32) pin32(v + c);
-                const int i0 = lo + j * KT + x * CT;
-                const unsigned *valid = &sh->valid[j & 7][x * CT / 32];
-                bool whole = i0 + CT <= to && i0 + CT <= hi && (i0 + CT <= sink_end || i0 >= from);
+            for (int c = 0; c < CT; c += 32) pin32(v + c);
+            const int i0 = lo + j * KT + x * CT;
+            const unsigned *valid = &sh->valid[j & 7][x * CT / 32];
+            bool whole = i0 + CT <= to && i0 + CT <= hi && (i0 + CT <= sink_end || i0 >= from);
 #pragma unroll
-                for (int c = 0; c < CT / 32; c++) whole = whole && valid[c] == 0xffffffffu;
-                if (!__all_sync(0xffffffffu, whole)) {
+            for (int c = 0; c < CT / 32; c++) whole = whole && valid[c] == 0xffffffffu;
+            if (!__all_sync(0xffffffffu, whole)) {
 #pragma unroll
-                    for (int c = 0; c < CT; c++) {
-                        const int i = i0 + c;
-                        const bool seen = i < to && (i < sink_end || i >= from) && ((valid[c >> 5] >> (c & 31)) & 1u);
-                        v[c] = seen ? v[c] : -INFINITY;
-                    }
+                for (int c = 0; c < CT; c++) {
+                    const int i = i0 + c;
+                    const bool seen = i < to && (i < sink_end || i >= from) && ((valid[c >> 5] >> (c & 31)) & 1u);
+                    v[c] = seen ? v[c] : -INFINITY;
                 }
-                float t0 = v[0], t1 = v[1], t2 = v[2], t3 = v[3];
-#pragma unroll
-                for (int c = 4; c < CT; c += 4) {
-                    t0 = fmaxf(t0, v[c]);
-                    t1 = fmaxf(t1, v[c + 1]);
-                    t2 = fmaxf(t2, v[c + 2]);
-                    t3 = fmaxf(t3, v[c + 3]);
-                }
-                top = __fmul_rn(fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)), sl2);
             }
-            // every score of the tile is in registers after this barrier, and
-            // the halves of each row move their reference together
-            float f = 1.0f;
-            const bool moved = named_bar_or(2, 256, top > m + PR_RESCALE || !ok);
-            if (moved) {
-                sh->row[x][r] = top;
-                if (named_bar_or(2, 256, !ok)) {
-                    ok = false;
-                    break;
-                }
-                const float both = fmaxf(top, sh->row[x ^ 1][r]);
-                if (both > m + PR_RESCALE) {
-                    f = ex2(__fsub_rn(m, both));
-                    m = both;
-                    l = __fmul_rn(l, f);
-                }
-                named_bar_sync(2, 256);  // read before the next tile's
-            }
-            float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;
+            float t0 = v[0], t1 = v[1], t2 = v[2], t3 = v[3];
 #pragma unroll
-            for (int c = 0; c < CT; c += 32) {
-                unsigned w[NQ][16];
+            for (int c = 4; c < CT; c += 4) {
+                t0 = fmaxf(t0, v[c]);
+                t1 = fmaxf(t1, v[c + 1]);
+                t2 = fmaxf(t2, v[c + 2]);
+                t3 = fmaxf(t3, v[c + 3]);
+            }
+            const float top = __fmul_rn(fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)), sl2);
+            // this thread has its scores, and says whether its row's reference
+            // has to move; the first weights are worked out meanwhile, as if none had
+            if (top > m + PR_RESCALE) *(volatile int *)&sh->move[j & 3] = 1;
+            mbar_arrive(&sh->seen_all);
+            uint64_t sum;  // of 32 weights
+            unsigned w[NQ][16];
+            auto weights = [&](int c) {
+                const uint64_t mm = pack2(-m, -m);
+                uint64_t s0 = 0ull, s1 = 0ull;
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {
-                    const float e0 = ex2(__fmaf_rn(v[c + i], sl2, -m)), e1 = ex2(__fmaf_rn(v[c + i + 1], sl2, -m));
-                    const float e2 = ex2(__fmaf_rn(v[c + i + 2], sl2, -m)), e3 = ex2(__fmaf_rn(v[c + i + 3], sl2, -m));
-                    l0 = __fadd_rn(l0, e0);
-                    l1 = __fadd_rn(l1, e1);
-                    l2 = __fadd_rn(l2, e2);
-                    l3 = __fadd_rn(l3, e3);
+                    float e0, e1, e2, e3;
+                    unpack2(fma2(pack2(v[c + i], v[c + i + 1]), sl22, mm), e0, e1);
+                    unpack2(fma2(pack2(v[c + i + 2], v[c + i + 3]), sl22, mm), e2, e3);
+                    const uint64_t a01 = pack2(exp2_approx(e0), exp2_approx(e1));
+                    const uint64_t a23 = pack2(exp2_approx(e2), exp2_approx(e3));
+                    s0 = add2(s0, a01);
+                    s1 = add2(s1, a23);
                     unsigned p[NQ], q[NQ];
-                    split2_weights<TYPE, NQ>(e0, e1, p);
-                    split2_weights<TYPE, NQ>(e2, e3, q);
+                    split2_weights<TYPE, NQ>(a01, p);
+                    split2_weights<TYPE, NQ>(a23, q);
 #pragma unroll
                     for (int n = 0; n < NQ; n++) w[n][i / 2] = p[n], w[n][i / 2 + 1] = q[n];
                 }
-                // the weights' parts take the scores' place
+                sum = add2(s0, s1);
+            };
+            weights(0);
+            wait(&sh->seen_all, j);
+            if (!ok) break;
+            float f = 1.0f;
+            const bool moved = *(volatile int *)&sh->move[j & 3] != 0;
+            if (tid == 0) *(volatile int *)&sh->move[(j + 2) & 3] = 0;  // last read two tiles ago
+            if (moved) {  // the halves of each row move their reference together
+                *(volatile float *)&sh->row[x][r] = top;
+                mbar_arrive(&sh->swapped);
+                wait(&sh->swapped, 0);
+                if (!ok) break;
+                const float both = fmaxf(top, *(volatile float *)&sh->row[x ^ 1][r]);
+                mbar_arrive(&sh->swapped);
+                wait(&sh->swapped, 1);  // read before the next exchange
+                if (!ok) break;
+                if (both > m + PR_RESCALE) {
+                    f = exp2_approx(__fsub_rn(m, both));
+                    m = both;
+                    l = __fmul_rn(l, f);
+                }
+                weights(0);
+            }
+            // every score of the tile is in registers: the weights take their place
+#pragma unroll
+            for (int c = 0; c < CT; c += 32) {
+                if (c > 0) weights(c);
+                float s0, s1;
+                unpack2(sum, s0, s1);
+                l = __fadd_rn(l, __fadd_rn(s0, s1));
 #pragma unroll
                 for (int n = 0; n < NQ; n++) tmem_st16(t_s + n * (KT / 2) + (x * CT + c) / 2, w[n]);
             }
-            l = __fadd_rn(l, __fadd_rn(__fadd_rn(l0, l1), __fadd_rn(l2, l3)));
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(&sh->p_full[j & 1]);
             if (j > 0) gather(j - 1);  // under w.v of this tile
             if (moved) {
+                const uint64_t ff = pack2(f, f);
 #pragma unroll
-                for (int i = 0; i < OC; i++) acc[i] = __fmul_rn(acc[i], f);
+                for (int i = 0; i < OC / 2; i++) acc[i] = mul2(acc[i], ff);
             }
         }
         if (ok && ntile > 0) gather(ntile - 1);
+        // (a thread that broke off leaves the others' waits to give up: all meet here)
+        const bool done = !named_bar_or(2, 256, !ok);
         sh->row[x][r] = l;
-        if (!named_bar_or(2, 256, !ok)) {
+        named_bar_sync(2, 256);
+        if (done) {
             l = __fadd_rn(sh->row[0][r], sh->row[1][r]);
             const bool whole = plan.splits == 1;
             const float inv = !whole ? 1.0f : l == 0.f ? 0.f : __fdiv_rn(1.0f, l);
-            const size_t part = ((size_t)row * a.num_heads + h) * plan.splits + split;
-            float *dst = (whole ? a.out + (size_t)row * a.ldo + (size_t)h * hd : plan.part_o + part * hd) + x * OC;
-            const bool vec = !whole || (((uintptr_t)a.out | (a.ldo * 4)) & 15) == 0;
+            // every product is complete: the results go through the q tiles,
+            // 16-byte chunk c of row r at chunk c ^ (r & 7), to whole rows
+            float4 *s_o = reinterpret_cast<float4 *>(s_q);
             bool finite = fabsf(l) < INFINITY;
 #pragma unroll
-            for (int i = 0; i < OC; i++) {
-                acc[i] = __fmul_rn(acc[i], inv);
-                if (x * OC + i < hd) finite = finite && fabsf(acc[i]) < INFINITY;
-            }
-            if (row_ok) {
+            for (int i = 0; i < OC; i += 4) {
+                float y[4];
+                unpack2(acc[i / 2], y[0], y[1]);
+                unpack2(acc[i / 2 + 1], y[2], y[3]);
 #pragma unroll
-                for (int i = 0; i < OC; i += 4) {
-                    if (x * OC + i >= hd) continue;
-                    if (vec)
-                        *reinterpret_cast<float4 *>(dst + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
-                    else
-#pragma unroll
-                        for (int u = 0; u < 4; u++) dst[i + u] = acc[i + u];
+                for (int u = 0; u < 4; u++) {
+                    y[u] = __fmul_rn(y[u], inv);
+                    if (x * OC + i < hd) finite = finite && fabsf(y[u]) < INFINITY;
                 }
-                if (!whole && x == 0) plan.part_ml[part] = make_float2(m, l);
+                s_o[r * (HDP / 4) + (((x * OC + i) / 4) ^ (r & 7))] = make_float4(y[0], y[1], y[2], y[3]);
+            }
+            if (!whole && x == 0 && row_ok)
+                plan.part_ml[((size_t)row * a.num_heads + h) * plan.splits + split] = make_float2(m, l);
+            named_bar_sync(2, 256);
+            const bool vec = !whole || (((uintptr_t)a.out | (a.ldo * 4)) & 15) == 0;
+            constexpr int LPR = HDP / 4, RPP = 32 / LPR;  // lanes a row, rows a pass
+            const int c = lane % LPR;
+#pragma unroll 4
+            for (int i = 0; i < 16; i += RPP) {
+                const int rr = warp * 16 + i + lane / LPR;
+                const unsigned fl = flat0 + (unsigned)rr, tk = fl / (unsigned)group;
+                if ((int)tk >= rows || c * 4 >= hd) continue;
+                const size_t orow = (size_t)(row0 + (int)tk);
+                const int oh = head * group + (int)(fl - tk * (unsigned)group);
+                float *dst = (whole ? a.out + orow * a.ldo + (size_t)oh * hd
+                                    : plan.part_o + ((orow * a.num_heads + oh) * plan.splits + split) * hd) + c * 4;
+                const float4 y = s_o[rr * LPR + (c ^ (rr & 7))];
+                if (vec)
+                    *reinterpret_cast<float4 *>(dst) = y;
+                else
+                    dst[0] = y.x, dst[1] = y.y, dst[2] = y.z, dst[3] = y.w;
             }
             // rows that met a value that is not finite, once their first
-            // results are written (the barrier orders the two halves' stores)
+            // results are written (the barrier orders the stores)
             if (named_bar_or(2, 256, row_ok && !finite)) {
                 sh->row[x][r] = finite ? 0.f : 1.f;
                 named_bar_sync(2, 256);
@@ -592,6 +637,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
                 }
             }
         }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(R_OTHER));
+    }
+    if (warp < 8) {
     } else if (warp == 8) {
         // --------------------------------------------------------- the MMAs
         if (ntile > 0) {

@@ -991,7 +991,11 @@ SLM_EXPORT int slm_paged_attention(const slm_kv_pages *pages, const slm_paged_ba
         launch_paged_decode(kv, b, a, plan, (cudaStream_t)stream);
         return launch_check("paged decode kernels");
     }
+    if ((uint64_t)b.num_rows * (uint64_t)(a.num_heads / kv.kv_heads) > (uint64_t)INT32_MAX - 256)
+        return fail(SLM_ERR_SHAPE, "too many rows of query heads");
     RowsPlan plan = plan_paged_rows(kv, b, a, batch->max_kv_len);
+    if (plan.tiles * kv.kv_heads * plan.splits > (uint64_t)INT32_MAX)
+        return fail(SLM_ERR_SHAPE, "too many row tiles");
     TRY(check_scratch(scratch, scratch_bytes, plan.scratch_bytes));
     plan.part_ml = (float2 *)scratch;
     plan.part_o = (float *)((char *)scratch + plan.ml_bytes);
