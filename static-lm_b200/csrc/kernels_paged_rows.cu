@@ -49,7 +49,9 @@ struct RowsCfg {
     static constexpr int SLOT = PART * NC;
     static constexpr int QPART = 128 * HDP * 2;
     static constexpr int QBYTES = NQ * QPART;
-    static constexpr int NSLOT = F16 ? (HDP == 128 ? 5 : 8) : TYPE == KV_BF16 ? 8 : (HDP == 128 ? 2 : 6);
+    // k and v of even and of odd tiles (one tile where f32 pages leave no room
+    // for two): the MMAs' operands are the same every second tile
+    static constexpr int NSLOT = TYPE == KV_F32 && HDP == 128 ? 2 : 4;
     // TMEM columns: score / weight buffers (128 or 3 x 32 used) at 0 and 128,
     // results at 256 and 256 + HDP: each buffer at a multiple of its width, as
     // an accumulator laid across column 256 faulted
@@ -63,8 +65,8 @@ struct RowsCfg {
 
 // The small shared data, after the tiles.
 struct RowsShared {
-    uint64_t full[8], empty[8], s_full[2], p_full[2], o_full[2], q_full, seen_all, swapped, drain;
-    long long off[128];       // element offsets of the newest tile's keys
+    uint64_t full[4], empty[4], s_full[2], p_full[2], o_full[2], q_full, seen_all, swapped, drain;
+    long long off[128];       // byte offsets of the newest tile's keys
     unsigned valid[8][4];     // held keys of the newest 8 tiles
     float row[2][128];        // exchanged between the halves of a row; 2^-e of q's rows before
     int move[4];              // some row's reference has to move, by tile
@@ -94,34 +96,35 @@ __device__ __forceinline__ uint64_t umma_desc_sw128_mn(unsigned saddr, unsigned 
 }
 // Instruction descriptor of kind::f16: f32 accumulator, f16 (0) or bf16 (1)
 // operands, A along K, B along K or (mn) along N.
-__device__ __forceinline__ unsigned umma_idesc_f16(bool bf16, int M, int N, bool b_mn) {
+__host__ __device__ constexpr unsigned umma_idesc_f16(bool bf16, int M, int N, bool b_mn) {
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn ? 1u : 0u) << 16) |
            ((unsigned)(N >> 3) << 17) | ((unsigned)(M >> 4) << 24);
 }
 // D[128 x N] (+)= A[128 x 16] B[N x 16]^T, A in shared memory or in TMEM, and
-// the commit of what a lane issued: the whole warp comes here with the same
-// operands and the lane with `me` issues.  (The operands are the warp's
-// uniform registers; issued from a branch of one lane, unrolled MMAs were
-// given each other's.)
-__device__ __forceinline__ void tc_mma_f16(bool me, unsigned d, uint64_t adesc, uint64_t bdesc, unsigned idesc, bool acc) {
+// the commit of what was issued: the whole warp comes here with the same
+// operands and its elected lane issues.  (The operands live in the warp's
+// uniform registers: issued from a branch of one lane, unrolled MMAs were
+// given each other's.  With the election inside, 128-wide MMAs issue every 64
+// cycles, their full rate, and 64-wide ones every 49; with a predicate kept
+// in a register every 73.)
+__device__ __forceinline__ void tc_mma_f16(unsigned d, uint64_t adesc, uint64_t bdesc, unsigned idesc, bool acc) {
     asm volatile(
-        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %9, 0;\n"
-        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n}\n" ::"r"(d),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"((unsigned)acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u), "r"((unsigned)me)
+        "{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"((unsigned)acc)
         : "memory");
 }
-__device__ __forceinline__ void tc_mma_f16_ta(bool me, unsigned d, unsigned a, uint64_t bdesc, unsigned idesc, bool acc) {
+__device__ __forceinline__ void tc_mma_f16_ta(unsigned d, unsigned a, uint64_t bdesc, unsigned idesc, bool acc) {
     asm volatile(
-        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %9, 0;\n"
-        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n}\n" ::"r"(d),
-        "r"(a), "l"(bdesc), "r"(idesc), "r"((unsigned)acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u), "r"((unsigned)me)
+        "{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(bdesc), "r"(idesc), "r"((unsigned)acc)
         : "memory");
 }
-__device__ __forceinline__ void tc_commit_by(bool me, uint64_t *bar) {
+__device__ __forceinline__ void tc_commit_elected(uint64_t *bar) {
     asm volatile(
-        "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
-        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_addr(bar)),
-        "r"((unsigned)me)
+        "{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_addr(bar))
         : "memory");
 }
 
@@ -369,7 +372,13 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const unsigned taddr = sh->taddr;
+    if (sh->taddr != 0) {  // never: all 512 columns start at column 0
+        if (tid == 0) paged_flag(kv, PAGED_WAIT_GAVE_UP);
+        __syncthreads();
+        if (warp == 0) tc_dealloc(sh->taddr, PR_TMEM_COLS);
+        return;
+    }
+    constexpr unsigned taddr = 0;
 
     // the softmax threads keep a tile's scores and the row's sums in registers:
     // they take some of the others' (256 x A + 128 x B = 384 x 168)
@@ -382,23 +391,35 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
         {  // a warp per row, eight rows at a time
             const bool vec = (((uintptr_t)a.q | (a.ldq * 4)) & 15) == 0;
             const int c4 = lane * 4;
+            // lane i < 16: the offset of the warp's row i in q, and whether it is one
+            const unsigned my_flat = flat0 + (unsigned)(warp * 16 + (lane & 15)), my_tok = my_flat / (unsigned)group;
+            const bool my_ok = (int)my_tok < rows;
+            const long long my_at = my_ok ? (long long)((size_t)(row0 + (int)my_tok) * a.ldq +
+                                                        (size_t)(head * group + (int)(my_flat - my_tok * (unsigned)group)) * hd)
+                                          : (long long)((size_t)row0 * a.ldq);
+            const unsigned oks = __ballot_sync(0xffffffffu, my_ok);
 #pragma unroll
             for (int r0 = 0; r0 < 16; r0 += 8) {
                 float f[8][4];
+                const int c_in = c4 < hd ? c4 : 0;  // every load is of some row's element: none is held up by a branch
+                if (vec) {
 #pragma unroll
-                for (int u = 0; u < 8; u++) {
-                    const unsigned flat = flat0 + (unsigned)(warp * 16 + r0 + u), tok = flat / (unsigned)group;
-                    const float *src = a.q + (size_t)(row0 + (int)tok) * a.ldq +
-                                       (size_t)(head * group + (int)(flat - tok * (unsigned)group)) * hd + c4;
-                    const bool in = (int)tok < rows && c4 < hd;
-                    if (in && vec) {
-                        const float4 t = *reinterpret_cast<const float4 *>(src);
+                    for (int u = 0; u < 8; u++) {
+                        const float4 t = *reinterpret_cast<const float4 *>(a.q + __shfl_sync(0xffffffffu, my_at, r0 + u) + c_in);
                         f[u][0] = t.x, f[u][1] = t.y, f[u][2] = t.z, f[u][3] = t.w;
-                    } else {
+                    }
+                } else {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) f[u][i] = in ? src[i] : 0.f;
+                    for (int u = 0; u < 8; u++) {
+                        const float *src = a.q + __shfl_sync(0xffffffffu, my_at, r0 + u) + c_in;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) f[u][i] = src[i];
                     }
                 }
+#pragma unroll
+                for (int u = 0; u < 8; u++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) f[u][i] = ((oks >> (r0 + u)) & 1u) && c4 < hd ? f[u][i] : 0.f;
 #pragma unroll
                 for (int u = 0; u < 8; u++) {
                     const int r = warp * 16 + r0 + u;
@@ -599,15 +620,19 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             const bool vec = !whole || (((uintptr_t)a.out | (a.ldo * 4)) & 15) == 0;
             constexpr int LPR = HDP / 4, RPP = 32 / LPR;  // lanes a row, rows a pass
             const int c = lane % LPR;
+            const unsigned my_flat = flat0 + (unsigned)(warp * 16 + (lane & 15)), my_tok = my_flat / (unsigned)group;
+            const size_t my_row = (size_t)(row0 + (int)my_tok);
+            const int my_head = head * group + (int)(my_flat - my_tok * (unsigned)group);
+            const long long my_at = (int)my_tok >= rows ? -1
+                                    : whole ? (long long)(my_row * a.ldo + (size_t)my_head * hd)
+                                            : (long long)(((my_row * a.num_heads + my_head) * plan.splits + split) * hd);
+            float *const to_base = (whole ? a.out : plan.part_o) + c * 4;
 #pragma unroll 4
             for (int i = 0; i < 16; i += RPP) {
                 const int rr = warp * 16 + i + lane / LPR;
-                const unsigned fl = flat0 + (unsigned)rr, tk = fl / (unsigned)group;
-                if ((int)tk >= rows || c * 4 >= hd) continue;
-                const size_t orow = (size_t)(row0 + (int)tk);
-                const int oh = head * group + (int)(fl - tk * (unsigned)group);
-                float *dst = (whole ? a.out + orow * a.ldo + (size_t)oh * hd
-                                    : plan.part_o + ((orow * a.num_heads + oh) * plan.splits + split) * hd) + c * 4;
+                const long long at = __shfl_sync(0xffffffffu, my_at, i + lane / LPR);
+                if (at < 0 || c * 4 >= hd) continue;
+                float *dst = to_base + at;
                 const float4 y = s_o[rr * LPR + (c ^ (rr & 7))];
                 if (vec)
                     *reinterpret_cast<float4 *>(dst) = y;
@@ -644,12 +669,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
     } else if (warp == 8) {
         // --------------------------------------------------------- the MMAs
         if (ntile > 0) {
-            const bool me = lane == 0;
-            const unsigned idesc_s = umma_idesc_f16(TYPE != KV_F16, 128, KT, false);
+            constexpr unsigned idesc_s = umma_idesc_f16(TYPE != KV_F16, 128, KT, false);
             const unsigned idesc_o = umma_idesc_f16(TYPE != KV_F16, 128, (hd + 15) / 16 * 16, true);
-            const int qk_steps = (hd + 15) / 16;
-            const uint64_t dq = umma_desc_sw128(smem_addr(s_q));
-            const uint64_t dk0 = umma_desc_sw128(smem_addr(s_kv)), dv0 = umma_desc_sw128_mn(smem_addr(s_kv), KT * 128);
+            const unsigned a_q = smem_addr(pr_smem), a_kv = a_q + Cfg::QBYTES;
             bool ok = true;
             auto wait = [&](uint64_t *bar, int phase) {  // the warp goes on together
                 ok = __all_sync(0xffffffffu, ok && pr_wait(bar, (unsigned)phase & 1u, sh, kv));
@@ -664,46 +686,53 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
                     f(2, 0, true), f(0, 2, false), f(1, 1, false), f(1, 0, false), f(0, 1, false), f(0, 0, false);
                 }
             };
-            // tile n of the ring: the keys of tile n / 2, or its values
-            auto scores = [&](int j) {
-                const int n = 2 * j, s = n % Cfg::NSLOT;
-                wait(&sh->full[s], n / Cfg::NSLOT);
+            // tile j, of parity P: every operand is a constant
+            auto scores = [&](auto parity, int j) {
+                constexpr int P = decltype(parity)::value, S = Cfg::NSLOT == 4 ? 2 * P : 0;
+                wait(&sh->full[S], Cfg::NSLOT == 4 ? j >> 1 : j);
                 if (!ok) return;
-                const uint64_t dk = dk0 + (uint64_t)(s * (Cfg::SLOT >> 4));
-                const unsigned d = taddr + (j & 1) * Cfg::T_S;
                 parts([&](int i, int c, bool first) {
 #pragma unroll
                     for (int ks = 0; ks < HDP / 16; ks++) {
                         const unsigned ao = i * Cfg::QPART + (ks >> 2) * 128 * 128 + (ks & 3) * 32;
-                        const unsigned bo = c * Cfg::PART + (ks >> 2) * KT * 128 + (ks & 3) * 32;
-                        if (ks < qk_steps) tc_mma_f16(me, d, dq + (ao >> 4), dk + (bo >> 4), idesc_s, !first || ks > 0);
+                        const unsigned bo = S * Cfg::SLOT + c * Cfg::PART + (ks >> 2) * KT * 128 + (ks & 3) * 32;
+                        tc_mma_f16(P * Cfg::T_S, umma_desc_sw128(a_q + ao), umma_desc_sw128(a_kv + bo), idesc_s,
+                                       !first || ks > 0);
                     }
                 });
-                tc_commit_by(me, &sh->s_full[j & 1]);
-                tc_commit_by(me, &sh->empty[s]);
+                tc_commit_elected(&sh->s_full[P]);
+                tc_commit_elected(&sh->empty[S]);
             };
-            wait(&sh->q_full, 0);
-            scores(0);
-            for (int j = 0; j < ntile && ok; j++) {
-                // over the weights of tile j - 1, which its w.v has read by then
-                if (j + 1 < ntile) scores(j + 1);
-                const int n = 2 * j + 1, s = n % Cfg::NSLOT;
-                wait(&sh->full[s], n / Cfg::NSLOT);
-                wait(&sh->p_full[j & 1], j >> 1);
-                if (!ok) break;
-                const uint64_t dv = dv0 + (uint64_t)(s * (Cfg::SLOT >> 4));
-                const unsigned d = taddr + Cfg::T_O + (j & 1) * HDP, w = taddr + (j & 1) * Cfg::T_S;
+            auto values = [&](auto parity, int j) {
+                constexpr int P = decltype(parity)::value, S = Cfg::NSLOT == 4 ? 2 * P + 1 : 1;
+                wait(&sh->full[S], Cfg::NSLOT == 4 ? j >> 1 : j);
+                wait(&sh->p_full[P], j >> 1);
+                if (!ok) return;
                 parts([&](int i, int c, bool first) {
 #pragma unroll
                     for (int ks = 0; ks < KT / 16; ks++)
-                        tc_mma_f16_ta(me, d, w + i * (KT / 2) + ks * 8, dv + ((c * Cfg::PART + ks * 2048) >> 4), idesc_o,
+                        tc_mma_f16_ta(Cfg::T_O + P * HDP, P * Cfg::T_S + i * (KT / 2) + ks * 8,
+                                      umma_desc_sw128_mn(a_kv + S * Cfg::SLOT + c * Cfg::PART + ks * 2048, KT * 128), idesc_o,
                                       !first || ks > 0);
                 });
-                tc_commit_by(me, &sh->o_full[j & 1]);
-                tc_commit_by(me, &sh->empty[s]);
+                tc_commit_elected(&sh->o_full[P]);
+                tc_commit_elected(&sh->empty[S]);
+            };
+            const std::integral_constant<int, 0> even{};
+            const std::integral_constant<int, 1> odd{};
+            wait(&sh->q_full, 0);
+            scores(even, 0);
+            // q.k of tile j + 1 goes over the weights of tile j - 1, which its
+            // w.v has read by then
+            for (int j = 0; j < ntile && ok; j += 2) {
+                if (j + 1 < ntile) scores(odd, j + 1);
+                values(even, j);
+                if (j + 1 == ntile) break;
+                if (j + 2 < ntile) scores(even, j + 2);
+                values(odd, j + 1);
             }
             // what was issued has to end before the TMEM is freed
-            tc_commit_by(me, &sh->drain);
+            tc_commit_elected(&sh->drain);
             const long long t0 = clock64();
             while (!mbar_test(&sh->drain, 0) && clock64() - t0 < WAIT_LIMIT) {
             }
@@ -713,17 +742,21 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
         // ------------------------------------------- keys and values to slots
         const int p = tid - 9 * 32;
         constexpr int CH = HDP / 8;               // 16-byte chunks of a row's part
-        constexpr int RSTEP = PR_PRODUCERS / CH;  // rows a pass
+        constexpr int RSTEP = PR_PRODUCERS / CH;  // rows a pass: 12 or 6
         constexpr int PASSES = (KT + RSTEP - 1) / RSTEP;
+        constexpr int ES = TYPE == KV_F32 ? 4 : 2;
         static_assert(PR_PRODUCERS % CH == 0, "a thread keeps its chunk");
         const int c = p % CH, r_first = p / CH;
-        const bool read = c < (hd + 15) / 16 * 2;  // a chunk some product reads
         const bool in_row = c * 8 < hd;
+        // the chunk's place in its row, swizzled, for the passes by four
+        unsigned place[4];
+#pragma unroll
+        for (int n = 0; n < 4; n++) place[n] = sw16_off((r_first + n * RSTEP) & 7, c, KT) - ((r_first + n * RSTEP) & 7) * 128;
         int slot = 0;
         unsigned turn = 1;  // phase of an empty slot: none is waited for in the first round
         bool first_round = true;
         int pending = -1;  // slot whose copies are under way
-        bool ok = true;
+        bool ok = true, all_held = false;
         auto land = [&]() {
             if (pending < 0) return;
             cp_async_wait<0>();
@@ -731,19 +764,13 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             mbar_arrive(&sh->full[pending]);
             pending = -1;
         };
-        // offsets of tile j's keys; the barriers order them with the copies
-        auto lookup = [&](int j) {
-            for (int i = p; i < KT; i += PR_PRODUCERS) {
-                const int at = lo + j * KT + i;
-                sh->off[i] = at < hi ? key_offset(kv, b, seq, (unsigned)keys.key(at), head) : -1;
-            }
-            named_bar_sync(1, PR_PRODUCERS);
-            if (p < KT / 32) {
-                unsigned bits = 0;
-                for (int i = 0; i < 32; i++) bits |= (sh->off[p * 32 + i] >= 0 ? 1u : 0u) << i;
-                sh->valid[j & 7][p] = bits;
-            }
+        // byte offset in the pools of key `i` of tile j, -1 for none
+        auto find = [&](int j, int i) -> long long {
+            const int at = lo + j * KT + i;
+            const long long o = i < KT && at < hi ? key_offset(kv, b, seq, (unsigned)keys.key(at), head) : -1;
+            return o < 0 ? -1 : o * ES;
         };
+        long long next0 = find(0, p), next1 = KT > PR_PRODUCERS ? find(0, p + PR_PRODUCERS) : -1;
         auto put = [&](const void *pool) {
             const int s = slot;
             if (!first_round && !mbar_test(&sh->empty[s], turn)) {
@@ -752,20 +779,24 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             }
             if (++slot == Cfg::NSLOT) slot = 0, turn ^= 1u, first_round = false;
             if (!ok) return;
-            const long long *off = sh->off;
             unsigned char *dst = s_kv + s * Cfg::SLOT;
             if constexpr (TYPE != KV_F32) {
-                const unsigned d0 = smem_addr(dst);
+                const unsigned d0 = smem_addr(dst) + r_first * 128;
                 const char *base = reinterpret_cast<const char *>(pool) + c * 16;
-                if (read) {
+                if (in_row && all_held) {
+#pragma unroll
+                    for (int n = 0; n < PASSES; n++)
+                        if (n < PASSES - 1 || r_first + n * RSTEP < KT)
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(d0 + n * RSTEP * 128 + place[n & 3]),
+                                         "l"(base + sh->off[r_first + n * RSTEP]));
+                } else {
 #pragma unroll 4
                     for (int n = 0; n < PASSES; n++) {
-                        const int r = r_first + n * RSTEP;
-                        if (r >= KT) break;
-                        const long long o = off[r];
+                        if (r_first + n * RSTEP >= KT) break;
+                        const long long o = sh->off[r_first + n * RSTEP];
                         const bool in = o >= 0 && in_row;
-                        const char *src = in ? base + o * 2 : reinterpret_cast<const char *>(pool);
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(d0 + sw16_off(r, c, KT)),
+                        const char *src = in ? base + o : reinterpret_cast<const char *>(pool);
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(d0 + n * RSTEP * 128 + place[n & 3]),
                                      "l"(src), "r"(in ? 16u : 0u));
                     }
                 }
@@ -781,9 +812,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
 #pragma unroll
                 for (int n = 0; n < PASSES; n++) {
                     const int r = r_first + n * RSTEP;
-                    const long long o = r < KT ? off[r] : -1;
+                    const long long o = r < KT ? sh->off[r] : -1;
                     if (o >= 0 && in_row) {
-                        const float4 *src = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(pool) + o + c * 8);
+                        const float4 *src = reinterpret_cast<const float4 *>(reinterpret_cast<const char *>(pool) + o + c * 32);
                         u[n][0] = src[0];
                         u[n][1] = src[1];
                     } else {
@@ -793,16 +824,15 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
 #pragma unroll
                 for (int n = 0; n < PASSES; n++) {
                     const int r = r_first + n * RSTEP;
-                    if (r >= KT || !read) continue;
+                    if (r >= KT) continue;
                     unsigned part[4][3];
                     split2<KV_BF16, 3>(u[n][0].x, u[n][0].y, part[0]);
                     split2<KV_BF16, 3>(u[n][0].z, u[n][0].w, part[1]);
                     split2<KV_BF16, 3>(u[n][1].x, u[n][1].y, part[2]);
                     split2<KV_BF16, 3>(u[n][1].z, u[n][1].w, part[3]);
-                    const unsigned at = sw16_off(r, c, KT);
 #pragma unroll
                     for (int i = 0; i < 3; i++)
-                        *reinterpret_cast<uint4 *>(dst + i * Cfg::PART + at) =
+                        *reinterpret_cast<uint4 *>(dst + i * Cfg::PART + r * 128 + place[n & 3]) =
                             make_uint4(part[0][i], part[1][i], part[2][i], part[3][i]);
                 }
                 fence_async_smem();
@@ -810,8 +840,21 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             }
         };
         for (int j = 0; j < ntile && ok; j++) {
-            lookup(j);
-            named_bar_sync(1, PR_PRODUCERS);
+            // tile j's offsets for all, then those of the next tile on their way
+            if (p < KT) sh->off[p] = next0;
+            const unsigned held0 = __ballot_sync(0xffffffffu, next0 >= 0);
+            if (lane == 0 && p < KT) sh->valid[j & 7][p >> 5] = held0;
+            unsigned held1 = 0xffffffffu;
+            if (KT > PR_PRODUCERS && warp == 9) {
+                sh->off[PR_PRODUCERS + p] = next1;
+                held1 = __ballot_sync(0xffffffffu, next1 >= 0);
+                if (lane == 0) sh->valid[j & 7][3] = held1;
+            }
+            all_held = !named_bar_or(1, PR_PRODUCERS, (p < KT && held0 != 0xffffffffu) || held1 != 0xffffffffu);
+            if (j + 1 < ntile) {
+                next0 = find(j + 1, p);
+                if (KT > PR_PRODUCERS && warp == 9) next1 = find(j + 1, p + PR_PRODUCERS);
+            }
             put(kv.k);
             if (ok) put(kv.v);
             ok = !named_bar_or(1, PR_PRODUCERS, !ok);
