@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(R_SOFTMAX));
         // ------------------------------------------------ q, softmax, output
         const float sl2_all = __fmul_rn(a.scale, 1.44269504088896340736f);
-        {  // a warp per row, eight rows at a time
+        {  // a warp per row, its sixteen rows' loads in flight together
             const bool vec = (((uintptr_t)a.q | (a.ldq * 4)) & 15) == 0;
             const int c4 = lane * 4;
             // lane i < 16: the offset of the warp's row i in q, and whether it is one
@@ -399,29 +399,29 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
                                           : (long long)((size_t)row0 * a.ldq);
             const unsigned oks = __ballot_sync(0xffffffffu, my_ok);
 #pragma unroll
-            for (int r0 = 0; r0 < 16; r0 += 8) {
-                float f[8][4];
+            for (int r0 = 0; r0 < 16; r0 += 16) {
+                float f[16][4];
                 const int c_in = c4 < hd ? c4 : 0;  // every load is of some row's element: none is held up by a branch
                 if (vec) {
 #pragma unroll
-                    for (int u = 0; u < 8; u++) {
+                    for (int u = 0; u < 16; u++) {
                         const float4 t = *reinterpret_cast<const float4 *>(a.q + __shfl_sync(0xffffffffu, my_at, r0 + u) + c_in);
                         f[u][0] = t.x, f[u][1] = t.y, f[u][2] = t.z, f[u][3] = t.w;
                     }
                 } else {
 #pragma unroll
-                    for (int u = 0; u < 8; u++) {
+                    for (int u = 0; u < 16; u++) {
                         const float *src = a.q + __shfl_sync(0xffffffffu, my_at, r0 + u) + c_in;
 #pragma unroll
                         for (int i = 0; i < 4; i++) f[u][i] = src[i];
                     }
                 }
 #pragma unroll
-                for (int u = 0; u < 8; u++)
+                for (int u = 0; u < 16; u++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) f[u][i] = ((oks >> (r0 + u)) & 1u) && c4 < hd ? f[u][i] : 0.f;
 #pragma unroll
-                for (int u = 0; u < 8; u++) {
+                for (int u = 0; u < 16; u++) {
                     const int r = warp * 16 + r0 + u;
                     if constexpr (Cfg::F16) {
                         // the bits of non-negative floats order as they do
@@ -488,15 +488,18 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             }
         };
         const uint64_t sl22 = pack2(sl2, sl2);
-        for (int j = 0; j < ntile; j++) {
-            const unsigned t_s = t_lane + (j & 1) * Cfg::T_S;
+        float v[CT];  // this thread's scores of a tile
+        auto fetch = [&](int j) {
             wait(&sh->s_full[j & 1], j >> 1);
-            if (!ok) break;
+            if (!ok) return;
             tc_fence_after();
-            float v[CT];
 #pragma unroll
-            for (int c = 0; c < CT; c += 32) tmem_ld32(t_s + x * CT + c, v + c);
-            tmem_wait_ld();
+            for (int c = 0; c < CT; c += 32) tmem_ld32(t_lane + (j & 1) * Cfg::T_S + x * CT + c, v + c);
+        };
+        if (ntile > 0) fetch(0);
+        for (int j = 0; j < ntile && ok; j++) {
+            const unsigned t_s = t_lane + (j & 1) * Cfg::T_S;
+            tmem_wait_ld();  // tile j's scores, on their way since the last tile's end
 #pragma unroll
             for (int c = 0; c < CT; c += 32) pin32(v + c);
             const int i0 = lo + j * KT + x * CT;
@@ -506,10 +509,15 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             for (int c = 0; c < CT / 32; c++) whole = whole && valid[c] == 0xffffffffu;
             if (!__all_sync(0xffffffffu, whole)) {
 #pragma unroll
-                for (int c = 0; c < CT; c++) {
-                    const int i = i0 + c;
-                    const bool seen = i < to && (i < sink_end || i >= from) && ((valid[c >> 5] >> (c & 31)) & 1u);
-                    v[c] = seen ? v[c] : -INFINITY;
+                for (int g = 0; g < CT; g += 32) {
+                    // bit c: list position i0 + g + c is seen
+                    auto below = [&](int end) -> unsigned {
+                        const int n = end - (i0 + g);
+                        return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+                    };
+                    const unsigned seen = below(to) & (below(sink_end) | ~below(from)) & valid[g >> 5];
+#pragma unroll
+                    for (int c = 0; c < 32; c++) v[g + c] = seen & (1u << c) ? v[g + c] : -INFINITY;
                 }
             }
             float t0 = v[0], t1 = v[1], t2 = v[2], t3 = v[3];
@@ -582,7 +590,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(&sh->p_full[j & 1]);
-            if (j > 0) gather(j - 1);  // under w.v of this tile
+            if (j + 1 < ntile) fetch(j + 1);
+            if (j > 0 && ok) gather(j - 1);  // under w.v of this tile
             if (moved) {
                 const uint64_t ff = pack2(f, f);
 #pragma unroll
@@ -676,6 +685,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             auto wait = [&](uint64_t *bar, int phase) {  // the warp goes on together
                 ok = __all_sync(0xffffffffu, ok && pr_wait(bar, (unsigned)phase & 1u, sh, kv));
                 tc_fence_after();
+                fence_async_smem();  // what the copies wrote, before the tensor core reads it
             };
             // the products of parts that count, the smallest first
             auto parts = [&](auto f) {
@@ -755,15 +765,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
         int slot = 0;
         unsigned turn = 1;  // phase of an empty slot: none is waited for in the first round
         bool first_round = true;
-        int pending = -1;  // slot whose copies are under way
         bool ok = true, all_held = false;
-        auto land = [&]() {
-            if (pending < 0) return;
-            cp_async_wait<0>();
-            fence_async_smem();
-            mbar_arrive(&sh->full[pending]);
-            pending = -1;
-        };
         // byte offset in the pools of key `i` of tile j, -1 for none
         auto find = [&](int j, int i) -> long long {
             const int at = lo + j * KT + i;
@@ -773,10 +775,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
         long long next0 = find(0, p), next1 = KT > PR_PRODUCERS ? find(0, p + PR_PRODUCERS) : -1;
         auto put = [&](const void *pool) {
             const int s = slot;
-            if (!first_round && !mbar_test(&sh->empty[s], turn)) {
-                land();
-                ok = pr_wait(&sh->empty[s], turn, sh, kv);
-            }
+            if (!first_round) ok = pr_wait(&sh->empty[s], turn, sh, kv);
             if (++slot == Cfg::NSLOT) slot = 0, turn ^= 1u, first_round = false;
             if (!ok) return;
             unsigned char *dst = s_kv + s * Cfg::SLOT;
@@ -800,13 +799,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
                                      "l"(src), "r"(in ? 16u : 0u));
                     }
                 }
-                cp_async_commit();
-                if (pending >= 0) {
-                    cp_async_wait<1>();
-                    fence_async_smem();
-                    mbar_arrive(&sh->full[pending]);
-                }
-                pending = s;
+                // arrives once this thread's copies are in; the MMA warp orders
+                // them before its own accesses
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(smem_addr(&sh->full[s])) : "memory");
             } else {
                 float4 u[PASSES][2];
 #pragma unroll
@@ -859,8 +854,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             if (ok) put(kv.v);
             ok = !named_bar_or(1, PR_PRODUCERS, !ok);
         }
-        land();
-        cp_async_wait<0>();
+        asm volatile("cp.async.wait_all;\n" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
