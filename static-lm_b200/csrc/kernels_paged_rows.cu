@@ -53,8 +53,7 @@ struct RowsCfg {
     // for two): the MMAs' operands are the same every second tile
     static constexpr int NSLOT = TYPE == KV_F32 && HDP == 128 ? 2 : 4;
     // TMEM columns: score / weight buffers (128 or 3 x 32 used) at 0 and 128,
-    // results at 256 and 256 + HDP: each buffer at a multiple of its width, as
-    // an accumulator laid across column 256 faulted
+    // results at 256 and 256 + HDP
     static constexpr int T_S = 128, T_O = 256;
     static constexpr int BIG = QBYTES + NSLOT * SLOT;
     // at least 120 KB: one CTA per SM, whose TMEM it takes whole
@@ -121,6 +120,12 @@ __device__ __forceinline__ void tc_mma_f16_ta(unsigned d, unsigned a, uint64_t b
         "r"(a), "l"(bdesc), "r"(idesc), "r"((unsigned)acc)
         : "memory");
 }
+// What the copies wrote, before the lane that issues has the tensor core read
+// it (by all 32 lanes after every wait it stood for about 1000 cycles a tile).
+__device__ __forceinline__ void fence_async_elected() {
+    asm volatile(
+        "{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n @q fence.proxy.async.shared::cta;\n}\n" ::: "memory");
+}
 __device__ __forceinline__ void tc_commit_elected(uint64_t *bar) {
     asm volatile(
         "{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n"
@@ -175,6 +180,13 @@ __device__ __forceinline__ bool pr_wait(uint64_t *bar, unsigned parity, RowsShar
     return true;
 }
 
+// One arrival for a warp's 32 threads (an arrival of each is worked off one by
+// one: at 256 a tile they took longer than the arithmetic).
+__device__ __forceinline__ void warp_arrive(uint64_t *bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
 // Two f32 values as the packed 16-bit parts of an operand.  A part that is
 // not finite is the whole value.
 template <int TYPE, int N>
@@ -200,23 +212,22 @@ __device__ __forceinline__ void split2(float a, float b, unsigned (&part)[N]) {
 }
 // The same of two softmax weights (finite, or NaN: then the row is redone).
 template <int TYPE, int N>
-__device__ __forceinline__ void split2_weights(uint64_t e, unsigned (&part)[N]) {
-    const uint64_t minus = 0xbf800000bf800000ull;  // (-1, -1)
-    float a, b;
+__device__ __forceinline__ void split2_weights(float a, float b, unsigned (&part)[N]) {
     if constexpr (TYPE == KV_F16) {
-        unpack2(e, a, b);
         const __half2 h = __floats2half2_rn(a, b);
         const float2 f = __half22float2(h);
-        unpack2(fma2(pack2(f.x, f.y), minus, e), a, b);
-        const __half2 r = __floats2half2_rn(a, b);
+        const __half2 r = __floats2half2_rn(__fsub_rn(a, f.x), __fsub_rn(b, f.y));
         part[0] = *reinterpret_cast<const unsigned *>(&h);
         part[1] = *reinterpret_cast<const unsigned *>(&r);
     } else {
 #pragma unroll
         for (int i = 0; i < N; i++) {  // cut, not rounded: 8 bits each
-            const uint64_t hi = e & 0xffff0000ffff0000ull;
-            part[i] = __byte_perm((unsigned)e, (unsigned)(e >> 32), 0x7632);
-            if (i + 1 < N) e = fma2(hi, minus, e);
+            const unsigned ua = __float_as_uint(a), ub = __float_as_uint(b);
+            part[i] = __byte_perm(ua, ub, 0x7632);
+            if (i + 1 < N) {
+                a = __fsub_rn(a, __uint_as_float(ua & 0xffff0000u));
+                b = __fsub_rn(b, __uint_as_float(ub & 0xffff0000u));
+            }
         }
     }
 }
@@ -344,12 +355,12 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
         }
         for (int x = 0; x < 2; x++) {
             mbar_init(&sh->s_full[x], 1);
-            mbar_init(&sh->p_full[x], 256);
+            mbar_init(&sh->p_full[x], 8);
             mbar_init(&sh->o_full[x], 1);
         }
-        mbar_init(&sh->q_full, 256);
-        mbar_init(&sh->seen_all, 256);
-        mbar_init(&sh->swapped, 256);
+        mbar_init(&sh->q_full, 8);
+        mbar_init(&sh->seen_all, 8);
+        mbar_init(&sh->swapped, 8);
         for (int i = 0; i < 4; i++) sh->move[i] = 0;
         mbar_init(&sh->drain, 1);
         sh->abort = 0;
@@ -448,7 +459,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
                 }
             }
             fence_async_smem();
-            mbar_arrive(&sh->q_full);
+            warp_arrive(&sh->q_full);
             if constexpr (Cfg::F16) named_bar_sync(2, 256);  // the rows' 2^-e
         }
         const int x = warp >> 2, r = tid & 127;  // half, row of the tile
@@ -465,9 +476,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
         const float sl2 = Cfg::F16 ? __fmul_rn(sl2_all, sh->row[0][r]) : sl2_all;
         const unsigned t_lane = taddr + ((unsigned)((warp & 3) * 32) << 16);
         float m = PR_NO_MAX, l = 0.f;
-        uint64_t acc[OC / 2];
+        float acc[OC];
 #pragma unroll
-        for (int i = 0; i < OC / 2; i++) acc[i] = 0ull;
+        for (int i = 0; i < OC; i++) acc[i] = 0.f;
         bool ok = true;
         auto wait = [&](uint64_t *bar, int phase) {  // a warp goes on together: TMEM accesses are warp-wide
             ok = __all_sync(0xffffffffu, ok && pr_wait(bar, (unsigned)phase & 1u, sh, kv));
@@ -484,10 +495,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
                 tmem_wait_ld();
                 pin32(o);
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) acc[(c + i) / 2] = add2(acc[(c + i) / 2], pack2(o[i], o[i + 1]));
+                for (int i = 0; i < 32; i++) acc[c + i] = __fadd_rn(acc[c + i], o[i]);
             }
         };
-        const uint64_t sl22 = pack2(sl2, sl2);
         float v[CT];  // this thread's scores of a tile
         auto fetch = [&](int j) {
             wait(&sh->s_full[j & 1], j >> 1);
@@ -532,28 +542,22 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             // this thread has its scores, and says whether its row's reference
             // has to move; the first weights are worked out meanwhile, as if none had
             if (top > m + PR_RESCALE) *(volatile int *)&sh->move[j & 3] = 1;
-            mbar_arrive(&sh->seen_all);
-            uint64_t sum;  // of 32 weights
+            warp_arrive(&sh->seen_all);
+            float sum;  // of 32 weights
             unsigned w[NQ][16];
             auto weights = [&](int c) {
-                const uint64_t mm = pack2(-m, -m);
-                uint64_t s0 = 0ull, s1 = 0ull;
+                float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-                for (int i = 0; i < 32; i += 4) {
-                    float e0, e1, e2, e3;
-                    unpack2(fma2(pack2(v[c + i], v[c + i + 1]), sl22, mm), e0, e1);
-                    unpack2(fma2(pack2(v[c + i + 2], v[c + i + 3]), sl22, mm), e2, e3);
-                    const uint64_t a01 = pack2(exp2_approx(e0), exp2_approx(e1));
-                    const uint64_t a23 = pack2(exp2_approx(e2), exp2_approx(e3));
-                    s0 = add2(s0, a01);
-                    s1 = add2(s1, a23);
-                    unsigned p[NQ], q[NQ];
-                    split2_weights<TYPE, NQ>(a01, p);
-                    split2_weights<TYPE, NQ>(a23, q);
+                for (int i = 0; i < 32; i += 2) {
+                    const float e0 = exp2_approx(__fmaf_rn(v[c + i], sl2, -m)), e1 = exp2_approx(__fmaf_rn(v[c + i + 1], sl2, -m));
+                    s0 = __fadd_rn(s0, e0);
+                    s1 = __fadd_rn(s1, e1);
+                    unsigned p[NQ];
+                    split2_weights<TYPE, NQ>(e0, e1, p);
 #pragma unroll
-                    for (int n = 0; n < NQ; n++) w[n][i / 2] = p[n], w[n][i / 2 + 1] = q[n];
+                    for (int n = 0; n < NQ; n++) w[n][i / 2] = p[n];
                 }
-                sum = add2(s0, s1);
+                sum = __fadd_rn(s0, s1);
             };
             weights(0);
             wait(&sh->seen_all, j);
@@ -563,11 +567,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             if (tid == 0) *(volatile int *)&sh->move[(j + 2) & 3] = 0;  // last read two tiles ago
             if (moved) {  // the halves of each row move their reference together
                 *(volatile float *)&sh->row[x][r] = top;
-                mbar_arrive(&sh->swapped);
+                warp_arrive(&sh->swapped);
                 wait(&sh->swapped, 0);
                 if (!ok) break;
                 const float both = fmaxf(top, *(volatile float *)&sh->row[x ^ 1][r]);
-                mbar_arrive(&sh->swapped);
+                warp_arrive(&sh->swapped);
                 wait(&sh->swapped, 1);  // read before the next exchange
                 if (!ok) break;
                 if (both > m + PR_RESCALE) {
@@ -581,21 +585,18 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
 #pragma unroll
             for (int c = 0; c < CT; c += 32) {
                 if (c > 0) weights(c);
-                float s0, s1;
-                unpack2(sum, s0, s1);
-                l = __fadd_rn(l, __fadd_rn(s0, s1));
+                l = __fadd_rn(l, sum);
 #pragma unroll
                 for (int n = 0; n < NQ; n++) tmem_st16(t_s + n * (KT / 2) + (x * CT + c) / 2, w[n]);
             }
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(&sh->p_full[j & 1]);
+            warp_arrive(&sh->p_full[j & 1]);
             if (j + 1 < ntile) fetch(j + 1);
             if (j > 0 && ok) gather(j - 1);  // under w.v of this tile
             if (moved) {
-                const uint64_t ff = pack2(f, f);
 #pragma unroll
-                for (int i = 0; i < OC / 2; i++) acc[i] = mul2(acc[i], ff);
+                for (int i = 0; i < OC; i++) acc[i] = __fmul_rn(acc[i], f);
             }
         }
         if (ok && ntile > 0) gather(ntile - 1);
@@ -613,9 +614,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             bool finite = fabsf(l) < INFINITY;
 #pragma unroll
             for (int i = 0; i < OC; i += 4) {
-                float y[4];
-                unpack2(acc[i / 2], y[0], y[1]);
-                unpack2(acc[i / 2 + 1], y[2], y[3]);
+                float y[4] = {acc[i], acc[i + 1], acc[i + 2], acc[i + 3]};
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
                     y[u] = __fmul_rn(y[u], inv);
@@ -685,7 +684,6 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             auto wait = [&](uint64_t *bar, int phase) {  // the warp goes on together
                 ok = __all_sync(0xffffffffu, ok && pr_wait(bar, (unsigned)phase & 1u, sh, kv));
                 tc_fence_after();
-                fence_async_smem();  // what the copies wrote, before the tensor core reads it
             };
             // the products of parts that count, the smallest first
             auto parts = [&](auto f) {
@@ -700,6 +698,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             auto scores = [&](auto parity, int j) {
                 constexpr int P = decltype(parity)::value, S = Cfg::NSLOT == 4 ? 2 * P : 0;
                 wait(&sh->full[S], Cfg::NSLOT == 4 ? j >> 1 : j);
+                fence_async_elected();
                 if (!ok) return;
                 parts([&](int i, int c, bool first) {
 #pragma unroll
@@ -716,6 +715,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             auto values = [&](auto parity, int j) {
                 constexpr int P = decltype(parity)::value, S = Cfg::NSLOT == 4 ? 2 * P + 1 : 1;
                 wait(&sh->full[S], Cfg::NSLOT == 4 ? j >> 1 : j);
+                fence_async_elected();
                 wait(&sh->p_full[P], j >> 1);
                 if (!ok) return;
                 parts([&](int i, int c, bool first) {
