@@ -187,8 +187,8 @@ __device__ __forceinline__ void warp_arrive(uint64_t *bar) {
     if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
-// Two f32 values as the packed 16-bit parts of an operand.  A part that is
-// not finite is the whole value.
+// Two f32 values as the packed 16-bit parts of an operand.  (The second part
+// of an infinity is NaN: rows that meet it come out NaN and are redone.)
 template <int TYPE, int N>
 __device__ __forceinline__ void split2(float a, float b, unsigned (&part)[N]) {
 #pragma unroll
@@ -205,8 +205,8 @@ __device__ __forceinline__ void split2(float a, float b, unsigned (&part)[N]) {
             ra = __uint_as_float(part[i] << 16), rb = __uint_as_float(part[i] & 0xffff0000u);
         }
         if (i + 1 < N) {
-            a = fabsf(ra) < INFINITY ? __fsub_rn(a, ra) : 0.f;
-            b = fabsf(rb) < INFINITY ? __fsub_rn(b, rb) : 0.f;
+            a = __fsub_rn(a, ra);
+            b = __fsub_rn(b, rb);
         }
     }
 }
@@ -850,8 +850,13 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
                 next0 = find(j + 1, p);
                 if (KT > PR_PRODUCERS && warp == 9) next1 = find(j + 1, p + PR_PRODUCERS);
             }
-            put(kv.k);
-            if (ok) put(kv.v);
+            if constexpr (TYPE == KV_F32) {  // one copy of the long conversion
+#pragma unroll 1
+                for (int i = 0; i < 2 && ok; i++) put(i == 0 ? kv.k : kv.v);
+            } else {
+                put(kv.k);
+                if (ok) put(kv.v);
+            }
             ok = !named_bar_or(1, PR_PRODUCERS, !ok);
         }
         asm volatile("cp.async.wait_all;\n" ::: "memory");
