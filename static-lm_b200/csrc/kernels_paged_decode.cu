@@ -15,11 +15,14 @@ namespace {
 
 constexpr int PD_WARPS = 4;
 constexpr int PD_THREADS = PD_WARPS * 32;
-constexpr int PD_STAGES = 3;
+constexpr int PD_STAGES = 2;  // 64 KB a CTA: three CTAs an SM (three stages and two CTAs: 8 % slower)
 constexpr int PD_PASSES = 8;               // 512-byte passes per K (or V) tile
 constexpr int PD_TILE = PD_PASSES * 512;   // bytes of a warp's K (or V) tile
 constexpr float PD_NO_MAX = -3.0e38f;      // below every finite score
 constexpr float PD_RESCALE = 8.0f;         // the reference moves when a score passes it by 2^8
+
+// CTAs of g query heads that an SM holds: by shared memory, and by registers.
+__host__ __device__ constexpr int ctas_per_sm(int g) { return g <= 4 ? 3 : 2; }
 
 __device__ __forceinline__ void cp_async16_zfill(unsigned dst, const void *src, unsigned bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes));
@@ -72,7 +75,7 @@ struct Chunk<KV_BF16> {
 // no barrier of the CTA before the join.  Slots past the end, and pages that
 // are not held, are filled with zeros and get weight zero.
 template <int TYPE, int LPR, int G>
-__global__ void __launch_bounds__(PD_THREADS, 2)
+__global__ void __launch_bounds__(PD_THREADS, ctas_per_sm(G))
     paged_decode_kernel(KvView kv, BatchView b, PagedAttnView a, DecodePlan plan) {
     constexpr int RPP = 32 / LPR;          // rows per pass
     constexpr int TK = RPP * PD_PASSES;    // keys per tile
@@ -408,13 +411,27 @@ DecodePlan plan_paged_decode(const KvView &kv, const BatchView &b, const PagedAt
     uint64_t most = max_kv_len;
     if (a.window) most = std::min<uint64_t>(most, (uint64_t)a.window + a.sinks);
     most = std::max<uint64_t>(most, 1);
-    const uint64_t units = (uint64_t)b.num_seqs * kv.kv_heads * p.head_groups;
-    const uint64_t slots = 2 * 148;
-    uint64_t chunk = most * std::max<uint64_t>(units, 1) / (slots * 4);
-    chunk = std::min<uint64_t>(std::max<uint64_t>(chunk, 256), 1024);
-    chunk = (chunk + 63) / 64 * 64;
-    p.splits = (int)((most + chunk - 1) / chunk);
-    p.chunk = (int)chunk;
+    const uint64_t units = std::max<uint64_t>((uint64_t)b.num_seqs * kv.kv_heads * p.head_groups, 1);
+    // A CTA costs its keys' bytes and about 150 KB more (its first look-ups and
+    // copies, its warps' join); the CTAs run in waves over the SMs; the second
+    // launch costs about 75 KB.  Of 1 to 64 splits the cheapest by that count.
+    // Measured (best of a sweep in brackets): 64 x 2049 f32, 192 units: 2
+    // splits, 50 us (1: 54, 4: 54); one sequence of 8192, 8 units: 24 to 37
+    // alike; 64 ragged to 8192, 512 units: 6, 218 us (8: 216, 4: 224, 1: 315);
+    // 128 windows of 1028, 1024 units: 1, 121 us (2: 126).
+    const uint64_t slots = 148 * (uint64_t)ctas_per_sm(p.heads);
+    const uint64_t key_bytes = 2ull * kv.hd * (kv.type == KV_F32 ? 4 : 2);
+    uint64_t best = UINT64_MAX;
+    for (uint64_t s = 1; s <= 64; s++) {
+        uint64_t chunk = ((most + s - 1) / s + 15) / 16 * 16;
+        if (s > 1 && chunk < 64) break;
+        const uint64_t waves = (units * s + slots - 1) / slots;
+        const uint64_t cost = waves * (chunk * key_bytes + (150 << 10)) + (s > 1 ? 75 << 10 : 0);
+        if (cost >= best) continue;
+        best = cost;
+        p.chunk = (int)std::min<uint64_t>(chunk, INT32_MAX);
+        p.splits = (int)((most + chunk - 1) / chunk);
+    }
     const uint64_t parts = (uint64_t)b.num_rows * a.num_heads * p.splits;
     p.ml_bytes = p.splits > 1 ? (parts * sizeof(float2) + 15) / 16 * 16 : 0;
     p.scratch_bytes = p.splits > 1 ? p.ml_bytes + parts * kv.hd * sizeof(float) : 0;
