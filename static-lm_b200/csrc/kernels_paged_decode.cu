@@ -18,7 +18,6 @@ constexpr int PD_THREADS = PD_WARPS * 32;
 constexpr int PD_STAGES = 2;  // 64 KB a CTA: three CTAs an SM (three stages and two CTAs: 8 % slower)
 constexpr int PD_PASSES = 8;               // 512-byte passes per K (or V) tile
 constexpr int PD_TILE = PD_PASSES * 512;   // bytes of a warp's K (or V) tile
-constexpr float PD_NO_MAX = -3.0e38f;      // below every finite score
 constexpr float PD_RESCALE = 8.0f;         // the reference moves when a score passes it by 2^8
 
 // CTAs of g query heads that an SM holds: by shared memory, and by registers.
@@ -29,59 +28,78 @@ __device__ __forceinline__ void cp_async16_zfill(unsigned dst, const void *src, 
 }
 
 // The 16 bytes of one lane as f32 pairs.
-template <int TYPE>
-struct Chunk;
-template <>
-struct Chunk<KV_F32> {
-    static constexpr int N = 2;
-    static __device__ __forceinline__ void get(unsigned a, uint64_t (&x)[2]) {
-        asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(x[0]), "=l"(x[1]) : "r"(a));
-    }
+__device__ __forceinline__ void load_chunk(unsigned a, uint64_t (&x)[2]) {
+    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(x[0]), "=l"(x[1]) : "r"(a));
+}
+
+// What the two kernels share of a CTA's work: keys [lo, hi) of the list that
+// the row of sequence `seq` sees, KV head `head`, ng query heads from h0 on.
+struct DecodeWork {
+    int split, seq, head, h0, ng, lo, hi;
+    SeenKeys keys;
 };
-template <>
-struct Chunk<KV_F16> {
-    static constexpr int N = 4;
-    static __device__ __forceinline__ void get(unsigned a, uint64_t (&x)[4]) {
-        unsigned w[4];
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a));
+__device__ __forceinline__ bool decode_work(const KvView &kv, const BatchView &b, const PagedAttnView &a,
+                                            const DecodePlan &plan, DecodeWork &w) {
+    w.split = blockIdx.x % plan.splits;
+    int unit = blockIdx.x / plan.splits;
+    const int hg = unit % plan.head_groups;
+    unit /= plan.head_groups;
+    w.head = unit % kv.kv_heads, w.seq = unit / kv.kv_heads;
+    const int group = a.num_heads / kv.kv_heads, g0 = hg * plan.heads;
+    w.ng = group - g0 < plan.heads ? group - g0 : plan.heads;
+    w.h0 = w.head * group + g0;
+    const int pos = b.kv_len[w.seq] - 1;
+    w.keys = seen_keys(pos, pos, a.window, a.sinks);
+    w.lo = w.split * plan.chunk;
+    if (w.split > 0 && w.lo >= w.keys.n) return false;  // the join knows
+    w.hi = w.split == plan.splits - 1 || w.lo + plan.chunk > w.keys.n ? w.keys.n : w.lo + plan.chunk;
+    return true;
+}
+// The warps' (m, l, o) of a CTA, in shared memory as [warp][G][hd], to the
+// output or to the split's place in the scratch.
+template <int G>
+__device__ __forceinline__ void decode_store(const KvView &kv, const PagedAttnView &a, const DecodePlan &plan,
+                                             const DecodeWork &w, const float *s_o, const float (*s_m)[G], const float (*s_l)[G]) {
+    for (int e = threadIdx.x; e < w.ng * kv.hd; e += PD_THREADS) {
+        const int g = e / kv.hd, d = e % kv.hd;
+        float top = s_m[0][g];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-            x[i] = pack2(f.x, f.y);
+        for (int i = 1; i < PD_WARPS; i++) top = fmaxf(top, s_m[i][g]);
+        float o = 0.f, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < PD_WARPS; i++) {
+            const float f = exp2_approx(__fsub_rn(s_m[i][g], top));
+            o = __fmaf_rn(f, s_o[(i * G + g) * kv.hd + d], o);
+            sum = __fmaf_rn(f, s_l[i][g], sum);
+        }
+        if (plan.splits == 1) {
+            a.out[(size_t)w.seq * a.ldo + (size_t)(w.h0 + g) * kv.hd + d] = sum == 0.f ? 0.f : __fdiv_rn(o, sum);
+        } else {
+            const size_t at = ((size_t)w.seq * a.num_heads + w.h0 + g) * plan.splits + w.split;
+            plan.part_o[at * kv.hd + d] = o;
+            if (d == 0) plan.part_ml[at] = make_float2(top, sum);
         }
     }
-};
-template <>
-struct Chunk<KV_BF16> {
-    static constexpr int N = 4;
-    static __device__ __forceinline__ void get(unsigned a, uint64_t (&x)[4]) {
-        unsigned w[4];
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a));
-#pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = pack2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
-    }
-};
+}
 
-// Work of one CTA: keys [split*chunk, ..) of the list of keys that the row of
-// sequence `seq` sees (the last split takes what is left), KV head `head`,
-// `g` query heads from h0 on.
+// f32 pages, on the CUDA cores.
 //
 // LPR lanes hold one key's row (16 bytes each), so a warp reads 32/LPR rows a
-// pass and a tile is 8 passes of 512 bytes whatever the type and head_dim.
-// Each lane dots its elements for every head; the 8 passes' partial sums are
-// summed over the row's lanes by halving exchanges (4 + 2 + 1 shuffles and
-// one more per doubling of LPR past 8), which leave lane i with the scores of
-// pass i & 7.  A warp's tiles come through its own ring of cp.async stages:
-// no barrier of the CTA before the join.  Slots past the end, and pages that
-// are not held, are filled with zeros and get weight zero.
-template <int TYPE, int LPR, int G>
+// pass and a tile is 8 passes of 512 bytes whatever the head_dim.  Each lane
+// dots its elements for every head; the 8 passes' partial sums are summed over
+// the row's lanes by halving exchanges (4 + 2 + 1 shuffles and one more per
+// doubling of LPR past 8), which leave lane i with the scores of pass i & 7.
+// A warp's tiles come through its own ring of cp.async stages: no barrier of
+// the CTA before its end.  Slots past the end, and pages that are not held, are
+// filled with zeros and get weight zero.
+template <int LPR, int G>
 __global__ void __launch_bounds__(PD_THREADS, ctas_per_sm(G))
     paged_decode_kernel(KvView kv, BatchView b, PagedAttnView a, DecodePlan plan) {
     constexpr int RPP = 32 / LPR;          // rows per pass
     constexpr int TK = RPP * PD_PASSES;    // keys per tile
-    constexpr int NV = Chunk<TYPE>::N;     // f32 pairs per lane and row
+    constexpr int NV = 2;                  // f32 pairs per lane and row
     constexpr int E = 2 * NV;
-    constexpr int ES = TYPE == KV_F32 ? 4 : 2;
+    constexpr int ES = 4;
     constexpr int GP = (G + 1) & ~1;
     extern __shared__ __align__(128) unsigned char pd_smem[];
     __shared__ __align__(16) uint64_t s_p[PD_WARPS][TK][GP];
@@ -90,20 +108,10 @@ __global__ void __launch_bounds__(PD_THREADS, ctas_per_sm(G))
 
     pdl_release();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int split = blockIdx.x % plan.splits;
-    int unit = blockIdx.x / plan.splits;
-    const int hg = unit % plan.head_groups;
-    unit /= plan.head_groups;
-    const int head = unit % kv.kv_heads, seq = unit / kv.kv_heads;
-    const int group = a.num_heads / kv.kv_heads;
-    const int g0 = hg * G, ng = group - g0 < G ? group - g0 : G;
-    const int h0 = head * group + g0;
-
-    const int pos = b.kv_len[seq] - 1;
-    const SeenKeys keys = seen_keys(pos, pos, a.window, a.sinks);
-    const int lo = split * plan.chunk;
-    if (split > 0 && lo >= keys.n) return;  // the join knows
-    const int hi = split == plan.splits - 1 || lo + plan.chunk > keys.n ? keys.n : lo + plan.chunk;
+    DecodeWork work;
+    if (!decode_work(kv, b, a, plan, work)) return;
+    const int seq = work.seq, head = work.head, h0 = work.h0, ng = work.ng, lo = work.lo, hi = work.hi;
+    const SeenKeys keys = work.keys;
 
     const int c = lane % LPR, rg = lane / LPR;
     const bool in_row = c * E < kv.hd;
@@ -141,7 +149,7 @@ __global__ void __launch_bounds__(PD_THREADS, ctas_per_sm(G))
     uint64_t acc[G][NV];
 #pragma unroll
     for (int g = 0; g < G; g++) {
-        m[g] = PD_NO_MAX;
+        m[g] = NO_MAX;
         l[g] = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; i++) acc[g][i] = 0ull;
@@ -173,7 +181,7 @@ __global__ void __launch_bounds__(PD_THREADS, ctas_per_sm(G))
 #pragma unroll
         for (int p = 0; p < PD_PASSES; p++) {
             uint64_t x[NV];
-            Chunk<TYPE>::get(kt + p * 512, x);
+            load_chunk(kt + p * 512, x);
 #pragma unroll
             for (int g = 0; g < G; g++) {
                 uint64_t d = mul2(q[g][0], x[0]);
@@ -235,7 +243,7 @@ __global__ void __launch_bounds__(PD_THREADS, ctas_per_sm(G))
 #pragma unroll
         for (int p = 0; p < PD_PASSES; p++) {
             uint64_t v[NV];
-            Chunk<TYPE>::get(vt + p * 512, v);
+            load_chunk(vt + p * 512, v);
             const uint64_t *w = s_p[warp][p * RPP + rg];
 #pragma unroll
             for (int g = 0; g < G; g++) {
@@ -272,26 +280,249 @@ __global__ void __launch_bounds__(PD_THREADS, ctas_per_sm(G))
         }
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < ng * kv.hd; e += PD_THREADS) {
-        const int g = e / kv.hd, d = e % kv.hd;
-        float top = s_m[0][g];
+    decode_store<G>(kv, a, plan, work, s_o, s_m, s_l);
+}
+
+// f16 and bf16 pages, on the tensor cores (mma.sync m16n8k16: a warp's own,
+// with fragments in registers; the 128-row tiles of tcgen05 would hold 8 rows).
+//
+// The 16 rows of A are up to 8 query heads in two 16-bit parts each, f16 with
+// the row scaled so that its largest element is near 2^15, or the first two of
+// three bf16 parts; the third has MMAs of its own.  A key's row is a column of
+// B straight from shared memory (ldmatrix).  Rows h and h + 8 of the scores
+// are one lane's, so it adds the parts itself, and its weights are, packed,
+// the A operand of w.v: nothing crosses lanes but the row maxima, on the tiles
+// where a reference moves.  Each step's w.v starts from zero and is added in
+// f32: the tensor core cuts its sums.  270 instructions per 16 keys of 128
+// elements; the same on the CUDA cores took 900 and the launch twice the time
+// that its bytes need.
+__device__ __forceinline__ void ldsm4(unsigned a, unsigned (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(unsigned a, unsigned (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a)
+                 : "memory");
+}
+template <int TYPE>
+__device__ __forceinline__ void mma16816(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
+                                         unsigned b1) {
+    if constexpr (TYPE == KV_F16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <int TYPE, int LPR>
+__global__ void __launch_bounds__(PD_THREADS, 3)
+    paged_decode_mma_kernel(KvView kv, BatchView b, PagedAttnView a, DecodePlan plan) {
+    constexpr int G = 8;
+    constexpr int RPP = 32 / LPR, TK = RPP * PD_PASSES;  // keys per tile: 16 or 32
+    constexpr int ROW = LPR * 16;                        // bytes of a key's row
+    constexpr int KS = LPR / 2;                          // 16-element steps of a row
+    constexpr int NQ = TYPE == KV_F16 ? 2 : 3;
+    extern __shared__ __align__(128) unsigned char pd_smem[];
+    __shared__ unsigned s_valid[PD_WARPS][PD_STAGES];
+    __shared__ float s_m[PD_WARPS][G], s_l[PD_WARPS][G];
+
+    pdl_release();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    DecodeWork work;
+    if (!decode_work(kv, b, a, plan, work)) return;
+    const int seq = work.seq, head = work.head, lo = work.lo, hi = work.hi;
+    const SeenKeys keys = work.keys;
+
+    // this lane's head and element pairs: 16 ks + 2 (lane & 3) + {0, 1} and 8 on
+    const int g = lane >> 2, e0 = (lane & 3) * 2;
+    float sl2 = __fmul_rn(a.scale, 1.44269504088896340736f);
+    unsigned qa[KS][2][NQ];  // [step][first or second half of it][part]
+    {
+        const float *src = a.q + (size_t)seq * a.ldq + (size_t)(work.h0 + (g < work.ng ? g : 0)) * kv.hd;
+        float f[KS][4];
+        unsigned top = 0;
 #pragma unroll
-        for (int w = 1; w < PD_WARPS; w++) top = fmaxf(top, s_m[w][g]);
-        float o = 0.f, sum = 0.f;
+        for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-        for (int w = 0; w < PD_WARPS; w++) {
-            const float f = exp2_approx(__fsub_rn(s_m[w][g], top));
-            o = __fmaf_rn(f, s_o[(w * G + g) * kv.hd + d], o);
-            sum = __fmaf_rn(f, s_l[w][g], sum);
+            for (int i = 0; i < 4; i++) {
+                const int d = ks * 16 + e0 + (i & 1) + (i >> 1) * 8;
+                f[ks][i] = d < kv.hd && g < work.ng ? src[d] : 0.f;
+                top = max(top, __float_as_uint(fabsf(f[ks][i])));
+            }
+        float up = 1.0f;
+        if constexpr (TYPE == KV_F16) {
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            int e = 141 - (int)(top >> 23);  // 2^14 <= top 2^e < 2^15
+            e = top == 0 || top >= 0x7f800000u ? 0 : e > 120 ? 120 : e;
+            up = __uint_as_float((unsigned)(127 + e) << 23);
+            sl2 = __fmul_rn(sl2, __uint_as_float((unsigned)(127 - e) << 23));
         }
-        if (plan.splits == 1) {
-            a.out[(size_t)seq * a.ldo + (size_t)(h0 + g) * kv.hd + d] = sum == 0.f ? 0.f : __fdiv_rn(o, sum);
-        } else {
-            const size_t at = ((size_t)seq * a.num_heads + h0 + g) * plan.splits + split;
-            plan.part_o[at * kv.hd + d] = o;
-            if (d == 0) plan.part_ml[at] = make_float2(top, sum);
-        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                split2<TYPE, NQ>(__fmul_rn(f[ks][2 * i], up), __fmul_rn(f[ks][2 * i + 1], up), qa[ks][i]);
     }
+
+    const unsigned ring = smem_addr(pd_smem) + warp * (PD_STAGES * 2 * PD_TILE);
+    const int ntile = (hi - lo + TK - 1) / TK;
+    const int c = lane % LPR, rg = lane / LPR;
+    const bool in_row = c * 8 < kv.hd;
+    auto lookup = [&](int t) -> long long {  // byte offset of key `lane` of tile t, -1 for none
+        const int i = lo + t * TK + lane;
+        const long long o = lane < TK && t < ntile && i < hi ? key_offset(kv, b, seq, (unsigned)keys.key(i), head) : -1;
+        return o < 0 ? -1 : 2 * o;
+    };
+    // 16-byte chunk c of row r is at chunk c ^ (r & 7): eight rows' chunks of
+    // one matrix lie in different banks
+    auto fill = [&](int stage, long long off) {
+        const unsigned valid = __ballot_sync(0xffffffffu, off >= 0);
+        if (lane == 0) s_valid[warp][stage] = valid;
+        const unsigned dst = ring + stage * (2 * PD_TILE);
+#pragma unroll
+        for (int p = 0; p < PD_PASSES; p++) {
+            const int r = p * RPP + rg;
+            const long long o = __shfl_sync(0xffffffffu, off, r);
+            const bool in = o >= 0 && in_row;
+            const size_t at = in ? (size_t)o + c * 16 : 0;
+            const unsigned n = in ? 16u : 0u, to = dst + r * ROW + ((c ^ (r & 7)) << 4);
+            cp_async16_zfill(to, reinterpret_cast<const char *>(kv.k) + at, n);
+            cp_async16_zfill(to + PD_TILE, reinterpret_cast<const char *>(kv.v) + at, n);
+        }
+    };
+
+    float m = NO_MAX, l = 0.f;
+    float acc[LPR][2];  // elements 8 t + e0 + {0, 1} of the head's output
+#pragma unroll
+    for (int t = 0; t < LPR; t++) acc[t][0] = acc[t][1] = 0.f;
+
+    int t_fill = warp, stage = 0;
+#pragma unroll
+    for (int s = 0; s < PD_STAGES - 1; s++) {
+        if (t_fill < ntile) fill(s, lookup(t_fill));
+        cp_async_commit();
+        t_fill += PD_WARPS;
+    }
+    long long off_next = lookup(t_fill);
+    const int lr = lane & 7, lm = lane >> 3;  // row and matrix this lane addresses
+    for (int t = warp; t < ntile; t += PD_WARPS) {
+        cp_async_wait<PD_STAGES - 2>();
+        __syncwarp();
+        {
+            const int to = stage == 0 ? PD_STAGES - 1 : stage - 1;
+            if (t_fill < ntile) fill(to, off_next);
+            cp_async_commit();
+            t_fill += PD_WARPS;
+            off_next = lookup(t_fill);
+        }
+        const unsigned kt = ring + stage * (2 * PD_TILE), vt = kt + PD_TILE;
+        const unsigned valid = s_valid[warp][stage];
+        float x[TK / 8][2];
+        bool move = false;
+#pragma unroll
+        for (int n = 0; n < TK / 8; n++) {  // eight keys
+            float s01[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k2 = 0; k2 < KS / 2; k2++) {
+                unsigned kb[4];
+                ldsm4(kt + (n * 8 + lr) * ROW + (((k2 * 4 + lm) ^ lr) << 4), kb);
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const unsigned(&q)[2][NQ] = qa[k2 * 2 + i];
+                    mma16816<TYPE>(s01, q[0][0], q[0][1], q[1][0], q[1][1], kb[2 * i], kb[2 * i + 1]);
+                    if constexpr (NQ == 3) mma16816<TYPE>(s2, q[0][2], 0u, q[1][2], 0u, kb[2 * i], kb[2 * i + 1]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                float s = __fadd_rn(s01[i], s01[2 + i]);
+                if constexpr (NQ == 3) s = __fadd_rn(s, s2[i]);
+                x[n][i] = (valid >> (n * 8 + e0 + i)) & 1u ? __fmul_rn(s, sl2) : -INFINITY;
+                move = move || x[n][i] > m + PD_RESCALE;
+            }
+        }
+        if (__any_sync(0xffffffffu, move)) {
+            float top = x[0][0];
+#pragma unroll
+            for (int n = 0; n < TK / 8; n++) top = fmaxf(top, fmaxf(x[n][0], x[n][1]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            top = fmaxf(top, m);
+            const float f = exp2_approx(__fsub_rn(m, top));
+            m = top;
+            l = __fmul_rn(l, f);
+#pragma unroll
+            for (int d = 0; d < LPR; d++) acc[d][0] = __fmul_rn(acc[d][0], f), acc[d][1] = __fmul_rn(acc[d][1], f);
+        }
+        unsigned w[TK / 8][NQ];
+#pragma unroll
+        for (int n = 0; n < TK / 8; n++) {
+            const float w0 = exp2_approx(__fsub_rn(x[n][0], m)), w1 = exp2_approx(__fsub_rn(x[n][1], m));
+            l = __fadd_rn(l, __fadd_rn(w0, w1));
+            split2_weights<TYPE, NQ>(w0, w1, w[n]);
+        }
+#pragma unroll
+        for (int d2 = 0; d2 < LPR / 2; d2++) {  // sixteen elements
+            float o0[4] = {0.f, 0.f, 0.f, 0.f}, o1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int u = 0; u < TK / 16; u++) {
+                unsigned vb[4];
+                ldsm4_t(vt + (u * 16 + (lm & 1) * 8 + lr) * ROW + (((d2 * 2 + (lm >> 1)) ^ lr) << 4), vb);
+                if constexpr (NQ == 3) {
+                    mma16816<TYPE>(o0, w[2 * u][2], 0u, w[2 * u + 1][2], 0u, vb[0], vb[1]);
+                    mma16816<TYPE>(o1, w[2 * u][2], 0u, w[2 * u + 1][2], 0u, vb[2], vb[3]);
+                }
+                mma16816<TYPE>(o0, w[2 * u][0], w[2 * u][1], w[2 * u + 1][0], w[2 * u + 1][1], vb[0], vb[1]);
+                mma16816<TYPE>(o1, w[2 * u][0], w[2 * u][1], w[2 * u + 1][0], w[2 * u + 1][1], vb[2], vb[3]);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                acc[2 * d2][i] = __fadd_rn(acc[2 * d2][i], __fadd_rn(o0[i], o0[2 + i]));
+                acc[2 * d2 + 1][i] = __fadd_rn(acc[2 * d2 + 1][i], __fadd_rn(o1[i], o1[2 + i]));
+            }
+        }
+        __syncwarp();  // the stage is filled again at the next turn
+        stage = stage == PD_STAGES - 1 ? 0 : stage + 1;
+    }
+    cp_async_wait<0>();
+    __syncthreads();  // every ring is free: the warps' results go there
+
+    float *s_o = reinterpret_cast<float *>(pd_smem);  // [warp][head][hd]
+    l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, 1));
+    l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, 2));
+    if ((lane & 3) == 0) s_m[warp][g] = m, s_l[warp][g] = l;
+#pragma unroll
+    for (int d = 0; d < LPR; d++)
+        if (d * 8 < kv.hd) {
+            s_o[(warp * G + g) * kv.hd + d * 8 + e0] = acc[d][0];
+            s_o[(warp * G + g) * kv.hd + d * 8 + e0 + 1] = acc[d][1];
+        }
+    bool finite = fabsf(l) < INFINITY;
+#pragma unroll
+    for (int d = 0; d < LPR; d++) finite = finite && fabsf(acc[d][0]) < INFINITY && fabsf(acc[d][1]) < INFINITY;
+    if (__syncthreads_or(!finite && g < work.ng)) {
+        // warp 0's place gets each head's whole result, the others' nothing
+        for (int h = warp; h < work.ng; h += PD_WARPS) {
+            const RowState st = attend_row<TYPE>(kv, b, seq, head, a.q + (size_t)seq * a.ldq + (size_t)(work.h0 + h) * kv.hd,
+                                                 __fmul_rn(a.scale, 1.44269504088896340736f), keys, lo, hi, 0, 0, 0x7fffffff);
+            for (int i = 0; i < PD_WARPS; i++) {
+#pragma unroll
+                for (int c4 = 0; c4 < 4; c4++)
+                    if (lane + 32 * c4 < kv.hd) s_o[(i * G + h) * kv.hd + lane + 32 * c4] = i == 0 ? st.acc[c4] : 0.f;
+                if (lane == 0) s_m[i][h] = i == 0 ? st.m : NO_MAX, s_l[i][h] = i == 0 ? st.l : 0.f;
+            }
+        }
+        __syncthreads();
+    }
+    decode_store<G>(kv, a, plan, work, s_o, s_m, s_l);
 }
 
 // Joins the splits of one (row, query head): warp w takes splits w, w + 4, ..
@@ -318,7 +549,7 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(KvView kv, Ba
     const float2 *ml = part_ml + item * splits;
     const float *po = part_o + item * splits * (uint64_t)kv.hd + 4 * lane;
     const bool mine = 4 * lane < kv.hd;
-    float top = PD_NO_MAX;
+    float top = NO_MAX;
     for (int s = lane; s < live; s += 32) top = fmaxf(top, ml[s].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -330,7 +561,7 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(KvView kv, Ba
 #pragma unroll
         for (int u = 0; u < 4; u++) {
             const int s = s0 + u * PJ_WARPS;
-            x[u] = s < live ? ml[s] : make_float2(PD_NO_MAX, 0.f);
+            x[u] = s < live ? ml[s] : make_float2(NO_MAX, 0.f);
             v[u] = s < live && mine ? *reinterpret_cast<const float4 *>(po + (size_t)s * kv.hd) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
 #pragma unroll
@@ -357,44 +588,32 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(KvView kv, Ba
 
 constexpr size_t PD_SMEM = (size_t)PD_WARPS * PD_STAGES * 2 * PD_TILE;
 
-template <int TYPE, int LPR, int G>
-void go(const KvView &kv, const BatchView &b, const PagedAttnView &a, const DecodePlan &plan, cudaStream_t s) {
+template <typename K>
+void go(K *kernel, SmemOptIn &opt, const KvView &kv, const BatchView &b, const PagedAttnView &a, const DecodePlan &plan,
+        cudaStream_t s) {
     const unsigned grid = (unsigned)((uint64_t)b.num_seqs * kv.kv_heads * plan.head_groups * plan.splits);
+    opt(kernel, (int)PD_SMEM);
+    launch_kernel(kernel, dim3(grid), dim3(PD_THREADS), PD_SMEM, s, false, kv, b, a, plan);
+}
+template <int TYPE, int LPR>
+void go_mma(const KvView &kv, const BatchView &b, const PagedAttnView &a, const DecodePlan &plan, cudaStream_t s) {
     static SmemOptIn opt;
-    opt(paged_decode_kernel<TYPE, LPR, G>, (int)PD_SMEM);
-    launch_kernel(paged_decode_kernel<TYPE, LPR, G>, dim3(grid), dim3(PD_THREADS), PD_SMEM, s, false, kv, b, a, plan);
+    go(paged_decode_mma_kernel<TYPE, LPR>, opt, kv, b, a, plan, s);
 }
-
-template <typename F>
-void for_heads(int g, F f) {
-    switch (g) {
-        case 1: f(std::integral_constant<int, 1>{}); break;
-        case 2: f(std::integral_constant<int, 2>{}); break;
-        case 3: f(std::integral_constant<int, 3>{}); break;
-        case 4: f(std::integral_constant<int, 4>{}); break;
-        case 6: f(std::integral_constant<int, 6>{}); break;
-        default: f(std::integral_constant<int, 8>{}); break;
-    }
+template <int LPR, int G>
+void go_fma(const KvView &kv, const BatchView &b, const PagedAttnView &a, const DecodePlan &plan, cudaStream_t s) {
+    static SmemOptIn opt;
+    go(paged_decode_kernel<LPR, G>, opt, kv, b, a, plan, s);
 }
-
-// f(type, lanes per row): rows of up to 64 or up to 128 elements
-template <typename F>
-void for_rows(int type, int hd, F f) {
-    if (type == KV_F32) {
-        if (hd <= 64)
-            f(std::integral_constant<int, KV_F32>{}, std::integral_constant<int, 16>{});
-        else
-            f(std::integral_constant<int, KV_F32>{}, std::integral_constant<int, 32>{});
-    } else if (type == KV_F16) {
-        if (hd <= 64)
-            f(std::integral_constant<int, KV_F16>{}, std::integral_constant<int, 8>{});
-        else
-            f(std::integral_constant<int, KV_F16>{}, std::integral_constant<int, 16>{});
-    } else {
-        if (hd <= 64)
-            f(std::integral_constant<int, KV_BF16>{}, std::integral_constant<int, 8>{});
-        else
-            f(std::integral_constant<int, KV_BF16>{}, std::integral_constant<int, 16>{});
+template <int LPR>
+void go_heads(const KvView &kv, const BatchView &b, const PagedAttnView &a, const DecodePlan &plan, cudaStream_t s) {
+    switch (plan.heads) {
+        case 1: go_fma<LPR, 1>(kv, b, a, plan, s); break;
+        case 2: go_fma<LPR, 2>(kv, b, a, plan, s); break;
+        case 3: go_fma<LPR, 3>(kv, b, a, plan, s); break;
+        case 4: go_fma<LPR, 4>(kv, b, a, plan, s); break;
+        case 6: go_fma<LPR, 6>(kv, b, a, plan, s); break;
+        default: go_fma<LPR, 8>(kv, b, a, plan, s); break;
     }
 }
 
@@ -406,7 +625,7 @@ DecodePlan plan_paged_decode(const KvView &kv, const BatchView &b, const PagedAt
     // query heads of a KV head in one CTA: up to 8 share each key they read
     p.head_groups = (group + 7) / 8;
     const int g = (group + p.head_groups - 1) / p.head_groups;
-    p.heads = g == 5 ? 6 : g == 7 ? 8 : g;
+    p.heads = kv.type != KV_F32 ? 8 : g == 5 ? 6 : g == 7 ? 8 : g;
     p.head_groups = (group + p.heads - 1) / p.heads;
     uint64_t most = max_kv_len;
     if (a.window) most = std::min<uint64_t>(most, (uint64_t)a.window + a.sinks);
@@ -419,7 +638,7 @@ DecodePlan plan_paged_decode(const KvView &kv, const BatchView &b, const PagedAt
     // splits, 50 us (1: 54, 4: 54); one sequence of 8192, 8 units: 24 to 37
     // alike; 64 ragged to 8192, 512 units: 6, 218 us (8: 216, 4: 224, 1: 315);
     // 128 windows of 1028, 1024 units: 1, 121 us (2: 126).
-    const uint64_t slots = 148 * (uint64_t)ctas_per_sm(p.heads);
+    const uint64_t slots = 148 * (uint64_t)(kv.type == KV_F32 ? ctas_per_sm(p.heads) : 3);
     const uint64_t key_bytes = 2ull * kv.hd * (kv.type == KV_F32 ? 4 : 2);
     uint64_t best = UINT64_MAX;
     for (uint64_t s = 1; s <= 64; s++) {
@@ -440,9 +659,12 @@ DecodePlan plan_paged_decode(const KvView &kv, const BatchView &b, const PagedAt
 
 void launch_paged_decode(const KvView &kv, const BatchView &b, const PagedAttnView &a, const DecodePlan &plan,
                          cudaStream_t s) {
-    for_rows(kv.type, kv.hd, [&](auto type, auto lpr) {
-        for_heads(plan.heads, [&](auto g) { go<decltype(type)::value, decltype(lpr)::value, decltype(g)::value>(kv, b, a, plan, s); });
-    });
+    if (kv.type == KV_F32)
+        kv.hd <= 64 ? go_heads<16>(kv, b, a, plan, s) : go_heads<32>(kv, b, a, plan, s);
+    else if (kv.type == KV_F16)
+        kv.hd <= 64 ? go_mma<KV_F16, 8>(kv, b, a, plan, s) : go_mma<KV_F16, 16>(kv, b, a, plan, s);
+    else
+        kv.hd <= 64 ? go_mma<KV_BF16, 8>(kv, b, a, plan, s) : go_mma<KV_BF16, 16>(kv, b, a, plan, s);
     if (plan.splits > 1) launch_paged_join(kv, b, a, plan.part_ml, plan.part_o, plan.chunk, plan.splits, s);
 }
 

@@ -35,7 +35,6 @@ namespace {
 
 constexpr int PR_THREADS = 384;
 constexpr int PR_PRODUCERS = 96;
-constexpr float PR_NO_MAX = -3.0e38f;
 constexpr float PR_RESCALE = 8.0f;
 constexpr unsigned PR_TMEM_COLS = 512;
 
@@ -185,105 +184,6 @@ __device__ __forceinline__ bool pr_wait(uint64_t *bar, unsigned parity, RowsShar
 __device__ __forceinline__ void warp_arrive(uint64_t *bar) {
     __syncwarp();
     if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
-}
-
-// Two f32 values as the packed 16-bit parts of an operand.  (The second part
-// of an infinity is NaN: rows that meet it come out NaN and are redone.)
-template <int TYPE, int N>
-__device__ __forceinline__ void split2(float a, float b, unsigned (&part)[N]) {
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        float ra, rb;
-        if constexpr (TYPE == KV_F16) {
-            const __half2 h = __floats2half2_rn(a, b);
-            part[i] = *reinterpret_cast<const unsigned *>(&h);
-            const float2 f = __half22float2(h);
-            ra = f.x, rb = f.y;
-        } else {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-            part[i] = *reinterpret_cast<const unsigned *>(&h);
-            ra = __uint_as_float(part[i] << 16), rb = __uint_as_float(part[i] & 0xffff0000u);
-        }
-        if (i + 1 < N) {
-            a = __fsub_rn(a, ra);
-            b = __fsub_rn(b, rb);
-        }
-    }
-}
-// The same of two softmax weights (finite, or NaN: then the row is redone).
-template <int TYPE, int N>
-__device__ __forceinline__ void split2_weights(float a, float b, unsigned (&part)[N]) {
-    if constexpr (TYPE == KV_F16) {
-        const __half2 h = __floats2half2_rn(a, b);
-        const float2 f = __half22float2(h);
-        const __half2 r = __floats2half2_rn(__fsub_rn(a, f.x), __fsub_rn(b, f.y));
-        part[0] = *reinterpret_cast<const unsigned *>(&h);
-        part[1] = *reinterpret_cast<const unsigned *>(&r);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) {  // cut, not rounded: 8 bits each
-            const unsigned ua = __float_as_uint(a), ub = __float_as_uint(b);
-            part[i] = __byte_perm(ua, ub, 0x7632);
-            if (i + 1 < N) {
-                a = __fsub_rn(a, __uint_as_float(ua & 0xffff0000u));
-                b = __fsub_rn(b, __uint_as_float(ub & 0xffff0000u));
-            }
-        }
-    }
-}
-
-// One row's keys [lo, hi) of the CTA's list on the CUDA cores, a warp per row:
-// 32 keys at a time, a key per lane for the scores, head_dim over the lanes
-// for the values.  Rows that met a value that is not finite are redone so:
-// on the tensor cores 0 x NaN of a key that a row does not see would reach it.
-struct RowState {
-    float m, l, acc[4];
-};
-template <int TYPE>
-__device__ __noinline__ RowState attend_row(const KvView &kv, const BatchView &b, int seq, int head, const float *q,
-                                            float sl2, SeenKeys keys, int lo, int hi, int from, int sink_end, int to) {
-    using T = typename KvElem<TYPE>::T;
-    const int lane = threadIdx.x & 31, hd = kv.hd;
-    RowState r;
-    r.m = PR_NO_MAX;
-    r.l = 0.f;
-#pragma unroll
-    for (int c = 0; c < 4; c++) r.acc[c] = 0.f;
-    if (hi > to) hi = to;
-    for (int i0 = lo; i0 < hi; i0 += 32) {
-        const int i = i0 + lane;
-        long long off = -1;
-        if (i < hi && (i < sink_end || i >= from)) off = key_offset(kv, b, seq, (unsigned)keys.key(i), head);
-        float x = -INFINITY;
-        if (off >= 0) {
-            const T *k = reinterpret_cast<const T *>(kv.k) + off;
-            float dot = 0.f;
-            for (int d = 0; d < hd; d++) dot = __fmaf_rn(q[d], KvElem<TYPE>::get(k + d), dot);
-            x = __fmul_rn(dot, sl2);
-        }
-        float top = x;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        top = fmaxf(top, r.m);
-        const float f = exp2_approx(__fsub_rn(r.m, top)), w = exp2_approx(__fsub_rn(x, top));
-        r.m = top;
-        float total = w;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) total = __fadd_rn(total, __shfl_xor_sync(0xffffffffu, total, o));
-        r.l = __fmaf_rn(r.l, f, total);
-#pragma unroll
-        for (int c = 0; c < 4; c++) r.acc[c] = __fmul_rn(r.acc[c], f);
-        for (int j = 0; j < 32; j++) {
-            const long long o = __shfl_sync(0xffffffffu, off, j);
-            const float wj = __shfl_sync(0xffffffffu, w, j);
-            if (o < 0) continue;
-            const T *v = reinterpret_cast<const T *>(kv.v) + o;
-#pragma unroll
-            for (int c = 0; c < 4; c++)
-                if (lane + 32 * c < hd) r.acc[c] = __fmaf_rn(wj, KvElem<TYPE>::get(v + lane + 32 * c), r.acc[c]);
-        }
-    }
-    return r;
 }
 
 template <int TYPE, int HDP>
@@ -475,7 +375,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
         if (a.window != 0 && pos >= 0 && (unsigned)pos >= a.window) from = pos - (int)a.window + 1 - keys.low + keys.sinks;
         const float sl2 = Cfg::F16 ? __fmul_rn(sl2_all, sh->row[0][r]) : sl2_all;
         const unsigned t_lane = taddr + ((unsigned)((warp & 3) * 32) << 16);
-        float m = PR_NO_MAX, l = 0.f;
+        float m = NO_MAX, l = 0.f;
         float acc[OC];
 #pragma unroll
         for (int i = 0; i < OC; i++) acc[i] = 0.f;

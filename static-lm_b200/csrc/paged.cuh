@@ -16,6 +16,8 @@ constexpr int PAGED_BAD_PAGE = 1;      // a page id at or past num_pages, or non
 constexpr int PAGED_BAD_POSITION = 2;  // a position past the page table or the rope table
 constexpr int PAGED_WAIT_GAVE_UP = 4;  // a bounded device wait gave up
 
+constexpr float NO_MAX = -3.0e38f;  // a running maximum before any key: below every finite score
+
 struct KvView {
     void *k, *v;
     uint64_t page_stride;  // elements
@@ -127,6 +129,52 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// ---- f32 values as sums of 16-bit parts
+// Two f32 values as the packed 16-bit parts of an operand.  (The second part
+// of an infinity is NaN: rows that meet it come out NaN and are redone.)
+template <int TYPE, int N>
+__device__ __forceinline__ void split2(float a, float b, unsigned (&part)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        float ra, rb;
+        if constexpr (TYPE == KV_F16) {
+            const __half2 h = __floats2half2_rn(a, b);
+            part[i] = *reinterpret_cast<const unsigned *>(&h);
+            const float2 f = __half22float2(h);
+            ra = f.x, rb = f.y;
+        } else {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+            part[i] = *reinterpret_cast<const unsigned *>(&h);
+            ra = __uint_as_float(part[i] << 16), rb = __uint_as_float(part[i] & 0xffff0000u);
+        }
+        if (i + 1 < N) {
+            a = __fsub_rn(a, ra);
+            b = __fsub_rn(b, rb);
+        }
+    }
+}
+// The same of two softmax weights (finite, or NaN: then the row is redone).
+template <int TYPE, int N>
+__device__ __forceinline__ void split2_weights(float a, float b, unsigned (&part)[N]) {
+    if constexpr (TYPE == KV_F16) {
+        const __half2 h = __floats2half2_rn(a, b);
+        const float2 f = __half22float2(h);
+        const __half2 r = __floats2half2_rn(__fsub_rn(a, f.x), __fsub_rn(b, f.y));
+        part[0] = *reinterpret_cast<const unsigned *>(&h);
+        part[1] = *reinterpret_cast<const unsigned *>(&r);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) {  // cut, not rounded: 8 bits each
+            const unsigned ua = __float_as_uint(a), ub = __float_as_uint(b);
+            part[i] = __byte_perm(ua, ub, 0x7632);
+            if (i + 1 < N) {
+                a = __fsub_rn(a, __uint_as_float(ua & 0xffff0000u));
+                b = __fsub_rn(b, __uint_as_float(ub & 0xffff0000u));
+            }
+        }
+    }
+}
+
 // Four values to / from a page's element type.
 template <int TYPE>
 struct KvElem;
@@ -159,5 +207,61 @@ struct KvElem<KV_BF16> {
     }
     static __device__ __forceinline__ float get(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
 };
+
+// One row and query head over the keys [lo, hi) of a list, of which it sees
+// those below sink_end and those in [from, to), on the CUDA cores by one warp:
+// 32 keys at a time, a key per lane for the scores, head_dim over the lanes
+// for the values.  The tensor-core kernels redo so what came out not finite:
+// 0 x NaN of a key in the tile that a row does not see reaches it there, and
+// the parts of an infinity are not its parts.
+struct RowState {
+    float m, l, acc[4];
+};
+template <int TYPE>
+__device__ __noinline__ RowState attend_row(const KvView &kv, const BatchView &b, int seq, int head, const float *q,
+                                            float sl2, SeenKeys keys, int lo, int hi, int from, int sink_end, int to) {
+    using T = typename KvElem<TYPE>::T;
+    const int lane = threadIdx.x & 31, hd = kv.hd;
+    RowState r;
+    r.m = NO_MAX;
+    r.l = 0.f;
+#pragma unroll
+    for (int c = 0; c < 4; c++) r.acc[c] = 0.f;
+    if (hi > to) hi = to;
+    for (int i0 = lo; i0 < hi; i0 += 32) {
+        const int i = i0 + lane;
+        long long off = -1;
+        if (i < hi && (i < sink_end || i >= from)) off = key_offset(kv, b, seq, (unsigned)keys.key(i), head);
+        float x = -INFINITY;
+        if (off >= 0) {
+            const T *k = reinterpret_cast<const T *>(kv.k) + off;
+            float dot = 0.f;
+            for (int d = 0; d < hd; d++) dot = __fmaf_rn(q[d], KvElem<TYPE>::get(k + d), dot);
+            x = __fmul_rn(dot, sl2);
+        }
+        float top = x;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        top = fmaxf(top, r.m);
+        const float f = exp2_approx(__fsub_rn(r.m, top)), w = exp2_approx(__fsub_rn(x, top));
+        r.m = top;
+        float total = w;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) total = __fadd_rn(total, __shfl_xor_sync(0xffffffffu, total, o));
+        r.l = __fmaf_rn(r.l, f, total);
+#pragma unroll
+        for (int c = 0; c < 4; c++) r.acc[c] = __fmul_rn(r.acc[c], f);
+        for (int j = 0; j < 32; j++) {
+            const long long o = __shfl_sync(0xffffffffu, off, j);
+            const float wj = __shfl_sync(0xffffffffu, w, j);
+            if (o < 0) continue;
+            const T *v = reinterpret_cast<const T *>(kv.v) + o;
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                if (lane + 32 * c < hd) r.acc[c] = __fmaf_rn(wj, KvElem<TYPE>::get(v + lane + 32 * c), r.acc[c]);
+        }
+    }
+    return r;
+}
 
 }  // namespace slm

@@ -505,6 +505,33 @@ def test_nan_in_a_seen_slot_reaches_its_rows(cuda):
         assert got[1].isnan().all() and got[0].isfinite().all()
 
 
+@pytest.mark.parametrize("kv", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_what_is_not_finite_reaches_the_rows_that_see_it_and_no_others(cuda, kv, hd, bad):
+    """In the middle of a tile, for keys and for values, with rows before it, in
+    its window and past its window."""
+    c = Cache(cuda, kv, [90, 30], 2, hd, 16, seed=23)
+    c.view(c.v)[int(c.table[0, 40 // 16]), 1, 40 % 16, 5] = bad
+    c.view(c.k)[int(c.table[1, 20 // 16]), 0, 20 % 16] = float("nan")
+    q = queries(cuda, 120, 4, hd, 7)
+    got = attend(cuda, c, q, 4, [90, 30], window=20, sinks=2).double().cpu().numpy().reshape(120, 4, hd)
+    with np.errstate(all="ignore"):
+        want = reference(c, q, [90, 30], 4, window=20, sinks=2).reshape(120, 4, hd)
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(np.isinf(got), np.isinf(want))
+    fine = np.isfinite(want)
+    assert fine.mean() > 0.9 and (~fine).any()
+    assert np.abs(got[fine] - want[fine]).max() <= MAX_TOL * np.abs(want[fine]).max()
+    assert np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
+    # one new row each
+    got = attend(cuda, c, q[:2], 4).double().cpu().numpy().reshape(2, 4, hd)
+    with np.errstate(all="ignore"):
+        want = reference(c, q[:2], [1, 1], 4).reshape(2, 4, hd)
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
+    fine = np.isfinite(want)
+    assert np.abs(got[fine] - want[fine]).max() <= MAX_TOL * np.abs(want[fine]).max()
+
+
 def test_offsets_past_32_bits(cuda):
     """Pages further apart than 2^31 elements."""
     stride = (1 << 31) // 2 + 2 * 16 * 64
