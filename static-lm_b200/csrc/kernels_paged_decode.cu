@@ -631,22 +631,27 @@ DecodePlan plan_paged_decode(const KvView &kv, const BatchView &b, const PagedAt
     if (a.window) most = std::min<uint64_t>(most, (uint64_t)a.window + a.sinks);
     most = std::max<uint64_t>(most, 1);
     const uint64_t units = std::max<uint64_t>((uint64_t)b.num_seqs * kv.kv_heads * p.head_groups, 1);
-    // A CTA costs its keys' bytes and about 150 KB more (its first look-ups and
-    // copies, its warps' join); the CTAs run in waves over the SMs; the second
-    // launch costs about 75 KB.  Of 1 to 64 splits the cheapest by that count.
-    // Measured (best of a sweep in brackets): 64 x 2049 f32, 192 units: 2
-    // splits, 50 us (1: 54, 4: 54); one sequence of 8192, 8 units: 24 to 37
-    // alike; 64 ragged to 8192, 512 units: 6, 218 us (8: 216, 4: 224, 1: 315);
-    // 128 windows of 1028, 1024 units: 1, 121 us (2: 126).
-    const uint64_t slots = 148 * (uint64_t)(kv.type == KV_F32 ? ctas_per_sm(p.heads) : 3);
+    // Of 1 to 64 splits the cheapest by this count, in bytes of an SM's share of
+    // the memory's rate: the keys of the SM with the most CTAs, a start and an
+    // end per wave of CTAs (about 5 us), and the join's launch (about 4 us).
+    // Where two are within 3 % the fewer splits win.  Measured, with cold
+    // pages: 64 x 2049 f32, 192 units: 1, 2, 3, 4 splits 54, 50, 59, 54 us; one
+    // sequence of 8192 f16, 8 units: 8, 16, 24, 32, 48 splits 28, 21.5, 23.5,
+    // 21.5, 23.6 us; 64 sequences of 500 to 8192 bf16, 512 units: 1, 2, 4, 8, 12
+    // splits 289, 257, 226, 228, 241 us; 128 windows of 1028 keys f16, 1024
+    // units: 1, 2, 3 splits 115, 120, 124 us.
+    constexpr uint64_t SMS = 148, WAVE = 215 << 10, JOIN = 170 << 10;
+    const uint64_t slots = SMS * (uint64_t)(kv.type == KV_F32 ? ctas_per_sm(p.heads) : 3);
     const uint64_t key_bytes = 2ull * kv.hd * (kv.type == KV_F32 ? 4 : 2);
     uint64_t best = UINT64_MAX;
-    for (uint64_t s = 1; s <= 64; s++) {
-        uint64_t chunk = ((most + s - 1) / s + 15) / 16 * 16;
-        if (s > 1 && chunk < 64) break;
-        const uint64_t waves = (units * s + slots - 1) / slots;
-        const uint64_t cost = waves * (chunk * key_bytes + (150 << 10)) + (s > 1 ? 75 << 10 : 0);
-        if (cost >= best) continue;
+    // lengths below the bound may be unlike: with at most 1 MB a CTA the last end together
+    const uint64_t fewest = std::min<uint64_t>(64, std::max<uint64_t>(1, (most * key_bytes) >> 20));
+    for (uint64_t s = fewest; s <= 64; s++) {
+        const uint64_t chunk = ((most + s - 1) / s + 15) / 16 * 16;
+        if (s > fewest && chunk < 64) break;
+        const uint64_t ctas = units * s, waves = (ctas + slots - 1) / slots, deep = (ctas + SMS - 1) / SMS;
+        const uint64_t cost = deep * chunk * key_bytes + waves * WAVE + (s > 1 ? JOIN : 0);
+        if (best != UINT64_MAX && cost + cost / 32 >= best) continue;
         best = cost;
         p.chunk = (int)std::min<uint64_t>(chunk, INT32_MAX);
         p.splits = (int)((most + chunk - 1) / chunk);
