@@ -346,8 +346,9 @@ int slm_paged_append(const slm_kv_pages *pages, const slm_paged_batch *batch,
  * it.  Sums and the softmax are f32.  out is apart from q.
  * `scratch` holds slm_paged_attention_scratch_bytes bytes, 16-byte aligned,
  * contents of no account before and after; calls that may overlap on the GPU
- * need scratches of their own.  Rows far outnumbering sequences (prompts) and
- * single new rows take different kernels; see slm_paged_batch.row_start. */
+ * need scratches of their own.  Sums are in an order that does not change from
+ * call to call.  A batch of single new rows is best given with row_start NULL:
+ * it then takes kernels made for one row per sequence. */
 typedef struct {
     const float *q;
     float *out;

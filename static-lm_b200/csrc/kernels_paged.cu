@@ -26,16 +26,24 @@ __device__ __forceinline__ void load4(const float *p, bool vec, float (&x)[4]) {
 // with (a, b) neighbours, or the two halves of the first rotary_dim elements.
 // Every product and sum is rounded on its own, so that the rotation gives the
 // bits of slm_apply_rope_cached.
+//
+// Bound by memory: 8 bytes in and out per query element, 4 + the page's type
+// per key and value element.  A thread's loads, its row's place (a search in
+// row_start, the length, the page id) and the two table rows are a chain of
+// latencies, so the registers are held to 32 for 64 warps an SM (40 registers:
+// 53.3 us, 32: 51.2 us for 8 x 4096 rows of 9 + 3 + 3 heads of 64, f16 pages,
+// cold: 4.6 TB/s of the 6.5 a copy reaches; single rows are a launch, 7 us
+// with the call).
 template <int TYPE, int LPV>
-__global__ void __launch_bounds__(AP_THREADS) paged_append_kernel(KvView kv, BatchView b, AppendView a) {
+__global__ void __launch_bounds__(AP_THREADS, 8) paged_append_kernel(KvView kv, BatchView b, AppendView a) {
     using T = typename KvElem<TYPE>::T;
     const int l = threadIdx.x % LPV, hd = kv.hd;
     const int per_row = a.num_heads + 2 * kv.kv_heads;
-    const uint64_t item = (uint64_t)blockIdx.x * (AP_THREADS / LPV) + threadIdx.x / LPV;
-    const uint64_t row64 = item / (unsigned)per_row;
-    const bool live = row64 < (uint64_t)b.num_rows && l * 8 < hd;
-    const int row = live ? (int)row64 : 0;
-    const int vec = live ? (int)(item - row64 * (unsigned)per_row) : 0;
+    const unsigned item = blockIdx.x * (AP_THREADS / LPV) + threadIdx.x / LPV;  // below 2^32: the host's check
+    const unsigned its_row = item / (unsigned)per_row;
+    const bool live = its_row < (unsigned)b.num_rows && l * 8 < hd;
+    const int row = live ? (int)its_row : 0;
+    const int vec = live ? (int)(item - its_row * (unsigned)per_row) : 0;
     // kind 0 = query head, 1 = key head, 2 = value head
     const int kind = vec < a.num_heads ? 0 : vec < a.num_heads + kv.kv_heads ? 1 : 2;
     const int head = kind == 0 ? vec : kind == 1 ? vec - a.num_heads : vec - a.num_heads - kv.kv_heads;

@@ -49,7 +49,8 @@ __device__ __forceinline__ bool decode_work(const KvView &kv, const BatchView &b
     w.ng = group - g0 < plan.heads ? group - g0 : plan.heads;
     w.h0 = w.head * group + g0;
     const int pos = b.kv_len[w.seq] - 1;
-    w.keys = seen_keys(pos, pos, a.window, a.sinks);
+    w.keys = seen_keys(b, pos, pos, a.window, a.sinks);
+    if (pos >= b.cap && threadIdx.x == 0) paged_flag(kv, PAGED_BAD_POSITION);
     w.lo = w.split * plan.chunk;
     if (w.split > 0 && w.lo >= w.keys.n) return false;  // the join knows
     w.hi = w.split == plan.splits - 1 || w.lo + plan.chunk > w.keys.n ? w.keys.n : w.lo + plan.chunk;
@@ -539,7 +540,7 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(KvView kv, Ba
     int live = splits;
     if (chunk > 0) {
         const int pos = b.kv_len[row] - 1;  // not written by the kernel waited for
-        const SeenKeys keys = seen_keys(pos, pos, a.window, a.sinks);
+        const SeenKeys keys = seen_keys(b, pos, pos, a.window, a.sinks);
         live = (keys.n + chunk - 1) / chunk;
         live = live < 1 ? 1 : live > splits ? splits : live;
     } else if (row >= b.row_start[b.num_seqs]) {

@@ -273,7 +273,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
     const int tok0 = (int)(flat0 / (unsigned)group);
     int tok1 = (int)((flat0 + 127u) / (unsigned)group);
     tok1 = tok1 < rows ? tok1 : rows - 1;
-    const SeenKeys keys = seen_keys(pos0 + tok0, pos0 + tok1, a.window, a.sinks);
+    const SeenKeys keys = seen_keys(b, pos0 + tok0, pos0 + tok1, a.window, a.sinks);
+    if (pos0 + tok1 >= b.cap && tid == 0) paged_flag(kv, PAGED_BAD_POSITION);
     const int all_tiles = (keys.n + KT - 1) / KT;
     const int per_split = (all_tiles + plan.splits - 1) / plan.splits;
     const int lo = split * per_split * KT;

@@ -32,6 +32,7 @@ struct BatchView {
     const int32_t *kv_len, *table;
     unsigned table_stride;
     int num_seqs, num_rows;
+    int cap;  // positions a row of the page table covers
 };
 
 __device__ __forceinline__ void paged_flag(const KvView &kv, int bit) {
@@ -82,19 +83,20 @@ __device__ __forceinline__ long long key_offset(const KvView &kv, const BatchVie
                        ((uint64_t)head * (unsigned)kv.page_size + slot) * (unsigned)kv.hd);
 }
 
-// The keys a row at position p sees, as a list of n_seen: key j of the list
-// is j below the sink count, and counts on from the window's first key after
-// it.  window 0 = every key up to p.
+// The keys that rows at positions first_pos..last_pos (the first may be
+// negative) see between them, as a list of n: the sinks, then from the first
+// row's window on (window 0: from the start) up to the last row.  Positions
+// past the page table are none.
 struct SeenKeys {
     int sinks, low, n;  // list index i -> i < sinks ? i : i - sinks + low
     __device__ __forceinline__ int key(int i) const { return i < sinks ? i : i - sinks + low; }
 };
-__device__ __forceinline__ SeenKeys seen_keys(int first_pos, int last_pos, unsigned window, unsigned sinks) {
-    // union over rows at first_pos..last_pos (first_pos may be negative)
+__device__ __forceinline__ SeenKeys seen_keys(const BatchView &b, int first_pos, int last_pos, unsigned window, unsigned sinks) {
     SeenKeys s;
-    const int end = last_pos + 1;
+    const int end = last_pos < b.cap ? last_pos + 1 : b.cap;
     s.low = 0;
     if (window != 0 && first_pos >= 0 && (unsigned)first_pos >= window) s.low = first_pos - (int)window + 1;
+    if (end > 0 && s.low > end) s.low = end;
     s.sinks = (unsigned)s.low < sinks ? s.low : (int)sinks;
     s.n = end > 0 ? s.sinks + end - s.low : 0;
     return s;

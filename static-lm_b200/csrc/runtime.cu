@@ -870,6 +870,7 @@ int check_batch(const slm_paged_batch *b, const KvView &kv, BatchView *v) {
     v->table_stride = b->table_stride;
     v->num_seqs = (int)b->num_seqs;
     v->num_rows = (int)b->num_rows;
+    v->cap = (int)(b->table_stride * (uint64_t)kv.page_size);
     return SLM_OK;
 }
 
@@ -938,6 +939,8 @@ SLM_EXPORT int slm_paged_append(const slm_kv_pages *pages, const slm_paged_batch
         return fail(SLM_ERR_INVALID_ARG, "null device pointer");
     if (args->num_heads && args->q_out == args->q && args->ldq_out != args->ldq)
         return fail(SLM_ERR_OVERLAP, "q_out is q with another row stride");
+    if ((uint64_t)b.num_rows * (args->num_heads + 2ull * kv.kv_heads) > (uint64_t)INT32_MAX)
+        return fail(SLM_ERR_SHAPE, "too many rows of heads");
     AppendView a{};
     a.q = args->q;
     a.k = args->k;
@@ -985,6 +988,9 @@ SLM_EXPORT int slm_paged_attention(const slm_kv_pages *pages, const slm_paged_ba
     if (a.q == a.out) return fail(SLM_ERR_OVERLAP, "out is q");
     if (!b.row_start) {
         DecodePlan plan = plan_paged_decode(kv, b, a, batch->max_kv_len);
+        if ((uint64_t)b.num_seqs * kv.kv_heads * plan.head_groups * plan.splits > (uint64_t)INT32_MAX ||
+            (uint64_t)b.num_rows * a.num_heads > (uint64_t)INT32_MAX)
+            return fail(SLM_ERR_SHAPE, "too many rows of query heads");
         TRY(check_scratch(scratch, scratch_bytes, plan.scratch_bytes));
         plan.part_ml = (float2 *)scratch;
         plan.part_o = (float *)((char *)scratch + plan.ml_bytes);
