@@ -19,6 +19,12 @@ __device__ __forceinline__ void load4(const float *p, bool vec, float (&x)[4]) {
     }
 }
 
+__device__ __forceinline__ void turn(float &p, float &q, float c, float s) {
+    const float t = __fsub_rn(__fmul_rn(p, c), __fmul_rn(q, s));
+    q = __fadd_rn(__fmul_rn(p, s), __fmul_rn(q, c));
+    p = t;
+}
+
 // LPV lanes (a power of two, 8 elements each) per head vector; the vectors of
 // a row are its query heads, its key heads, then its value heads.
 //   norm:  y = x * (1 / sqrt(sum(x^2) / head_dim + eps)) * w      (q and k)
@@ -27,120 +33,132 @@ __device__ __forceinline__ void load4(const float *p, bool vec, float (&x)[4]) {
 // Every product and sum is rounded on its own, so that the rotation gives the
 // bits of slm_apply_rope_cached.
 //
-// Bound by memory: 8 bytes in and out per query element, 4 + the page's type
-// per key and value element.  A thread's loads, its row's place (a search in
-// row_start, the length, the page id) and the two table rows are a chain of
-// latencies, so the registers are held to 32 for 64 warps an SM (40 registers:
-// 53.3 us, 32: 51.2 us for 8 x 4096 rows of 9 + 3 + 3 heads of 64, f16 pages,
-// cold: 4.6 TB/s of the 6.5 a copy reaches; single rows are a launch, 7 us
-// with the call).
+// A group of LPV lanes takes AP_VECS vectors of one row: what they share (the
+// row's place, found by a search in row_start, its page's offset, its row of
+// the rope tables) is worked out once for them, with all their loads in flight.
+// 8 bytes in and out per query element, 4 + the page's type per key and value
+// element are its bytes.  With a vector a group it was bound by instructions
+// (issue 77 % of the cycles, DRAM 49 %): 8 x 4096 rows of 9 + 3 + 3 heads of 64
+// into f16 pages, cold, 51.2 us; two vectors 47.1, three 45.1 (5.2 TB/s), four
+// (three CTAs an SM) 49.2.  Single rows are one launch's time.
+constexpr int AP_VECS = 3;
+
 template <int TYPE, int LPV>
-__global__ void __launch_bounds__(AP_THREADS, 8) paged_append_kernel(KvView kv, BatchView b, AppendView a) {
+__global__ void __launch_bounds__(AP_THREADS, 4) paged_append_kernel(KvView kv, BatchView b, AppendView a) {
     using T = typename KvElem<TYPE>::T;
     const int l = threadIdx.x % LPV, hd = kv.hd;
-    const int per_row = a.num_heads + 2 * kv.kv_heads;
+    const int per_row = a.num_heads + 2 * kv.kv_heads, parts = (per_row + AP_VECS - 1) / AP_VECS;
     const unsigned item = blockIdx.x * (AP_THREADS / LPV) + threadIdx.x / LPV;  // below 2^32: the host's check
-    const unsigned its_row = item / (unsigned)per_row;
+    const unsigned its_row = item / (unsigned)parts;
     const bool live = its_row < (unsigned)b.num_rows && l * 8 < hd;
     const int row = live ? (int)its_row : 0;
-    const int vec = live ? (int)(item - its_row * (unsigned)per_row) : 0;
-    // kind 0 = query head, 1 = key head, 2 = value head
-    const int kind = vec < a.num_heads ? 0 : vec < a.num_heads + kv.kv_heads ? 1 : 2;
-    const int head = kind == 0 ? vec : kind == 1 ? vec - a.num_heads : vec - a.num_heads - kv.kv_heads;
-    const float *src = kind == 0   ? a.q + (size_t)row * a.ldq
-                       : kind == 1 ? a.k + (size_t)row * a.ldk
-                                   : a.v + (size_t)row * a.ldv;
+    const int first = live ? (int)(item - its_row * (unsigned)parts) * AP_VECS : 0;
     const int rd = a.rotary_dim;
-    const bool turned = kind != 2 && 8 * l < rd;
-    const bool split = turned && a.halves;
+    const bool turns = 8 * l < rd;          // this lane's elements of q and k are rotated,
+    const bool split = turns && a.halves;   // as pairs half of rotary_dim apart
     const int i0 = split ? 4 * l : 8 * l, i1 = split ? rd / 2 + 4 * l : 8 * l + 4;
+    const float *const rq = a.q + (size_t)row * a.ldq, *const rk = a.k + (size_t)row * a.ldk,
+                *const rv = a.v + (size_t)row * a.ldv;
+    const int k0 = a.num_heads, v0 = a.num_heads + kv.kv_heads;  // the first key's and value's vector
 
-    float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-    if (live) {
-        load4(src + (size_t)head * hd + i0, a.vec, x);
-        load4(src + (size_t)head * hd + i1, a.vec, y);
+    float x[AP_VECS][4], y[AP_VECS][4];
+#pragma unroll
+    for (int n = 0; n < AP_VECS; n++) {
+        const int vec = first + n;
+        const float *src = vec < k0 ? rq + vec * hd : vec < v0 ? rk + (vec - k0) * hd : rv + (vec - v0) * hd;
+        if (live && vec < per_row) {
+            load4(src + i0, a.vec, x[n]);
+            load4(src + i1, a.vec, y[n]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[n][j] = y[n][j] = 0.f;
+        }
     }
     int seq = 0, pos = -1;
     if (live) row_place(b, row, seq, pos);
-
-    const float *w = kind == 0 ? a.q_norm : a.k_norm;
-    if (kind == 2) w = nullptr;
-    float ss = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; j++) ss = __fmaf_rn(x[j], x[j], __fmaf_rn(y[j], y[j], ss));
-#pragma unroll
-    for (int o = LPV / 2; o > 0; o >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, o));
-    if (!live) return;
-    if (w) {
-        const float r = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)hd), a.eps)));
-        float wx[4], wy[4];
-        load4(w + i0, a.vec, wx);
-        load4(w + i1, a.vec, wy);
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            x[j] = __fmul_rn(__fmul_rn(x[j], r), wx[j]);
-            y[j] = __fmul_rn(__fmul_rn(y[j], r), wy[j]);
+    bool ok = pos >= 0;
+    float c[4], s[4];
+    if (ok && rd > 0) {
+        if (pos >= a.rope_rows) {
+            paged_flag(kv, PAGED_BAD_POSITION);
+            ok = false;
+        } else if (turns) {
+            const size_t at = (size_t)pos * (rd / 2) + 4 * l;
+            load4(a.cos + at, a.vec, c);
+            load4(a.sin + at, a.vec, s);
         }
     }
-    bool ok = pos >= 0;
-    if (ok && turned && pos >= a.rope_rows) {
-        paged_flag(kv, PAGED_BAD_POSITION);
-        ok = false;
+    // the row's slot in KV head 0
+    long long slot = -1;
+    if (ok && first + AP_VECS > k0) {
+        slot = key_offset(kv, b, seq, (unsigned)pos, 0);
+        if (slot < 0) paged_flag(kv, PAGED_BAD_PAGE);
     }
-    if (ok && turned) {
-        float c[4], s[4];
-        const size_t at = (size_t)pos * (rd / 2) + 4 * l;
-        load4(a.cos + at, a.vec, c);
-        load4(a.sin + at, a.vec, s);
-        if (split) {
+    if (a.q_norm || a.k_norm) {
+#pragma unroll
+        for (int n = 0; n < AP_VECS; n++) {
+            float ss = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) ss = __fmaf_rn(x[n][j], x[n][j], __fmaf_rn(y[n][j], y[n][j], ss));
+#pragma unroll
+            for (int o = LPV / 2; o > 0; o >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, o));
+            const int vec = first + n;
+            const float *w = vec < k0 ? a.q_norm : vec < v0 ? a.k_norm : nullptr;
+            if (live && w) {
+                const float r = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)hd), a.eps)));
+                float wx[4], wy[4];
+                load4(w + i0, a.vec, wx);
+                load4(w + i1, a.vec, wy);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    x[n][j] = __fmul_rn(__fmul_rn(x[n][j], r), wx[j]);
+                    y[n][j] = __fmul_rn(__fmul_rn(y[n][j], r), wy[j]);
+                }
+            }
+        }
+    }
+    if (!live) return;
+#pragma unroll
+    for (int n = 0; n < AP_VECS; n++) {
+        const int vec = first + n;
+        if (vec >= per_row) break;
+        if (ok && turns && vec < v0) {
+            if (split) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) turn(x[n][j], y[n][j], c[j], s[j]);
+            } else {
+                turn(x[n][0], x[n][1], c[0], s[0]);
+                turn(x[n][2], x[n][3], c[1], s[1]);
+                turn(y[n][0], y[n][1], c[2], s[2]);
+                turn(y[n][2], y[n][3], c[3], s[3]);
+            }
+        }
+        if (vec < k0) {
+            float *dst = a.q_out + (size_t)row * a.ldq_out + vec * hd;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const float p = x[j], q = y[j];
-                x[j] = __fsub_rn(__fmul_rn(p, c[j]), __fmul_rn(q, s[j]));
-                y[j] = __fadd_rn(__fmul_rn(p, s[j]), __fmul_rn(q, c[j]));
+                x[n][j] = ok ? x[n][j] : 0.f;
+                y[n][j] = ok ? y[n][j] : 0.f;
             }
-        } else {
+            if (a.vec) {
+                *reinterpret_cast<float4 *>(dst + i0) = make_float4(x[n][0], x[n][1], x[n][2], x[n][3]);
+                *reinterpret_cast<float4 *>(dst + i1) = make_float4(y[n][0], y[n][1], y[n][2], y[n][3]);
+            } else {
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                float p = x[2 * j], q = x[2 * j + 1];
-                x[2 * j] = __fsub_rn(__fmul_rn(p, c[j]), __fmul_rn(q, s[j]));
-                x[2 * j + 1] = __fadd_rn(__fmul_rn(p, s[j]), __fmul_rn(q, c[j]));
-                p = y[2 * j], q = y[2 * j + 1];
-                y[2 * j] = __fsub_rn(__fmul_rn(p, c[j + 2]), __fmul_rn(q, s[j + 2]));
-                y[2 * j + 1] = __fadd_rn(__fmul_rn(p, s[j + 2]), __fmul_rn(q, c[j + 2]));
+                for (int j = 0; j < 4; j++) dst[i0 + j] = x[n][j], dst[i1 + j] = y[n][j];
             }
+        } else if (slot >= 0) {
+            const bool key = vec < v0;
+            T *pool = reinterpret_cast<T *>(key ? kv.k : kv.v) + slot + (long long)(vec - (key ? k0 : v0)) * kv.page_size * hd;
+            KvElem<TYPE>::store4(pool + i0, x[n]);
+            KvElem<TYPE>::store4(pool + i1, y[n]);
         }
     }
-    if (kind == 0) {
-        float *dst = a.q_out + (size_t)row * a.ldq_out + (size_t)head * hd;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            x[j] = ok ? x[j] : 0.f;
-            y[j] = ok ? y[j] : 0.f;
-        }
-        if (a.vec) {
-            *reinterpret_cast<float4 *>(dst + i0) = make_float4(x[0], x[1], x[2], x[3]);
-            *reinterpret_cast<float4 *>(dst + i1) = make_float4(y[0], y[1], y[2], y[3]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; j++) dst[i0 + j] = x[j], dst[i1 + j] = y[j];
-        }
-        return;
-    }
-    if (!ok) return;
-    const long long off = key_offset(kv, b, seq, (unsigned)pos, head);
-    if (off < 0) {
-        paged_flag(kv, PAGED_BAD_PAGE);
-        return;
-    }
-    T *pool = reinterpret_cast<T *>(kind == 1 ? kv.k : kv.v) + off;
-    KvElem<TYPE>::store4(pool + i0, x);
-    KvElem<TYPE>::store4(pool + i1, y);
 }
 
 template <int TYPE>
 void append_typed(const KvView &kv, const BatchView &b, const AppendView &a, cudaStream_t s) {
-    const uint64_t items = (uint64_t)b.num_rows * (unsigned)(a.num_heads + 2 * kv.kv_heads);
+    const uint64_t items = (uint64_t)b.num_rows * (unsigned)((a.num_heads + 2 * kv.kv_heads + AP_VECS - 1) / AP_VECS);
     auto go = [&](auto kernel, int lpv) {
         const uint64_t per = AP_THREADS / lpv;
         kernel<<<(unsigned)((items + per - 1) / per), AP_THREADS, 0, s>>>(kv, b, a);
