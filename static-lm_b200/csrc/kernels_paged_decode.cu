@@ -322,6 +322,20 @@ __device__ __forceinline__ void mma16816(float (&c)[4], unsigned a0, unsigned a1
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// The same from zero.
+template <int TYPE>
+__device__ __forceinline__ void mma16816_zero(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
+                                              unsigned b1) {
+    if constexpr (TYPE == KV_F16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 template <int TYPE, int LPR>
 __global__ void __launch_bounds__(PD_THREADS, 3)
     paged_decode_mma_kernel(KvView kv, BatchView b, PagedAttnView a, DecodePlan plan) {
@@ -384,19 +398,21 @@ __global__ void __launch_bounds__(PD_THREADS, 3)
     };
     // 16-byte chunk c of row r is at chunk c ^ (r & 7): eight rows' chunks of
     // one matrix lie in different banks
+    const char *const k_at = reinterpret_cast<const char *>(kv.k) + (in_row ? c * 16 : 0);
+    const char *const v_at = reinterpret_cast<const char *>(kv.v) + (in_row ? c * 16 : 0);
     auto fill = [&](int stage, long long off) {
         const unsigned valid = __ballot_sync(0xffffffffu, off >= 0);
         if (lane == 0) s_valid[warp][stage] = valid;
+        if (off < 0) off = 0;
+        const unsigned mine = in_row ? valid : 0u;
         const unsigned dst = ring + stage * (2 * PD_TILE);
 #pragma unroll
         for (int p = 0; p < PD_PASSES; p++) {
             const int r = p * RPP + rg;
             const long long o = __shfl_sync(0xffffffffu, off, r);
-            const bool in = o >= 0 && in_row;
-            const size_t at = in ? (size_t)o + c * 16 : 0;
-            const unsigned n = in ? 16u : 0u, to = dst + r * ROW + ((c ^ (r & 7)) << 4);
-            cp_async16_zfill(to, reinterpret_cast<const char *>(kv.k) + at, n);
-            cp_async16_zfill(to + PD_TILE, reinterpret_cast<const char *>(kv.v) + at, n);
+            const unsigned n = (mine >> r) << 4 & 16u, to = dst + r * ROW + ((c ^ (r & 7)) << 4);
+            cp_async16_zfill(to, k_at + o, n);
+            cp_async16_zfill(to + PD_TILE, v_at + o, n);
         }
     };
 
@@ -430,7 +446,7 @@ __global__ void __launch_bounds__(PD_THREADS, 3)
         bool move = false;
 #pragma unroll
         for (int n = 0; n < TK / 8; n++) {  // eight keys
-            float s01[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
+            float s01[4], s2[4];
 #pragma unroll
             for (int k2 = 0; k2 < KS / 2; k2++) {
                 unsigned kb[4];
@@ -438,8 +454,13 @@ __global__ void __launch_bounds__(PD_THREADS, 3)
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     const unsigned(&q)[2][NQ] = qa[k2 * 2 + i];
-                    mma16816<TYPE>(s01, q[0][0], q[0][1], q[1][0], q[1][1], kb[2 * i], kb[2 * i + 1]);
-                    if constexpr (NQ == 3) mma16816<TYPE>(s2, q[0][2], 0u, q[1][2], 0u, kb[2 * i], kb[2 * i + 1]);
+                    if (k2 + i == 0) {
+                        mma16816_zero<TYPE>(s01, q[0][0], q[0][1], q[1][0], q[1][1], kb[0], kb[1]);
+                        if constexpr (NQ == 3) mma16816_zero<TYPE>(s2, q[0][2], 0u, q[1][2], 0u, kb[0], kb[1]);
+                    } else {
+                        mma16816<TYPE>(s01, q[0][0], q[0][1], q[1][0], q[1][1], kb[2 * i], kb[2 * i + 1]);
+                        if constexpr (NQ == 3) mma16816<TYPE>(s2, q[0][2], 0u, q[1][2], 0u, kb[2 * i], kb[2 * i + 1]);
+                    }
                 }
             }
 #pragma unroll
@@ -472,17 +493,22 @@ __global__ void __launch_bounds__(PD_THREADS, 3)
         }
 #pragma unroll
         for (int d2 = 0; d2 < LPR / 2; d2++) {  // sixteen elements
-            float o0[4] = {0.f, 0.f, 0.f, 0.f}, o1[4] = {0.f, 0.f, 0.f, 0.f};
+            float o0[4], o1[4];
 #pragma unroll
             for (int u = 0; u < TK / 16; u++) {
                 unsigned vb[4];
                 ldsm4_t(vt + (u * 16 + (lm & 1) * 8 + lr) * ROW + (((d2 * 2 + (lm >> 1)) ^ lr) << 4), vb);
-                if constexpr (NQ == 3) {
-                    mma16816<TYPE>(o0, w[2 * u][2], 0u, w[2 * u + 1][2], 0u, vb[0], vb[1]);
-                    mma16816<TYPE>(o1, w[2 * u][2], 0u, w[2 * u + 1][2], 0u, vb[2], vb[3]);
-                }
-                mma16816<TYPE>(o0, w[2 * u][0], w[2 * u][1], w[2 * u + 1][0], w[2 * u + 1][1], vb[0], vb[1]);
-                mma16816<TYPE>(o1, w[2 * u][0], w[2 * u][1], w[2 * u + 1][0], w[2 * u + 1][1], vb[2], vb[3]);
+                auto add = [&](bool zero, unsigned a0, unsigned a1, unsigned a2, unsigned a3) {
+                    if (zero) {
+                        mma16816_zero<TYPE>(o0, a0, a1, a2, a3, vb[0], vb[1]);
+                        mma16816_zero<TYPE>(o1, a0, a1, a2, a3, vb[2], vb[3]);
+                    } else {
+                        mma16816<TYPE>(o0, a0, a1, a2, a3, vb[0], vb[1]);
+                        mma16816<TYPE>(o1, a0, a1, a2, a3, vb[2], vb[3]);
+                    }
+                };
+                if constexpr (NQ == 3) add(u == 0, w[2 * u][2], 0u, w[2 * u + 1][2], 0u);
+                add(u == 0 && NQ == 2, w[2 * u][0], w[2 * u][1], w[2 * u + 1][0], w[2 * u + 1][1]);
             }
 #pragma unroll
             for (int i = 0; i < 2; i++) {
