@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(KvView kv, Ba
         const SeenKeys keys = seen_keys(b, pos, pos, a.window, a.sinks);
         live = (keys.n + chunk - 1) / chunk;
         live = live < 1 ? 1 : live > splits ? splits : live;
-    } else if (row >= b.row_start[b.num_seqs]) {
+    } else if (row < b.row_start[0] || row >= b.row_start[b.num_seqs]) {
         return;  // no sequence's: zeroed already
     }
     pdl_wait();

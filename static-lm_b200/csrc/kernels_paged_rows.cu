@@ -206,9 +206,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
 
     // rows that no sequence owns
     {
-        const int end = b.row_start[b.num_seqs];
-        for (long long r = (long long)(end < 0 ? 0 : end) + blockIdx.x; r < b.num_rows; r += gridDim.x)
+        const int start = min(max(b.row_start[0], 0), b.num_rows), end = max(b.row_start[b.num_seqs], start);
+        for (long long i = blockIdx.x; i < (long long)b.num_rows - end + start; i += gridDim.x) {
+            const long long r = i < start ? i : i - start + end;
             for (int e = tid; e < a.num_heads * hd; e += PR_THREADS) a.out[(size_t)r * a.ldo + e] = 0.f;
+        }
     }
     // this CTA's row tile: tiles are counted from the last sequence's last
     // (the longest under the causal mask) to the first

@@ -403,6 +403,37 @@ def test_rows_that_see_nothing_are_zero(cuda, kv, rows):
 
 
 @pytest.mark.parametrize("kv", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("length", [70, 2000])  # one CTA a tile, and keys split over CTAs
+def test_rows_of_no_sequence_are_zero(cuda, kv, length):
+    """Places of a padded batch before the first sequence's rows and after the last's."""
+    c = Cache(cuda, kv, [length, 9], 2, 64, 16, seed=10)
+    q = queries(cuda, 3 + 8 + 4, 4, 64, 3)
+    want = reference(c, q[3:11], [5, 3], 4)
+    c.batch([5, 3])
+    start = cuda.tensor([3, 8, 11], dtype=cuda.int32).cuda()
+    out = cuda.full((15, 256), 7.0, device="cuda")
+    batch = S.PagedBatch(row_start=start.data_ptr(), kv_len=c.len_d.data_ptr(), page_table=c.table_d.data_ptr(),
+                         table_stride=c.table.shape[1], num_seqs=2, num_rows=15, max_kv_len=length)
+    args = S.PagedAttentionArgs(q=q.data_ptr(), out=out.data_ptr(), ldq=256, ldo=256, num_heads=4)
+    size = S.paged_attention_scratch_bytes(c.pages, batch, args)
+    scratch = cuda.full((size + 16,), 0xFF, dtype=cuda.uint8, device="cuda")
+    cuda.cuda.synchronize()
+    S.paged_attention(c.pages, batch, args, scratch.data_ptr(), size)
+    cuda.cuda.synchronize()
+    near(out[3:11], want)
+    assert (out[:3] == 0).all() and (out[11:] == 0).all()
+    cos, sin = (cuda.from_numpy(t).cuda() for t in rope_table(length, 64))
+    x = queries(cuda, 15, 4 + 4, 64, 4)
+    q_out = cuda.full((15, 256), 7.0, device="cuda")
+    S.paged_append(c.pages, batch, S.PagedAppendArgs(
+        q=x.data_ptr(), k=x.data_ptr() + 4 * 256, v=x.data_ptr() + 4 * 384, q_out=q_out.data_ptr(), ldq=512, ldk=512, ldv=512,
+        ldq_out=256, num_heads=4, rope_cos=cos.data_ptr(), rope_sin=sin.data_ptr(), rope_rows=length, rotary_dim=64))
+    cuda.cuda.synchronize()
+    assert (q_out[:3] == 0).all() and (q_out[11:] == 0).all() and (q_out[3:11].abs().sum(1) > 0).all()
+    assert int(c.status) == 0
+
+
+@pytest.mark.parametrize("kv", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("rows", [None, [9, 60]])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 def test_slots_not_seen_do_not_matter(cuda, kv, rows, bad):
