@@ -22,8 +22,8 @@
 // head side by side (row = token * group + head in group), so every key read
 // serves all of them.  Warps 0-7 run the softmax: thread r and r + 128 hold
 // the two halves of row r's keys of a tile, and of its head_dim.  Warp 8
-// issues the MMAs, warps 9-11 bring keys and values from the pages into a
-// ring of shared-memory slots.  Scores and tile results are double-buffered in
+// issues the MMAs, warps 9-11 (9-15 for f32 pages) bring keys and values from
+// the pages into a ring of shared-memory slots.  Scores and tile results are double-buffered in
 // TMEM: q.k of tile j + 1 and w.v of tile j - 1 run under the softmax of j.
 #include "async.cuh"
 #include "kernels.h"
@@ -33,8 +33,6 @@ namespace slm {
 
 namespace {
 
-constexpr int PR_THREADS = 384;
-constexpr int PR_PRODUCERS = 96;
 constexpr float PR_RESCALE = 8.0f;
 constexpr unsigned PR_TMEM_COLS = 512;
 
@@ -44,6 +42,13 @@ struct RowsCfg {
     static constexpr int KT = F16 ? 128 : 64;    // keys per tile
     static constexpr int NQ = F16 ? 2 : 3;       // parts of q and of the weights
     static constexpr int NC = TYPE == KV_F32 ? 3 : 1;  // parts of k and v
+    // warps 0-7 and 8, and those that copy: f32 pages are split into parts on
+    // the way, and three warps of it held the rest up (16 chunks of up to 512 rows
+    // behind up to 2048 keys: 178 us, with seven 146)
+    static constexpr int PRODUCERS = TYPE == KV_F32 ? 224 : 96, THREADS = 288 + PRODUCERS;
+    static constexpr int R_LAUNCH = TYPE == KV_F32 ? 128 : 168;  // registers of a thread at launch, and after the split
+    static constexpr int R_SOFTMAX = F16 ? 200 : TYPE == KV_F32 ? 152 : 184, R_OTHER = F16 ? 104 : TYPE == KV_F32 ? 104 : 136;
+    static_assert(256 * R_SOFTMAX + (THREADS - 256) * R_OTHER == THREADS * R_LAUNCH, "registers");
     static constexpr int PART = KT * HDP * 2;    // bytes of one part of a key tile
     static constexpr int SLOT = PART * NC;
     static constexpr int QPART = 128 * HDP * 2;
@@ -187,7 +192,7 @@ __device__ __forceinline__ void warp_arrive(uint64_t *bar) {
 }
 
 template <int TYPE, int HDP>
-__global__ void __launch_bounds__(PR_THREADS, 1)
+__global__ void __launch_bounds__(RowsCfg<TYPE, HDP>::THREADS, 1)
     paged_rows_kernel(KvView kv, BatchView b, PagedAttnView a, RowsPlan plan) {
     using Cfg = RowsCfg<TYPE, HDP>;
     constexpr int KT = Cfg::KT, NQ = Cfg::NQ, NC = Cfg::NC;
@@ -209,7 +214,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
         const int start = min(max(b.row_start[0], 0), b.num_rows), end = max(b.row_start[b.num_seqs], start);
         for (long long i = blockIdx.x; i < (long long)b.num_rows - end + start; i += gridDim.x) {
             const long long r = i < start ? i : i - start + end;
-            for (int e = tid; e < a.num_heads * hd; e += PR_THREADS) a.out[(size_t)r * a.ldo + e] = 0.f;
+            for (int e = tid; e < a.num_heads * hd; e += Cfg::THREADS) a.out[(size_t)r * a.ldo + e] = 0.f;
         }
     }
     // this CTA's row tile: tiles are counted from the last sequence's last
@@ -252,7 +257,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
     if (warp == 0) tc_alloc(&sh->taddr, PR_TMEM_COLS);
     if (tid == 32) {
         for (int i = 0; i < Cfg::NSLOT; i++) {
-            mbar_init(&sh->full[i], PR_PRODUCERS);
+            mbar_init(&sh->full[i], Cfg::PRODUCERS);
             mbar_init(&sh->empty[i], 1);
         }
         for (int x = 0; x < 2; x++) {
@@ -295,11 +300,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
     constexpr unsigned taddr = 0;
 
     // the softmax threads keep a tile's scores and the row's sums in registers:
-    // they take some of the others' (256 x A + 128 x B = 384 x 168)
-    constexpr int R_SOFTMAX = Cfg::F16 ? 200 : 184, R_OTHER = Cfg::F16 ? 104 : 136;
-    static_assert(256 * R_SOFTMAX + 128 * R_OTHER == 384 * 168, "registers");
+    // they take some of the others'
     if (warp < 8) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(R_SOFTMAX));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(Cfg::R_SOFTMAX));
         // ------------------------------------------------ q, softmax, output
         const float sl2_all = __fmul_rn(a.scale, 1.44269504088896340736f);
         {  // a warp per row, its sixteen rows' loads in flight together
@@ -574,7 +577,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             }
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(R_OTHER));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(Cfg::R_OTHER));
     }
     if (warp < 8) {
     } else if (warp == 8) {
@@ -655,10 +658,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
         // ------------------------------------------- keys and values to slots
         const int p = tid - 9 * 32;
         constexpr int CH = HDP / 8;               // 16-byte chunks of a row's part
-        constexpr int RSTEP = PR_PRODUCERS / CH;  // rows a pass: 12 or 6
+        constexpr int RSTEP = Cfg::PRODUCERS / CH;  // rows a pass: 12, 6, 28 or 14
         constexpr int PASSES = (KT + RSTEP - 1) / RSTEP;
         constexpr int ES = TYPE == KV_F32 ? 4 : 2;
-        static_assert(PR_PRODUCERS % CH == 0, "a thread keeps its chunk");
+        static_assert(Cfg::PRODUCERS % CH == 0, "a thread keeps its chunk");
         const int c = p % CH, r_first = p / CH;
         const bool in_row = c * 8 < hd;
         // the chunk's place in its row, swizzled, for the passes by four
@@ -675,7 +678,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             const long long o = i < KT && at < hi ? key_offset(kv, b, seq, (unsigned)keys.key(at), head) : -1;
             return o < 0 ? -1 : o * ES;
         };
-        long long next0 = find(0, p), next1 = KT > PR_PRODUCERS ? find(0, p + PR_PRODUCERS) : -1;
+        long long next0 = find(0, p), next1 = KT > Cfg::PRODUCERS ? find(0, p + Cfg::PRODUCERS) : -1;
         auto put = [&](const void *pool) {
             const int s = slot;
             if (!first_round) ok = pr_wait(&sh->empty[s], turn, sh, kv);
@@ -743,15 +746,15 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             const unsigned held0 = __ballot_sync(0xffffffffu, next0 >= 0);
             if (lane == 0 && p < KT) sh->valid[j & 7][p >> 5] = held0;
             unsigned held1 = 0xffffffffu;
-            if (KT > PR_PRODUCERS && warp == 9) {
-                sh->off[PR_PRODUCERS + p] = next1;
+            if (KT > Cfg::PRODUCERS && warp == 9) {
+                sh->off[Cfg::PRODUCERS + p] = next1;
                 held1 = __ballot_sync(0xffffffffu, next1 >= 0);
                 if (lane == 0) sh->valid[j & 7][3] = held1;
             }
-            all_held = !named_bar_or(1, PR_PRODUCERS, (p < KT && held0 != 0xffffffffu) || held1 != 0xffffffffu);
+            all_held = !named_bar_or(1, Cfg::PRODUCERS, (p < KT && held0 != 0xffffffffu) || held1 != 0xffffffffu);
             if (j + 1 < ntile) {
                 next0 = find(j + 1, p);
-                if (KT > PR_PRODUCERS && warp == 9) next1 = find(j + 1, p + PR_PRODUCERS);
+                if (KT > Cfg::PRODUCERS && warp == 9) next1 = find(j + 1, p + Cfg::PRODUCERS);
             }
             if constexpr (TYPE == KV_F32) {  // one copy of the long conversion
 #pragma unroll 1
@@ -760,7 +763,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
                 put(kv.k);
                 if (ok) put(kv.v);
             }
-            ok = !named_bar_or(1, PR_PRODUCERS, !ok);
+            ok = !named_bar_or(1, Cfg::PRODUCERS, !ok);
         }
         asm volatile("cp.async.wait_all;\n" ::: "memory");
     }
@@ -775,7 +778,7 @@ void go(const KvView &kv, const BatchView &b, const PagedAttnView &a, const Rows
     static SmemOptIn opt;
     opt(paged_rows_kernel<TYPE, HDP>, RowsCfg<TYPE, HDP>::SMEM);
     const unsigned grid = (unsigned)(plan.tiles * kv.kv_heads * plan.splits);
-    launch_kernel(paged_rows_kernel<TYPE, HDP>, dim3(grid), dim3(PR_THREADS), RowsCfg<TYPE, HDP>::SMEM, s, false, kv, b, a,
+    launch_kernel(paged_rows_kernel<TYPE, HDP>, dim3(grid), dim3(RowsCfg<TYPE, HDP>::THREADS), RowsCfg<TYPE, HDP>::SMEM, s, false, kv, b, a,
                   plan);
 }
 
