@@ -18,7 +18,6 @@ constexpr int PD_THREADS = PD_WARPS * 32;
 constexpr int PD_STAGES = 2;  // 64 KB a CTA: three CTAs an SM (three stages and two CTAs: 8 % slower)
 constexpr int PD_PASSES = 8;               // 512-byte passes per K (or V) tile
 constexpr int PD_TILE = PD_PASSES * 512;   // bytes of a warp's K (or V) tile
-constexpr float PD_RESCALE = 8.0f;         // the reference moves when a score passes it by 2^8
 
 // CTAs of g query heads that an SM holds: by shared memory, and by registers.
 __host__ __device__ constexpr int ctas_per_sm(int g) { return g <= 4 ? 3 : 2; }
@@ -217,7 +216,7 @@ __global__ void __launch_bounds__(PD_THREADS, ctas_per_sm(G))
 #pragma unroll
             for (int o = 8; o < LPR; o <<= 1) u1 = __fadd_rn(u1, __shfl_xor_sync(0xffffffffu, u1, o));
             x[g] = seen ? __fmul_rn(u1, sl2) : -INFINITY;
-            move = move || x[g] > m[g] + PD_RESCALE;
+            move = move || x[g] > m[g] + WeightRange<KV_F32>::rescale;
         }
         if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
@@ -345,6 +344,11 @@ __global__ void __launch_bounds__(PD_THREADS, 3)
     constexpr int ROW = LPR * 16;                        // bytes of a key's row
     constexpr int KS = LPR / 2;                          // 16-element steps of a row
     constexpr int NQ = TYPE == KV_F16 ? 2 : 3;
+    using Range = WeightRange<TYPE>;
+    // the products of the first and of the second part
+    auto sum2 = [](float p0, float p1) {
+        return TYPE == KV_F16 ? __fmaf_rn(p1, F16_PART2_INV, p0) : __fadd_rn(p0, p1);
+    };
     extern __shared__ __align__(128) unsigned char pd_smem[];
     __shared__ unsigned s_valid[PD_WARPS][PD_STAGES];
     __shared__ float s_m[PD_WARPS][G], s_l[PD_WARPS][G];
@@ -466,10 +470,10 @@ __global__ void __launch_bounds__(PD_THREADS, 3)
             }
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                float s = __fadd_rn(s01[i], s01[2 + i]);
+                float s = sum2(s01[i], s01[2 + i]);
                 if constexpr (NQ == 3) s = __fadd_rn(s, s2[i]);
                 x[n][i] = (valid >> (n * 8 + e0 + i)) & 1u ? __fmul_rn(s, sl2) : -INFINITY;
-                move = move || x[n][i] > m + PD_RESCALE;
+                move = move || x[n][i] > m + Range::rescale;
             }
         }
         if (__any_sync(0xffffffffu, move)) {
@@ -478,7 +482,7 @@ __global__ void __launch_bounds__(PD_THREADS, 3)
             for (int n = 0; n < TK / 8; n++) top = fmaxf(top, fmaxf(x[n][0], x[n][1]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            top = fmaxf(top, m);
+            top = fmaxf(__fsub_rn(top, Range::margin), m);
             const float f = exp2_approx(__fsub_rn(m, top));
             m = top;
             l = __fmul_rn(l, f);
@@ -513,8 +517,8 @@ __global__ void __launch_bounds__(PD_THREADS, 3)
             }
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                acc[2 * d2][i] = __fadd_rn(acc[2 * d2][i], __fadd_rn(o0[i], o0[2 + i]));
-                acc[2 * d2 + 1][i] = __fadd_rn(acc[2 * d2 + 1][i], __fadd_rn(o1[i], o1[2 + i]));
+                acc[2 * d2][i] = __fadd_rn(acc[2 * d2][i], sum2(o0[i], o0[2 + i]));
+                acc[2 * d2 + 1][i] = __fadd_rn(acc[2 * d2 + 1][i], sum2(o1[i], o1[2 + i]));
             }
         }
         __syncwarp();  // the stage is filled again at the next turn

@@ -5,9 +5,10 @@
 // The tensor cores multiply 16-bit operands exactly and add in f32, so an f32
 // operand is written as a sum of 16-bit parts and the products of the parts
 // are added up:
-//   f16 pages:  q 2^e = q0 + q1 (e per row, so that the row's largest element
-//               is near 2^15: 22 bits of it survive), w = w0 + w1 for the
-//               softmax weights w <= 2^8; 2 products each for q.k and w.v.
+//   f16 pages:  q 2^e = q0 + q1 / 2^12 (e per row, so that the row's largest
+//               element is near 2^15), w = w0 + w1 / 2^12 for the softmax weights
+//               w <= 2^15; 2 products each for q.k and w.v, the second parts'
+//               first and the others onto them as the MMA takes D / 2^12.
 //   bf16 pages: three bf16 parts of q and w (24 bits), 3 products each.
 //   f32 pages:  three bf16 parts of q, w, k and v; the 6 products whose size
 //               is above 2^-24 of the leading one.
@@ -33,7 +34,6 @@ namespace slm {
 
 namespace {
 
-constexpr float PR_RESCALE = 8.0f;
 constexpr unsigned PR_TMEM_COLS = 512;
 
 template <int TYPE, int HDP>
@@ -117,6 +117,22 @@ __device__ __forceinline__ void tc_mma_f16(unsigned d, uint64_t adesc, uint64_t 
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"((unsigned)acc)
         : "memory");
 }
+// The same on top of D / 2^12: D holds the products of the second f16 parts.
+static_assert(F16_PART2_LOG2 == 12, "the immediate below");
+__device__ __forceinline__ void tc_mma_f16_onto_part2(unsigned d, uint64_t adesc, uint64_t bdesc, unsigned idesc) {
+    asm volatile(
+        "{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.eq.u32 p, 0, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p, 12;\n}\n" ::"r"(d),
+        "l"(adesc), "l"(bdesc), "r"(idesc)
+        : "memory");
+}
+__device__ __forceinline__ void tc_mma_f16_ta_onto_part2(unsigned d, unsigned a, uint64_t bdesc, unsigned idesc) {
+    asm volatile(
+        "{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.eq.u32 p, 0, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p, 12;\n}\n" ::"r"(d),
+        "r"(a), "l"(bdesc), "r"(idesc)
+        : "memory");
+}
 __device__ __forceinline__ void tc_mma_f16_ta(unsigned d, unsigned a, uint64_t bdesc, unsigned idesc, bool acc) {
     asm volatile(
         "{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
@@ -195,6 +211,7 @@ template <int TYPE, int HDP>
 __global__ void __launch_bounds__(RowsCfg<TYPE, HDP>::THREADS, 1)
     paged_rows_kernel(KvView kv, BatchView b, PagedAttnView a, RowsPlan plan) {
     using Cfg = RowsCfg<TYPE, HDP>;
+    using Range = WeightRange<TYPE>;
     constexpr int KT = Cfg::KT, NQ = Cfg::NQ, NC = Cfg::NC;
     constexpr int CT = KT / 2, OC = HDP / 2;        // a thread's keys of a tile, and its part of head_dim
     extern __shared__ __align__(1024) unsigned char pr_smem[];
@@ -447,7 +464,7 @@ __global__ void __launch_bounds__(RowsCfg<TYPE, HDP>::THREADS, 1)
             const float top = __fmul_rn(fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)), sl2);
             // this thread has its scores, and says whether its row's reference
             // has to move; the first weights are worked out meanwhile, as if none had
-            if (top > m + PR_RESCALE) *(volatile int *)&sh->move[j & 3] = 1;
+            if (top > m + Range::rescale) *(volatile int *)&sh->move[j & 3] = 1;
             warp_arrive(&sh->seen_all);
             float sum;  // of 32 weights
             unsigned w[NQ][16];
@@ -480,9 +497,10 @@ __global__ void __launch_bounds__(RowsCfg<TYPE, HDP>::THREADS, 1)
                 warp_arrive(&sh->swapped);
                 wait(&sh->swapped, 1);  // read before the next exchange
                 if (!ok) break;
-                if (both > m + PR_RESCALE) {
-                    f = exp2_approx(__fsub_rn(m, both));
-                    m = both;
+                if (both > m + Range::rescale) {
+                    const float to_m = __fsub_rn(both, Range::margin);
+                    f = exp2_approx(__fsub_rn(m, to_m));
+                    m = to_m;
                     l = __fmul_rn(l, f);
                 }
                 weights(0);
@@ -611,7 +629,10 @@ __global__ void __launch_bounds__(RowsCfg<TYPE, HDP>::THREADS, 1)
                     for (int ks = 0; ks < HDP / 16; ks++) {
                         const unsigned ao = i * Cfg::QPART + (ks >> 2) * 128 * 128 + (ks & 3) * 32;
                         const unsigned bo = S * Cfg::SLOT + c * Cfg::PART + (ks >> 2) * KT * 128 + (ks & 3) * 32;
-                        tc_mma_f16(P * Cfg::T_S, umma_desc_sw128(a_q + ao), umma_desc_sw128(a_kv + bo), idesc_s,
+                        if (Cfg::F16 && i == 0 && ks == 0)
+                            tc_mma_f16_onto_part2(P * Cfg::T_S, umma_desc_sw128(a_q + ao), umma_desc_sw128(a_kv + bo), idesc_s);
+                        else
+                            tc_mma_f16(P * Cfg::T_S, umma_desc_sw128(a_q + ao), umma_desc_sw128(a_kv + bo), idesc_s,
                                        !first || ks > 0);
                     }
                 });
@@ -626,10 +647,14 @@ __global__ void __launch_bounds__(RowsCfg<TYPE, HDP>::THREADS, 1)
                 if (!ok) return;
                 parts([&](int i, int c, bool first) {
 #pragma unroll
-                    for (int ks = 0; ks < KT / 16; ks++)
-                        tc_mma_f16_ta(Cfg::T_O + P * HDP, P * Cfg::T_S + i * (KT / 2) + ks * 8,
-                                      umma_desc_sw128_mn(a_kv + S * Cfg::SLOT + c * Cfg::PART + ks * 2048, KT * 128), idesc_o,
-                                      !first || ks > 0);
+                    for (int ks = 0; ks < KT / 16; ks++) {
+                        const unsigned w_at = P * Cfg::T_S + i * (KT / 2) + ks * 8;
+                        const uint64_t v_desc = umma_desc_sw128_mn(a_kv + S * Cfg::SLOT + c * Cfg::PART + ks * 2048, KT * 128);
+                        if (Cfg::F16 && i == 0 && ks == 0)
+                            tc_mma_f16_ta_onto_part2(Cfg::T_O + P * HDP, w_at, v_desc, idesc_o);
+                        else
+                            tc_mma_f16_ta(Cfg::T_O + P * HDP, w_at, v_desc, idesc_o, !first || ks > 0);
+                    }
                 });
                 tc_commit_elected(&sh->o_full[P]);
                 tc_commit_elected(&sh->empty[S]);

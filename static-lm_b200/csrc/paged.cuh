@@ -127,26 +127,51 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return r;
 }
 // ---- f32 values as sums of 16-bit parts
+// bf16: every part is what the ones before it leave; the exponents are f32's.
+// f16: the first part and 2^12 times what it leaves.  f16 ends at 2^-24, so
+// that an unscaled second part of a value below 2^-2 would keep fewer and fewer
+// bits and none of one below 2^-25; scaled, the parts hold values from 2^-14
+// (where the first one's own bits begin to go) to 2^15 to 2^-24 of themselves
+// and smaller ones to 2^-37.
+constexpr float F16_PART2 = 4096.0f, F16_PART2_INV = 1.0f / 4096.0f;
+constexpr int F16_PART2_LOG2 = 12;
+// Where a softmax's weights 2^(x - m) lie: m is set `margin` below the largest
+// score, and set anew once a score passes it by `rescale`.  bf16 parts and f32
+// weights have room on either side.  f16 parts need the weights as high as
+// their type goes: at most 2^15, a row's largest at least 2^9, so that weights
+// down to 2^-23 of it are held to 2^-24 of themselves and smaller ones to 2^-46
+// of it: those of e^-17 beside one of 1 to 3e-7 of themselves, those of e^-20 to
+// 7e-6.  (At most 2^8, the largest at least 1, with an unscaled second part: 40 %
+// and nothing left.)  Each bit less between margin and rescale doubles that
+// range and has references move more often: 8 x 4096 rows of 9 / 3 heads of 64
+// 644 us with 7, 645 with 6, 653 with 5, 678 with 4.
+template <int TYPE>
+struct WeightRange {
+    static constexpr float margin = TYPE == KV_F16 ? 9.0f : 0.0f, rescale = TYPE == KV_F16 ? 15.0f : 8.0f;
+};
+
 // Two f32 values as the packed 16-bit parts of an operand.  (The second part
 // of an infinity is NaN: rows that meet it come out NaN and are redone.)
 template <int TYPE, int N>
 __device__ __forceinline__ void split2(float a, float b, unsigned (&part)[N]) {
+    if constexpr (TYPE == KV_F16) {
+        static_assert(N == 2, "two parts");
+        const __half2 h = __floats2half2_rn(a, b);
+        const float2 f = __half22float2(h);
+        float ra, rb;  // (a - f) 2^12, exact
+        unpack2(fma2(pack2(f.x, f.y), pack2(-F16_PART2, -F16_PART2), mul2(pack2(a, b), pack2(F16_PART2, F16_PART2))), ra, rb);
+        const __half2 r = __floats2half2_rn(ra, rb);
+        part[0] = *reinterpret_cast<const unsigned *>(&h);
+        part[1] = *reinterpret_cast<const unsigned *>(&r);
+    } else {
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        float ra, rb;
-        if constexpr (TYPE == KV_F16) {
-            const __half2 h = __floats2half2_rn(a, b);
-            part[i] = *reinterpret_cast<const unsigned *>(&h);
-            const float2 f = __half22float2(h);
-            ra = f.x, rb = f.y;
-        } else {
+        for (int i = 0; i < N; i++) {
             const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
             part[i] = *reinterpret_cast<const unsigned *>(&h);
-            ra = __uint_as_float(part[i] << 16), rb = __uint_as_float(part[i] & 0xffff0000u);
-        }
-        if (i + 1 < N) {
-            a = __fsub_rn(a, ra);
-            b = __fsub_rn(b, rb);
+            if (i + 1 < N) {
+                a = __fsub_rn(a, __uint_as_float(part[i] << 16));
+                b = __fsub_rn(b, __uint_as_float(part[i] & 0xffff0000u));
+            }
         }
     }
 }
@@ -154,11 +179,7 @@ __device__ __forceinline__ void split2(float a, float b, unsigned (&part)[N]) {
 template <int TYPE, int N>
 __device__ __forceinline__ void split2_weights(float a, float b, unsigned (&part)[N]) {
     if constexpr (TYPE == KV_F16) {
-        const __half2 h = __floats2half2_rn(a, b);
-        const float2 f = __half22float2(h);
-        const __half2 r = __floats2half2_rn(__fsub_rn(a, f.x), __fsub_rn(b, f.y));
-        part[0] = *reinterpret_cast<const unsigned *>(&h);
-        part[1] = *reinterpret_cast<const unsigned *>(&r);
+        split2<KV_F16, N>(a, b, part);
     } else {
 #pragma unroll
         for (int i = 0; i < N; i++) {  // cut, not rounded: 8 bits each
