@@ -81,15 +81,10 @@ class PagedServer:
         self.next = torch.zeros(max_rows, dtype=torch.int32, device="cuda")
         self.requests: list[Request] = []
         self.stream = torch.cuda.current_stream().cuda_stream
-        # the scratch of the largest call of this loop serves all of them
-        size = 0
-        for rows in (None, 1):
-            b = S.PagedBatch(row_start=rows, kv_len=1, page_table=1, table_stride=self.per_seq, num_seqs=max_rows,
-                             num_rows=max_rows, max_kv_len=cfg.max_seq_len)
-            for n_rows in (1, max_rows):
-                b.num_rows = n_rows
-                b.num_seqs = n_rows if rows is None else max(1, min(n_rows, 64))
-                size = max(size, S.paged_attention_scratch_bytes(self.pages[0], b, self._attention_args()))
+        # the scratch of the largest call of this loop, in either form, serves all of them
+        batch = lambda start: S.PagedBatch(row_start=start, kv_len=1, page_table=1, table_stride=self.per_seq,  # noqa: E731
+                                           num_seqs=max_rows, num_rows=max_rows, max_kv_len=cfg.max_seq_len)
+        size = max(S.paged_attention_scratch_bytes(self.pages[0], batch(start), self._attention_args()) for start in (None, 1))
         self.scratch = torch.empty(size + 16, dtype=torch.uint8, device="cuda")
 
     def _attention_args(self):

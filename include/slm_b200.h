@@ -360,9 +360,12 @@ typedef struct {
 int slm_paged_attention(const slm_kv_pages *pages, const slm_paged_batch *batch,
                         const slm_paged_attention_args *args, void *scratch, uint64_t scratch_bytes,
                         void *stream);
-/* Bytes of scratch for such a call (0 may be returned; then scratch may be
- * NULL).  It grows with num_rows, num_seqs and max_kv_len: the size for the
- * largest values of a serving loop serves every smaller call of it. */
+/* Bytes of scratch for such a call and for every one like it with fewer rows,
+ * sequences or keys: with the descriptors' other fields and the form (row_start
+ * NULL or not) kept, the size does not fall as num_rows, num_seqs or max_kv_len
+ * grow.  The size for the largest values of a serving loop, the larger of the two
+ * forms' where it takes both, serves every call of it.  0 may be returned; then
+ * scratch may be NULL. */
 uint64_t slm_paged_attention_scratch_bytes(const slm_kv_pages *pages, const slm_paged_batch *batch,
                                            const slm_paged_attention_args *args);
 

@@ -349,6 +349,10 @@ struct PagedAttnView {
     float scale;
     unsigned window, sinks;
 };
+// Scratch of n partial results: their (maximum, sum) first, then their values.
+inline uint64_t parts_ml_bytes(uint64_t n) { return (n * sizeof(float2) + 15) / 16 * 16; }
+inline uint64_t parts_bytes(uint64_t n, int hd) { return parts_ml_bytes(n) + n * (uint64_t)hd * sizeof(float); }
+
 // One new row per sequence (kernels_paged_decode.cu): how its keys are split
 // over CTAs, and where the partial results go.
 struct DecodePlan {
@@ -356,7 +360,8 @@ struct DecodePlan {
     int chunk, splits;       // keys per split; the last split takes what is left
     float2 *part_ml;         // [row][query head][split] running maximum and sum
     float *part_o;           // [row][query head][split][head_dim]
-    uint64_t ml_bytes, scratch_bytes;
+    uint64_t ml_bytes;       // of the scratch in use, before part_o
+    uint64_t scratch_bytes;  // does not fall as rows, sequences and keys grow: no less than this call uses
 };
 DecodePlan plan_paged_decode(const KvView &kv, const BatchView &b, const PagedAttnView &a, uint32_t max_kv_len);
 void launch_paged_decode(const KvView &kv, const BatchView &b, const PagedAttnView &a, const DecodePlan &plan,
@@ -373,7 +378,7 @@ struct RowsPlan {
     int splits;      // CTAs that share a tile's keys
     float2 *part_ml;
     float *part_o;
-    uint64_t ml_bytes, scratch_bytes;
+    uint64_t ml_bytes, scratch_bytes;  // as in DecodePlan
 };
 RowsPlan plan_paged_rows(const KvView &kv, const BatchView &b, const PagedAttnView &a, uint32_t max_kv_len);
 void launch_paged_rows(const KvView &kv, const BatchView &b, const PagedAttnView &a, const RowsPlan &plan, cudaStream_t s);

@@ -680,17 +680,25 @@ DecodePlan plan_paged_decode(const KvView &kv, const BatchView &b, const PagedAt
     const uint64_t fewest = std::min<uint64_t>(64, std::max<uint64_t>(1, (most * key_bytes) >> 20));
     for (uint64_t s = fewest; s <= 64; s++) {
         const uint64_t chunk = ((most + s - 1) / s + 15) / 16 * 16;
-        if (s > fewest && chunk < 64) break;
-        const uint64_t ctas = units * s, waves = (ctas + slots - 1) / slots, deep = (ctas + SMS - 1) / SMS;
+        const uint64_t ctas = units * s;
+        // (past eight waves the count seldom wins, and the scratch has its bound)
+        if (s > fewest && (chunk < 64 || ctas > 8 * slots)) break;
+        const uint64_t waves = (ctas + slots - 1) / slots, deep = (ctas + SMS - 1) / SMS;
         const uint64_t cost = deep * chunk * key_bytes + waves * WAVE + (s > 1 ? JOIN : 0);
         if (best != UINT64_MAX && cost + cost / 32 >= best) continue;
         best = cost;
         p.chunk = (int)std::min<uint64_t>(chunk, INT32_MAX);
         p.splits = (int)((most + chunk - 1) / chunk);
     }
-    const uint64_t parts = (uint64_t)b.num_rows * a.num_heads * p.splits;
-    p.ml_bytes = p.splits > 1 ? (parts * sizeof(float2) + 15) / 16 * 16 : 0;
-    p.scratch_bytes = p.splits > 1 ? p.ml_bytes + parts * kv.hd * sizeof(float) : 0;
+    const uint64_t rows = (uint64_t)b.num_rows * a.num_heads, parts = p.splits > 1 ? rows * p.splits : 0;
+    p.ml_bytes = parts_ml_bytes(parts);
+    // The bound for every call of as many rows and keys or fewer, which may be
+    // split more: as often as `fewest` says, or with chunks of 64 keys (so that
+    // the splits are fewer than most / 48) and at most 8 x slots CTAs.
+    const uint64_t more = std::min<uint64_t>(64, most / 48);
+    uint64_t bound = fewest > 1 ? rows * fewest : 0;
+    if (more > 1) bound = std::max(bound, std::min(rows * more, 8 * slots * (uint64_t)p.heads));
+    p.scratch_bytes = parts_bytes(std::max(parts, bound), kv.hd);
     return p;
 }
 

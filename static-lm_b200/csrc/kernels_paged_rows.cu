@@ -820,11 +820,16 @@ RowsPlan plan_paged_rows(const KvView &kv, const BatchView &b, const PagedAttnVi
     if (a.window) most = std::min<uint64_t>(most, (uint64_t)a.window + a.sinks + rt / group + 1);
     const uint64_t key_tiles = (most + kt - 1) / kt;
     // fewer tiles than SMs: split the keys, at least four key tiles each
-    uint64_t splits = units < 148 ? std::min<uint64_t>(148 / units, key_tiles / 4) : 1;
+    const uint64_t splits = units < 148 ? std::min<uint64_t>(148 / units, key_tiles / 4) : 1;
     p.splits = (int)std::max<uint64_t>(splits, 1);
-    const uint64_t parts = (uint64_t)b.num_rows * a.num_heads * p.splits;
-    p.ml_bytes = p.splits > 1 ? (parts * sizeof(float2) + 15) / 16 * 16 : 0;
-    p.scratch_bytes = p.splits > 1 ? p.ml_bytes + parts * kv.hd * sizeof(float) : 0;
+    const uint64_t rows = (uint64_t)b.num_rows * a.num_heads, parts = p.splits > 1 ? rows * p.splits : 0;
+    p.ml_bytes = parts_ml_bytes(parts);
+    // The bound for every call of as many rows and keys or fewer, which may be
+    // split more: units tiles hold at most 128 x units (row, query head) pairs,
+    // and units x splits is at most 148.
+    const uint64_t more = std::min<uint64_t>(148, key_tiles / 4);
+    const uint64_t bound = more > 1 ? std::min(rows * more, 148 * rt) : 0;
+    p.scratch_bytes = parts_bytes(std::max(parts, bound), kv.hd);
     return p;
 }
 

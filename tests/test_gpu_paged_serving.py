@@ -55,3 +55,18 @@ def test_window_gives_pages_back(cuda):
     r = server.submit(list(range(1, 121)), 40)  # 160 positions: twenty pages without the window
     server.run()
     assert len(r.out) == 40 and len(server.free) == 12
+
+
+def test_long_prompts_and_few_long_requests(cuda):
+    """Calls that are split over more CTAs than the loop's largest: the last
+    chunk of a prompt near max_seq_len, and a handful of long sequences.  (Which
+    tokens come is not compared: Q8_0 activations turn differences of 1e-7 into
+    some 1e-2 of a logit, and over so many positions some logits lie that near.)"""
+    cfg, w, vocab = model()
+    rng = np.random.default_rng(5)
+    server = example().PagedServer(cfg, w, num_pages=256)
+    made = [server.submit([int(t) for t in rng.integers(0, vocab, n)], 8)
+            for n in (cfg.max_seq_len - 8, 430, 433, 410, 417, 440)]
+    server.run()
+    assert all(len(r.out) == 8 and all(0 <= t < vocab for t in r.out) for r in made)
+    assert len(server.free) == 256
