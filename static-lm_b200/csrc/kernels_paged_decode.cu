@@ -569,15 +569,19 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(KvView kv, Ba
     const uint64_t item = blockIdx.x;
     const int row = (int)(item / (unsigned)a.num_heads), h = (int)(item % (unsigned)a.num_heads);
     int live = splits;
+    bool owned = true;
     if (chunk > 0) {
         const int pos = b.kv_len[row] - 1;  // not written by the kernel waited for
         const SeenKeys keys = seen_keys(b, pos, pos, a.window, a.sinks);
         live = (keys.n + chunk - 1) / chunk;
         live = live < 1 ? 1 : live > splits ? splits : live;
-    } else if (row < b.row_start[0] || row >= b.row_start[b.num_seqs]) {
-        return;  // no sequence's: zeroed already
+    } else {
+        owned = row >= b.row_start[0] && row < b.row_start[b.num_seqs];
     }
+    // every CTA waits, those without work too: else a join of rows that are no
+    // sequence's would end, and let its own successor start, before they are zeroed
     pdl_wait();
+    if (!owned) return;
     const float2 *ml = part_ml + item * splits;
     const float *po = part_o + item * splits * (uint64_t)kv.hd + 4 * lane;
     const bool mine = 4 * lane < kv.hd;
