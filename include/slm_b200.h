@@ -271,7 +271,8 @@ enum { SLM_ROPE_PAIRS = 0, SLM_ROPE_HALVES = 1 };
 enum {
     SLM_PAGED_BAD_PAGE = 1,     /* a page id >= num_pages, or none where a key is written */
     SLM_PAGED_BAD_POSITION = 2, /* a position past the page table or the rope table */
-    SLM_PAGED_WAIT_GAVE_UP = 4  /* a bounded device wait gave up */
+    SLM_PAGED_WAIT_GAVE_UP = 4, /* a bounded device wait gave up */
+    SLM_PAGED_BAD_ROWS = 8      /* row_start is negative, falls, or ends past num_rows */
 };
 
 /* One layer's pages.  K and V of (page, KV head, slot) are head_dim elements
@@ -292,7 +293,10 @@ typedef struct {
 /* The rows of one call.  Sequence s owns rows row_start[s]..row_start[s+1]-1
  * of the activations (any number, zero included), which are its last
  * positions: row i of them sits at position kv_len[s] - rows + i, kv_len
- * counting them.  row_start NULL means one new row per sequence
+ * counting them.  row_start does not fall and lies in 0..num_rows: of a
+ * sequence that ends past num_rows the rows before it are worked on, at their
+ * positions, and what it holds of a falling one is of no account
+ * (SLM_PAGED_BAD_ROWS).  row_start NULL means one new row per sequence
  * (num_rows = num_seqs).  Key j of sequence s is in page
  * page_table[s*table_stride + j/page_size], slot j%page_size; a negative id
  * is a page that is not held (given back, or not needed yet): its keys are

@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(AP_THREADS, 4) paged_append_kernel(KvView kv, 
         }
     }
     int seq = 0, pos = -1;
-    if (live) row_place(b, row, seq, pos);
+    if (live) row_place(kv, b, row, seq, pos);
     bool ok = pos >= 0;
     float c[4], s[4];
     if (ok && rd > 0) {

@@ -76,7 +76,7 @@ struct RowsShared {
     unsigned taddr;
     int abort;
     // the CTA's work
-    int seq, row0, rows, tile, found;  // row0: first activation row of the sequence
+    int seq, row0, rows, past, tile, found;  // row0: first activation row of the sequence
 };
 static_assert(sizeof(RowsShared) <= 3072, "small shared data");
 
@@ -228,7 +228,8 @@ __global__ void __launch_bounds__(RowsCfg<TYPE, HDP>::THREADS, 1)
 
     // rows that no sequence owns
     {
-        const int start = min(max(b.row_start[0], 0), b.num_rows), end = max(b.row_start[b.num_seqs], start);
+        const int start = min(max(b.row_start[0], 0), b.num_rows);
+        const int end = min(max(b.row_start[b.num_seqs], start), b.num_rows);
         for (long long i = blockIdx.x; i < (long long)b.num_rows - end + start; i += gridDim.x) {
             const long long r = i < start ? i : i - start + end;
             for (int e = tid; e < a.num_heads * hd; e += Cfg::THREADS) a.out[(size_t)r * a.ldo + e] = 0.f;
@@ -239,15 +240,23 @@ __global__ void __launch_bounds__(RowsCfg<TYPE, HDP>::THREADS, 1)
     const int split = blockIdx.x % plan.splits;
     const int head = blockIdx.x / plan.splits % kv.kv_heads;
     const int index = blockIdx.x / plan.splits / kv.kv_heads;
+    if (blockIdx.x == 0 && warp == 1) {
+        bool bad = b.row_start[0] < 0 || b.row_start[b.num_seqs] > b.num_rows;
+        for (int s = lane; s < b.num_seqs; s += 32) bad = bad || b.row_start[s + 1] < b.row_start[s];
+        if (bad) paged_flag(kv, PAGED_BAD_ROWS);
+    }
     if (warp == 0) {
         int before = 0, found = 0;
         for (int s0 = b.num_seqs - 1; s0 >= 0 && !found; s0 -= 32) {
             const int s = s0 - lane;
-            int start = 0, rows = 0;
+            int start = 0, rows = 0, past = 0;  // rows of the sequence in the call, and past its end
             if (s >= 0) {
                 start = b.row_start[s];
-                rows = b.row_start[s + 1] - start;
-                if (start < 0 || rows < 0 || rows > b.num_rows - start) rows = 0;
+                const int end = b.row_start[s + 1];
+                if (start >= 0 && start <= end) {
+                    rows = max(min(end, b.num_rows) - start, 0);
+                    past = end - start - rows;
+                }
             }
             const int n = (int)(((long long)rows * group + 127) >> 7);
             int sum = n;
@@ -262,6 +271,7 @@ __global__ void __launch_bounds__(RowsCfg<TYPE, HDP>::THREADS, 1)
                 sh->seq = s;
                 sh->row0 = start;
                 sh->rows = rows;
+                sh->past = past;
                 sh->tile = n - 1 - (index - (before + sum - n));
             }
             found = who != 0;
@@ -291,7 +301,7 @@ __global__ void __launch_bounds__(RowsCfg<TYPE, HDP>::THREADS, 1)
         mbar_fence_init();
     }
     const int seq = sh->seq, row0 = sh->row0, rows = sh->rows, tile = sh->tile;
-    const int pos0 = b.kv_len[seq] - rows;  // position of the sequence's first row
+    const int pos0 = b.kv_len[seq] - rows - sh->past;  // position of the sequence's first row
     // tokens of this tile, and the list of keys any of them sees
     const unsigned flat0 = (unsigned)tile * 128u;
     const int tok0 = (int)(flat0 / (unsigned)group);

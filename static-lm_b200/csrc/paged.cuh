@@ -15,6 +15,7 @@ enum KvType : int { KV_F32 = 0, KV_F16 = 1, KV_BF16 = 2 };
 constexpr int PAGED_BAD_PAGE = 1;      // a page id at or past num_pages, or none where one is written
 constexpr int PAGED_BAD_POSITION = 2;  // a position past the page table or the rope table
 constexpr int PAGED_WAIT_GAVE_UP = 4;  // a bounded device wait gave up
+constexpr int PAGED_BAD_ROWS = 8;      // row_start is negative, falls, or ends past num_rows
 
 constexpr float NO_MAX = -3.0e38f;  // a running maximum before any key: below every finite score
 
@@ -40,8 +41,9 @@ __device__ __forceinline__ void paged_flag(const KvView &kv, int bit) {
 }
 
 // Sequence and position of an activation row; position -1 for a row that
-// belongs to no sequence or lies before its sequence's start.
-__device__ __forceinline__ void row_place(const BatchView &b, int row, int &seq, int &pos) {
+// belongs to no sequence or lies before its sequence's start.  (A sequence
+// whose rows end past num_rows keeps their positions.)
+__device__ __forceinline__ void row_place(const KvView &kv, const BatchView &b, int row, int &seq, int &pos) {
     seq = row;
     if (!b.row_start) {
         pos = b.kv_len[row] - 1;
@@ -57,6 +59,7 @@ __device__ __forceinline__ void row_place(const BatchView &b, int row, int &seq,
     }
     seq = lo;
     const int end = b.row_start[lo + 1];
+    if (end > b.num_rows) paged_flag(kv, PAGED_BAD_ROWS);
     pos = b.row_start[lo] <= row && row < end ? b.kv_len[lo] - (end - row) : -1;
 }
 

@@ -1022,6 +1022,7 @@ SLM_EXPORT int slm_paged_check(const slm_kv_pages *pages, void *stream) {
     std::string what;
     if (bits & SLM_PAGED_BAD_PAGE) what += "a page id is not a page of the pool; ";
     if (bits & SLM_PAGED_BAD_POSITION) what += "a position is past the page table or the rope table; ";
+    if (bits & SLM_PAGED_BAD_ROWS) what += "row_start is negative, falls or ends past num_rows; ";
     if (bits & SLM_PAGED_WAIT_GAVE_UP) what += "a device wait timed out; ";
     return fail(SLM_ERR_DEVICE_INPUT, what.substr(0, what.size() - 2));
 }
