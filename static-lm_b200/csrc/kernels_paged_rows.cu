@@ -545,7 +545,10 @@ __global__ void __launch_bounds__(RowsCfg<TYPE, HDP>::THREADS, 1)
             // every product is complete: the results go through the q tiles,
             // 16-byte chunk c of row r at chunk c ^ (r & 7), to whole rows
             float4 *s_o = reinterpret_cast<float4 *>(s_q);
-            bool finite = fabsf(l) < INFINITY;
+            // Once a reference was set, l is 2^margin or more, but for scores past
+            // 2^24, of which x - m keeps the bits that m, rounded, has lost: they
+            // may add up to any power of two, and the weights to zero or infinity.
+            bool finite = fabsf(l) < INFINITY && (m == NO_MAX || l >= Range::least);
 #pragma unroll
             for (int i = 0; i < OC; i += 4) {
                 float y[4] = {acc[i], acc[i + 1], acc[i + 2], acc[i + 3]};
@@ -581,7 +584,7 @@ __global__ void __launch_bounds__(RowsCfg<TYPE, HDP>::THREADS, 1)
                 else
                     dst[0] = y.x, dst[1] = y.y, dst[2] = y.z, dst[3] = y.w;
             }
-            // rows that met a value that is not finite, once their first
+            // rows that met a value that is not finite, or scores so large, once their first
             // results are written (the barrier orders the stores)
             if (named_bar_or(2, 256, row_ok && !finite)) {
                 sh->row[x][r] = finite ? 0.f : 1.f;

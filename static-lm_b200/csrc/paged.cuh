@@ -151,6 +151,7 @@ constexpr int F16_PART2_LOG2 = 12;
 template <int TYPE>
 struct WeightRange {
     static constexpr float margin = TYPE == KV_F16 ? 9.0f : 0.0f, rescale = TYPE == KV_F16 ? 15.0f : 8.0f;
+    static constexpr float least = TYPE == KV_F16 ? 256.0f : 0.5f;  // half of 2^margin
 };
 
 // Two f32 values as the packed 16-bit parts of an operand.  (The second part

@@ -15,7 +15,7 @@ weights, which is the difference of the errors of two scores.  u = 2^-24:
 import numpy as np
 import pytest
 
-from test_gpu_paged import Cache, attend, queries, reference
+from test_gpu_paged import Cache, attend, near, queries, reference
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
@@ -58,3 +58,15 @@ def test_values_of_small_weights(cuda, kv, parts, hd, gap, rows, sink, spread):
     off, size = np.linalg.norm(got - want, axis=1), np.linalg.norm(want, axis=1)
     assert (off <= tol * size).all(), (off / size).max() / tol
     assert (np.abs(got - want).max(1) <= 4 * tol * np.abs(want).max(1)).all()
+
+
+@pytest.mark.parametrize("kv", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("factor", [1e5, 1e7, 1e9, 1e15, 1e25])
+@pytest.mark.parametrize("rows", [None, [150]])
+def test_scores_of_any_size(cuda, kv, factor, rows):
+    """So far apart that one key takes the whole weight: the output is its value
+    (two of a row's scores nearer than their error, 1e-6 of them, would be a rare draw)."""
+    c = Cache(cuda, kv, [150], 2, 64, 16, seed=31)
+    n = [1] if rows is None else rows
+    q = queries(cuda, sum(n), 4, 64, 12) * factor
+    near(attend(cuda, c, q, 4, rows), reference(c, q, n, 4))
