@@ -76,7 +76,7 @@ struct RowsShared {
     unsigned taddr;
     int abort;
     // the CTA's work
-    int seq, row0, rows, past, tile, found;  // row0: first activation row of the sequence
+    int seq, row0, rows, past, tile, found, bits;  // row0: first activation row of the sequence
 };
 static_assert(sizeof(RowsShared) <= 3072, "small shared data");
 
@@ -240,19 +240,17 @@ __global__ void __launch_bounds__(RowsCfg<TYPE, HDP>::THREADS, 1)
     const int split = blockIdx.x % plan.splits;
     const int head = blockIdx.x / plan.splits % kv.kv_heads;
     const int index = blockIdx.x / plan.splits / kv.kv_heads;
-    if (blockIdx.x == 0 && warp == 1) {
-        bool bad = b.row_start[0] < 0 || b.row_start[b.num_seqs] > b.num_rows;
-        for (int s = lane; s < b.num_seqs; s += 32) bad = bad || b.row_start[s + 1] < b.row_start[s];
-        if (bad) paged_flag(kv, PAGED_BAD_ROWS);
-    }
     if (warp == 0) {
         int before = 0, found = 0;
-        for (int s0 = b.num_seqs - 1; s0 >= 0 && !found; s0 -= 32) {
+        bool bad = b.row_start[0] < 0 || b.row_start[b.num_seqs] > b.num_rows;
+        // (the first CTA goes over all sequences, for the check)
+        for (int s0 = b.num_seqs - 1; s0 >= 0 && (!found || blockIdx.x == 0); s0 -= 32) {
             const int s = s0 - lane;
             int start = 0, rows = 0, past = 0;  // rows of the sequence in the call, and past its end
             if (s >= 0) {
                 start = b.row_start[s];
                 const int end = b.row_start[s + 1];
+                bad = bad || end < start;
                 if (start >= 0 && start <= end) {
                     rows = max(min(end, b.num_rows) - start, 0);
                     past = end - start - rows;
@@ -274,13 +272,17 @@ __global__ void __launch_bounds__(RowsCfg<TYPE, HDP>::THREADS, 1)
                 sh->past = past;
                 sh->tile = n - 1 - (index - (before + sum - n));
             }
-            found = who != 0;
+            found |= who != 0;
             before += __shfl_sync(0xffffffffu, sum, 31);
         }
-        if (lane == 0) sh->found = found;
+        bad = __any_sync(0xffffffffu, bad);
+        if (lane == 0) sh->found = found, sh->bits = bad ? PAGED_BAD_ROWS : 0;
     }
     __syncthreads();
-    if (!sh->found) return;
+    if (!sh->found) {
+        if (tid == 0 && sh->bits) paged_flag(kv, sh->bits);
+        return;
+    }
     if (warp == 0) tc_alloc(&sh->taddr, PR_TMEM_COLS);
     if (tid == 32) {
         for (int i = 0; i < Cfg::NSLOT; i++) {
@@ -308,7 +310,8 @@ __global__ void __launch_bounds__(RowsCfg<TYPE, HDP>::THREADS, 1)
     int tok1 = (int)((flat0 + 127u) / (unsigned)group);
     tok1 = tok1 < rows ? tok1 : rows - 1;
     const SeenKeys keys = seen_keys(b, pos0 + tok0, pos0 + tok1, a.window, a.sinks);
-    if (pos0 + tok1 >= b.cap && tid == 0) paged_flag(kv, PAGED_BAD_POSITION);
+    const int bits = sh->bits | (pos0 + tok1 >= b.cap ? PAGED_BAD_POSITION : 0);
+    if (bits && tid == 0) paged_flag(kv, bits);
     const int all_tiles = (keys.n + KT - 1) / KT;
     const int per_split = (all_tiles + plan.splits - 1) / plan.splits;
     const int lo = split * per_split * KT;
