@@ -6,6 +6,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <float.h>
 #include <stdint.h>
 
 namespace slm {
@@ -17,7 +18,7 @@ constexpr int PAGED_BAD_POSITION = 2;  // a position past the page table or the 
 constexpr int PAGED_WAIT_GAVE_UP = 4;  // a bounded device wait gave up
 constexpr int PAGED_BAD_ROWS = 8;      // row_start is negative, falls, or ends past num_rows
 
-constexpr float NO_MAX = -3.0e38f;  // a running maximum before any key: below every finite score
+constexpr float NO_MAX = -FLT_MAX;  // a running maximum before any key: no finite score is below it
 
 struct KvView {
     void *k, *v;

@@ -70,3 +70,17 @@ def test_scores_of_any_size(cuda, kv, factor, rows):
     n = [1] if rows is None else rows
     q = queries(cuda, sum(n), 4, 64, 12) * factor
     near(attend(cuda, c, q, 4, rows), reference(c, q, n, 4))
+
+
+@pytest.mark.parametrize("kv,q0,k0", [("f32", 1e19, -2.2e19), ("bf16", 1e19, -2.2e19), ("f16", 3.36e33, -65504.0)])
+@pytest.mark.parametrize("rows", [None, [40]])
+@pytest.mark.parametrize("length", [50, 1500])
+def test_scores_near_the_lowest_f32(cuda, kv, q0, k0, rows, length):
+    """-2.2e38, times log2(e) -3.2e38: finite, and the same for every key, whose values are averaged."""
+    c = Cache(cuda, kv, [length], 2, 64, 16, seed=32)
+    c.k.zero_()
+    c.view(c.k)[..., 0] = k0
+    n = [1] if rows is None else rows
+    q = cuda.zeros(sum(n), 4 * 64, device="cuda")
+    q.view(-1, 4, 64)[..., 0] = q0
+    near(attend(cuda, c, q, 4, rows, scale=1.0), reference(c, q, n, 4, scale=1.0))
