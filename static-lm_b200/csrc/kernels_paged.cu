@@ -92,7 +92,8 @@ __global__ void __launch_bounds__(AP_THREADS, 4) paged_append_kernel(KvView kv, 
     long long slot = -1;
     if (ok && first + AP_VECS > k0) {
         slot = key_offset(kv, b, seq, (unsigned)pos, 0);
-        if (slot < 0) paged_flag(kv, PAGED_BAD_PAGE);
+        // (a position past the table has its own flag)
+        if (slot < 0 && page_index(kv, (unsigned)pos) < b.table_stride) paged_flag(kv, PAGED_BAD_PAGE);
     }
     if (a.q_norm || a.k_norm) {
 #pragma unroll

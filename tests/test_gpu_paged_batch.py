@@ -4,7 +4,7 @@ import pytest
 
 import static_lm as S
 from static_lm._lib import SlmError
-from test_gpu_paged import Cache, append_reference, near, queries, reference, rope_table
+from test_gpu_paged import Cache, append_reference, near, queries, reference, rope_table, run_append
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +77,18 @@ def test_row_starts_that_fall_or_are_negative_are_flagged(cuda, start):
     out = cuda.full((10, 256), 7.0, device="cuda")
     call(cuda, c, q, 4, start, 9, 40, out)
     assert int(c.status) == 8 and (out[9] == 7.0).all()
+
+
+@pytest.mark.parametrize("table,length,rope,bits", [
+    ([-1, -1], 5, 9, 1),  # a page that is not held
+    ([90, 0], 1, 9, 1),   # an id past the pool
+    ([0, 1], 9, 9, 2),    # a position past the table
+    ([0, 1], 8, 7, 2),    # one past the rope table
+    ([0, 1], 8, 9, 0),
+])
+def test_append_flags_what_it_met_and_nothing_else(cuda, table, length, rope, bits):
+    c = Cache(cuda, "f32", [length], 1, 64, 4, seed=7)
+    c.table = np.array([table], np.int32)
+    c.table_d = cuda.from_numpy(c.table).cuda()
+    run_append(cuda, c, queries(cuda, 1, 2 + 2, 64, 7), None, 2, *rope_table(rope, 64), 64)
+    assert int(c.status) == bits
