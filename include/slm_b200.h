@@ -302,6 +302,8 @@ typedef struct {
  * is a page that is not held (given back, or not needed yet): its keys are
  * not seen.  kv_len 0 marks an unused place of a padded batch.  max_kv_len is
  * the host's upper bound of kv_len: it sizes grids and scratch, never results.
+ * table_stride * page_size, the positions a row of the table covers, is at most
+ * 2^31 - 65537.
  * Arrays are device memory (int32). */
 typedef struct {
     const int32_t *row_start;  /* [num_seqs + 1], or NULL */

@@ -573,7 +573,7 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(KvView kv, Ba
     if (chunk > 0) {
         const int pos = b.kv_len[row] - 1;  // not written by the kernel waited for
         const SeenKeys keys = seen_keys(b, pos, pos, a.window, a.sinks);
-        live = (keys.n + chunk - 1) / chunk;
+        live = (int)(((unsigned)keys.n + (unsigned)chunk - 1u) / (unsigned)chunk);
         live = live < 1 ? 1 : live > splits ? splits : live;
     } else {
         owned = row >= b.row_start[0] && row < b.row_start[b.num_seqs];

@@ -861,7 +861,8 @@ int check_batch(const slm_paged_batch *b, const KvView &kv, BatchView *v) {
     if (b->num_rows && b->num_seqs == 0) return fail(SLM_ERR_SHAPE, "rows without a sequence");
     if (b->num_rows && (!b->kv_len || !b->page_table)) return fail(SLM_ERR_INVALID_ARG, "null device pointer");
     if (b->num_rows && b->table_stride == 0) return fail(SLM_ERR_SHAPE, "table_stride must be positive");
-    if ((uint64_t)b->table_stride * (uint64_t)kv.page_size > (uint64_t)INT32_MAX)
+    // (the kernels' 32-bit key indices run up to 148 tiles of 128 keys past the last)
+    if ((uint64_t)b->table_stride * (uint64_t)kv.page_size > (uint64_t)INT32_MAX - 65536)
         return fail(SLM_ERR_SHAPE, "page table covers too many positions");
     if (b->max_kv_len > (uint32_t)INT32_MAX) return fail(SLM_ERR_SHAPE, "max_kv_len too large");
     v->row_start = b->row_start;
