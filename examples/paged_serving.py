@@ -164,7 +164,9 @@ class PagedServer:
 
     # -------------------------------------------------------------- steps
     def submit(self, prompt, n_out) -> Request:
-        if len(prompt) + n_out > self.cfg.max_seq_len or not prompt:
+        if not prompt or n_out < 1:
+            raise S.SlmError(1, "a request has a prompt and asks for a token at least")
+        if len(prompt) + n_out > self.cfg.max_seq_len:
             raise S.SlmError(2, "prompt and output exceed max_seq_len")
         self.requests.append(Request(prompt, n_out))
         return self.requests[-1]

@@ -70,3 +70,12 @@ def test_long_prompts_and_few_long_requests(cuda):
     server.run()
     assert all(len(r.out) == 8 and all(0 <= t < vocab for t in r.out) for r in made)
     assert len(server.free) == 256
+
+
+@pytest.mark.parametrize("prompt,n_out,code", [([], 4, 1), ([5], 0, 1), ([5], -1, 1), ([5] * 500, 13, 2)])
+def test_requests_that_could_not_end_are_refused(cuda, prompt, n_out, code):
+    cfg, w, vocab = model()
+    server = example().PagedServer(cfg, w, num_pages=4)
+    with pytest.raises(S.SlmError) as e:
+        server.submit(prompt, n_out)
+    assert e.value.code == code and not server.step()
