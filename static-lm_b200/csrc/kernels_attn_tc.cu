@@ -268,20 +268,20 @@ __global__ void __launch_bounds__(TC_THREADS) attn_prefill_tc_kernel(AttnArgs a,
             },
             tid);
     };
-    // Thread 0 issues MMAs after every thread's shared-memory writes (the
+    // Warp 0 issues MMAs after every thread's shared-memory writes (the
     // barrier orders them, and the TMEM reads before it), then commits them
     // to `done` (bar_s for S, bar_p for PV: a commit covers everything the
-    // thread issued before it).  The same barrier tells every thread whether
+    // warp issued before it).  The same barrier tells every thread whether
     // any thread's wait gave up (then nothing is issued and the caller stops).
     bool waits_ok = true;
     auto issue = [&](auto body, uint64_t *done, unsigned &n_done) {
         fence_async_smem();
         tc_fence_before();
         if (__syncthreads_or(!waits_ok)) return false;
-        if (tid == 0) {
+        if (warp == 0) {
             tc_fence_after();
             body();
-            tc_commit(done);
+            tc_commit_elected(done);
         }
         n_done++;
         return true;

@@ -103,11 +103,8 @@ __host__ __device__ constexpr unsigned umma_idesc_f16(bool bf16, int M, int N, b
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn ? 1u : 0u) << 16) |
            ((unsigned)(N >> 3) << 17) | ((unsigned)(M >> 4) << 24);
 }
-// D[128 x N] (+)= A[128 x 16] B[N x 16]^T, A in shared memory or in TMEM, and
-// the commit of what was issued: the whole warp comes here with the same
-// operands and its elected lane issues.  (The operands live in the warp's
-// uniform registers: issued from a branch of one lane, unrolled MMAs were
-// given each other's.  With the election inside, 128-wide MMAs issue every 64
+// D[128 x N] (+)= A[128 x 16] B[N x 16]^T, A in shared memory or in TMEM, called
+// by the whole warp.  (With the election inside, 128-wide MMAs issue every 64
 // cycles, their full rate, and 64-wide ones every 49; with a predicate kept
 // in a register every 73.)
 __device__ __forceinline__ void tc_mma_f16(unsigned d, uint64_t adesc, uint64_t bdesc, unsigned idesc, bool acc) {
@@ -146,13 +143,6 @@ __device__ __forceinline__ void fence_async_elected() {
     asm volatile(
         "{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n @q fence.proxy.async.shared::cta;\n}\n" ::: "memory");
 }
-__device__ __forceinline__ void tc_commit_elected(uint64_t *bar) {
-    asm volatile(
-        "{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n"
-        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_addr(bar))
-        : "memory");
-}
-
 // ---- TMEM <-> registers, 32 columns of this thread's lane
 __device__ __forceinline__ void tmem_ld32(unsigned taddr, float *v) {
     asm volatile(

@@ -1,6 +1,13 @@
 // tc.cuh -- 5th-generation tensor core (tcgen05) helpers for sm_100a: TMEM
 // allocation, kind::tf32 MMA on shared-memory operands, completion through an
 // mbarrier, TMEM loads and the fences that order them with thread barriers.
+//
+// An MMA's operands live in the warp's uniform registers.  Where many are
+// unrolled, the whole, converged warp calls them with the same operands and
+// each elects its lane inside: in a branch of one lane, unrolled MMAs were once
+// seen with each other's operands (in a kernel no longer here; why was not
+// narrowed further).  A loop of one or two MMAs and a commit by one lane is
+// kept in the GEMM: elected, its whole step took 2 to 4 % longer.
 #pragma once
 
 #include "async.cuh"
@@ -38,12 +45,12 @@ __host__ __device__ constexpr unsigned umma_idesc_tf32(int M, int N) {
     return (1u << 4) | (2u << 7) | (2u << 10) | ((unsigned)(N >> 3) << 17) | ((unsigned)(M >> 4) << 24);
 }
 
-// D[M x N] (+)= A[M x K=8] . B[N x K=8]^T, issued by one thread.
+// D[M x N] (+)= A[M x K=8] . B[N x K=8]^T, called by a whole warp.
 __device__ __forceinline__ void tc_mma_tf32(unsigned d_tmem, uint64_t adesc, uint64_t bdesc,
                                             unsigned idesc, bool accumulate) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n}\n" ::"r"(d_tmem),
+        "{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n}\n" ::"r"(d_tmem),
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"((unsigned)accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
         : "memory");
 }
@@ -71,6 +78,15 @@ __device__ __forceinline__ void tc_commit(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(
                      smem_addr(bar))
                  : "memory");
+}
+
+// The same of what a warp's elected lane issued (the same lane every time),
+// called by the whole warp.
+__device__ __forceinline__ void tc_commit_elected(uint64_t *bar) {
+    asm volatile(
+        "{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_addr(bar))
+        : "memory");
 }
 
 // Warp-wide: allocate `ncols` TMEM columns (power of two >= 32), address to *dst.
