@@ -349,7 +349,8 @@ int slm_paged_append(const slm_kv_pages *pages, const slm_paged_batch *batch,
  * 1/sqrt(head_dim).  A row that sees no key (outside every sequence, before
  * position 0, no page held), or whose every score is -infinity, is zero.
  * What is in slots a row does not see (stale, infinite, NaN) does not reach
- * it.  Sums and the softmax are f32.  out is apart from q.
+ * it.  Sums and the softmax are f32; with f16 pages weights below 2^-23 of a
+ * row's largest are held to 2^-46 of it.  out is apart from q.
  * `scratch` holds slm_paged_attention_scratch_bytes bytes, 16-byte aligned,
  * contents of no account before and after; calls that may overlap on the GPU
  * need scratches of their own.  Sums are in an order that does not change from

@@ -38,9 +38,17 @@ __device__ __forceinline__ void turn(float &p, float &q, float c, float s) {
 // the rope tables) is worked out once for them, with all their loads in flight.
 // 8 bytes in and out per query element, 4 + the page's type per key and value
 // element are its bytes.  With a vector a group it was bound by instructions
-// (issue 77 % of the cycles, DRAM 49 %): 8 x 4096 rows of 9 + 3 + 3 heads of 64
-// into f16 pages, cold, 51.2 us; two vectors 47.1, three 45.1 (5.2 TB/s), four
-// (three CTAs an SM) 49.2.  Single rows are one launch's time.
+// (issue 77 % of the cycles, DRAM 49 %; now 62 and 56).  With one, two, three and
+// four vectors a group (64 registers each), prompts of 4096 rows into f16
+// pages:
+//   8 x 9 + 3 + 3 heads of 64          49.9  44.5  43.1  44.8 us (f32 pages 45.4, bf16 43.1)
+//   2 x 32 + 8 + 8 of 128, normed      83.8  75.0  73.7  73.5
+//   8 x 6 + 6 + 6 of 48                57.3  49.0  43.1  46.9 (two of eight lanes idle)
+//   6 x 12 + 2 + 2 of 80               69.6  56.7  52.4  49.9 (six of sixteen)
+//   4 x 20 + 4 + 4 of 96               81.8  67.8  63.8  61.5 (four of sixteen)
+//   12 x 4 + 4 + 4 of 32, bf16 pages   34.8  30.6  28.2  28.7
+// Three are best or within 5 % everywhere: 4.5 to 5.7 TB/s.  Single rows are one
+// launch's time.
 constexpr int AP_VECS = 3;
 
 template <int TYPE, int LPV>

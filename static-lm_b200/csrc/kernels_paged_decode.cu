@@ -294,9 +294,11 @@ __global__ void __launch_bounds__(PD_THREADS, ctas_per_sm(G))
 // the A operand of w.v: nothing crosses lanes but the row maxima, on the tiles
 // where a reference moves.  Each step's w.v starts from zero and is added in
 // f32: the tensor core cuts its sums.  About 500 instructions per 16 keys of
-// 128 elements (f16); the same on the CUDA cores took 900: cold, 128 windows
-// of 1028 keys 121 us there and 115 here, 64 sequences of 500 to 8192 in bf16
-// 224 us.  It is bound by memory (5 TB/s of pages scattered over the pool).
+// 128 elements (f16); the same on the CUDA cores took 900: 64 sequences of 500
+// to 8192 keys in f16 238 us there and 194 here, 64 of 2049 (9 / 3 heads of 64)
+// 28.7 and 25.6.  bf16 pays for its third part: 230 and 223, 28.1 and 28.5; 128
+// windows of 1028 keys 112.5 and 114.5, one sequence of 8192 18.5 and 19.1.  It is
+// bound by memory (5 to 5.9 TB/s of pages scattered over the pool).
 __device__ __forceinline__ void ldsm4(unsigned a, unsigned (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])

@@ -15,9 +15,13 @@
 //
 // The tensor core cuts each sum at the last bit of its largest addend, always
 // towards zero: about 2e-8 of the sum per MMA, which over the hundreds of MMAs
-// of a long row adds up.  So no chain of MMAs is longer than one key tile (at
-// most 24, the smallest products first): every tile's w.v goes to TMEM afresh
-// and is added to the row's sums in registers.
+// of a long row adds up.  So no chain of MMAs is longer than one key tile (8 to
+// 24, 48 for q.k of f32 pages with head_dim above 64; the smallest products
+// first): every tile's w.v goes to TMEM afresh and is added to the row's sums in
+// registers.  Against 64 bits, in the 2-norm, 300 rows behind 3000 keys are off by
+// 2e-7 to 7e-7 with q of N(0, 1) and 1.5 times it, and by 5e-7 (head_dim 64) and 8e-7
+// (f32 and bf16 pages, 128) or 1.1e-6 (f16, 128) with q sixteen times as large,
+// where f32 arithmetic itself gives 1.7e-6 and 2.6e-6.
 //
 // A CTA takes 128 rows of one (sequence, KV head), the query heads of the KV
 // head side by side (row = token * group + head in group), so every key read
