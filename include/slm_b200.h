@@ -293,11 +293,11 @@ typedef struct {
 /* The rows of one call.  Sequence s owns rows row_start[s]..row_start[s+1]-1
  * of the activations (any number, zero included), which are its last
  * positions: row i of them sits at position kv_len[s] - rows + i, kv_len
- * counting them.  row_start does not fall and lies in 0..num_rows: of a
- * sequence that ends past num_rows the rows before it are worked on, at their
- * positions, and what it holds of a falling one is of no account
- * (SLM_PAGED_BAD_ROWS).  row_start NULL means one new row per sequence
- * (num_rows = num_seqs).  Key j of sequence s is in page
+ * counting them.  row_start lies in 0..num_rows and does not fall.  Where one
+ * does not (SLM_PAGED_BAD_ROWS), a sequence that ends past num_rows has its rows
+ * before num_rows worked on, at their positions; one whose range falls or starts
+ * below 0 is left out, and its rows' outputs mean nothing.  row_start NULL means
+ * one new row per sequence (num_rows = num_seqs).  Key j of sequence s is in page
  * page_table[s*table_stride + j/page_size], slot j%page_size; a negative id
  * is a page that is not held (given back, or not needed yet): its keys are
  * not seen.  kv_len 0 marks an unused place of a padded batch.  max_kv_len is
