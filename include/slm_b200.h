@@ -256,13 +256,14 @@ int slm_sample_argmax(const float *logits_dev, uint64_t n, int32_t *out_dev, voi
  * one sequence of max_seq_len positions).  Sequences of unlike and changing
  * lengths share one pool of pages; a table says which pages hold a sequence's
  * positions.  Activations are f32 as everywhere in this library, the pages
- * f32, f16 or bf16.  All pointers are the caller's device memory; the calls
+ * f32, f16, bf16 or 8-bit.  All pointers are the caller's device memory; the calls
  * allocate nothing, copy nothing to the host and are stream-ordered, so they
  * can be captured in a CUDA graph. */
 enum {
     SLM_KV_F32 = 0,
     SLM_KV_F16 = 1, /* rounded to nearest even; past 65504 to infinity */
-    SLM_KV_BF16 = 2
+    SLM_KV_BF16 = 2,
+    SLM_KV_Q8 = 3 /* signed bytes with an f32 scale per (KV head, slot) */
 };
 /* Pair layout of the rotation: neighbours (v[2j], v[2j+1]) as
  * apply_rope_cached, or halves (v[j], v[j + rotary_dim/2]). */
@@ -280,6 +281,11 @@ enum {
  * num_kv_heads*page_size*head_dim, a larger one lets layers or K and V share
  * an allocation.  k, v and page_stride (in bytes) are multiples of 16.
  * head_dim is a multiple of 8, at most 128; page_size is any positive number.
+ * An element of 8-bit pages is a byte, and a page ends with its scales: the f32
+ * scale of (KV head, slot) at byte num_kv_heads*page_size*head_dim +
+ * (head*page_size + slot)*4 of the page; the row's values are its signed bytes
+ * times it.  page_stride 0 means num_kv_heads*page_size*(head_dim + 4) rounded up
+ * to 16; head_dim is a multiple of 16.  slm_paged_page_bytes gives a page's size.
  * `status` (optional) is one zeroed device word that the kernels set bits in
  * (SLM_PAGED_*); slm_paged_check reads it. */
 typedef struct {
@@ -326,7 +332,10 @@ typedef struct {
  * so does one past the rope table (SLM_PAGED_BAD_POSITION).  A page id that
  * is not a page of the pool stores nothing (SLM_PAGED_BAD_PAGE).  Two rows at
  * one slot of one page leave either's values.  Pairs without a norm into f32
- * pages give the bits of slm_apply_rope_cached. */
+ * pages give the bits of slm_apply_rope_cached.  Into 8-bit pages a row of k or
+ * v of a head goes as q = x*(127/max|x|) rounded to the nearest, ties to even,
+ * and scale = max|x|/127; one whose values are all below 2^-100 in size as zeros,
+ * one that holds an infinity or a NaN as NaN throughout (its scale). */
 typedef struct {
     const float *q, *k, *v;
     float *q_out;
@@ -375,6 +384,90 @@ int slm_paged_attention(const slm_kv_pages *pages, const slm_paged_batch *batch,
  * scratch may be NULL. */
 uint64_t slm_paged_attention_scratch_bytes(const slm_kv_pages *pages, const slm_paged_batch *batch,
                                            const slm_paged_attention_args *args);
+
+/* Bytes from one page to the next of such pages with page_stride 0 (from dtype,
+ * num_kv_heads, page_size and head_dim alone; k and v may be NULL); 0 where no
+ * such pages can be. */
+uint64_t slm_paged_page_bytes(const slm_kv_pages *pages);
+
+/* Rows of the cache back: for every row of the batch (its sequence's positions
+ * as in slm_paged_append) the keys and values that its slot holds, as rows of
+ * num_kv_heads*head_dim elements of type out_dtype (SLM_KV_F32, SLM_KV_F16 or
+ * SLM_KV_BF16, rounded to the nearest), ldk and ldv elements apart.  Either
+ * output may be NULL.  A row outside every sequence, before position 0, past
+ * the page table or whose page is not held is zero.  The outputs are apart from
+ * the pages and from each other. */
+typedef struct {
+    void *k_out, *v_out;
+    uint64_t ldk, ldv;
+    int32_t out_dtype;
+} slm_paged_read_args;
+int slm_paged_read(const slm_kv_pages *pages, const slm_paged_batch *batch, const slm_paged_read_args *args,
+                   void *stream);
+
+/* Sequences that go on from others (the beams of a search, samples of one
+ * prompt): new sequence i has the positions below kv_len[p] of sequence p =
+ * parent[i], and page_table_out[i] its pages.  The successor of p with the
+ * lowest i keeps p's row of the table; the others share its full pages, and are
+ * given spare[i] for the page of position kv_len[p], into which the used slots
+ * of p's page are copied, keys and values of all layers.  Where kv_len[p] is a
+ * multiple of page_size that page holds no position yet: nothing is copied, and
+ * the first successor too is given spare[i] if p's row holds none.  Entries
+ * past it are -1 but for the first.  taken[i] (optional) is 1 where spare[i] is
+ * in the table now, else 0.
+ *
+ * parent[i] < 0 is an unused place: length 0, every entry -1.  parent[i] >=
+ * num_seqs is treated so and sets SLM_PAGED_BAD_ROWS.  A page that p does not hold
+ * its successors do not hold either.  spare is NULL or [num_new]; where a page
+ * is needed for a copy and there is none (negative, or >= num_pages), the entry
+ * is -1 and SLM_PAGED_BAD_PAGE set.  A length past the page table sets
+ * SLM_PAGED_BAD_POSITION.  Spare pages are apart from each other and from every
+ * page in the tables; a page whose slots two sequences would fill must not be
+ * in two rows of page_table.  The outputs are apart from the inputs.
+ * pages[0..num_layers-1] are layers with pages of one shape, indexed by one
+ * table; pages[0].status takes the flags.  At most 65536 new sequences. */
+typedef struct {
+    const int32_t *parent;     /* [num_new] */
+    const int32_t *kv_len;     /* [num_seqs] */
+    const int32_t *page_table; /* [num_seqs][table_stride] */
+    const int32_t *spare;      /* [num_new], or NULL */
+    int32_t *kv_len_out;       /* [num_new] */
+    int32_t *page_table_out;   /* [num_new][table_stride] */
+    int32_t *taken;            /* [num_new], or NULL */
+    uint32_t table_stride, num_seqs, num_new;
+} slm_paged_fork_args;
+int slm_paged_fork(const slm_kv_pages *pages, uint32_t num_layers, const slm_paged_fork_args *args, void *stream);
+
+/* The best continuations of num_groups groups of beams: of all
+ *   scores[r] + log softmax(logits[r])[t]
+ * over the rows r = g*beams .. g*beams + beams - 1 of group g and the tokens t
+ * the num_out largest, in falling order, as out_scores, out_rows (r, which is
+ * the parent for slm_paged_fork) and out_tokens, [num_groups][num_out].  Sums
+ * that are equal go by the lower row, then the larger logit, then the lower
+ * token.  A row whose score is not finite proposes nothing (an unused beam has
+ * -infinity); one with ended[r] != 0 (ended is optional) proposes end_token once,
+ * at its own score, and its logits are not read.  NaN logits are skipped, as
+ * in slm_sample_argmax, and count nothing in the softmax; logits of -infinity
+ * are never proposed; a row that holds +infinity proposes nothing.  Places for
+ * which there is no candidate are (-infinity, -1, -1).
+ * The exponentials are f32, their sums over a row's parts and the candidates'
+ * sums 64 bits, rounded once.  1 to 256 beams, num_out 1 to 64, vocab at most
+ * 2^30, 2^24 rows.  out_scores may be scores where num_out = beams; the outputs
+ * are apart otherwise.  `scratch` as for slm_paged_attention. */
+typedef struct {
+    const float *logits; /* rows of vocab, ld floats apart */
+    uint64_t ld;
+    const float *scores;
+    const int32_t *ended;
+    uint32_t num_groups, beams, vocab, num_out;
+    int32_t end_token;
+    float *out_scores;
+    int32_t *out_rows, *out_tokens;
+} slm_beam_select_args;
+int slm_beam_select(const slm_beam_select_args *args, void *scratch, uint64_t scratch_bytes, void *stream);
+/* Bytes of scratch for such a call and for every one like it with fewer groups,
+ * beams, tokens or outputs. */
+uint64_t slm_beam_select_scratch_bytes(const slm_beam_select_args *args);
 
 /* Wait for `stream`, read the pages' status word and zero it: SLM_OK, or
  * SLM_ERR_DEVICE_INPUT with what the kernels of earlier calls met. */

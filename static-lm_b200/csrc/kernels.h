@@ -341,6 +341,46 @@ struct AppendView {
 };
 void launch_paged_append(const KvView &kv, const BatchView &b, const AppendView &a, cudaStream_t s);
 
+struct ReadView {
+    void *k, *v;  // either may be null; rows ldk, ldv elements apart
+    size_t ldk, ldv;
+    int type;  // KV_F32, KV_F16 or KV_BF16
+    bool vec;  // 16-byte aligned pointers and rows
+};
+void launch_paged_read(const KvView &kv, const BatchView &b, const ReadView &a, cudaStream_t s);
+
+// New sequence i goes on from sequence parent[i].
+constexpr int FORK_LAYERS = 64;  // layers a launch takes: their pools are its parameters
+struct ForkPools {
+    void *k[FORK_LAYERS], *v[FORK_LAYERS];
+};
+struct ForkView {
+    const int32_t *parent, *kv_len, *table, *spare;  // spare may be null
+    int32_t *len_out, *table_out, *taken;            // table_out null: pages alone; taken may be null
+    int stride, num_seqs, num_new;
+};
+void launch_paged_fork(const ForkPools &pools, const KvView &kv, const ForkView &a, int layers, cudaStream_t s);
+
+// ---- beam search (kernels_beam.cu)
+struct BeamView {
+    const float *logits, *scores;
+    const int32_t *ended;  // may be null
+    size_t ld;
+    int groups, beams, vocab, num_out, end_token;
+    float *out_scores;
+    int32_t *out_rows, *out_tokens;
+    bool vec;  // logits 16-byte aligned, ld a multiple of 4
+};
+// Every row of logits is cut into `parts` of `part` tokens (a multiple of 16).
+struct BeamPlan {
+    int part, parts;
+    double2 *part_ms;    // [row][part] maximum and sum of exponentials
+    uint64_t *part_best; // [row][part][num_out] best tokens, best first
+    uint64_t scratch_bytes;
+};
+BeamPlan plan_beam_select(const BeamView &a);
+void launch_beam_select(const BeamView &a, const BeamPlan &plan, cudaStream_t s);
+
 struct PagedAttnView {
     const float *q;
     float *out;
@@ -366,6 +406,7 @@ struct DecodePlan {
 DecodePlan plan_paged_decode(const KvView &kv, const BatchView &b, const PagedAttnView &a, uint32_t max_kv_len);
 void launch_paged_decode(const KvView &kv, const BatchView &b, const PagedAttnView &a, const DecodePlan &plan,
                          cudaStream_t s);
+void launch_paged_q8(const KvView &kv, const BatchView &b, const PagedAttnView &a, cudaStream_t s);
 // Joins the partial results of a row's splits into out.  chunk > 0: splits of
 // `chunk` seen keys, of which only those that have a key were written;
 // chunk 0: every split was written.

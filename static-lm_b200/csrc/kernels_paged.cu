@@ -51,6 +51,33 @@ __device__ __forceinline__ void turn(float &p, float &q, float c, float s) {
 // launch's time.
 constexpr int AP_VECS = 3;
 
+// 8-bit rows: x = q scale with scale = max|x| / 127 and q = x (127 / max|x|)
+// rounded to the nearest, ties to even: off by half a step, max|x| / 254, and
+// the roundings of the two quotients and the product.  A row of magnitudes
+// below 2^-100, whose scale would be near f32's smallest, is stored as zeros; one
+// that holds an infinity or a NaN as NaN throughout, by its scale.
+struct Q8Row {
+    float scale, up;
+};
+__device__ __forceinline__ Q8Row q8_row(unsigned top) {
+    Q8Row r;
+    r.scale = r.up = 0.f;
+    if (top >= 0x7f800000u) {
+        r.scale = __uint_as_float(0x7fc00000u);
+    } else if (top >= (unsigned)(127 - 100) << 23) {
+        r.scale = __fdiv_rn(__uint_as_float(top), 127.0f);
+        r.up = __fdiv_rn(127.0f, __uint_as_float(top));
+    }
+    return r;
+}
+__device__ __forceinline__ unsigned q8_pack(const float (&x)[4], float up) {
+    // 1.5 2^23 + q: q is rounded to the nearest by the sum, and its low byte is the sum's
+    unsigned u[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) u[j] = __float_as_uint(__fadd_rn(__fmul_rn(x[j], up), 12582912.0f));
+    return __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+}
+
 template <int TYPE, int LPV>
 __global__ void __launch_bounds__(AP_THREADS, 4) paged_append_kernel(KvView kv, BatchView b, AppendView a) {
     using T = typename KvElem<TYPE>::T;
@@ -96,12 +123,17 @@ __global__ void __launch_bounds__(AP_THREADS, 4) paged_append_kernel(KvView kv, 
             load4(a.sin + at, a.vec, s);
         }
     }
-    // the row's slot in KV head 0
-    long long slot = -1;
+    // the row's slot in KV head 0, and its scale's place
+    long long slot = -1, scale = -1;
     if (ok && first + AP_VECS > k0) {
-        slot = key_offset(kv, b, seq, (unsigned)pos, 0);
-        // (a position past the table has its own flag)
-        if (slot < 0 && page_index(kv, (unsigned)pos) < b.table_stride) paged_flag(kv, PAGED_BAD_PAGE);
+        unsigned in_page;
+        const int page = key_page(kv, b, seq, (unsigned)pos, in_page);
+        if (page >= 0) {
+            slot = row_offset(kv, page, 0, in_page);
+            if constexpr (TYPE == KV_Q8) scale = scale_offset(kv, page, 0, in_page);
+        } else if (page_index(kv, (unsigned)pos) < b.table_stride) {  // (a position past the table has its own flag)
+            paged_flag(kv, PAGED_BAD_PAGE);
+        }
     }
     if (a.q_norm || a.k_norm) {
 #pragma unroll
@@ -126,11 +158,9 @@ __global__ void __launch_bounds__(AP_THREADS, 4) paged_append_kernel(KvView kv, 
             }
         }
     }
-    if (!live) return;
 #pragma unroll
     for (int n = 0; n < AP_VECS; n++) {
         const int vec = first + n;
-        if (vec >= per_row) break;
         if (ok && turns && vec < v0) {
             if (split) {
 #pragma unroll
@@ -142,6 +172,24 @@ __global__ void __launch_bounds__(AP_THREADS, 4) paged_append_kernel(KvView kv, 
                 turn(y[n][2], y[n][3], c[3], s[3]);
             }
         }
+    }
+    unsigned top[AP_VECS];  // of the vector's magnitudes, as bits, which order as they do
+    if constexpr (TYPE == KV_Q8) {
+#pragma unroll
+        for (int n = 0; n < AP_VECS; n++) {
+            top[n] = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                top[n] = max(top[n], max(__float_as_uint(fabsf(x[n][j])), __float_as_uint(fabsf(y[n][j]))));
+#pragma unroll
+            for (int o = LPV / 2; o > 0; o >>= 1) top[n] = max(top[n], __shfl_xor_sync(0xffffffffu, top[n], o));
+        }
+    }
+    if (!live) return;
+#pragma unroll
+    for (int n = 0; n < AP_VECS; n++) {
+        const int vec = first + n;
+        if (vec >= per_row) break;
         if (vec < k0) {
             float *dst = a.q_out + (size_t)row * a.ldq_out + vec * hd;
 #pragma unroll
@@ -158,9 +206,18 @@ __global__ void __launch_bounds__(AP_THREADS, 4) paged_append_kernel(KvView kv, 
             }
         } else if (slot >= 0) {
             const bool key = vec < v0;
-            T *pool = reinterpret_cast<T *>(key ? kv.k : kv.v) + slot + (long long)(vec - (key ? k0 : v0)) * kv.page_size * hd;
-            KvElem<TYPE>::store4(pool + i0, x[n]);
-            KvElem<TYPE>::store4(pool + i1, y[n]);
+            const long long above = (long long)(vec - (key ? k0 : v0)) * kv.page_size;  // rows of the heads before
+            T *pool = reinterpret_cast<T *>(key ? kv.k : kv.v) + slot + above * hd;
+            if constexpr (TYPE == KV_Q8) {
+                const Q8Row r = q8_row(top[n]);
+                *reinterpret_cast<unsigned *>(pool + i0) = q8_pack(x[n], r.up);
+                *reinterpret_cast<unsigned *>(pool + i1) = q8_pack(y[n], r.up);
+                if (l == 0)
+                    *reinterpret_cast<float *>(reinterpret_cast<char *>(key ? kv.k : kv.v) + scale + above * 4) = r.scale;
+            } else {
+                KvElem<TYPE>::store4(pool + i0, x[n]);
+                KvElem<TYPE>::store4(pool + i1, y[n]);
+            }
         }
     }
 }
@@ -180,15 +237,194 @@ void append_typed(const KvView &kv, const BatchView &b, const AppendView &a, cud
         go(paged_append_kernel<TYPE, 16>, 16);
 }
 
+// Rows of the cache as they were appended: a group of `lanes` lanes (a power of
+// two, 8 elements each) per (row, KV head) takes its K and its V.
+constexpr int RD_THREADS = 256;
+
+template <int TYPE>
+__device__ __forceinline__ void read8(const void *pool, long long at, long long scale, float (&x)[8]) {
+    if constexpr (TYPE == KV_F32) {
+        const float4 *p = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(pool) + at);
+        const float4 u = p[0], v = p[1];
+        x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+    } else if constexpr (TYPE == KV_Q8) {
+        const uint2 u = *reinterpret_cast<const uint2 *>(reinterpret_cast<const char *>(pool) + at);
+        const float f = scale_get(pool, scale);
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            x[j] = __fmul_rn((float)(int8_t)((j < 4 ? u.x : u.y) >> (8 * (j & 3))), f);
+    } else {
+        const uint4 u = *reinterpret_cast<const uint4 *>(reinterpret_cast<const char *>(pool) + 2 * at);
+        const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            float2 f;
+            if constexpr (TYPE == KV_F16)
+                f = __half22float2(*reinterpret_cast<const __half2 *>(&w[j]));
+            else
+                f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&w[j]));
+            x[2 * j] = f.x, x[2 * j + 1] = f.y;
+        }
+    }
+}
+template <int OUT>
+__device__ __forceinline__ void write8(void *out, size_t at, const float (&x)[8], bool vec) {
+    using T = typename KvElem<OUT>::T;
+    T *p = reinterpret_cast<T *>(out) + at;
+    T y[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        if constexpr (OUT == KV_F32)
+            y[j] = x[j];
+        else if constexpr (OUT == KV_F16)
+            y[j] = __float2half_rn(x[j]);
+        else
+            y[j] = __float2bfloat16_rn(x[j]);
+    }
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof y / 16; i++) reinterpret_cast<uint4 *>(p)[i] = reinterpret_cast<const uint4 *>(y)[i];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) p[j] = y[j];
+    }
+}
+
+template <int TYPE, int OUT>
+__global__ void __launch_bounds__(RD_THREADS) paged_read_kernel(KvView kv, BatchView b, ReadView a, int lanes_log2) {
+    const unsigned item = (blockIdx.x * (unsigned)RD_THREADS + threadIdx.x) >> lanes_log2;
+    const int l = threadIdx.x & ((1 << lanes_log2) - 1);
+    const unsigned row = item / (unsigned)kv.kv_heads, head = item - row * (unsigned)kv.kv_heads;
+    if (row >= (unsigned)b.num_rows || l * 8 >= kv.hd) return;
+    int seq, pos;
+    row_place(kv, b, (int)row, seq, pos);
+    int page = -1;
+    unsigned slot = 0;
+    if (pos >= 0) page = key_page(kv, b, seq, (unsigned)pos, slot);
+    const long long at = page < 0 ? 0 : row_offset(kv, page, (int)head, slot) + l * 8;
+    const long long scale = page < 0 || TYPE != KV_Q8 ? 0 : scale_offset(kv, page, (int)head, slot);
+    const size_t to = (size_t)head * kv.hd + l * 8;
+    float k[8] = {}, v[8] = {};
+    if (page >= 0 && a.k) read8<TYPE>(kv.k, at, scale, k);
+    if (page >= 0 && a.v) read8<TYPE>(kv.v, at, scale, v);
+    if (a.k) write8<OUT>(a.k, (size_t)row * a.ldk + to, k, a.vec);
+    if (a.v) write8<OUT>(a.v, (size_t)row * a.ldv + to, v, a.vec);
+}
+
+template <int TYPE>
+void read_typed(const KvView &kv, const BatchView &b, const ReadView &a, cudaStream_t s) {
+    const int log2 = kv.hd <= 8 ? 0 : kv.hd <= 16 ? 1 : kv.hd <= 32 ? 2 : kv.hd <= 64 ? 3 : 4;
+    const uint64_t threads = ((uint64_t)b.num_rows * kv.kv_heads) << log2;
+    const unsigned grid = (unsigned)((threads + RD_THREADS - 1) / RD_THREADS);
+    if (a.type == KV_F32)
+        paged_read_kernel<TYPE, KV_F32><<<grid, RD_THREADS, 0, s>>>(kv, b, a, log2);
+    else if (a.type == KV_F16)
+        paged_read_kernel<TYPE, KV_F16><<<grid, RD_THREADS, 0, s>>>(kv, b, a, log2);
+    else
+        paged_read_kernel<TYPE, KV_BF16><<<grid, RD_THREADS, 0, s>>>(kv, b, a, log2);
+}
+
+// Sequences that go on from others: CTA (i, y) makes sequence i's row of the
+// table (y 0) and copies the used slots of its parent's last page, layers y *
+// per_cta on, where i needs a page of its own.
+constexpr int FK_THREADS = 256;
+
+__global__ void __launch_bounds__(FK_THREADS) paged_fork_kernel(ForkPools pools, KvView kv, ForkView a, int layers, int per_cta,
+                                                                int el) {
+    const int i = blockIdx.x, tid = threadIdx.x;
+    int p = a.parent[i];
+    if (p >= a.num_seqs) {
+        if (tid == 0 && blockIdx.y == 0) paged_flag(kv, PAGED_BAD_ROWS);
+        p = -1;
+    }
+    const bool table = blockIdx.y == 0 && a.table_out != nullptr;
+    if (p < 0) {
+        if (table) {
+            for (int j = tid; j < a.stride; j += FK_THREADS) a.table_out[(size_t)i * a.stride + j] = -1;
+            if (tid == 0) a.len_out[i] = 0;
+            if (tid == 0 && a.taken) a.taken[i] = 0;
+        }
+        return;
+    }
+    // the first successor of a parent goes on in its pages
+    int before = 0;
+    for (int j = tid; j < i && !before; j += FK_THREADS) before = a.parent[j] == p;
+    const bool first = !__syncthreads_or(before);
+    const int len = max(a.kv_len[p], 0);
+    const unsigned tail = page_index(kv, (unsigned)len), used = (unsigned)len - tail * (unsigned)kv.page_size;
+    const int32_t *old = a.table + (size_t)p * a.stride;
+    const bool in_table = tail < (unsigned)a.stride;
+    if (tid == 0 && blockIdx.y == 0 && (tail > (unsigned)a.stride || (!in_table && used))) paged_flag(kv, PAGED_BAD_POSITION);
+    int source = in_table ? old[tail] : -1;
+    const bool held = (unsigned)source < (unsigned)kv.num_pages;
+    if (source >= 0 && !held && tid == 0 && blockIdx.y == 0) paged_flag(kv, PAGED_BAD_PAGE);
+    // a page of its own: for the used slots that another goes on to fill, or for the next position
+    const bool copies = !first && in_table && used && held;
+    const bool wants = copies || (in_table && !used && (!first || source < 0));
+    int spare = wants && a.spare ? a.spare[i] : -1;
+    if ((unsigned)spare >= (unsigned)kv.num_pages) {
+        if (tid == 0 && blockIdx.y == 0 && (spare >= 0 || copies)) paged_flag(kv, PAGED_BAD_PAGE);
+        spare = -1;
+    }
+    if (table) {
+        for (int j = tid; j < a.stride; j += FK_THREADS) {
+            int id = first || (unsigned)j < tail ? old[j] : -1;
+            if ((unsigned)j == tail && wants) id = spare;
+            a.table_out[(size_t)i * a.stride + j] = id;
+        }
+        if (tid == 0) a.len_out[i] = len;
+        if (tid == 0 && a.taken) a.taken[i] = wants && spare >= 0;
+    }
+    if (!copies || spare < 0) return;
+    const unsigned chunks = used * (unsigned)(kv.hd * el) / 16u;  // of a KV head's used slots
+    const uint64_t from = (uint64_t)source * kv.page_stride * el, to = (uint64_t)spare * kv.page_stride * el;
+    const uint64_t head_bytes = (uint64_t)kv.page_size * kv.hd * el;
+    for (int layer = blockIdx.y * per_cta; layer < min(layers, (int)(blockIdx.y + 1) * per_cta); layer++)
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            char *pool = reinterpret_cast<char *>(x ? pools.v[layer] : pools.k[layer]);
+            for (unsigned e = tid; e < chunks * (unsigned)kv.kv_heads; e += FK_THREADS) {
+                const unsigned h = e / chunks;
+                const uint64_t at = h * head_bytes + (uint64_t)(e - h * chunks) * 16u;
+                *reinterpret_cast<uint4 *>(pool + to + at) = *reinterpret_cast<const uint4 *>(pool + from + at);
+            }
+            if (kv.type == KV_Q8)
+                for (unsigned e = tid; e < used * (unsigned)kv.kv_heads; e += FK_THREADS) {
+                    const unsigned h = e / used;
+                    const uint64_t at = kv.scale_at + ((uint64_t)h * (unsigned)kv.page_size + (e - h * used)) * 4u;
+                    *reinterpret_cast<float *>(pool + to + at) = *reinterpret_cast<const float *>(pool + from + at);
+                }
+        }
+}
+
 }  // namespace
+
+void launch_paged_read(const KvView &kv, const BatchView &b, const ReadView &a, cudaStream_t s) {
+    if (kv.type == KV_F32)
+        read_typed<KV_F32>(kv, b, a, s);
+    else if (kv.type == KV_F16)
+        read_typed<KV_F16>(kv, b, a, s);
+    else if (kv.type == KV_BF16)
+        read_typed<KV_BF16>(kv, b, a, s);
+    else
+        read_typed<KV_Q8>(kv, b, a, s);
+}
+
+void launch_paged_fork(const ForkPools &pools, const KvView &kv, const ForkView &a, int layers, cudaStream_t s) {
+    const int el = kv.type == KV_F32 ? 4 : kv.type == KV_Q8 ? 1 : 2, per_cta = 4;
+    paged_fork_kernel<<<dim3((unsigned)a.num_new, (unsigned)((layers + per_cta - 1) / per_cta)), FK_THREADS, 0, s>>>(
+        pools, kv, a, layers, per_cta, el);
+}
 
 void launch_paged_append(const KvView &kv, const BatchView &b, const AppendView &a, cudaStream_t s) {
     if (kv.type == KV_F32)
         append_typed<KV_F32>(kv, b, a, s);
     else if (kv.type == KV_F16)
         append_typed<KV_F16>(kv, b, a, s);
-    else
+    else if (kv.type == KV_BF16)
         append_typed<KV_BF16>(kv, b, a, s);
+    else
+        append_typed<KV_Q8>(kv, b, a, s);
 }
 
 }  // namespace slm

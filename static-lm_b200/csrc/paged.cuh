@@ -11,7 +11,9 @@
 
 namespace slm {
 
-enum KvType : int { KV_F32 = 0, KV_F16 = 1, KV_BF16 = 2 };
+// KV_Q8: signed bytes, then an f32 scale per (KV head, slot) at scale_at; an
+// element of its strides and offsets is a byte.
+enum KvType : int { KV_F32 = 0, KV_F16 = 1, KV_BF16 = 2, KV_Q8 = 3 };
 // bits of the status word
 constexpr int PAGED_BAD_PAGE = 1;      // a page id at or past num_pages, or none where one is written
 constexpr int PAGED_BAD_POSITION = 2;  // a position past the page table or the rope table
@@ -27,6 +29,7 @@ struct KvView {
     int page_shift;  // log2(page_size), or -1
     int kv_heads, hd, type;
     int32_t *status;
+    uint64_t scale_at;  // KV_Q8: byte offset of a page's scales
 };
 
 struct BatchView {
@@ -68,11 +71,12 @@ __device__ __forceinline__ unsigned page_index(const KvView &kv, unsigned key) {
     return kv.page_shift >= 0 ? key >> kv.page_shift : key / (unsigned)kv.page_size;
 }
 
-// Element offset of (sequence, key, KV head) in the pools, or -1 where the
-// key's page is not held (a negative id) or the id or the key is out of
-// range (the latter two set the status word).
-__device__ __forceinline__ long long key_offset(const KvView &kv, const BatchView &b, int seq, unsigned key, int head) {
+// The page of (sequence, key) and the key's slot in it, or -1 where the key's
+// page is not held (a negative id) or the id or the key is out of range (the
+// latter two set the status word).
+__device__ __forceinline__ int key_page(const KvView &kv, const BatchView &b, int seq, unsigned key, unsigned &slot) {
     const unsigned pi = page_index(kv, key);
+    slot = key - pi * (unsigned)kv.page_size;
     if (pi >= b.table_stride) {
         paged_flag(kv, PAGED_BAD_POSITION);
         return -1;
@@ -82,9 +86,25 @@ __device__ __forceinline__ long long key_offset(const KvView &kv, const BatchVie
         if (page >= 0) paged_flag(kv, PAGED_BAD_PAGE);
         return -1;
     }
-    const unsigned slot = key - pi * (unsigned)kv.page_size;
+    return page;
+}
+__device__ __forceinline__ long long row_offset(const KvView &kv, int page, int head, unsigned slot) {
     return (long long)((uint64_t)page * kv.page_stride +
                        ((uint64_t)head * (unsigned)kv.page_size + slot) * (unsigned)kv.hd);
+}
+// Byte offset of the row's scale (KV_Q8).
+__device__ __forceinline__ long long scale_offset(const KvView &kv, int page, int head, unsigned slot) {
+    return (long long)((uint64_t)page * kv.page_stride + kv.scale_at +
+                       ((uint64_t)head * (unsigned)kv.page_size + slot) * 4u);
+}
+__device__ __forceinline__ float scale_get(const void *pool, long long at) {
+    return *reinterpret_cast<const float *>(reinterpret_cast<const char *>(pool) + at);
+}
+// Element offset of (sequence, key, KV head) in the pools, or -1 as key_page.
+__device__ __forceinline__ long long key_offset(const KvView &kv, const BatchView &b, int seq, unsigned key, int head) {
+    unsigned slot;
+    const int page = key_page(kv, b, seq, key, slot);
+    return page < 0 ? -1 : row_offset(kv, page, head, slot);
 }
 
 // The keys that rows at positions first_pos..last_pos (the first may be
@@ -230,6 +250,11 @@ struct KvElem<KV_BF16> {
     }
     static __device__ __forceinline__ float get(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
 };
+template <>
+struct KvElem<KV_Q8> {
+    using T = int8_t;
+    static __device__ __forceinline__ float get(const int8_t *p) { return (float)*p; }
+};
 
 // One row and query head over the keys [lo, hi) of a list, of which it sees
 // those below sink_end and those in [from, to), on the CUDA cores by one warp:
@@ -254,13 +279,23 @@ __device__ __noinline__ RowState attend_row(const KvView &kv, const BatchView &b
     for (int i0 = lo; i0 < hi; i0 += 32) {
         const int i = i0 + lane;
         long long off = -1;
-        if (i < hi && (i < sink_end || i >= from)) off = key_offset(kv, b, seq, (unsigned)keys.key(i), head);
+        float v_scale = 1.0f;
         float x = -INFINITY;
-        if (off >= 0) {
-            const T *k = reinterpret_cast<const T *>(kv.k) + off;
-            float dot = 0.f;
-            for (int d = 0; d < hd; d++) dot = __fmaf_rn(q[d], KvElem<TYPE>::get(k + d), dot);
-            x = __fmul_rn(dot, sl2);
+        if (i < hi && (i < sink_end || i >= from)) {
+            unsigned slot;
+            const int page = key_page(kv, b, seq, (unsigned)keys.key(i), slot);
+            if (page >= 0) {
+                off = row_offset(kv, page, head, slot);
+                const T *k = reinterpret_cast<const T *>(kv.k) + off;
+                float dot = 0.f;
+                for (int d = 0; d < hd; d++) dot = __fmaf_rn(q[d], KvElem<TYPE>::get(k + d), dot);
+                if constexpr (TYPE == KV_Q8) {
+                    const long long at = scale_offset(kv, page, head, slot);
+                    dot = __fmul_rn(dot, scale_get(kv.k, at));
+                    v_scale = scale_get(kv.v, at);
+                }
+                x = __fmul_rn(dot, sl2);
+            }
         }
         float top = x;
 #pragma unroll
@@ -274,9 +309,10 @@ __device__ __noinline__ RowState attend_row(const KvView &kv, const BatchView &b
         r.l = __fmaf_rn(r.l, f, total);
 #pragma unroll
         for (int c = 0; c < 4; c++) r.acc[c] = __fmul_rn(r.acc[c], f);
+        const float wv = TYPE == KV_Q8 ? __fmul_rn(w, v_scale) : w;
         for (int j = 0; j < 32; j++) {
             const long long o = __shfl_sync(0xffffffffu, off, j);
-            const float wj = __shfl_sync(0xffffffffu, w, j);
+            const float wj = __shfl_sync(0xffffffffu, wv, j);
             if (o < 0) continue;
             const T *v = reinterpret_cast<const T *>(kv.v) + o;
 #pragma unroll

@@ -818,22 +818,30 @@ namespace {
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
+// Elements from one page to the next; an 8-bit page's, bytes, end with its scales.
+uint64_t page_elements(int32_t dtype, uint64_t kv_heads, uint64_t page_size, uint64_t head_dim) {
+    const uint64_t rows = kv_heads * page_size;
+    return dtype == SLM_KV_Q8 ? (rows * (head_dim + 4) + 15) / 16 * 16 : rows * head_dim;
+}
+
 int check_pages(const slm_kv_pages *p, KvView *kv) {
     if (!p) return fail(SLM_ERR_INVALID_ARG, "pages are null");
     if (!p->k || !p->v) return fail(SLM_ERR_INVALID_ARG, "null page pool");
-    if (p->dtype != SLM_KV_F32 && p->dtype != SLM_KV_F16 && p->dtype != SLM_KV_BF16)
+    if (p->dtype != SLM_KV_F32 && p->dtype != SLM_KV_F16 && p->dtype != SLM_KV_BF16 && p->dtype != SLM_KV_Q8)
         return fail(SLM_ERR_INVALID_ARG, "unknown page type");
+    const bool q8 = p->dtype == SLM_KV_Q8;
     if (p->num_pages == 0 || p->page_size == 0 || p->num_kv_heads == 0)
         return fail(SLM_ERR_SHAPE, "page counts and sizes must be positive");
     if (p->head_dim == 0 || p->head_dim % 8 || p->head_dim > 128)
         return fail(SLM_ERR_SHAPE, "head_dim must be a multiple of 8, at most 128");
+    if (q8 && p->head_dim % 16) return fail(SLM_ERR_SHAPE, "head_dim of 8-bit pages must be a multiple of 16");
     if (p->num_pages > (uint32_t)INT32_MAX || p->page_size > (1u << 24) || p->num_kv_heads > (1u << 16))
         return fail(SLM_ERR_SHAPE, "page pool too large");
-    const uint64_t dense = (uint64_t)p->num_kv_heads * p->page_size * p->head_dim;
+    const uint64_t dense = page_elements(p->dtype, p->num_kv_heads, p->page_size, p->head_dim);
     const uint64_t stride = p->page_stride ? p->page_stride : dense;
     if (stride < dense) return fail(SLM_ERR_SHAPE, "page_stride below one page");
     if (stride > (uint64_t)1 << 40) return fail(SLM_ERR_SHAPE, "page_stride too large");
-    const uint64_t bytes = stride * (p->dtype == SLM_KV_F32 ? 4 : 2);
+    const uint64_t bytes = stride * (p->dtype == SLM_KV_F32 ? 4 : q8 ? 1 : 2);
     if (!aligned16(p->k) || !aligned16(p->v) || bytes % 16)
         return fail(SLM_ERR_INVALID_ARG, "pages must be 16-byte aligned");
     if ((uintptr_t)p->status & 3) return fail(SLM_ERR_INVALID_ARG, "status word is misaligned");
@@ -849,6 +857,7 @@ int check_pages(const slm_kv_pages *p, KvView *kv) {
     kv->hd = (int)p->head_dim;
     kv->type = p->dtype;
     kv->status = p->status;
+    kv->scale_at = q8 ? (uint64_t)p->num_kv_heads * p->page_size * p->head_dim : 0;
     return SLM_OK;
 }
 
@@ -973,6 +982,7 @@ SLM_EXPORT uint64_t slm_paged_attention_scratch_bytes(const slm_kv_pages *pages,
     BatchView b{};
     PagedAttnView a{};
     if (check_attention(pages, batch, args, &kv, &b, &a) != SLM_OK) return 0;
+    if (kv.type == KV_Q8) return 0;
     return b.row_start ? plan_paged_rows(kv, b, a, batch->max_kv_len).scratch_bytes
                        : plan_paged_decode(kv, b, a, batch->max_kv_len).scratch_bytes;
 }
@@ -987,6 +997,10 @@ SLM_EXPORT int slm_paged_attention(const slm_kv_pages *pages, const slm_paged_ba
     if (b.num_rows == 0) return SLM_OK;
     if (!a.q || !a.out) return fail(SLM_ERR_INVALID_ARG, "null device pointer");
     if (a.q == a.out) return fail(SLM_ERR_OVERLAP, "out is q");
+    if (kv.type == KV_Q8) {
+        launch_paged_q8(kv, b, a, (cudaStream_t)stream);
+        return launch_check("paged q8 kernel");
+    }
     if (!b.row_start) {
         DecodePlan plan = plan_paged_decode(kv, b, a, batch->max_kv_len);
         if ((uint64_t)b.num_seqs * kv.kv_heads * plan.head_groups * plan.splits > (uint64_t)INT32_MAX ||
@@ -1008,6 +1022,146 @@ SLM_EXPORT int slm_paged_attention(const slm_kv_pages *pages, const slm_paged_ba
     plan.part_o = (float *)((char *)scratch + plan.ml_bytes);
     launch_paged_rows(kv, b, a, plan, (cudaStream_t)stream);
     return launch_check("paged rows kernels");
+}
+
+SLM_EXPORT uint64_t slm_paged_page_bytes(const slm_kv_pages *pages) {
+    if (!pages) return fail(SLM_ERR_INVALID_ARG, "pages are null"), 0;
+    slm_kv_pages p = *pages;
+    p.k = p.v = (void *)16;  // the size does not hang on where the pages are
+    p.page_stride = 0;
+    p.num_pages = 1;
+    p.status = nullptr;
+    KvView kv{};
+    if (check_pages(&p, &kv) != SLM_OK) return 0;
+    return kv.page_stride * (kv.type == KV_F32 ? 4 : kv.type == KV_Q8 ? 1 : 2);
+}
+
+SLM_EXPORT int slm_paged_read(const slm_kv_pages *pages, const slm_paged_batch *batch, const slm_paged_read_args *args,
+                              void *stream) {
+    KvView kv{};
+    BatchView b{};
+    TRY(check_pages(pages, &kv));
+    TRY(check_batch(batch, kv, &b));
+    if (!args) return fail(SLM_ERR_INVALID_ARG, "arguments are null");
+    if (args->out_dtype != SLM_KV_F32 && args->out_dtype != SLM_KV_F16 && args->out_dtype != SLM_KV_BF16)
+        return fail(SLM_ERR_INVALID_ARG, "unknown output type");
+    const uint64_t width = (uint64_t)kv.kv_heads * kv.hd, el = args->out_dtype == SLM_KV_F32 ? 4 : 2;
+    if ((args->k_out && args->ldk < width) || (args->v_out && args->ldv < width))
+        return fail(SLM_ERR_SHAPE, "row stride below one row");
+    if (((uintptr_t)args->k_out | (uintptr_t)args->v_out) & (el - 1))
+        return fail(SLM_ERR_INVALID_ARG, "output is misaligned");
+    if (b.num_rows == 0) return SLM_OK;
+    if (!args->k_out && !args->v_out) return fail(SLM_ERR_INVALID_ARG, "null device pointer");
+    if (args->k_out == args->v_out) return fail(SLM_ERR_OVERLAP, "k_out is v_out");
+    if ((uint64_t)b.num_rows * kv.kv_heads > (uint64_t)INT32_MAX / 16) return fail(SLM_ERR_SHAPE, "too many rows of heads");
+    ReadView a{};
+    a.k = args->k_out;
+    a.v = args->v_out;
+    a.ldk = args->ldk;
+    a.ldv = args->ldv;
+    a.type = args->out_dtype;
+    a.vec = aligned16(a.k) && aligned16(a.v) && (!a.k || a.ldk * el % 16 == 0) && (!a.v || a.ldv * el % 16 == 0);
+    launch_paged_read(kv, b, a, (cudaStream_t)stream);
+    return launch_check("paged read kernel");
+}
+
+SLM_EXPORT int slm_paged_fork(const slm_kv_pages *pages, uint32_t num_layers, const slm_paged_fork_args *args, void *stream) {
+    if (!pages || num_layers == 0) return fail(SLM_ERR_INVALID_ARG, "no pages");
+    if (num_layers > (1u << 16)) return fail(SLM_ERR_SHAPE, "too many layers");
+    KvView kv{};
+    for (uint32_t i = 0; i < num_layers; i++) {
+        KvView one{};
+        TRY(check_pages(&pages[i], &one));
+        if (i == 0)
+            kv = one;
+        else if (one.page_stride != kv.page_stride || one.num_pages != kv.num_pages || one.page_size != kv.page_size ||
+                 one.kv_heads != kv.kv_heads || one.hd != kv.hd || one.type != kv.type)
+            return fail(SLM_ERR_SHAPE, "layers with pages of unlike shapes");
+    }
+    if (!args) return fail(SLM_ERR_INVALID_ARG, "arguments are null");
+    if (args->num_new > (1u << 16)) return fail(SLM_ERR_SHAPE, "too many new sequences");
+    if (args->num_seqs > (uint32_t)INT32_MAX) return fail(SLM_ERR_SHAPE, "too many sequences");
+    if (args->num_new == 0) return SLM_OK;
+    if (args->num_seqs == 0) return fail(SLM_ERR_SHAPE, "new sequences without old ones");
+    if (args->table_stride == 0) return fail(SLM_ERR_SHAPE, "table_stride must be positive");
+    if ((uint64_t)args->table_stride * (uint64_t)kv.page_size > (uint64_t)INT32_MAX - 65536)
+        return fail(SLM_ERR_SHAPE, "page table covers too many positions");
+    if (!args->parent || !args->kv_len || !args->page_table || !args->kv_len_out || !args->page_table_out)
+        return fail(SLM_ERR_INVALID_ARG, "null device pointer");
+    if (args->page_table_out == args->page_table) return fail(SLM_ERR_OVERLAP, "page_table_out is page_table");
+    if (args->kv_len_out == args->kv_len) return fail(SLM_ERR_OVERLAP, "kv_len_out is kv_len");
+    ForkView a{};
+    a.parent = args->parent;
+    a.kv_len = args->kv_len;
+    a.table = args->page_table;
+    a.spare = args->spare;
+    a.len_out = args->kv_len_out;
+    a.table_out = args->page_table_out;
+    a.taken = args->taken;
+    a.stride = (int)args->table_stride;
+    a.num_seqs = (int)args->num_seqs;
+    a.num_new = (int)args->num_new;
+    for (uint32_t at = 0; at < num_layers; at += FORK_LAYERS) {
+        ForkPools pools{};
+        const int n = (int)std::min<uint32_t>(num_layers - at, FORK_LAYERS);
+        for (int i = 0; i < n; i++) pools.k[i] = pages[at + i].k, pools.v[i] = pages[at + i].v;
+        launch_paged_fork(pools, kv, a, n, (cudaStream_t)stream);
+        TRY(launch_check("paged fork kernel"));
+        a.table_out = nullptr;  // made by the first launch
+    }
+    return SLM_OK;
+}
+
+// ============================================================ beam search
+
+namespace {
+
+int check_beams(const slm_beam_select_args *args, BeamView *a) {
+    if (!args) return fail(SLM_ERR_INVALID_ARG, "arguments are null");
+    if (args->beams == 0 || args->beams > 256) return fail(SLM_ERR_SHAPE, "a group has 1 to 256 beams");
+    if (args->num_out == 0 || args->num_out > 64) return fail(SLM_ERR_SHAPE, "num_out is 1 to 64");
+    if (args->vocab == 0 || args->vocab > (1u << 30)) return fail(SLM_ERR_SHAPE, "vocab is 1 to 2^30");
+    if (args->ld < args->vocab) return fail(SLM_ERR_SHAPE, "row stride below one row");
+    if ((uint64_t)args->num_groups * args->beams > (1u << 24)) return fail(SLM_ERR_SHAPE, "too many rows");
+    a->logits = args->logits;
+    a->scores = args->scores;
+    a->ended = args->ended;
+    a->ld = args->ld;
+    a->groups = (int)args->num_groups;
+    a->beams = (int)args->beams;
+    a->vocab = (int)args->vocab;
+    a->num_out = (int)args->num_out;
+    a->end_token = args->end_token;
+    a->out_scores = args->out_scores;
+    a->out_rows = args->out_rows;
+    a->out_tokens = args->out_tokens;
+    a->vec = aligned16(a->logits) && a->ld % 4 == 0;
+    return SLM_OK;
+}
+
+}  // namespace
+
+SLM_EXPORT uint64_t slm_beam_select_scratch_bytes(const slm_beam_select_args *args) {
+    BeamView a{};
+    if (check_beams(args, &a) != SLM_OK) return 0;
+    return plan_beam_select(a).scratch_bytes;
+}
+
+SLM_EXPORT int slm_beam_select(const slm_beam_select_args *args, void *scratch, uint64_t scratch_bytes, void *stream) {
+    BeamView a{};
+    TRY(check_beams(args, &a));
+    if (a.groups == 0) return SLM_OK;
+    if (!a.logits || !a.scores || !a.out_scores || !a.out_rows || !a.out_tokens)
+        return fail(SLM_ERR_INVALID_ARG, "null device pointer");
+    if (a.out_rows == a.out_tokens) return fail(SLM_ERR_OVERLAP, "out_rows is out_tokens");
+    if (a.out_scores == a.scores && a.num_out != a.beams)
+        return fail(SLM_ERR_OVERLAP, "out_scores is scores, of another number a group");
+    BeamPlan plan = plan_beam_select(a);
+    TRY(check_scratch(scratch, scratch_bytes, plan.scratch_bytes));
+    plan.part_ms = (double2 *)scratch;
+    plan.part_best = (uint64_t *)((double2 *)scratch + (uint64_t)a.groups * a.beams * plan.parts);
+    launch_beam_select(a, plan, (cudaStream_t)stream);
+    return launch_check("beam select kernels");
 }
 
 SLM_EXPORT int slm_paged_check(const slm_kv_pages *pages, void *stream) {

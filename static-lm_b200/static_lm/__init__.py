@@ -15,14 +15,16 @@ import ctypes as C
 
 import numpy as np
 
-from ._lib import (JIT_KERNEL_FN, JIT_OPS, KV_BF16, KV_DTYPES, KV_F16, KV_F32, PHASES, ROPE_HALVES, ROPE_PAIRS,
-                   Config, KvPages, LayerWeights, ModelWeights, PagedAppendArgs, PagedAttentionArgs, PagedBatch,
-                   SlmError, Slice, lib)
+from ._lib import (JIT_KERNEL_FN, JIT_OPS, KV_BF16, KV_DTYPES, KV_F16, KV_F32, KV_Q8, PHASES, ROPE_HALVES,
+                   ROPE_PAIRS, BeamSelectArgs, Config, KvPages, LayerWeights, ModelWeights, PagedAppendArgs,
+                   PagedAttentionArgs, PagedBatch, PagedForkArgs, PagedReadArgs, SlmError, Slice, lib)
 
 __all__ = ["Config", "Slice", "SlmError", "Arena", "QMatrix", "Model", "JitEngine", "lib",
            "gemv_q4_0_arena", "gemm_q4_0_arena", "rope_tables", "KvPages", "PagedBatch", "PagedAppendArgs",
            "PagedAttentionArgs", "KV_F32", "KV_F16", "KV_BF16", "KV_DTYPES", "ROPE_PAIRS", "ROPE_HALVES",
-           "paged_append", "paged_attention", "paged_attention_scratch_bytes", "paged_check"]
+           "paged_append", "paged_attention", "paged_attention_scratch_bytes", "paged_check", "KV_Q8", "PagedReadArgs",
+           "PagedForkArgs", "BeamSelectArgs", "paged_page_bytes", "paged_read", "paged_fork", "beam_select",
+           "beam_select_scratch_bytes"]
 
 Q4_BLOCK_BYTES = 18
 Q8_BLOCK_BYTES = 34
@@ -145,6 +147,34 @@ def paged_attention(pages: KvPages, batch: PagedBatch, args: PagedAttentionArgs,
 def paged_attention_scratch_bytes(pages: KvPages, batch: PagedBatch, args: PagedAttentionArgs) -> int:
     """Bytes of device scratch paged_attention needs for such a call."""
     return int(lib().slm_paged_attention_scratch_bytes(pages, batch, args))
+
+
+def paged_page_bytes(pages: KvPages) -> int:
+    """Bytes from one page to the next with page_stride 0 (slm_paged_page_bytes)."""
+    return int(lib().slm_paged_page_bytes(pages))
+
+
+def paged_read(pages: KvPages, batch: PagedBatch, args: PagedReadArgs, stream: int = 0) -> None:
+    """Keys and values of the batch's rows out of their pages (slm_paged_read)."""
+    lib().slm_paged_read(pages, batch, args, stream)
+
+
+def paged_fork(pages, args: PagedForkArgs, stream: int = 0) -> None:
+    """Tables of the sequences that go on from others, and the pages they do not
+    share (slm_paged_fork); `pages` holds a KvPages for every layer."""
+    n = len(pages)
+    layers = pages if isinstance(pages, C.Array) else (KvPages * n)(*pages)
+    lib().slm_paged_fork(layers, n, args, stream)
+
+
+def beam_select(args: BeamSelectArgs, scratch: int = 0, scratch_bytes: int = 0, stream: int = 0) -> None:
+    """The best continuations of every group of beams (slm_beam_select)."""
+    lib().slm_beam_select(args, scratch, scratch_bytes, stream)
+
+
+def beam_select_scratch_bytes(args: BeamSelectArgs) -> int:
+    """Bytes of device scratch beam_select needs for such a call."""
+    return int(lib().slm_beam_select_scratch_bytes(args))
 
 
 def paged_check(pages: KvPages, stream: int = 0) -> None:

@@ -84,7 +84,28 @@ class PagedAttentionArgs(C.Structure):
                 ("sinks", C.c_uint32)]
 
 
-KV_F32, KV_F16, KV_BF16 = 0, 1, 2
+class PagedReadArgs(C.Structure):
+    """slm_paged_read_args."""
+    _fields_ = [("k_out", C.c_void_p), ("v_out", C.c_void_p), ("ldk", C.c_uint64), ("ldv", C.c_uint64),
+                ("out_dtype", C.c_int32)]
+
+
+class PagedForkArgs(C.Structure):
+    """slm_paged_fork_args."""
+    _fields_ = [("parent", C.c_void_p), ("kv_len", C.c_void_p), ("page_table", C.c_void_p), ("spare", C.c_void_p),
+                ("kv_len_out", C.c_void_p), ("page_table_out", C.c_void_p), ("taken", C.c_void_p),
+                ("table_stride", C.c_uint32), ("num_seqs", C.c_uint32), ("num_new", C.c_uint32)]
+
+
+class BeamSelectArgs(C.Structure):
+    """slm_beam_select_args."""
+    _fields_ = [("logits", C.c_void_p), ("ld", C.c_uint64), ("scores", C.c_void_p), ("ended", C.c_void_p),
+                ("num_groups", C.c_uint32), ("beams", C.c_uint32), ("vocab", C.c_uint32), ("num_out", C.c_uint32),
+                ("end_token", C.c_int32), ("out_scores", C.c_void_p), ("out_rows", C.c_void_p),
+                ("out_tokens", C.c_void_p)]
+
+
+KV_F32, KV_F16, KV_BF16, KV_Q8 = 0, 1, 2, 3
 KV_DTYPES = {"f32": KV_F32, "f16": KV_F16, "bf16": KV_BF16}
 ROPE_PAIRS, ROPE_HALVES = 0, 1
 
@@ -137,6 +158,11 @@ SIGNATURES = {
                                       _V, _U64, _V], True),
     "slm_paged_attention_scratch_bytes": (_U64, [C.POINTER(KvPages), C.POINTER(PagedBatch),
                                                  C.POINTER(PagedAttentionArgs)], False),
+    "slm_paged_page_bytes": (_U64, [C.POINTER(KvPages)], False),
+    "slm_paged_read": (C.c_int, [C.POINTER(KvPages), C.POINTER(PagedBatch), C.POINTER(PagedReadArgs), _V], True),
+    "slm_paged_fork": (C.c_int, [C.POINTER(KvPages), _U32, C.POINTER(PagedForkArgs), _V], True),
+    "slm_beam_select": (C.c_int, [C.POINTER(BeamSelectArgs), _V, _U64, _V], True),
+    "slm_beam_select_scratch_bytes": (_U64, [C.POINTER(BeamSelectArgs)], False),
     "slm_paged_check": (C.c_int, [C.POINTER(KvPages), _V], True),
     "slm_model_create": (C.c_int, [C.c_int, C.POINTER(Config), C.POINTER(ModelWeights), _U32, _U32,
                                    C.POINTER(_V)], True),
