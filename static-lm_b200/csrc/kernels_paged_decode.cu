@@ -642,6 +642,302 @@ __global__ void __launch_bounds__(PD_THREADS) paged_q8_kernel(KvView kv, BatchVi
         if (lane + 32 * c < kv.hd) d[lane + 32 * c] = r.l == 0.f ? 0.f : __fdiv_rn(r.acc[c], r.l);
 }
 
+// 8-bit pages, on the tensor cores.
+//
+// A signed byte is exact in f16, so the bytes go into the MMAs as they are and a
+// row's scale is taken once: the key's by its score, the value's by its weight.
+// Keys, and d of the values, are the 16 rows of A, and the 8 columns of B four
+// query heads in two f16 parts (NG twice that), column 2 h + part: a lane's
+// products of the parts lie side by side, it holds no score twice, and its
+// weights, packed {first, second part}, are after one transposition (movmatrix)
+// the B operand of v.w.  ldmatrix on pairs of bytes leaves a lane with four bytes
+// of one key, of which any two may be the pair of an A register, since q is laid
+// out to match, or (transposed) with two elements of each of two keys, whose
+// pairing by element is part of the conversion: no byte moves between lanes.
+// Weights are at most 2^15 (WeightRange); a value's scale enters them relative to
+// a power of two at or above the tile's largest, which the f32 sums take back.
+__device__ __forceinline__ unsigned movm(unsigned a) {
+    unsigned r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+    return r;
+}
+// Bytes i and j of four signed ones, their top bits flipped, as f16: 1024 + b + 128
+// is b + 128 under an exponent byte of 0x64.
+template <int I, int J>
+__device__ __forceinline__ unsigned bytes_f16(unsigned flipped) {
+    const unsigned h = __byte_perm(flipped, 0x64646464u, 0x4040 | I | J << 8);
+    unsigned r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(0x64806480u));
+    return r;
+}
+__device__ __forceinline__ void cp_async4_zfill(unsigned dst, const void *src, unsigned bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(bytes));
+}
+
+template <int LPR, int NG>
+__global__ void __launch_bounds__(PD_THREADS, 3) paged_decode_q8_kernel(KvView kv, BatchView b, PagedAttnView a, DecodePlan plan) {
+    constexpr int G = 4 * NG, TK = 32;        // heads of a CTA, keys of a tile
+    constexpr int ROW = LPR * 16, RPP = 32 / LPR, PASSES = TK / RPP, TILE = TK * ROW;
+    constexpr int STAGES = LPR == 8 ? 2 : 4;  // the same bytes in either case
+    static_assert(STAGES * TILE == PD_STAGES * PD_TILE, "shared memory");
+    using Range = WeightRange<KV_F16>;
+    extern __shared__ __align__(128) unsigned char pd_smem[];
+    __shared__ unsigned s_valid[PD_WARPS][STAGES];
+    __shared__ float s_scale[PD_WARPS][STAGES][2][TK];  // of a tile's keys and values
+    __shared__ float s_m[PD_WARPS][G], s_l[PD_WARPS][G];
+
+    pdl_release();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    DecodeWork work;
+    if (!decode_work(kv, b, a, plan, work)) return;
+    const int seq = work.seq, head = work.head, lo = work.lo, hi = work.hi;
+    const SeenKeys keys = work.keys;
+    const int g = lane >> 2, t4 = lane & 3;
+
+    // q as B: this lane's column is head g / 2, part g & 1; elements 16 ks + 4 t4 + {0, 1}, {2, 3}
+    unsigned qb[NG][LPR][2];
+    float sl2[NG];  // of this lane's scores: head t4
+#pragma unroll
+    for (int n = 0; n < NG; n++) {
+        const int h = n * 4 + (g >> 1);
+        const float *src = a.q + (size_t)seq * a.ldq + (size_t)(work.h0 + (h < work.ng ? h : 0)) * kv.hd;
+        float f[LPR][4];
+        unsigned top = 0;
+#pragma unroll
+        for (int ks = 0; ks < LPR; ks++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int d = ks * 16 + t4 * 4 + i;
+                f[ks][i] = d < kv.hd && h < work.ng ? src[d] : 0.f;
+                top = max(top, __float_as_uint(fabsf(f[ks][i])));
+            }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        int e = 141 - (int)(top >> 23);  // 2^14 <= top 2^e < 2^15
+        e = top == 0 || top >= 0x7f800000u ? 0 : e > 120 ? 120 : e;
+        const float up = __uint_as_float((unsigned)(127 + e) << 23);
+        const float down = __uint_as_float((unsigned)(127 - e) << 23);
+        sl2[n] = __fmul_rn(__fmul_rn(a.scale, 1.44269504088896340736f), __shfl_sync(0xffffffffu, down, t4 * 8));
+#pragma unroll
+        for (int ks = 0; ks < LPR; ks++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                unsigned part[2];
+                split2<KV_F16, 2>(__fmul_rn(f[ks][2 * i], up), __fmul_rn(f[ks][2 * i + 1], up), part);
+                qb[n][ks][i] = g & 1 ? part[1] : part[0];
+            }
+    }
+
+    const unsigned ring = smem_addr(pd_smem) + warp * (STAGES * 2 * TILE);
+    const int ntile = (hi - lo + TK - 1) / TK;
+    const int c = lane % LPR, rg = lane / LPR;
+    const bool in_row = c * 16 < kv.hd;
+    auto place = [](int r, int chunk) {  // eight rows' chunks of one matrix lie in different banks
+        return (unsigned)(r * ROW + ((chunk ^ (LPR == 8 ? r & 7 : (r >> 1) & 3)) << 4));
+    };
+    struct At {
+        long long row, scale;  // byte offsets of a key in the pools; row -1 for none
+    };
+    auto lookup = [&](int t) -> At {  // key `lane` of tile t
+        const int i = lo + t * TK + lane;
+        unsigned slot;
+        const int page = t < ntile && i < hi ? key_page(kv, b, seq, (unsigned)keys.key(i), slot) : -1;
+        return page < 0 ? At{-1, 0} : At{row_offset(kv, page, head, slot), scale_offset(kv, page, head, slot)};
+    };
+    const char *const k_at = reinterpret_cast<const char *>(kv.k) + (in_row ? c * 16 : 0);
+    const char *const v_at = reinterpret_cast<const char *>(kv.v) + (in_row ? c * 16 : 0);
+    auto fill = [&](int stage, At at) {
+        const unsigned valid = __ballot_sync(0xffffffffu, at.row >= 0);
+        if (lane == 0) s_valid[warp][stage] = valid;
+        const unsigned ns = at.row >= 0 ? 4u : 0u;
+        cp_async4_zfill(smem_addr(&s_scale[warp][stage][0][lane]), reinterpret_cast<const char *>(kv.k) + at.scale, ns);
+        cp_async4_zfill(smem_addr(&s_scale[warp][stage][1][lane]), reinterpret_cast<const char *>(kv.v) + at.scale, ns);
+        if (at.row < 0) at.row = 0;
+        const unsigned mine = in_row ? valid : 0u;
+        const unsigned dst = ring + stage * (2 * TILE);
+#pragma unroll
+        for (int p = 0; p < PASSES; p++) {
+            const int r = p * RPP + rg;
+            const long long o = __shfl_sync(0xffffffffu, at.row, r);
+            const unsigned n = (mine >> r) << 4 & 16u, to = dst + place(r, c);
+            cp_async16_zfill(to, k_at + o, n);
+            cp_async16_zfill(to + TILE, v_at + o, n);
+        }
+    };
+
+    float m[NG], l[NG];
+    float acc[NG][LPR][2];  // elements 16 c + 2 g + {0, 1} of the output of head t4
+#pragma unroll
+    for (int n = 0; n < NG; n++) {
+        m[n] = NO_MAX, l[n] = 0.f;
+#pragma unroll
+        for (int d = 0; d < LPR; d++) acc[n][d][0] = acc[n][d][1] = 0.f;
+    }
+
+    int t_fill = warp, stage = 0;
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; s++) {
+        if (t_fill < ntile) fill(s, lookup(t_fill));
+        cp_async_commit();
+        t_fill += PD_WARPS;
+    }
+    At next = lookup(t_fill);
+    // ldmatrix: rows 8 (lane >> 3 & 1) + lane & 7 of 16, chunk lane >> 4 of two
+    const int lr = (lane & 15), lc = lane >> 4;
+    for (int t = warp; t < ntile; t += PD_WARPS) {
+        cp_async_wait<STAGES - 2>();
+        __syncwarp();
+        {
+            const int to = stage == 0 ? STAGES - 1 : stage - 1;
+            if (t_fill < ntile) fill(to, next);
+            cp_async_commit();
+            t_fill += PD_WARPS;
+            next = lookup(t_fill);
+        }
+        const unsigned kt = ring + stage * (2 * TILE), vt = kt + TILE;
+        const unsigned valid = s_valid[warp][stage];
+        const float *ks = s_scale[warp][stage][0], *vs = s_scale[warp][stage][1];
+        // 2^e above the tile's largest scale of a value that is finite
+        const unsigned bits = __float_as_uint(fabsf(vs[lane]));
+        const int e = min(max((int)(__reduce_max_sync(0xffffffffu, bits < 0x7f800000u ? bits : 0u) >> 23) - 126, -125), 126);
+        const float v_up = __uint_as_float((unsigned)(127 - e) << 23), v_down = __uint_as_float((unsigned)(127 + e) << 23);
+        float x[NG][TK / 8];  // keys g + 8 i
+        bool move = false;
+#pragma unroll
+        for (int u = 0; u < TK / 16; u++) {
+            float s[NG][4];
+#pragma unroll
+            for (int c2 = 0; c2 < LPR / 2; c2++) {
+                unsigned kb[4];
+                ldsm4(kt + place(u * 16 + lr, c2 * 2 + lc), kb);
+#pragma unroll
+                for (int i = 0; i < 4; i++) kb[i] ^= 0x80808080u;
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const unsigned a0 = bytes_f16<0, 1>(kb[2 * i]), a1 = bytes_f16<0, 1>(kb[2 * i + 1]),
+                                   a2 = bytes_f16<2, 3>(kb[2 * i]), a3 = bytes_f16<2, 3>(kb[2 * i + 1]);
+#pragma unroll
+                    for (int n = 0; n < NG; n++) {
+                        const unsigned(&q)[2] = qb[n][c2 * 2 + i];
+                        if (c2 + i == 0)
+                            mma16816_zero<KV_F16>(s[n], a0, a1, a2, a3, q[0], q[1]);
+                        else
+                            mma16816<KV_F16>(s[n], a0, a1, a2, a3, q[0], q[1]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int key = u * 16 + i * 8 + g;
+                const float k_scale = ks[key];
+#pragma unroll
+                for (int n = 0; n < NG; n++) {
+                    const float dot = __fmaf_rn(s[n][2 * i + 1], F16_PART2_INV, s[n][2 * i]);
+                    x[n][2 * u + i] = (valid >> key) & 1u ? __fmul_rn(__fmul_rn(dot, k_scale), sl2[n]) : -INFINITY;
+                    move = move || x[n][2 * u + i] > m[n] + Range::rescale;
+                }
+            }
+        }
+        if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+            for (int n = 0; n < NG; n++) {
+                float top = x[n][0];
+#pragma unroll
+                for (int i = 1; i < TK / 8; i++) top = fmaxf(top, x[n][i]);
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                top = fmaxf(__fsub_rn(top, Range::margin), m[n]);
+                const float f = exp2_approx(__fsub_rn(m[n], top));
+                m[n] = top;
+                l[n] = __fmul_rn(l[n], f);
+#pragma unroll
+                for (int d = 0; d < LPR; d++) acc[n][d][0] = __fmul_rn(acc[n][d][0], f), acc[n][d][1] = __fmul_rn(acc[n][d][1], f);
+            }
+        }
+        unsigned w[NG][TK / 8];
+#pragma unroll
+        for (int i = 0; i < TK / 8; i++) {
+            const float v_scale = __fmul_rn(vs[i * 8 + g], v_up);
+#pragma unroll
+            for (int n = 0; n < NG; n++) {
+                const float y = exp2_approx(__fsub_rn(x[n][i], m[n]));
+                l[n] = __fadd_rn(l[n], y);
+                const float z = __fmul_rn(y, v_scale);
+                const __half z0 = __float2half_rn(z);
+                const __half z1 = __float2half_rn(__fmul_rn(__fsub_rn(z, __half2float(z0)), F16_PART2));
+                w[n][i] = movm((unsigned)__half_as_ushort(z1) << 16 | __half_as_ushort(z0));
+            }
+        }
+#pragma unroll
+        for (int c2 = 0; c2 < LPR / 2; c2++) {
+            float o[2][NG][4];
+#pragma unroll
+            for (int u = 0; u < TK / 16; u++) {
+                unsigned vb[4];
+                ldsm4_t(vt + place(u * 16 + lr, c2 * 2 + lc), vb);
+#pragma unroll
+                for (int i = 0; i < 4; i++) vb[i] ^= 0x80808080u;
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const unsigned a0 = bytes_f16<0, 2>(vb[2 * i]), a1 = bytes_f16<1, 3>(vb[2 * i]),
+                                   a2 = bytes_f16<0, 2>(vb[2 * i + 1]), a3 = bytes_f16<1, 3>(vb[2 * i + 1]);
+#pragma unroll
+                    for (int n = 0; n < NG; n++)
+                        if (u == 0)
+                            mma16816_zero<KV_F16>(o[i][n], a0, a1, a2, a3, w[n][2 * u], w[n][2 * u + 1]);
+                        else
+                            mma16816<KV_F16>(o[i][n], a0, a1, a2, a3, w[n][2 * u], w[n][2 * u + 1]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int n = 0; n < NG; n++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++)
+                        acc[n][2 * c2 + i][j] = __fmaf_rn(__fmaf_rn(o[i][n][2 * j + 1], F16_PART2_INV, o[i][n][2 * j]), v_down,
+                                                          acc[n][2 * c2 + i][j]);
+        }
+        __syncwarp();  // the stage is filled again at the next turn
+        stage = stage == STAGES - 1 ? 0 : stage + 1;
+    }
+    cp_async_wait<0>();
+    __syncthreads();  // every ring is free: the warps' results go there
+
+    float *s_o = reinterpret_cast<float *>(pd_smem);  // [warp][head][hd]
+    bool finite = true;
+#pragma unroll
+    for (int n = 0; n < NG; n++) {
+        const int h = n * 4 + t4;
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[n] = __fadd_rn(l[n], __shfl_xor_sync(0xffffffffu, l[n], o));
+        if (g == 0) s_m[warp][h] = m[n], s_l[warp][h] = l[n];
+        bool fine = fabsf(l[n]) < INFINITY;
+#pragma unroll
+        for (int d = 0; d < LPR; d++) {
+            if (d * 16 < kv.hd)
+                *reinterpret_cast<float2 *>(s_o + (warp * G + h) * kv.hd + d * 16 + 2 * g) = make_float2(acc[n][d][0], acc[n][d][1]);
+            fine = fine && fabsf(acc[n][d][0]) < INFINITY && fabsf(acc[n][d][1]) < INFINITY;
+        }
+        finite = finite && (fine || h >= work.ng);
+    }
+    if (__syncthreads_or(!finite)) {
+        // warp 0's place gets each head's whole result, the others' nothing
+        for (int h = warp; h < work.ng; h += PD_WARPS) {
+            const RowState st = attend_row<KV_Q8>(kv, b, seq, head, a.q + (size_t)seq * a.ldq + (size_t)(work.h0 + h) * kv.hd,
+                                                  __fmul_rn(a.scale, 1.44269504088896340736f), keys, lo, hi, 0, 0, 0x7fffffff);
+            for (int i = 0; i < PD_WARPS; i++) {
+#pragma unroll
+                for (int c4 = 0; c4 < 4; c4++)
+                    if (lane + 32 * c4 < kv.hd) s_o[(i * G + h) * kv.hd + lane + 32 * c4] = i == 0 ? st.acc[c4] : 0.f;
+                if (lane == 0) s_m[i][h] = i == 0 ? st.m : NO_MAX, s_l[i][h] = i == 0 ? st.l : 0.f;
+            }
+        }
+        __syncthreads();
+    }
+    decode_store<G>(kv, a, plan, work, s_o, s_m, s_l);
+}
+
 constexpr size_t PD_SMEM = (size_t)PD_WARPS * PD_STAGES * 2 * PD_TILE;
 
 template <typename K>
@@ -655,6 +951,14 @@ template <int TYPE, int LPR>
 void go_mma(const KvView &kv, const BatchView &b, const PagedAttnView &a, const DecodePlan &plan, cudaStream_t s) {
     static SmemOptIn opt;
     go(paged_decode_mma_kernel<TYPE, LPR>, opt, kv, b, a, plan, s);
+}
+template <int LPR>
+void go_q8(const KvView &kv, const BatchView &b, const PagedAttnView &a, const DecodePlan &plan, cudaStream_t s) {
+    static SmemOptIn one, two;
+    if (plan.heads <= 4)
+        go(paged_decode_q8_kernel<LPR, 1>, one, kv, b, a, plan, s);
+    else
+        go(paged_decode_q8_kernel<LPR, 2>, two, kv, b, a, plan, s);
 }
 template <int LPR, int G>
 void go_fma(const KvView &kv, const BatchView &b, const PagedAttnView &a, const DecodePlan &plan, cudaStream_t s) {
@@ -686,7 +990,7 @@ DecodePlan plan_paged_decode(const KvView &kv, const BatchView &b, const PagedAt
     // query heads of a KV head in one CTA: up to 8 share each key they read
     p.head_groups = (group + 7) / 8;
     const int g = (group + p.head_groups - 1) / p.head_groups;
-    p.heads = kv.type != KV_F32 ? 8 : g == 5 ? 6 : g == 7 ? 8 : g;
+    p.heads = kv.type == KV_Q8 ? (g <= 4 ? 4 : 8) : kv.type != KV_F32 ? 8 : g == 5 ? 6 : g == 7 ? 8 : g;
     p.head_groups = (group + p.heads - 1) / p.heads;
     uint64_t most = max_kv_len;
     if (a.window) most = std::min<uint64_t>(most, (uint64_t)a.window + a.sinks);
@@ -703,7 +1007,7 @@ DecodePlan plan_paged_decode(const KvView &kv, const BatchView &b, const PagedAt
     // units: 1, 2, 3 splits 115, 120, 124 us.
     constexpr uint64_t SMS = 148, WAVE = 215 << 10, JOIN = 170 << 10;
     const uint64_t slots = SMS * (uint64_t)(kv.type == KV_F32 ? ctas_per_sm(p.heads) : 3);
-    const uint64_t key_bytes = 2ull * kv.hd * (kv.type == KV_F32 ? 4 : 2);
+    const uint64_t key_bytes = 2ull * (kv.type == KV_Q8 ? kv.hd + 4 : kv.hd * (kv.type == KV_F32 ? 4 : 2));
     uint64_t best = UINT64_MAX;
     // lengths below the bound may be unlike: with at most 1 MB a CTA the last end together
     const uint64_t fewest = std::min<uint64_t>(64, std::max<uint64_t>(1, (most * key_bytes) >> 20));
@@ -737,6 +1041,8 @@ void launch_paged_decode(const KvView &kv, const BatchView &b, const PagedAttnVi
         kv.hd <= 64 ? go_heads<16>(kv, b, a, plan, s) : go_heads<32>(kv, b, a, plan, s);
     else if (kv.type == KV_F16)
         kv.hd <= 64 ? go_mma<KV_F16, 8>(kv, b, a, plan, s) : go_mma<KV_F16, 16>(kv, b, a, plan, s);
+    else if (kv.type == KV_Q8)
+        kv.hd <= 64 ? go_q8<4>(kv, b, a, plan, s) : go_q8<8>(kv, b, a, plan, s);
     else
         kv.hd <= 64 ? go_mma<KV_BF16, 8>(kv, b, a, plan, s) : go_mma<KV_BF16, 16>(kv, b, a, plan, s);
     if (plan.splits > 1) launch_paged_join(kv, b, a, plan.part_ml, plan.part_o, plan.chunk, plan.splits, s);
