@@ -406,7 +406,6 @@ struct DecodePlan {
 DecodePlan plan_paged_decode(const KvView &kv, const BatchView &b, const PagedAttnView &a, uint32_t max_kv_len);
 void launch_paged_decode(const KvView &kv, const BatchView &b, const PagedAttnView &a, const DecodePlan &plan,
                          cudaStream_t s);
-void launch_paged_q8(const KvView &kv, const BatchView &b, const PagedAttnView &a, cudaStream_t s);
 // Joins the partial results of a row's splits into out.  chunk > 0: splits of
 // `chunk` seen keys, of which only those that have a key were written;
 // chunk 0: every split was written.
@@ -422,6 +421,7 @@ struct RowsPlan {
     uint64_t ml_bytes, scratch_bytes;  // as in DecodePlan
 };
 RowsPlan plan_paged_rows(const KvView &kv, const BatchView &b, const PagedAttnView &a, uint32_t max_kv_len);
+void launch_paged_rows_q8(const KvView &kv, const BatchView &b, const PagedAttnView &a, const RowsPlan &plan, cudaStream_t s);
 void launch_paged_rows(const KvView &kv, const BatchView &b, const PagedAttnView &a, const RowsPlan &plan, cudaStream_t s);
 
 }  // namespace slm

@@ -624,24 +624,6 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(KvView kv, Ba
     }
 }
 
-// 8-bit pages, a warp per row and query head.
-__global__ void __launch_bounds__(PD_THREADS) paged_q8_kernel(KvView kv, BatchView b, PagedAttnView a) {
-    const uint64_t item = (uint64_t)blockIdx.x * PD_WARPS + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31, row = (int)(item / (unsigned)a.num_heads), h = (int)(item % (unsigned)a.num_heads);
-    if (row >= b.num_rows) return;
-    int seq, pos;
-    row_place(kv, b, row, seq, pos);
-    if (pos >= b.cap && lane == 0) paged_flag(kv, PAGED_BAD_POSITION);
-    const SeenKeys keys = seen_keys(b, pos, pos, a.window, a.sinks);
-    const RowState r = attend_row<KV_Q8>(kv, b, seq, h / (a.num_heads / kv.kv_heads),
-                                         a.q + (size_t)row * a.ldq + (size_t)h * kv.hd,
-                                         __fmul_rn(a.scale, 1.44269504088896340736f), keys, 0, keys.n, 0, 0, 0x7fffffff);
-    float *d = a.out + (size_t)row * a.ldo + (size_t)h * kv.hd;
-#pragma unroll
-    for (int c = 0; c < 4; c++)
-        if (lane + 32 * c < kv.hd) d[lane + 32 * c] = r.l == 0.f ? 0.f : __fdiv_rn(r.acc[c], r.l);
-}
-
 // 8-bit pages, on the tensor cores.
 //
 // A signed byte is exact in f16, so the bytes go into the MMAs as they are and a
@@ -978,11 +960,6 @@ void go_heads(const KvView &kv, const BatchView &b, const PagedAttnView &a, cons
 }
 
 }  // namespace
-
-void launch_paged_q8(const KvView &kv, const BatchView &b, const PagedAttnView &a, cudaStream_t s) {
-    const uint64_t items = (uint64_t)b.num_rows * a.num_heads;
-    paged_q8_kernel<<<(unsigned)((items + PD_WARPS - 1) / PD_WARPS), PD_THREADS, 0, s>>>(kv, b, a);
-}
 
 DecodePlan plan_paged_decode(const KvView &kv, const BatchView &b, const PagedAttnView &a, uint32_t max_kv_len) {
     DecodePlan p{};

@@ -982,7 +982,6 @@ SLM_EXPORT uint64_t slm_paged_attention_scratch_bytes(const slm_kv_pages *pages,
     BatchView b{};
     PagedAttnView a{};
     if (check_attention(pages, batch, args, &kv, &b, &a) != SLM_OK) return 0;
-    if (kv.type == KV_Q8 && b.row_start) return 0;
     return b.row_start ? plan_paged_rows(kv, b, a, batch->max_kv_len).scratch_bytes
                        : plan_paged_decode(kv, b, a, batch->max_kv_len).scratch_bytes;
 }
@@ -997,10 +996,6 @@ SLM_EXPORT int slm_paged_attention(const slm_kv_pages *pages, const slm_paged_ba
     if (b.num_rows == 0) return SLM_OK;
     if (!a.q || !a.out) return fail(SLM_ERR_INVALID_ARG, "null device pointer");
     if (a.q == a.out) return fail(SLM_ERR_OVERLAP, "out is q");
-    if (kv.type == KV_Q8 && b.row_start) {
-        launch_paged_q8(kv, b, a, (cudaStream_t)stream);
-        return launch_check("paged q8 kernel");
-    }
     if (!b.row_start) {
         DecodePlan plan = plan_paged_decode(kv, b, a, batch->max_kv_len);
         if ((uint64_t)b.num_seqs * kv.kv_heads * plan.head_groups * plan.splits > (uint64_t)INT32_MAX ||
