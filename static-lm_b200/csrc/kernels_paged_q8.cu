@@ -31,15 +31,15 @@ struct Q8Cfg {
     static constexpr int KT = 64;             // keys per tile: a thread holds a tile's scores in registers
     static constexpr bool Q_TMEM = HDP == 64;  // q's parts in TMEM (from shared memory an MMA of 64 columns takes 48 cycles, not 32)
     static constexpr int PRODUCERS = 96, THREADS = 384;
-    static constexpr int R_LAUNCH = 168, R_SOFTMAX = HDP == 64 ? 200 : 224, R_OTHER = HDP == 64 ? 104 : 56;
+    static constexpr int R_LAUNCH = 168, R_SOFTMAX = 208, R_OTHER = 88;
     static_assert(256 * R_SOFTMAX + (THREADS - 256) * R_OTHER == THREADS * R_LAUNCH, "registers");
     static constexpr int QPART = 128 * HDP * 2;
     static constexpr int STREAM = 2 * QPART;  // q's parts, and after them the results, f32
     static constexpr int SLOT = KT * HDP * 2;  // k and v of even and of odd tiles, f16
     static constexpr int RAW = KT * HDP;       // the same as bytes
     static constexpr int A_KV = 2 * STREAM, A_RAW = A_KV + 4 * SLOT, BIG = A_RAW + 4 * RAW;
-    // TMEM columns: scores / weights of (stream, parity) 64 each, q's parts, results
-    static constexpr int T_S = 64, T_Q = 256, T_O = Q_TMEM ? 384 : 256;
+    // TMEM columns, of both streams: scores from 0 on, weights, q's parts, results
+    static constexpr int T_W = 2 * KT, T_Q = 4 * KT, T_O = Q_TMEM ? T_Q + 128 : 256;
     static_assert(T_O + 2 * HDP <= (int)PQ_TMEM_COLS, "TMEM");
     // at least 120 KB: one CTA per SM, whose TMEM it takes whole
     static constexpr int SMALL = 3 * 1024, SMEM = (BIG > 120 * 1024 ? BIG : 120 * 1024) + SMALL;
@@ -48,7 +48,7 @@ struct Q8Cfg {
 
 // The small shared data, after the tiles.
 struct Q8Shared {
-    uint64_t full[4], empty[4], s_full[2][2], p_full[2], o_full[2], q_full[2], drain;
+    uint64_t full[4], empty[4], s_full[2], p_full[2], o_full[2], q_full[2], drain;
     long long off[64];        // byte offsets of the newest tile's keys
     alignas(16) float scale[4][2][64];  // of the keys and values of the newest 4 tiles
     unsigned valid[8][2];     // held keys of the newest 8 tiles
@@ -75,6 +75,16 @@ __device__ __forceinline__ bool pq_wait(uint64_t *bar, unsigned parity, Q8Shared
         }
     }
     return true;
+}
+
+// A load that is issued here, not where its result is used.
+__device__ __forceinline__ unsigned ldg_now(const void *p) {
+    unsigned v;
+    asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ void lds_b64x2(unsigned a, uint64_t &x, uint64_t &y) {
+    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(x), "=l"(y) : "r"(a));
 }
 
 // Bytes 0, 1 and 2, 3 of four signed ones as f16 pairs: 1024 + b + 128 is b + 128
@@ -121,8 +131,7 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
             mbar_init(&sh->empty[i], 1);
         }
         for (int x = 0; x < 2; x++) {
-            mbar_init(&sh->s_full[x][0], 1);
-            mbar_init(&sh->s_full[x][1], 1);
+            mbar_init(&sh->s_full[x], 1);
             mbar_init(&sh->p_full[x], 4);
             mbar_init(&sh->o_full[x], 1);
             mbar_init(&sh->q_full[x], 4);
@@ -173,7 +182,7 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
             const int row = row0 + (row_ok ? tok : 0);
             const int pos = row_ok ? pos0 + tok : -1;
             const unsigned t_lane = (unsigned)((warp & 3) * 32) << 16;
-            const unsigned t_s = t_lane + (unsigned)(x * 2 * Cfg::T_S), t_o = t_lane + (unsigned)(Cfg::T_O + x * HDP);
+            const unsigned t_s = t_lane + (unsigned)(x * KT), t_w = t_lane + (unsigned)(Cfg::T_W + x * KT), t_o = t_lane + (unsigned)(Cfg::T_O + x * HDP);
             float sl2;
             {  // the row of q in two parts, scaled so that its largest element is near 2^15
                 const float *src = a.q + (size_t)row * a.ldq + (size_t)(row_ok ? h : head * group) * hd;
@@ -238,10 +247,10 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
             const int sink_end = a.sinks < 0x7fffffffu ? (int)a.sinks : 0x7fffffff;
             int from = 0;
             if (a.window != 0 && pos >= 0 && (unsigned)pos >= a.window) from = pos - (int)a.window + 1 - keys.low + keys.sinks;
-            float m = NO_MAX, l = 0.f;
-            float acc[HDP];
+            float m = NO_MAX;
+            uint64_t l2 = 0, acc[HDP / 2];  // pairs
 #pragma unroll
-            for (int i = 0; i < HDP; i++) acc[i] = 0.f;
+            for (int i = 0; i < HDP / 2; i++) acc[i] = 0;
             bool ok = true;
             auto wait = [&](uint64_t *bar, int phase) {  // a warp goes on together: TMEM accesses are warp-wide
                 ok = __all_sync(0xffffffffu, ok && pq_wait(bar, (unsigned)phase & 1u, sh, kv));
@@ -251,7 +260,7 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
                 wait(&sh->o_full[x], j);
                 if (!ok) return;
                 tc_fence_after();
-                const float down = sh->down[j & 7];
+                const uint64_t down = pack2(sh->down[j & 7], sh->down[j & 7]);
 #pragma unroll
                 for (int c = 0; c < HDP; c += 32) {
                     float o[32];
@@ -259,94 +268,91 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
                     tmem_wait_ld();
                     pin32(o);
 #pragma unroll
-                    for (int i = 0; i < 32; i++) acc[c + i] = __fmaf_rn(o[i], down, acc[c + i]);
+                    for (int i = 0; i < 32; i += 2) acc[(c + i) / 2] = fma2(pack2(o[i], o[i + 1]), down, acc[(c + i) / 2]);
                 }
             };
+            const uint64_t sl2_2 = pack2(sl2, sl2);
             for (int j = 0; j < ntile; j++) {
-                wait(&sh->s_full[x][j & 1], j >> 1);
+                if (j > 0) gather(j - 1);  // which ends w.v of the weights whose place is taken next
+                wait(&sh->s_full[x], j);
                 if (!ok) break;
                 tc_fence_after();
-                const unsigned t_w = t_s + (unsigned)((j & 1) * Cfg::T_S);
-                float v[KT];
-                tmem_ld32(t_w, v);
-                tmem_ld32(t_w + 32, v + 32);
-                const float4 *k_scale = reinterpret_cast<const float4 *>(sh->scale[j & 3][0]);
-                const float4 *v_scale = reinterpret_cast<const float4 *>(sh->scale[j & 3][1]);
                 const int i0 = lo + j * KT;
                 const unsigned *valid = sh->valid[j & 7];
                 const bool whole = i0 + KT <= to && i0 + KT <= hi && (i0 + KT <= sink_end || i0 >= from) &&
                                    (valid[0] & valid[1]) == 0xffffffffu;
-                tmem_wait_ld();
-                pin32(v);
-                pin32(v + 32);
+                const bool masks = !__all_sync(0xffffffffu, whole);
+                // The weights by the reference as it is, and the largest score under way:
+                // where one has passed the reference by too much, all over again by a new
+                // one.  (A pass for the maximum alone before each tile: 601 us, 8 x 4096 rows.)
+                uint64_t l_before = l2;
+                for (;;) {
+                    const uint64_t minus_m = pack2(-m, -m);
+                    float top = -INFINITY;
+                    l2 = l_before;
+#pragma unroll 1
+                    for (int g = 0; g < 2; g++) {
+                        float v[32];
+                        tmem_ld32(t_s + g * 32, v);
+                        const unsigned k_scales = smem_addr(sh->scale[j & 3][0] + g * 32);
+                        const unsigned v_scales = smem_addr(sh->scale[j & 3][1] + g * 32);
+                        uint64_t s[16];
 #pragma unroll
-                for (int c = 0; c < KT; c += 4) {
-                    const float4 s = k_scale[c / 4];
-                    v[c] = __fmul_rn(v[c], s.x);
-                    v[c + 1] = __fmul_rn(v[c + 1], s.y);
-                    v[c + 2] = __fmul_rn(v[c + 2], s.z);
-                    v[c + 3] = __fmul_rn(v[c + 3], s.w);
-                }
-                if (!__all_sync(0xffffffffu, whole)) {
+                        for (int i = 0; i < 16; i += 2) lds_b64x2(k_scales + i * 8, s[i], s[i + 1]);
+                        tmem_wait_ld();
+                        pin32(v);
+                        uint64_t y[16];
 #pragma unroll
-                    for (int g = 0; g < KT; g += 32) {
-                        // bit c: list position i0 + g + c is seen
-                        auto below = [&](int end) -> unsigned {
-                            const int n = end - (i0 + g);
-                            return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
-                        };
-                        const unsigned seen = below(to) & (below(sink_end) | ~below(from)) & valid[g >> 5];
+                        for (int i = 0; i < 16; i++) y[i] = mul2(pack2(v[2 * i], v[2 * i + 1]), s[i]);
+                        if (masks) {
+                            // bit c: list position i0 + 32 g + c is seen
+                            auto below = [&](int end) -> unsigned {
+                                const int n = end - (i0 + g * 32);
+                                return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+                            };
+                            const unsigned seen = below(to) & (below(sink_end) | ~below(from)) & valid[g];
 #pragma unroll
-                        for (int c = 0; c < 32; c++) v[g + c] = seen & (1u << c) ? v[g + c] : -INFINITY;
+                            for (int i = 0; i < 16; i++) {
+                                float s0, s1;
+                                unpack2(y[i], s0, s1);
+                                y[i] = pack2(seen & (1u << (2 * i)) ? s0 : -INFINITY, seen & (1u << (2 * i + 1)) ? s1 : -INFINITY);
+                            }
+                        }
+                        unsigned w[2][16];
+#pragma unroll
+                        for (int i = 0; i < 16; i += 2) {
+                            uint64_t vs[2];
+                            lds_b64x2(v_scales + i * 8, vs[0], vs[1]);
+#pragma unroll
+                            for (int u = 0; u < 2; u++) {
+                                float e0, e1;
+                                unpack2(y[i + u], e0, e1);
+                                top = fmaxf(top, fmaxf(e0, e1));
+                                unpack2(fma2(y[i + u], sl2_2, minus_m), e0, e1);
+                                const uint64_t e = pack2(exp2_approx(e0), exp2_approx(e1));
+                                l2 = add2(l2, e);
+                                unpack2(mul2(e, vs[u]), e0, e1);
+                                unsigned part[2];
+                                split2<KV_F16, 2>(e0, e1, part);
+                                w[0][i + u] = part[0], w[1][i + u] = part[1];
+                            }
+                        }
+                        // part n of 32 keys at column 16 n
+                        tmem_st16(t_w + g * 32, w[0]);
+                        tmem_st16(t_w + g * 32 + 16, w[1]);
                     }
-                }
-                float t0 = v[0], t1 = v[1], t2 = v[2], t3 = v[3];
+                    top = __fmul_rn(top, sl2);
+                    const bool move = top > m + Range::rescale;
+                    if (!__any_sync(0xffffffffu, move)) break;
+                    if (move) {
+                        const float to_m = __fsub_rn(top, Range::margin);
+                        const float f = exp2_approx(__fsub_rn(m, to_m));
+                        m = to_m;
+                        const uint64_t f2 = pack2(f, f);
+                        l_before = mul2(l_before, f2);
 #pragma unroll
-                for (int c = 4; c < KT; c += 4) {
-                    t0 = fmaxf(t0, v[c]);
-                    t1 = fmaxf(t1, v[c + 1]);
-                    t2 = fmaxf(t2, v[c + 2]);
-                    t3 = fmaxf(t3, v[c + 3]);
-                }
-                const float top = __fmul_rn(fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)), sl2);
-                float f = 1.0f;
-                const bool moved = __any_sync(0xffffffffu, top > m + Range::rescale);
-                if (moved && top > m + Range::rescale) {
-                    const float to_m = __fsub_rn(top, Range::margin);
-                    f = exp2_approx(__fsub_rn(m, to_m));
-                    m = to_m;
-                    l = __fmul_rn(l, f);
-                }
-                // every score of the tile is in registers: the weights take their place
-#pragma unroll
-                for (int c = 0; c < KT; c += 32) {
-                    float s0 = 0.f, s1 = 0.f;
-                    unsigned w[2][16];
-#pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const float4 s = v_scale[(c + i) / 4];
-                        float e[4];
-#pragma unroll
-                        for (int u = 0; u < 4; u++) e[u] = exp2_approx(__fmaf_rn(v[c + i + u], sl2, -m));
-                        s0 = __fadd_rn(s0, __fadd_rn(e[0], e[2]));
-                        s1 = __fadd_rn(s1, __fadd_rn(e[1], e[3]));
-                        unsigned p[2];
-                        split2<KV_F16, 2>(__fmul_rn(e[0], s.x), __fmul_rn(e[1], s.y), p);
-                        w[0][i / 2] = p[0], w[1][i / 2] = p[1];
-                        split2<KV_F16, 2>(__fmul_rn(e[2], s.z), __fmul_rn(e[3], s.w), p);
-                        w[0][i / 2 + 1] = p[0], w[1][i / 2 + 1] = p[1];
+                        for (int i = 0; i < HDP / 2; i++) acc[i] = mul2(acc[i], f2);
                     }
-                    l = __fadd_rn(l, __fadd_rn(s0, s1));
-                    tmem_st16(t_w + c / 2, w[0]);
-                    tmem_st16(t_w + KT / 2 + c / 2, w[1]);
-                }
-                if (j > 0) {  // before w.v of this tile takes the place of the last one's
-                    gather(j - 1);
-                    if (!ok) break;
-                }
-                if (moved) {
-#pragma unroll
-                    for (int i = 0; i < HDP; i++) acc[i] = __fmul_rn(acc[i], f);
                 }
                 tmem_wait_st();
                 tc_fence_before();
@@ -355,6 +361,9 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
             if (ok && ntile > 0) gather(ntile - 1);
             // (a warp that broke off leaves the others' waits to give up: all meet here)
             if (!named_bar_or(2 + x, 128, !ok)) {
+                float l, l_odd;
+                unpack2(l2, l, l_odd);
+                l = __fadd_rn(l, l_odd);
                 const bool split_up = plan.splits > 1;
                 const float inv = split_up ? 1.0f : l == 0.f ? 0.f : __fdiv_rn(1.0f, l);
                 // Once a reference was set, l is 2^margin or more, but for scores past
@@ -365,7 +374,9 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
                 float4 *s_o = reinterpret_cast<float4 *>(pq_smem + x * Cfg::STREAM + (warp & 3) * 32 * HDP * 4);
 #pragma unroll
                 for (int i = 0; i < HDP; i += 4) {
-                    float y[4] = {acc[i], acc[i + 1], acc[i + 2], acc[i + 3]};
+                    float y[4];
+                    unpack2(acc[i / 2], y[0], y[1]);
+                    unpack2(acc[i / 2 + 1], y[2], y[3]);
 #pragma unroll
                     for (int u = 0; u < 4; u++) {
                         y[u] = __fmul_rn(y[u], inv);
@@ -431,40 +442,54 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
                 ok = __all_sync(0xffffffffu, ok && pq_wait(bar, (unsigned)phase & 1u, sh, kv));
                 tc_fence_after();
             };
-            // tile j, of parity P, stream X: every operand is a constant; the second parts' products first
+            // A descriptor is a base's low word plus a constant (in 16 bytes; no carry: the
+            // address has 14 bits there).  The base is made anew for every tile, else
+            // all the descriptors are kept, more than the registers hold.
+            auto plus = [](unsigned base, unsigned bytes, uint64_t of) -> uint64_t {
+                return (of & 0xffffffff00000000ull) | (base + (bytes >> 4));
+            };
+            auto base_of = [](uint64_t desc) -> unsigned {
+                unsigned lo = (unsigned)desc;
+                asm volatile("" : "+r"(lo));
+                return lo;
+            };
+            // k of slot parity P, stream X; the second parts' products first
             auto scores = [&](auto parity, auto stream) {
                 constexpr int P = decltype(parity)::value, X = decltype(stream)::value;
-                constexpr unsigned d = (X * 2 + P) * Cfg::T_S;
+                const uint64_t k_desc = umma_desc_sw128(a_kv + 2 * P * Cfg::SLOT), q_desc = umma_desc_sw128(a_q + X * Cfg::STREAM);
+                const unsigned k_base = base_of(k_desc), q_base = base_of(q_desc);
 #pragma unroll
                 for (int i = 1; i >= 0; i--)
 #pragma unroll
                     for (int ks = 0; ks < HDP / 16; ks++) {
-                        const uint64_t bd = umma_desc_sw128(a_kv + 2 * P * Cfg::SLOT + (ks >> 2) * KT * 128 + (ks & 3) * 32);
+                        const uint64_t bd = plus(k_base, (ks >> 2) * KT * 128 + (ks & 3) * 32, k_desc);
                         if constexpr (Cfg::Q_TMEM) {
                             const unsigned at = Cfg::T_Q + X * 64 + i * 32 + ks * 8;
                             if (i == 0 && ks == 0)
-                                tc_mma_f16_ta_onto_part2(d, at, bd, idesc_s);
+                                tc_mma_f16_ta_onto_part2(X * KT, at, bd, idesc_s);
                             else
-                                tc_mma_f16_ta(d, at, bd, idesc_s, i == 0 || ks > 0);
+                                tc_mma_f16_ta(X * KT, at, bd, idesc_s, i == 0 || ks > 0);
                         } else {
-                            const uint64_t ad = umma_desc_sw128(a_q + X * Cfg::STREAM + i * Cfg::QPART + (ks >> 2) * 128 * 128 + (ks & 3) * 32);
+                            const uint64_t ad = plus(q_base, i * Cfg::QPART + (ks >> 2) * 128 * 128 + (ks & 3) * 32, q_desc);
                             if (i == 0 && ks == 0)
-                                tc_mma_f16_onto_part2(d, ad, bd, idesc_s);
+                                tc_mma_f16_onto_part2(X * KT, ad, bd, idesc_s);
                             else
-                                tc_mma_f16(d, ad, bd, idesc_s, i == 0 || ks > 0);
+                                tc_mma_f16(X * KT, ad, bd, idesc_s, i == 0 || ks > 0);
                         }
                     }
-                tc_commit_elected(&sh->s_full[X][P]);
+                tc_commit_elected(&sh->s_full[X]);
             };
             auto values = [&](auto parity, auto stream) {
                 constexpr int P = decltype(parity)::value, X = decltype(stream)::value;
                 constexpr unsigned d = Cfg::T_O + X * HDP;
+                const uint64_t v_desc = umma_desc_sw128_mn(a_kv + (2 * P + 1) * Cfg::SLOT, KT * 128);
+                const unsigned v_base = base_of(v_desc);
 #pragma unroll
                 for (int i = 1; i >= 0; i--)
 #pragma unroll
                     for (int ks = 0; ks < KT / 16; ks++) {
-                        const unsigned at = (X * 2 + P) * Cfg::T_S + i * (KT / 2) + ks * 8;
-                        const uint64_t bd = umma_desc_sw128_mn(a_kv + (2 * P + 1) * Cfg::SLOT + ks * 2048, KT * 128);
+                        const unsigned at = Cfg::T_W + X * KT + (ks >> 1) * 32 + i * 16 + (ks & 1) * 8;
+                        const uint64_t bd = plus(v_base, ks * 2048, v_desc);
                         if (i == 0 && ks == 0)
                             tc_mma_f16_ta_onto_part2(d, at, bd, idesc_o);
                         else
@@ -474,40 +499,46 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
             };
             const std::integral_constant<int, 0> zero{};
             const std::integral_constant<int, 1> one{};
-            // q.k of tile j for both streams; it goes over the weights of tile j - 2,
-            // which its w.v, issued before, has read by then
-            auto all_scores = [&](auto parity, int j) {
+            // w.v of tile j, then q.k of tile j + 1 in the place of the scores that the
+            // weights were made of, stream by stream
+            auto step = [&](auto parity, int j) {
                 constexpr int P = decltype(parity)::value;
-                wait(&sh->full[2 * P], j >> 1);
-                fence_async_elected();
-                if (!ok) return;
-                scores(parity, zero);
-                if (streams == 2) scores(parity, one);
-                tc_commit_elected(&sh->empty[2 * P]);
-            };
-            auto all_values = [&](auto parity, int j) {
-                constexpr int P = decltype(parity)::value;
+                const std::integral_constant<int, 1 - P> other{};
+                const bool more = j + 1 < ntile;
                 wait(&sh->full[2 * P + 1], j >> 1);
-                fence_async_elected();
                 wait(&sh->p_full[0], j);
+                fence_async_elected();
                 if (!ok) return;
                 values(parity, zero);
+                if (more) {
+                    wait(&sh->full[2 * (1 - P)], (j + 1) >> 1);
+                    fence_async_elected();
+                    if (!ok) return;
+                    scores(other, zero);
+                }
                 if (streams == 2) {
                     wait(&sh->p_full[1], j);
                     if (!ok) return;
                     values(parity, one);
                 }
                 tc_commit_elected(&sh->empty[2 * P + 1]);
+                if (more) {
+                    if (streams == 2) scores(other, one);
+                    tc_commit_elected(&sh->empty[2 * (1 - P)]);
+                }
             };
             wait(&sh->q_full[0], 0);
-            if (streams == 2) wait(&sh->q_full[1], 0);
-            if (ok) all_scores(zero, 0);
+            wait(&sh->full[0], 0);
+            fence_async_elected();
+            if (ok) scores(zero, zero);
+            if (streams == 2) {
+                wait(&sh->q_full[1], 0);
+                if (ok) scores(zero, one);
+            }
+            if (ok) tc_commit_elected(&sh->empty[0]);
             for (int j = 0; j < ntile && ok; j += 2) {
-                if (j + 1 < ntile) all_scores(one, j + 1);
-                if (ok) all_values(zero, j);
-                if (j + 1 == ntile || !ok) break;
-                if (j + 2 < ntile) all_scores(zero, j + 2);
-                if (ok) all_values(one, j + 1);
+                step(zero, j);
+                if (j + 1 < ntile && ok) step(one, j + 1);
             }
             // what was issued has to end before the TMEM is freed
             tc_commit_elected(&sh->drain);
@@ -526,17 +557,30 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
         const int c = p % CH, r_first = p / CH;
         const bool in_row = c * 16 < hd;
         bool ok = true;
+        // Key p of a tile: its page id is on its way for a tile while that of the
+        // tile before is made offsets, whose scales are on theirs.
+        struct Id {
+            int page;
+            unsigned slot;
+        };
         struct At {
             long long row;  // byte offset in the pools, -1 for none
             float k_scale, v_scale;
         };
-        auto find = [&](int j) -> At {  // key p of tile j
+        auto look = [&](int j) -> Id {
             const int at = lo + j * KT + p;
-            unsigned slot;
-            const int page = p < KT && at < hi ? key_page(kv, b, seq, (unsigned)keys.key(at), slot) : -1;
-            if (page < 0) return At{-1, 0.f, 0.f};
-            const long long s = scale_offset(kv, page, head, slot);
-            return At{row_offset(kv, page, head, slot), scale_get(kv.k, s), scale_get(kv.v, s)};
+            if (p >= KT || at >= hi) return Id{-1, 0};  // (every list position is below the table's end)
+            const unsigned key = (unsigned)keys.key(at), pi = page_index(kv, key);
+            return Id{(int)ldg_now(b.table + (size_t)seq * b.table_stride + pi), key - pi * (unsigned)kv.page_size};
+        };
+        auto find = [&](Id id) -> At {
+            if ((unsigned)id.page >= (unsigned)kv.num_pages) {
+                if (id.page >= 0) paged_flag(kv, PAGED_BAD_PAGE);
+                return At{-1, 0.f, 0.f};
+            }
+            const long long s = scale_offset(kv, id.page, head, id.slot);
+            return At{row_offset(kv, id.page, head, id.slot), __uint_as_float(ldg_now(reinterpret_cast<const char *>(kv.k) + s)),
+                      __uint_as_float(ldg_now(reinterpret_cast<const char *>(kv.v) + s))};
         };
         // tile j's bytes, by the thread that will turn them into f16
         auto copy = [&](int j) {
@@ -561,19 +605,23 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
             if (!ok) return;
             const unsigned char *raw = pq_smem + Cfg::A_RAW + ((j & 1) * 2 + i) * Cfg::RAW + p * 16;
             unsigned char *dst = pq_smem + Cfg::A_KV + s * Cfg::SLOT;
+            uint4 w[PASSES];
+#pragma unroll
+            for (int n = 0; n < PASSES; n++)
+                if (r_first + n * RSTEP < KT) w[n] = *reinterpret_cast<const uint4 *>(raw + n * Cfg::PRODUCERS * 16);
 #pragma unroll
             for (int n = 0; n < PASSES; n++) {
                 const int row = r_first + n * RSTEP;
                 if (row >= KT) break;
-                const uint4 w = *reinterpret_cast<const uint4 *>(raw + n * Cfg::PRODUCERS * 16);
-                const uint2 b0 = bytes_f16(w.x), b1 = bytes_f16(w.y), b2 = bytes_f16(w.z), b3 = bytes_f16(w.w);
+                const uint2 b0 = bytes_f16(w[n].x), b1 = bytes_f16(w[n].y), b2 = bytes_f16(w[n].z), b3 = bytes_f16(w[n].w);
                 *reinterpret_cast<uint4 *>(dst + sw16_off(row, 2 * c, KT)) = make_uint4(b0.x, b0.y, b1.x, b1.y);
                 *reinterpret_cast<uint4 *>(dst + sw16_off(row, 2 * c + 1, KT)) = make_uint4(b2.x, b2.y, b3.x, b3.y);
             }
-            fence_async_smem();
+            // (the MMA warp orders these stores before its own accesses)
             mbar_arrive(&sh->full[s]);
         };
-        At next = find(0);
+        At next = find(look(0));
+        Id ahead = look(1);
         for (int j = 0; j < ntile && ok; j++) {
             // tile j's offsets and scales for all, its copies on their way, then the next tile's look-ups
             if (warp < 11) {
@@ -593,7 +641,8 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
                 sh->scale[j & 3][1][p] = __fmul_rn(next.v_scale, __uint_as_float((unsigned)(127 - e) << 23));
                 if (p == 0) sh->down[j & 7] = __uint_as_float((unsigned)(127 + e) << 23);
             }
-            if (j + 1 < ntile) next = find(j + 1);
+            next = find(ahead);
+            ahead = look(j + 2);
             if (j > 0) {
                 cp_async_wait<1>();
                 convert(j - 1, 0);
