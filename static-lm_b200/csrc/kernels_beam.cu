@@ -13,9 +13,10 @@ namespace slm {
 
 namespace {
 
-constexpr int BS_THREADS = 256, BS_WARPS = BS_THREADS / 32;
-constexpr int BS_PER = 16, BS_CHUNK = BS_THREADS * BS_PER;  // logits of a thread, and of a CTA, at a time
 constexpr int BS_MAX_OUT = 64;
+constexpr int BS_THREADS = 128, BS_WARPS = BS_THREADS / 32;
+constexpr int BS_STAGES = 3, BS_PER = 16, BS_CHUNK = 32 * BS_PER;  // logits of a lane, and of a warp, at a time
+constexpr int BJ_THREADS = 256, BJ_WARPS = BJ_THREADS / 32, BS_MAX_PARTS = 128;
 
 // Logit and token as one number: larger for a larger logit, and for the lower
 // token of two that are equal.  Zeros of either sign are equal.
@@ -41,57 +42,137 @@ __device__ __forceinline__ bool row_lives(const BeamView &a, int row) {
     return fabsf(a.scores[row]) < INFINITY && !(a.ended && a.ended[row] != 0);
 }
 
-// CTA (row, part).  The list of the part's best so far has a threshold, its
-// num_out-th: most chunks hold no logit above it, and cost a maximum, an exp and
-// a vote.  Where more pass than the buffer takes (the first chunk, rising
-// logits), the num_out-th largest of the threads' own maxima is a bound below
-// which nothing can be among the best, and at most 16 num_out pass that.
-template <bool VEC>
-__global__ void __launch_bounds__(BS_THREADS) beam_part_kernel(BeamView a, BeamPlan plan) {
-    __shared__ uint64_t s_cand[17 * BS_MAX_OUT], s_best[BS_MAX_OUT], s_top[BS_THREADS];
-    __shared__ int s_count[BS_WARPS];
+// CTA (row, part); its warps take chunks of 512 logits in turn, each through its
+// own ring of cp.async stages.  A chunk costs a maximum, an exp and a vote unless a
+// logit reaches the CTA's threshold, a number that num_out of its logits are known
+// to reach: those that do go one by one into the warp's best so far, a list over
+// its lanes, rank r in lane r (and r - 32), by a count of the ranks above and a
+// shift.  The threshold is first a bound from the first chunks, by the lanes' own
+// largest; then the least of num_out slots in shared memory, the least of which
+// every logit that passes replaces (where two warps replace the same one the
+// smaller is lost there, and the threshold only lower than it could be); or the
+// last place of a warp's full list.  Where more than a few of a chunk reach it
+// (rising logits), the chunk's own bound comes first: at most 16 num_out are not
+// below that.  No warp waits for another but after the first chunk and before the
+// lists are merged.
+// 256 rows of 131072 (134 MB, 20 us), both launches: one list a CTA, with a barrier
+// a chunk, 85 us; a list a warp without a common threshold 63; with the least of
+// the warps' own places as the threshold, loads to registers, 55.
+template <bool VEC, bool TWO>
+__global__ void __launch_bounds__(BS_THREADS, 8) beam_part_kernel(BeamView a, BeamPlan plan) {
+    extern __shared__ __align__(16) float s_ring[];  // [warp][stage][512]
+    __shared__ uint64_t s_best[BS_WARPS * BS_MAX_OUT];
+    __shared__ unsigned long long s_least;
+    __shared__ volatile uint64_t s_place[BS_WARPS];  // the warps' r-th best
     __shared__ float s_m[BS_WARPS];
     __shared__ double s_s[BS_WARPS];
     pdl_release();
-    const int row = blockIdx.x / plan.parts, part = blockIdx.x % plan.parts;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.num_out, cap = 17 * K;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, K = a.num_out;
+    const int row = (int)(blockIdx.x / (unsigned)plan.parts), part = (int)(blockIdx.x % (unsigned)plan.parts);
     if (!row_lives(a, row)) return;  // the join knows
     const int begin = part * plan.part, end = min(a.vocab, begin + plan.part);
     const float *x = a.logits + (size_t)row * a.ld;
-    auto token = [&](int at, int i) { return VEC ? at + (i >> 2) * (4 * BS_THREADS) + tid * 4 + (i & 3) : at + i * BS_THREADS + tid; };
-    auto load = [&](int at, float (&v)[BS_PER]) {
-        if constexpr (VEC) {
+    float *const ring = s_ring + warp * (BS_STAGES * BS_CHUNK);
+    // element i of this lane in a chunk
+    auto place = [&](int i, int l) { return (i >> 2) * 128 + l * 4 + (i & 3); };
+    auto fetch = [&](int at, int stage) {
+        const unsigned dst = smem_addr(ring + stage * BS_CHUNK);
+        if (at < end) {
+            if constexpr (VEC) {  // (rows are multiples of 16 bytes apart: what is past the row's end is not read)
 #pragma unroll
-            for (int i = 0; i < BS_PER; i += 4) {
-                const int t = token(at, i);
-                float4 f = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                if (t + 3 < end) {
-                    f = *reinterpret_cast<const float4 *>(x + t);
-                } else if (t < end) {
-                    f.x = x[t];
-                    if (t + 1 < end) f.y = x[t + 1];
-                    if (t + 2 < end) f.z = x[t + 2];
+                for (int i = 0; i < BS_PER; i += 4) {
+                    const int o = place(i, lane), n = min(max(end - at - o, 0), 4);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst + o * 4), "l"(x + (n ? at + o : 0)), "r"(n * 4));
                 }
-                v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
-            }
-        } else {
+            } else {
 #pragma unroll
-            for (int i = 0; i < BS_PER; i++) {
-                const int t = token(at, i);
-                v[i] = t < end ? x[t] : -INFINITY;
+                for (int i = 0; i < BS_PER; i++) {
+                    const int o = i * 32 + lane;
+                    const bool in = at + o < end;
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst + o * 4), "l"(x + (in ? at + o : 0)),
+                                 "r"(in ? 4u : 0u));
+                }
             }
+        }
+        cp_async_commit();
+    };
+    auto load = [&](int at, int stage, float (&v)[BS_PER]) {
+        const unsigned src = smem_addr(ring + stage * BS_CHUNK);
+#pragma unroll
+        for (int i = 0; i < BS_PER; i += 4) {
+            const float4 f = lds_f32x4(src + place(i, lane) * 4);
+            v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
+        }
+        if (at + BS_CHUNK > end) {
+#pragma unroll
+            for (int i = 0; i < BS_PER; i++) v[i] = at + place(i, lane) < end ? v[i] : -INFINITY;
         }
 #pragma unroll
         for (int i = 0; i < BS_PER; i++) v[i] = fmaxf(v[i], -INFINITY);  // NaN is no candidate and adds nothing
     };
-    float m = -INFINITY, s = 0.f, least = -INFINITY;  // least: of the list, once it is full
-    int held = 0;
-    for (int at = begin; at < end; at += BS_CHUNK) {
+    constexpr int STEP = BS_WARPS * BS_CHUNK;
+    const int first = begin + warp * BS_CHUNK;
+#pragma unroll
+    for (int i = 0; i < BS_STAGES - 1; i++) fetch(first + i * STEP, i);
+    const int r = (K + BS_WARPS - 1) / BS_WARPS - 1;  // (below 16)
+    if (threadIdx.x < BS_WARPS) s_place[threadIdx.x] = 0;
+    if (threadIdx.x == 0) s_least = 0;
+    __syncthreads();
+    float m = -INFINITY, s = 0.f;
+    uint64_t low = 0;         // the threshold as this warp last saw it; 0: none
+    float least = -FLT_MAX;   // its logit (-infinity is no candidate)
+    auto see = [&](uint64_t key) {
+        if (key > low) low = key, least = key_logit(key);
+    };
+    uint64_t k0 = 0, k1 = 0;  // ranks lane and 32 + lane; 0: none
+    auto last = [&]() -> uint64_t { return __shfl_sync(0xffffffffu, TWO && K > 32 ? k1 : k0, (K - 1) & 31); };
+    auto insert = [&](uint64_t key) {
+        const int above = __popc(__ballot_sync(0xffffffffu, k0 > key));
+        const uint64_t up = __shfl_up_sync(0xffffffffu, k0, 1);
+        if constexpr (TWO) {
+            const int above1 = above + __popc(__ballot_sync(0xffffffffu, k1 > key));
+            uint64_t up1 = __shfl_up_sync(0xffffffffu, k1, 1);
+            const uint64_t carry = __shfl_sync(0xffffffffu, k0, 31);
+            if (lane == 0) up1 = carry;
+            if (lane + 32 > above1) k1 = up1;
+            if (lane + 32 == above1) k1 = key;
+        }
+        if (lane > above) k0 = up;
+        if (lane == above) k0 = key;
+    };
+    int stage = 0;
+    for (int at = first; at < end || at == first; at += STEP) {
+        cp_async_wait<BS_STAGES - 2>();
+        __syncwarp();
         float v[BS_PER];
-        load(at, v);
+        load(at, stage, v);
+        const int here = stage * BS_CHUNK;
+        fetch(at + (BS_STAGES - 1) * STEP, stage == 0 ? BS_STAGES - 1 : stage - 1);
+        stage = stage == BS_STAGES - 1 ? 0 : stage + 1;
         float top = v[0];
 #pragma unroll
         for (int i = 1; i < BS_PER; i++) top = fmaxf(top, v[i]);
+        if (at == first) {
+            // a first threshold: num_out lanes' largest reach it (up to 32), or all lanes' second largest
+            float bound;
+            if (TWO && K > 32) {
+                float two = -INFINITY, one = v[0];
+#pragma unroll
+                for (int i = 1; i < BS_PER; i++) two = fmaxf(two, fminf(one, v[i])), one = fmaxf(one, v[i]);
+                bound = -warp_max_nan(-two);
+            } else {
+                float rest = top;
+                int n = 0;
+                do {
+                    bound = warp_max_nan(rest);
+                    n += __popc(__ballot_sync(0xffffffffu, rest == bound));
+                    if (rest == bound) rest = -INFINITY;
+                } while (n < K && bound > -INFINITY);
+            }
+            if (lane == 0 && bound > -INFINITY) atomicMax(&s_least, (unsigned long long)(beam_key(bound, 0) | 0xffffffffu) - 0xffffffffull - 1);
+            __syncthreads();
+        }
+        see(*(volatile unsigned long long *)&s_least);
         if (top > m) {
             s = __fmul_rn(s, exp2_approx(__fmul_rn(__fsub_rn(m, top), 1.44269504088896340736f)));
             m = top;
@@ -105,114 +186,82 @@ __global__ void __launch_bounds__(BS_THREADS) beam_part_kernel(BeamView a, BeamP
             }
             s = __fadd_rn(s, __fadd_rn(s0, s1));
         }
-        if (!__syncthreads_or(top > least)) continue;
-        uint64_t bound = 0;
-        int mine = 0, base = 0, total = 0;
-        auto count = [&]() {  // of this thread's that pass, its place among all, and all
-            mine = 0;
+        if (!__any_sync(0xffffffffu, top >= least)) continue;
+        unsigned pass = 0;  // of this lane's
 #pragma unroll
-            for (int i = 0; i < BS_PER; i++) mine += v[i] > least && beam_key(v[i], token(at, i)) >= bound;
-            int sum = mine;
+        for (int i = 0; i < BS_PER; i++) pass |= (unsigned)(v[i] >= least) << i;
+        if (__reduce_add_sync(0xffffffffu, __popc(pass)) > 32u) {
+            uint64_t one = 0, two = 0;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int t = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= o) sum += t;
+            for (int i = 0; i < BS_PER; i++) {
+                const uint64_t key = pass >> i & 1u ? beam_key(v[i], at + place(i, lane)) : 0;
+                if (key > one)
+                    two = one, one = key;
+                else if (TWO && key > two)
+                    two = key;
             }
-            if (lane == 31) s_count[warp] = sum;
-            __syncthreads();
-            base = sum - mine;
-            total = 0;
-#pragma unroll
-            for (int w = 0; w < BS_WARPS; w++) {
-                if (w < warp) base += s_count[w];
-                total += s_count[w];
-            }
-        };
-        count();
-        if (held + total > cap) {
-            float best = v[0];
-            int which = 0;
-#pragma unroll
-            for (int i = 1; i < BS_PER; i++)
-                if (v[i] > best) best = v[i], which = i;
-            s_top[tid] = best > least ? beam_key(best, token(at, which)) : 0;
-            __syncthreads();
-            if (warp == 0) {
-                uint64_t t[BS_WARPS], one = 0;
-#pragma unroll
-                for (int i = 0; i < BS_WARPS; i++) t[i] = s_top[i * 32 + lane];
+            uint64_t bound = 0;
+            if (TWO && K > 32) {
+                bound = ~warp_max64(~two);
+            } else {
                 for (int k = 0; k < K; k++) {
-                    uint64_t mx = 0;
-#pragma unroll
-                    for (int i = 0; i < BS_WARPS; i++) mx = t[i] > mx ? t[i] : mx;
-                    one = warp_max64(mx);
-#pragma unroll
-                    for (int i = 0; i < BS_WARPS; i++) t[i] = t[i] == one ? 0 : t[i];
+                    bound = warp_max64(one);
+                    if (one == bound) one = 0;
                 }
-                if (lane == 0) s_top[0] = one;
             }
-            __syncthreads();
-            bound = s_top[0];
-            count();
-        }
-        int place = held + base;
+            if (bound) see(bound - 1);
+            pass = 0;
 #pragma unroll
-        for (int i = 0; i < BS_PER; i++) {
-            if (mine && v[i] > least) {
-                const uint64_t key = beam_key(v[i], token(at, i));
-                if (key >= bound) s_cand[place++] = key;
+            for (int i = 0; i < BS_PER; i++) pass |= (unsigned)(v[i] >= least && beam_key(v[i], at + place(i, lane)) > low) << i;
+        }
+        for (unsigned lanes = __ballot_sync(0xffffffffu, pass); lanes; lanes &= lanes - 1) {
+            const int l = __ffs(lanes) - 1;
+            for (unsigned its = __shfl_sync(0xffffffffu, pass, l); its; its &= its - 1) {
+                const int o = place(__ffs(its) - 1, l);
+                const uint64_t key = beam_key(ring[here + o], at + o);
+                if (key <= low) continue;
+                insert(key);
+                see(last());
             }
         }
-        held += total;
-        __syncthreads();
-        if (held > K) {  // every candidate's rank; the first K stay, in order
-            for (int e = tid; e < held; e += BS_THREADS) {
-                const uint64_t key = s_cand[e];
-                int rank = 0;
-                for (int o = 0; o < held; o++) rank += s_cand[o] > key;
-                if (rank < K) s_best[rank] = key;
-            }
-            __syncthreads();
-            if (tid < K) s_cand[tid] = s_best[tid];
-            held = K;
-            least = key_logit(s_best[K - 1]);
-            __syncthreads();
-        } else if (held == K) {
-            uint64_t low = s_cand[0];
-            for (int o = 1; o < held; o++) low = s_cand[o] < low ? s_cand[o] : low;
-            least = key_logit(low);
-        }
+        // (places only rise: one that is read late is a lower bound too)
+        const uint64_t mine = __shfl_sync(0xffffffffu, k0, r);
+        if (lane == 0) s_place[warp] = mine;
+        const uint64_t all = ~warp_max64(lane < BS_WARPS ? ~(lane == warp ? mine : s_place[lane]) : 0);
+        if (all) see(all - 1);
+        if (lane == 0 && low > *(volatile unsigned long long *)&s_least) atomicMax(&s_least, (unsigned long long)low);
     }
-    // the list, sorted, and the part's maximum and sum
+    cp_async_wait<0>();
+    // the warps' lists become one
+    if (lane < K) s_best[warp * K + lane] = k0;
+    if (TWO && lane + 32 < K) s_best[warp * K + lane + 32] = k1;
+    const size_t list = (size_t)row * plan.parts + part;
     float all = m;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
-    if (lane == 0) s_m[warp] = all;
-    __syncthreads();
-    all = s_m[0];
-#pragma unroll
-    for (int w = 1; w < BS_WARPS; w++) all = fmaxf(all, s_m[w]);
     double sum = m > -INFINITY ? (double)__fmul_rn(s, exp2_approx(__fmul_rn(__fsub_rn(m, all), 1.44269504088896340736f))) : 0.0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) s_s[warp] = sum;
+    if (lane == 0) s_m[warp] = all, s_s[warp] = sum;
     __syncthreads();
-    const size_t list = (size_t)row * plan.parts + part;
-    if (tid == 0) {
+    if (threadIdx.x == BS_THREADS - 1) {
+        all = s_m[0];
+        for (int w = 1; w < BS_WARPS; w++) all = fmaxf(all, s_m[w]);
         sum = 0.0;
-        for (int w = 0; w < BS_WARPS; w++) sum += s_s[w];
+        for (int w = 0; w < BS_WARPS; w++)
+            if (s_m[w] > -INFINITY) sum += s_s[w] * exp((double)s_m[w] - (double)all);
         plan.part_ms[list] = make_double2((double)all, sum);
     }
     uint64_t *best = plan.part_best + list * K;
-    for (int e = tid; e < K; e += BS_THREADS) {
-        if (e < held) {
-            const uint64_t key = s_cand[e];
-            int rank = 0;
-            for (int o = 0; o < held; o++) rank += s_cand[o] > key;
-            best[rank] = key;
-        } else {
-            best[e] = 0;  // no token
-        }
+    const int held = BS_WARPS * K;
+    for (int e0 = 0; e0 < held; e0 += BS_THREADS / 4) {  // an entry's rank, by four lanes; among those that are none, by place
+        const int e = e0 + threadIdx.x / 4;
+        const uint64_t key = e < held ? s_best[e] : 0;
+        int rank = 0;
+        for (int o = threadIdx.x & 3; o < held; o += 4) rank += s_best[o] > key || (key == 0 && s_best[o] == 0 && o < e);
+        rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+        rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+        if (e < held && (threadIdx.x & 3) == 0 && rank < K) best[rank] = key;
     }
 }
 
@@ -223,14 +272,17 @@ __device__ __forceinline__ uint64_t ordered64(double v) {
     return u >> 63 ? ~u : u | 1ull << 63;
 }
 
-__global__ void __launch_bounds__(BS_THREADS) beam_join_kernel(BeamView a, BeamPlan plan) {
+__global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(BeamView a, BeamPlan plan, int staged) {
     extern __shared__ double s_lse[];  // [beams]: log sum exp; NaN for a row without candidates
-    __shared__ uint64_t s_head[2][BS_WARPS];
-    __shared__ int s_list[2][BS_WARPS];
+    // staged: the lists in shared memory
+    __shared__ uint64_t s_head[2][BJ_WARPS];
+    __shared__ int s_list[2][BJ_WARPS];
     double *const s_score = s_lse + a.beams;
-    unsigned char *const s_next = reinterpret_cast<unsigned char *>(s_score + a.beams);  // [list]: places taken
+    uint64_t *const s_keys = reinterpret_cast<uint64_t *>(s_score + a.beams);
+    unsigned char *const s_next = reinterpret_cast<unsigned char *>(s_keys + staged);  // [list]: places taken
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
     const int row0 = blockIdx.x * a.beams, lists = a.beams * plan.parts, K = a.num_out;
+    for (int i = tid; i < lists; i += blockDim.x) s_next[i] = 0;
     pdl_wait();
     for (int i = warp; i < a.beams; i += warps) {
         const int row = row0 + i;
@@ -255,7 +307,8 @@ __global__ void __launch_bounds__(BS_THREADS) beam_join_kernel(BeamView a, BeamP
         }
         if (lane == 0) s_lse[i] = lse, s_score[i] = (double)score;
     }
-    for (int i = tid; i < lists; i += blockDim.x) s_next[i] = 0;
+    const uint64_t *const keys = plan.part_best + (size_t)row0 * plan.parts * K;
+    for (int i = tid; i < staged; i += blockDim.x) s_keys[i] = keys[i];
     __syncthreads();
     // the candidate at a list's head, 0 for none
     auto head = [&](int list, int &tok) -> uint64_t {
@@ -266,15 +319,18 @@ __global__ void __launch_bounds__(BS_THREADS) beam_join_kernel(BeamView a, BeamP
             tok = a.end_token;
             return list % plan.parts == 0 && at == 0 ? ordered64(s_score[beam]) : 0;
         }
-        const uint64_t key = plan.part_best[((size_t)row0 * plan.parts + list) * K + at];
+        const uint64_t key = staged ? s_keys[list * K + at] : keys[(size_t)list * K + at];
         tok = key_token(key);
         return key ? ordered64(s_score[beam] + ((double)key_logit(key) - lse)) : 0;
     };
+    // up to four lists a lane are one warp's, which needs no barriers
+    const int pickers = lists <= 128 ? 32 : (int)blockDim.x;
+    if (tid >= pickers) return;
     uint64_t best = 0;
     int from = 0, tok = 0;
     auto refresh = [&]() {
         best = 0;
-        for (int i = tid; i < lists; i += blockDim.x) {
+        for (int i = tid; i < lists; i += pickers) {
             int t;
             const uint64_t h = head(i, t);
             if (h > best) best = h, from = i, tok = t;
@@ -282,16 +338,16 @@ __global__ void __launch_bounds__(BS_THREADS) beam_join_kernel(BeamView a, BeamP
     };
     refresh();
     for (int k = 0; k < K; k++) {
-        const uint64_t w = warp_max64(best);
-        const int list = (int)__reduce_min_sync(0xffffffffu, best == w && w ? (unsigned)from : 0x7fffffffu);
-        if (lane == 0) s_head[k & 1][warp] = w, s_list[k & 1][warp] = list;
-        __syncthreads();
-        uint64_t win = 0;
-        int which = 0x7fffffff;
-        for (int i = 0; i < warps; i++) {
-            const uint64_t h = s_head[k & 1][i];
-            const int li = s_list[k & 1][i];
-            if (h > win || (h == win && li < which)) win = h, which = li;
+        uint64_t win = warp_max64(best);
+        int which = (int)__reduce_min_sync(0xffffffffu, best == win && win ? (unsigned)from : 0x7fffffffu);
+        if (pickers > 32) {
+            if (lane == 0) s_head[k & 1][warp] = win, s_list[k & 1][warp] = which;
+            __syncthreads();
+            for (int i = 0; i < warps; i++) {
+                const uint64_t h = s_head[k & 1][i];
+                const int li = s_list[k & 1][i];
+                if (h > win || (h == win && li < which)) win = h, which = li;
+            }
         }
         const size_t to = (size_t)blockIdx.x * K + k;
         if (win == 0) {
@@ -313,28 +369,46 @@ BeamPlan plan_beam_select(const BeamView &a) {
     BeamPlan p{};
     const uint64_t rows = (uint64_t)a.groups * a.beams;
     const uint64_t chunks = std::max<uint64_t>(((uint64_t)a.vocab + BS_CHUNK - 1) / BS_CHUNK, 1);
-    // parts enough to fill the GPU, at most 64
-    constexpr uint64_t CTAS = 148 * 6;
-    const uint64_t most = std::min<uint64_t>(chunks, 64);
-    const uint64_t want = std::max<uint64_t>(std::min<uint64_t>((CTAS + rows - 1) / std::max<uint64_t>(rows, 1), most), 1);
-    const uint64_t per = (chunks + want - 1) / want;
-    p.part = (int)std::min<uint64_t>(per * BS_CHUNK, INT32_MAX / 2 + 1);
-    p.parts = (int)((chunks + per - 1) / per);
-    // no fewer for fewer rows or tokens: rows x parts is below rows + CTAS and at most rows x most
-    const uint64_t lists = std::min(rows * most, rows + CTAS);
+    // Parts of at least a chunk for every warp, the number with the least work by
+    // this count: of the SM with the most CTAs the rounds of chunks, and for each
+    // CTA about four more for its start and end; fewer than four CTAs an SM leave
+    // the memory idle.  (256 rows of 131072, 1, 2, 3, 4, 5, 6, 8 parts: 57, 50.7,
+    // 50.2, 48.2, 54.4, 54.5, 56.5 us; four of 49152, 2, 4, 6, 8, 12: 19.5, 17.2,
+    // 16.1, 16.1, 16.3.)
+    constexpr uint64_t SMS = 148, MOST = 32 * SMS;  // CTAs where rows are split
+    const uint64_t most = std::max<uint64_t>(std::min<uint64_t>(chunks / BS_WARPS, BS_MAX_PARTS), 1);
+    uint64_t best = UINT64_MAX;
+    for (uint64_t n = 1; n <= most && (n == 1 || rows * n <= MOST); n++) {
+        const uint64_t per = (chunks + n - 1) / n, parts = (chunks + per - 1) / per;
+        const uint64_t cost = std::max<uint64_t>((rows * parts + SMS - 1) / SMS, 4) * ((per + BS_WARPS - 1) / BS_WARPS + 4);
+        if (cost >= best) continue;
+        best = cost;
+        p.part = (int)std::min<uint64_t>(per * BS_CHUNK, INT32_MAX / 2 + 1);
+        p.parts = (int)parts;
+    }
+    // no fewer for fewer rows or tokens
+    const uint64_t lists = std::max(rows, std::min(rows * most, MOST));
     p.scratch_bytes = lists * (sizeof(double2) + 8ull * a.num_out);
     return p;
 }
 
 void launch_beam_select(const BeamView &a, const BeamPlan &plan, cudaStream_t s) {
-    const unsigned grid = (unsigned)((uint64_t)a.groups * a.beams * plan.parts);
-    if (a.vec)
-        launch_kernel(beam_part_kernel<true>, dim3(grid), dim3(BS_THREADS), 0, s, false, a, plan);
+    const dim3 grid((unsigned)((uint64_t)a.groups * a.beams * plan.parts)), block(BS_THREADS);
+    auto go = [&](auto *kernel, SmemOptIn &opt) {
+        constexpr int bytes = BS_WARPS * BS_STAGES * BS_CHUNK * 4;
+        opt(kernel, bytes);
+        launch_kernel(kernel, grid, block, bytes, s, false, a, plan);
+    };
+    static SmemOptIn opt[4];
+    if (a.num_out <= 32)
+        a.vec ? go(beam_part_kernel<true, false>, opt[0]) : go(beam_part_kernel<false, false>, opt[1]);
     else
-        launch_kernel(beam_part_kernel<false>, dim3(grid), dim3(BS_THREADS), 0, s, false, a, plan);
-    const int lists = a.beams * plan.parts, warps = std::min((lists + 31) / 32, BS_WARPS);
-    launch_kernel(beam_join_kernel, dim3((unsigned)a.groups), dim3((unsigned)warps * 32), (size_t)a.beams * 16 + lists, s, true, a,
-                  plan);
+        a.vec ? go(beam_part_kernel<true, true>, opt[2]) : go(beam_part_kernel<false, true>, opt[3]);
+    const int lists = a.beams * plan.parts, warps = std::min(std::max((lists + 31) / 32, a.beams), BJ_WARPS);
+    // (at most 4 KB of sums, 32 KB of lists and a byte for each of 32768)
+    const int staged = lists * a.num_out <= (lists <= 4096 ? 4096 : 0) ? lists * a.num_out : 0;
+    launch_kernel(beam_join_kernel, dim3((unsigned)a.groups), dim3((unsigned)warps * 32), (size_t)a.beams * 16 + staged * 8 + lists,
+                  s, true, a, plan, staged);
 }
 
 }  // namespace slm

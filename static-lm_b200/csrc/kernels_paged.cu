@@ -326,12 +326,14 @@ void read_typed(const KvView &kv, const BatchView &b, const ReadView &a, cudaStr
 
 // Sequences that go on from others: CTA (i, y) makes sequence i's row of the
 // table (y 0) and copies the used slots of its parent's last page, layers y *
-// per_cta on, where i needs a page of its own.
-constexpr int FK_THREADS = 256;
+// per_cta on, where i needs a page of its own.  A warp takes a (layer, K or V) at
+// a time, its lanes 16-byte pieces of the used slots of all KV heads, four loads
+// in flight: the pages lie scattered and hold 2 to 8 KB of a layer's keys.
+constexpr int FK_THREADS = 128, FK_WARPS = FK_THREADS / 32, FK_PER = 2;
 
 __global__ void __launch_bounds__(FK_THREADS) paged_fork_kernel(ForkPools pools, KvView kv, ForkView a, int layers, int per_cta,
                                                                 int el) {
-    const int i = blockIdx.x, tid = threadIdx.x;
+    const int i = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int p = a.parent[i];
     if (p >= a.num_seqs) {
         if (tid == 0 && blockIdx.y == 0) paged_flag(kv, PAGED_BAD_ROWS);
@@ -349,19 +351,20 @@ __global__ void __launch_bounds__(FK_THREADS) paged_fork_kernel(ForkPools pools,
     // the first successor of a parent goes on in its pages
     int before = 0;
     for (int j = tid; j < i && !before; j += FK_THREADS) before = a.parent[j] == p;
-    const bool first = !__syncthreads_or(before);
     const int len = max(a.kv_len[p], 0);
     const unsigned tail = page_index(kv, (unsigned)len), used = (unsigned)len - tail * (unsigned)kv.page_size;
     const int32_t *old = a.table + (size_t)p * a.stride;
     const bool in_table = tail < (unsigned)a.stride;
-    if (tid == 0 && blockIdx.y == 0 && (tail > (unsigned)a.stride || (!in_table && used))) paged_flag(kv, PAGED_BAD_POSITION);
     int source = in_table ? old[tail] : -1;
+    int spare = a.spare ? a.spare[i] : -1;
+    const bool first = !__syncthreads_or(before);
+    if (tid == 0 && blockIdx.y == 0 && (tail > (unsigned)a.stride || (!in_table && used))) paged_flag(kv, PAGED_BAD_POSITION);
     const bool held = (unsigned)source < (unsigned)kv.num_pages;
     if (source >= 0 && !held && tid == 0 && blockIdx.y == 0) paged_flag(kv, PAGED_BAD_PAGE);
     // a page of its own: for the used slots that another goes on to fill, or for the next position
     const bool copies = !first && in_table && used && held;
     const bool wants = copies || (in_table && !used && (!first || source < 0));
-    int spare = wants && a.spare ? a.spare[i] : -1;
+    if (!wants) spare = -1;
     if ((unsigned)spare >= (unsigned)kv.num_pages) {
         if (tid == 0 && blockIdx.y == 0 && (spare >= 0 || copies)) paged_flag(kv, PAGED_BAD_PAGE);
         spare = -1;
@@ -377,24 +380,33 @@ __global__ void __launch_bounds__(FK_THREADS) paged_fork_kernel(ForkPools pools,
     }
     if (!copies || spare < 0) return;
     const unsigned chunks = used * (unsigned)(kv.hd * el) / 16u;  // of a KV head's used slots
+    const unsigned all = chunks * (unsigned)kv.kv_heads, gap = (unsigned)kv.page_size * (unsigned)(kv.hd * el) / 16u - chunks;
     const uint64_t from = (uint64_t)source * kv.page_stride * el, to = (uint64_t)spare * kv.page_stride * el;
-    const uint64_t head_bytes = (uint64_t)kv.page_size * kv.hd * el;
-    for (int layer = blockIdx.y * per_cta; layer < min(layers, (int)(blockIdx.y + 1) * per_cta); layer++)
+    const int end = min(layers, (int)(blockIdx.y + 1) * per_cta) * 2;
+    for (int x = blockIdx.y * per_cta * 2 + warp; x < end; x += FK_WARPS) {
+        char *pool = reinterpret_cast<char *>(x & 1 ? pools.v[x >> 1] : pools.k[x >> 1]);
+        const uint4 *src = reinterpret_cast<const uint4 *>(pool + from);
+        uint4 *dst = reinterpret_cast<uint4 *>(pool + to);
+        for (unsigned e = lane; e < all; e += 128) {
+            uint4 v[4];
+            unsigned at[4];
 #pragma unroll
-        for (int x = 0; x < 2; x++) {
-            char *pool = reinterpret_cast<char *>(x ? pools.v[layer] : pools.k[layer]);
-            for (unsigned e = tid; e < chunks * (unsigned)kv.kv_heads; e += FK_THREADS) {
-                const unsigned h = e / chunks;
-                const uint64_t at = h * head_bytes + (uint64_t)(e - h * chunks) * 16u;
-                *reinterpret_cast<uint4 *>(pool + to + at) = *reinterpret_cast<const uint4 *>(pool + from + at);
+            for (int u = 0; u < 4; u++) {
+                const unsigned c = e + u * 32;
+                at[u] = c + c / chunks * gap;
+                if (c < all) v[u] = src[at[u]];
             }
-            if (kv.type == KV_Q8)
-                for (unsigned e = tid; e < used * (unsigned)kv.kv_heads; e += FK_THREADS) {
-                    const unsigned h = e / used;
-                    const uint64_t at = kv.scale_at + ((uint64_t)h * (unsigned)kv.page_size + (e - h * used)) * 4u;
-                    *reinterpret_cast<float *>(pool + to + at) = *reinterpret_cast<const float *>(pool + from + at);
-                }
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (e + u * 32 < all) dst[at[u]] = v[u];
         }
+        if (kv.type == KV_Q8)
+            for (unsigned e = lane; e < used * (unsigned)kv.kv_heads; e += 32) {
+                const unsigned h = e / used;
+                const uint64_t at = kv.scale_at + ((uint64_t)h * (unsigned)kv.page_size + (e - h * used)) * 4u;
+                *reinterpret_cast<float *>(pool + to + at) = *reinterpret_cast<const float *>(pool + from + at);
+            }
+    }
 }
 
 }  // namespace
@@ -411,7 +423,8 @@ void launch_paged_read(const KvView &kv, const BatchView &b, const ReadView &a, 
 }
 
 void launch_paged_fork(const ForkPools &pools, const KvView &kv, const ForkView &a, int layers, cudaStream_t s) {
-    const int el = kv.type == KV_F32 ? 4 : kv.type == KV_Q8 ? 1 : 2, per_cta = 4;
+    // a (layer, K or V) for each warp; fewer, longer CTAs where there are many
+    const int el = kv.type == KV_F32 ? 4 : kv.type == KV_Q8 ? 1 : 2, per_cta = FK_PER;
     paged_fork_kernel<<<dim3((unsigned)a.num_new, (unsigned)((layers + per_cta - 1) / per_cta)), FK_THREADS, 0, s>>>(
         pools, kv, a, layers, per_cta, el);
 }
