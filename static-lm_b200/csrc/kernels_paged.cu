@@ -48,8 +48,10 @@ __device__ __forceinline__ void turn(float &p, float &q, float c, float s) {
 //   4 x 20 + 4 + 4 of 96               81.8  67.8  63.8  61.5 (four of sixteen)
 //   12 x 4 + 4 + 4 of 32, bf16 pages   34.8  30.6  28.2  28.7
 // Three are best or within 5 % everywhere: 4.5 to 5.7 TB/s.  Single rows are one
-// launch's time.
-constexpr int AP_VECS = 3;
+// launch's time.  8-bit pages (amax and two quotients a vector on top: issue, not
+// memory, bounds them): one, two, three 62.3, 48.1, 50.3 us for the first.
+template <int TYPE>
+constexpr int AP_VECS = TYPE == KV_Q8 ? 2 : 3;
 
 // 8-bit rows: x = q scale with scale = max|x| / 127 and q = x (127 / max|x|)
 // rounded to the nearest, ties to even: off by half a step, max|x| / 254, and
@@ -65,7 +67,10 @@ __device__ __forceinline__ Q8Row q8_row(unsigned top) {
     if (top >= 0x7f800000u) {
         r.scale = __uint_as_float(0x7fc00000u);
     } else if (top >= (unsigned)(127 - 100) << 23) {
-        r.scale = __fdiv_rn(__uint_as_float(top), 127.0f);
+        // max|x| / 127 rounded once: the quotient by the rounded 1/127 and what its exact
+        // remainder adds (Markstein's theorem); a third of the division's instructions
+        const float a = __uint_as_float(top), y = 1.0f / 127.0f, q = __fmul_rn(a, y);
+        r.scale = __fmaf_rn(__fmaf_rn(-127.0f, q, a), y, q);
         r.up = __fdiv_rn(127.0f, __uint_as_float(top));
     }
     return r;
@@ -82,12 +87,12 @@ template <int TYPE, int LPV>
 __global__ void __launch_bounds__(AP_THREADS, 4) paged_append_kernel(KvView kv, BatchView b, AppendView a) {
     using T = typename KvElem<TYPE>::T;
     const int l = threadIdx.x % LPV, hd = kv.hd;
-    const int per_row = a.num_heads + 2 * kv.kv_heads, parts = (per_row + AP_VECS - 1) / AP_VECS;
+    const int per_row = a.num_heads + 2 * kv.kv_heads, parts = (per_row + AP_VECS<TYPE> - 1) / AP_VECS<TYPE>;
     const unsigned item = blockIdx.x * (AP_THREADS / LPV) + threadIdx.x / LPV;  // below 2^32: the host's check
     const unsigned its_row = item / (unsigned)parts;
     const bool live = its_row < (unsigned)b.num_rows && l * 8 < hd;
     const int row = live ? (int)its_row : 0;
-    const int first = live ? (int)(item - its_row * (unsigned)parts) * AP_VECS : 0;
+    const int first = live ? (int)(item - its_row * (unsigned)parts) * AP_VECS<TYPE> : 0;
     const int rd = a.rotary_dim;
     const bool turns = 8 * l < rd;          // this lane's elements of q and k are rotated,
     const bool split = turns && a.halves;   // as pairs half of rotary_dim apart
@@ -96,9 +101,9 @@ __global__ void __launch_bounds__(AP_THREADS, 4) paged_append_kernel(KvView kv, 
                 *const rv = a.v + (size_t)row * a.ldv;
     const int k0 = a.num_heads, v0 = a.num_heads + kv.kv_heads;  // the first key's and value's vector
 
-    float x[AP_VECS][4], y[AP_VECS][4];
+    float x[AP_VECS<TYPE>][4], y[AP_VECS<TYPE>][4];
 #pragma unroll
-    for (int n = 0; n < AP_VECS; n++) {
+    for (int n = 0; n < AP_VECS<TYPE>; n++) {
         const int vec = first + n;
         const float *src = vec < k0 ? rq + vec * hd : vec < v0 ? rk + (vec - k0) * hd : rv + (vec - v0) * hd;
         if (live && vec < per_row) {
@@ -125,7 +130,7 @@ __global__ void __launch_bounds__(AP_THREADS, 4) paged_append_kernel(KvView kv, 
     }
     // the row's slot in KV head 0, and its scale's place
     long long slot = -1, scale = -1;
-    if (ok && first + AP_VECS > k0) {
+    if (ok && first + AP_VECS<TYPE> > k0) {
         unsigned in_page;
         const int page = key_page(kv, b, seq, (unsigned)pos, in_page);
         if (page >= 0) {
@@ -137,7 +142,7 @@ __global__ void __launch_bounds__(AP_THREADS, 4) paged_append_kernel(KvView kv, 
     }
     if (a.q_norm || a.k_norm) {
 #pragma unroll
-        for (int n = 0; n < AP_VECS; n++) {
+        for (int n = 0; n < AP_VECS<TYPE>; n++) {
             float ss = 0.f;
 #pragma unroll
             for (int j = 0; j < 4; j++) ss = __fmaf_rn(x[n][j], x[n][j], __fmaf_rn(y[n][j], y[n][j], ss));
@@ -159,7 +164,7 @@ __global__ void __launch_bounds__(AP_THREADS, 4) paged_append_kernel(KvView kv, 
         }
     }
 #pragma unroll
-    for (int n = 0; n < AP_VECS; n++) {
+    for (int n = 0; n < AP_VECS<TYPE>; n++) {
         const int vec = first + n;
         if (ok && turns && vec < v0) {
             if (split) {
@@ -173,10 +178,10 @@ __global__ void __launch_bounds__(AP_THREADS, 4) paged_append_kernel(KvView kv, 
             }
         }
     }
-    unsigned top[AP_VECS];  // of the vector's magnitudes, as bits, which order as they do
+    unsigned top[AP_VECS<TYPE>];  // of the vector's magnitudes, as bits, which order as they do
     if constexpr (TYPE == KV_Q8) {
 #pragma unroll
-        for (int n = 0; n < AP_VECS; n++) {
+        for (int n = 0; n < AP_VECS<TYPE>; n++) {
             top[n] = 0;
 #pragma unroll
             for (int j = 0; j < 4; j++)
@@ -187,7 +192,7 @@ __global__ void __launch_bounds__(AP_THREADS, 4) paged_append_kernel(KvView kv, 
     }
     if (!live) return;
 #pragma unroll
-    for (int n = 0; n < AP_VECS; n++) {
+    for (int n = 0; n < AP_VECS<TYPE>; n++) {
         const int vec = first + n;
         if (vec >= per_row) break;
         if (vec < k0) {
@@ -224,7 +229,7 @@ __global__ void __launch_bounds__(AP_THREADS, 4) paged_append_kernel(KvView kv, 
 
 template <int TYPE>
 void append_typed(const KvView &kv, const BatchView &b, const AppendView &a, cudaStream_t s) {
-    const uint64_t items = (uint64_t)b.num_rows * (unsigned)((a.num_heads + 2 * kv.kv_heads + AP_VECS - 1) / AP_VECS);
+    const uint64_t items = (uint64_t)b.num_rows * (unsigned)((a.num_heads + 2 * kv.kv_heads + AP_VECS<TYPE> - 1) / AP_VECS<TYPE>);
     auto go = [&](auto kernel, int lpv) {
         const uint64_t per = AP_THREADS / lpv;
         kernel<<<(unsigned)((items + per - 1) / per), AP_THREADS, 0, s>>>(kv, b, a);
@@ -237,8 +242,10 @@ void append_typed(const KvView &kv, const BatchView &b, const AppendView &a, cud
         go(paged_append_kernel<TYPE, 16>, 16);
 }
 
-// Rows of the cache as they were appended: a group of `lanes` lanes (a power of
-// two, 8 elements each) per (row, KV head) takes its K and its V.
+// Rows of the cache as they were appended: a group of lanes (a power of two, 8
+// elements each) takes the K and the V of one KV head of a row.  (8 x 4096 rows of 3
+// heads of 64, 8-bit to f16: 15.2 us, 3.3 TB/s with the launch; two, three, four
+// heads a group, for which the row's place is found once, 19.2, 17.4, 21.4.)
 constexpr int RD_THREADS = 256;
 
 template <int TYPE>
@@ -292,7 +299,7 @@ __device__ __forceinline__ void write8(void *out, size_t at, const float (&x)[8]
 
 template <int TYPE, int OUT>
 __global__ void __launch_bounds__(RD_THREADS) paged_read_kernel(KvView kv, BatchView b, ReadView a, int lanes_log2) {
-    const unsigned item = (blockIdx.x * (unsigned)RD_THREADS + threadIdx.x) >> lanes_log2;
+    const unsigned item = (blockIdx.x * (unsigned)RD_THREADS + threadIdx.x) >> lanes_log2;  // below 2^32: the host's check
     const int l = threadIdx.x & ((1 << lanes_log2) - 1);
     const unsigned row = item / (unsigned)kv.kv_heads, head = item - row * (unsigned)kv.kv_heads;
     if (row >= (unsigned)b.num_rows || l * 8 >= kv.hd) return;

@@ -29,9 +29,13 @@ constexpr unsigned PQ_TMEM_COLS = 512;
 template <int HDP>
 struct Q8Cfg {
     static constexpr int KT = 64;             // keys per tile: a thread holds a tile's scores in registers
+    // Of which it works on 16 at a time, in a loop: code that is unrolled further leaves
+    // the instruction cache.  (8 x 4096 rows of 9 / 3 heads of 64 and chunks of 32 / 8 of
+    // 128: 16 keys 541 and 765 us, 32 541 and 818, all 64 660 and 1073.)
+    static constexpr int KC = 16;
     static constexpr bool Q_TMEM = HDP == 64;  // q's parts in TMEM (from shared memory an MMA of 64 columns takes 48 cycles, not 32)
     static constexpr int PRODUCERS = 96, THREADS = 384;
-    static constexpr int R_LAUNCH = 168, R_SOFTMAX = 208, R_OTHER = 88;
+    static constexpr int R_LAUNCH = 168, R_SOFTMAX = HDP == 64 ? 208 : 200, R_OTHER = HDP == 64 ? 88 : 104;
     static_assert(256 * R_SOFTMAX + (THREADS - 256) * R_OTHER == THREADS * R_LAUNCH, "registers");
     static constexpr int QPART = 128 * HDP * 2;
     static constexpr int STREAM = 2 * QPART;  // q's parts, and after them the results, f32
@@ -77,16 +81,6 @@ __device__ __forceinline__ bool pq_wait(uint64_t *bar, unsigned parity, Q8Shared
     return true;
 }
 
-// A load that is issued here, not where its result is used.
-__device__ __forceinline__ unsigned ldg_now(const void *p) {
-    unsigned v;
-    asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-    return v;
-}
-__device__ __forceinline__ void lds_b64x2(unsigned a, uint64_t &x, uint64_t &y) {
-    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(x), "=l"(y) : "r"(a));
-}
-
 // Bytes 0, 1 and 2, 3 of four signed ones as f16 pairs: 1024 + b + 128 is b + 128
 // under an exponent byte of 0x64.
 __device__ __forceinline__ uint2 bytes_f16(unsigned w) {
@@ -102,7 +96,7 @@ template <int HDP>
 __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(KvView kv, BatchView b, PagedAttnView a, RowsPlan plan) {
     using Cfg = Q8Cfg<HDP>;
     using Range = WeightRange<KV_F16>;
-    constexpr int KT = Cfg::KT;
+    constexpr int KT = Cfg::KT, KC = Cfg::KC;
     extern __shared__ __align__(1024) unsigned char pq_smem[];
     Q8Shared *sh = reinterpret_cast<Q8Shared *>(pq_smem + Cfg::SMEM - Cfg::SMALL);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -187,40 +181,30 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
             {  // the row of q in two parts, scaled so that its largest element is near 2^15
                 const float *src = a.q + (size_t)row * a.ldq + (size_t)(row_ok ? h : head * group) * hd;
                 const bool vec = (((uintptr_t)a.q | (a.ldq * 4)) & 15) == 0;
-                auto load4 = [&](int d, float (&f)[4]) {  // elements d .. d + 3
-                    const bool in = row_ok && d < hd;
-                    if (in && vec) {
+                float f[HDP];  // (the row's sums are not yet in the registers)
+#pragma unroll
+                for (int d = 0; d < HDP; d += 4) {
+                    if (row_ok && d < hd && vec) {
                         const float4 t = *reinterpret_cast<const float4 *>(src + d);
-                        f[0] = t.x, f[1] = t.y, f[2] = t.z, f[3] = t.w;
+                        f[d] = t.x, f[d + 1] = t.y, f[d + 2] = t.z, f[d + 3] = t.w;
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) f[i] = in ? src[d + i] : 0.f;
+                        for (int i = 0; i < 4; i++) f[d + i] = row_ok && d < hd ? src[d + i] : 0.f;
                     }
-                };
-                unsigned top = 0;  // the bits of non-negative floats order as they do
-#pragma unroll 8
-                for (int d = 0; d < HDP; d += 4) {
-                    float f[4];
-                    load4(d, f);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) top = max(top, __float_as_uint(fabsf(f[i])));
                 }
+                unsigned top = 0;  // the bits of non-negative floats order as they do
+#pragma unroll
+                for (int d = 0; d < HDP; d++) top = max(top, __float_as_uint(fabsf(f[d])));
                 int e = 141 - (int)(top >> 23);  // 2^14 <= top 2^e < 2^15
                 e = top == 0 || top >= 0x7f800000u ? 0 : e > 120 ? 120 : e;
                 const float up = __uint_as_float((unsigned)(127 + e) << 23);
                 sl2 = __fmul_rn(sl2_all, __uint_as_float((unsigned)(127 - e) << 23));
-#pragma unroll 2
+#pragma unroll
                 for (int d = 0; d < HDP; d += 32) {
                     unsigned part[2][16];
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        float f[4];
-                        load4(d + i, f);
-                        unsigned p[2];
-                        split2<KV_F16, 2>(__fmul_rn(f[0], up), __fmul_rn(f[1], up), p);
-                        part[0][i / 2] = p[0], part[1][i / 2] = p[1];
-                        split2<KV_F16, 2>(__fmul_rn(f[2], up), __fmul_rn(f[3], up), p);
-                        part[0][i / 2 + 1] = p[0], part[1][i / 2 + 1] = p[1];
+                    for (int i = 0; i < 32; i += 2) {
+                        split2_f16(__fmul_rn(f[d + i], up), __fmul_rn(f[d + i + 1], up), part[0][i / 2], part[1][i / 2]);
                     }
 #pragma unroll
                     for (int n = 0; n < 2; n++) {
@@ -291,38 +275,36 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
                     float top = -INFINITY;
                     l2 = l_before;
 #pragma unroll 1
-                    for (int g = 0; g < 2; g++) {
-                        float v[32];
-                        tmem_ld32(t_s + g * 32, v);
-                        const unsigned k_scales = smem_addr(sh->scale[j & 3][0] + g * 32);
-                        const unsigned v_scales = smem_addr(sh->scale[j & 3][1] + g * 32);
-                        uint64_t s[16];
+                    for (int g = 0; g < KT / KC; g++) {
+                        float v[KC];
+                        tmem_ld16(t_s + g * KC, v);
+                        const ulonglong2 *k_scales = reinterpret_cast<const ulonglong2 *>(sh->scale[j & 3][0] + g * KC);
+                        const ulonglong2 *v_scales = reinterpret_cast<const ulonglong2 *>(sh->scale[j & 3][1] + g * KC);
+                        uint64_t y[KC / 2];
 #pragma unroll
-                        for (int i = 0; i < 16; i += 2) lds_b64x2(k_scales + i * 8, s[i], s[i + 1]);
+                        for (int i = 0; i < KC / 2; i += 2) y[i] = k_scales[i / 2].x, y[i + 1] = k_scales[i / 2].y;
                         tmem_wait_ld();
-                        pin32(v);
-                        uint64_t y[16];
+                        pin16(v);
 #pragma unroll
-                        for (int i = 0; i < 16; i++) y[i] = mul2(pack2(v[2 * i], v[2 * i + 1]), s[i]);
+                        for (int i = 0; i < KC / 2; i++) y[i] = mul2(pack2(v[2 * i], v[2 * i + 1]), y[i]);
                         if (masks) {
-                            // bit c: list position i0 + 32 g + c is seen
+                            // bit c: list position i0 + KC g + c is seen
                             auto below = [&](int end) -> unsigned {
-                                const int n = end - (i0 + g * 32);
+                                const int n = end - (i0 + g * KC);
                                 return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
                             };
-                            const unsigned seen = below(to) & (below(sink_end) | ~below(from)) & valid[g];
+                            const unsigned seen = below(to) & (below(sink_end) | ~below(from)) & (valid[g * KC / 32] >> (g * KC % 32));
 #pragma unroll
-                            for (int i = 0; i < 16; i++) {
+                            for (int i = 0; i < KC / 2; i++) {
                                 float s0, s1;
                                 unpack2(y[i], s0, s1);
                                 y[i] = pack2(seen & (1u << (2 * i)) ? s0 : -INFINITY, seen & (1u << (2 * i + 1)) ? s1 : -INFINITY);
                             }
                         }
-                        unsigned w[2][16];
+                        unsigned w[2][KC / 2];
 #pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
-                            uint64_t vs[2];
-                            lds_b64x2(v_scales + i * 8, vs[0], vs[1]);
+                        for (int i = 0; i < KC / 2; i += 2) {
+                            const ulonglong2 vs = v_scales[i / 2];
 #pragma unroll
                             for (int u = 0; u < 2; u++) {
                                 float e0, e1;
@@ -331,15 +313,13 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
                                 unpack2(fma2(y[i + u], sl2_2, minus_m), e0, e1);
                                 const uint64_t e = pack2(exp2_approx(e0), exp2_approx(e1));
                                 l2 = add2(l2, e);
-                                unpack2(mul2(e, vs[u]), e0, e1);
-                                unsigned part[2];
-                                split2<KV_F16, 2>(e0, e1, part);
-                                w[0][i + u] = part[0], w[1][i + u] = part[1];
+                                unpack2(mul2(e, u ? vs.y : vs.x), e0, e1);
+                                split2_f16(e0, e1, w[0][i + u], w[1][i + u]);
                             }
                         }
-                        // part n of 32 keys at column 16 n
-                        tmem_st16(t_w + g * 32, w[0]);
-                        tmem_st16(t_w + g * 32 + 16, w[1]);
+                        // part n of KC keys at column n KC / 2
+                        tmem_st8(t_w + g * KC, w[0]);
+                        tmem_st8(t_w + g * KC + KC / 2, w[1]);
                     }
                     top = __fmul_rn(top, sl2);
                     const bool move = top > m + Range::rescale;
@@ -488,7 +468,7 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
                 for (int i = 1; i >= 0; i--)
 #pragma unroll
                     for (int ks = 0; ks < KT / 16; ks++) {
-                        const unsigned at = Cfg::T_W + X * KT + (ks >> 1) * 32 + i * 16 + (ks & 1) * 8;
+                        const unsigned at = Cfg::T_W + X * KT + ks * KC + i * (KC / 2);
                         const uint64_t bd = plus(v_base, ks * 2048, v_desc);
                         if (i == 0 && ks == 0)
                             tc_mma_f16_ta_onto_part2(d, at, bd, idesc_o);
@@ -553,6 +533,7 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
         constexpr int CH = HDP / 16;                // 16-byte chunks of a row
         constexpr int RSTEP = Cfg::PRODUCERS / CH;  // rows a pass: 24 or 12
         constexpr int PASSES = (KT + RSTEP - 1) / RSTEP;
+        static_assert(KC == 16, "an MMA's keys");
         static_assert(Cfg::PRODUCERS % CH == 0 && RSTEP % 4 == 0, "a thread keeps its chunk");
         const int c = p % CH, r_first = p / CH;
         const bool in_row = c * 16 < hd;

@@ -92,6 +92,12 @@ __device__ __forceinline__ long long row_offset(const KvView &kv, int page, int 
     return (long long)((uint64_t)page * kv.page_stride +
                        ((uint64_t)head * (unsigned)kv.page_size + slot) * (unsigned)kv.hd);
 }
+// A load that is issued here, not where its result is used.
+__device__ __forceinline__ unsigned ldg_now(const void *p) {
+    unsigned v;
+    asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
 // Byte offset of the row's scale (KV_Q8).
 __device__ __forceinline__ long long scale_offset(const KvView &kv, int page, int head, unsigned slot) {
     return (long long)((uint64_t)page * kv.page_stride + kv.scale_at +
@@ -205,6 +211,22 @@ __device__ __forceinline__ void split2(float a, float b, unsigned (&part)[N]) {
         }
     }
 }
+// The same of f16, what the first part leaves by multiply-adds that take it as it is
+// (two instructions fewer): b's in the upper halves.
+__device__ __forceinline__ void split2_f16(float a, float b, unsigned &first, unsigned &second) {
+    const __half2 h = __floats2half2_rn(a, b);
+    first = *reinterpret_cast<const unsigned *>(&h);
+    float ra, rb;
+    unpack2(mul2(pack2(a, b), pack2(F16_PART2, F16_PART2)), ra, rb);
+    asm("{\n .reg .b16 x, y, c;\n mov.b32 {x, y}, %2;\n mov.b16 c, 0xEC00;\n"  // -4096
+        " fma.rn.f32.f16 %0, x, c, %0;\n fma.rn.f32.f16 %1, y, c, %1;\n}\n"
+        : "+f"(ra), "+f"(rb)
+        : "r"(first));
+    const __half2 r = __floats2half2_rn(ra, rb);
+    second = *reinterpret_cast<const unsigned *>(&r);
+}
+static_assert(F16_PART2 == 4096.0f, "the constant above");
+
 // The same of two softmax weights (finite, or NaN: then the row is redone).
 template <int TYPE, int N>
 __device__ __forceinline__ void split2_weights(float a, float b, unsigned (&part)[N]) {
