@@ -9,7 +9,7 @@ from a free list and go back when a request ends, or, for a model with an
 attention window, as soon as no later row sees them.
 
   python examples/paged_serving.py [--model cfg1] [--requests 6] [--tokens 24]
-                                   [--pages f32|f16|bf16] [--window W --sinks S]
+                                   [--pages f32|f16|bf16|q8] [--window W --sinks S]
 """
 from __future__ import annotations
 
@@ -26,7 +26,8 @@ sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), ".."
 import static_lm as S  # noqa: E402
 from static_lm import synth  # noqa: E402
 
-TORCH = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+TORCH = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16, "q8": torch.uint8}
+PAGES = {**S.KV_DTYPES, "q8": S.KV_Q8}
 
 
 def dequantize_rows(blocks: np.ndarray, rows, cols: int) -> np.ndarray:
@@ -66,13 +67,13 @@ class PagedServer:
         cos, sin = S.rope_tables(cfg.max_seq_len, self.hd)
         self.cos, self.sin = torch.from_numpy(cos).cuda(), torch.from_numpy(sin).cuda()
         # every layer's keys and values of a page lie together: page_stride spans the layers
-        n, one = len(self.layers), cfg.num_kv_heads * page_size * self.hd
+        shape = dict(page_size=page_size, num_kv_heads=cfg.num_kv_heads, head_dim=self.hd, dtype=PAGES[kv])
+        n, one = len(self.layers), S.paged_page_bytes(S.KvPages(**shape)) // TORCH[kv].itemsize
         self.pool = torch.zeros(num_pages, n, 2, one, dtype=TORCH[kv], device="cuda")
         self.status = torch.zeros(1, dtype=torch.int32, device="cuda")
         self.pages = [S.KvPages(k=self.pool[0, i, 0].data_ptr(), v=self.pool[0, i, 1].data_ptr(),
-                                page_stride=n * 2 * one, num_pages=num_pages, page_size=page_size,
-                                num_kv_heads=cfg.num_kv_heads, head_dim=self.hd, dtype=S.KV_DTYPES[kv],
-                                status=self.status.data_ptr()) for i in range(n)]
+                                page_stride=n * 2 * one, num_pages=num_pages, status=self.status.data_ptr(), **shape)
+                      for i in range(n)]
         self.free = list(range(num_pages))[::-1]
         buf = lambda cols: torch.zeros(max_rows, cols, device="cuda")  # noqa: E731
         self.x, self.xb, self.qkv, self.att, self.y = buf(d), buf(d), buf(d + 2 * k), buf(d), buf(d)
