@@ -353,3 +353,45 @@ def test_select_and_fork_captured_and_replayed(cuda):
         tables = fork_reference(table, lengths, want[1].reshape(-1), spare, pool.shape[0], page, slots(want_pool, "q8", kvh, page, hd))
         assert all(np.array_equal(a.cpu().numpy(), b) for a, b in zip((new_table, new_len, taken), tables))
         assert cuda.equal(pool, want_pool) and int(status) == 0
+
+
+def test_fork_of_pages_far_apart(cuda):
+    """Pages further apart than 2^31 bytes."""
+    kvh, page, hd = 2, 16, 64
+    far, one = (1 << 31) + 4096, kvh * page * (hd + 4)
+    pool = cuda.zeros(2 * far + 2 * one, dtype=cuda.uint8, device="cuda")
+    g = cuda.Generator().manual_seed(1)
+    pool[:2 * one] = cuda.randint(0, 256, (2 * one,), dtype=cuda.uint8, generator=g).cuda()
+    pages = [S.KvPages(k=pool.data_ptr(), v=pool.data_ptr() + one, page_stride=far, num_pages=3, page_size=page,
+                       num_kv_heads=kvh, head_dim=hd, dtype=S.KV_Q8)]
+    got = fork(cuda, pages, np.array([[0]], np.int32), [11], [0, 0, 0], [1, 1, 2])
+    assert got[0].tolist() == [[0], [1], [2]] and got[2].tolist() == [0, 1, 1]
+    for first in (far, 2 * far):
+        for base in (0, one):
+            a, b = pool[base:base + one], pool[first + base:first + base + one]
+            x, y = (t[:kvh * page * hd].view(kvh, page, hd) for t in (a, b))
+            assert cuda.equal(x[:, :11], y[:, :11]) and (y[:, 11:] == 0).all()
+            x, y = (t[kvh * page * hd:].view(kvh, page, 4) for t in (a, b))
+            assert cuda.equal(x[:, :11], y[:, :11]) and (y[:, 11:] == 0).all()
+
+
+def test_two_selections_at_once(cuda):
+    """On two streams, with a scratch each."""
+    work = []
+    for seed, (groups, beams, vocab, out) in enumerate(((5, 4, 30000, 8), (2, 3, 50000, 6))):
+        wide, scores = inputs(cuda, groups, beams, vocab, 0, 30 + seed)
+        logits, scores = wide.cuda(), scores.cuda()
+        want = select(cuda, logits, scores, beams, out)
+        o = [cuda.zeros(groups, out, dtype=t, device="cuda") for t in (cuda.float32, cuda.int32, cuda.int32)]
+        args = S.BeamSelectArgs(logits=logits.data_ptr(), ld=vocab, scores=scores.data_ptr(), num_groups=groups, beams=beams,
+                                vocab=vocab, num_out=out, out_scores=o[0].data_ptr(), out_rows=o[1].data_ptr(),
+                                out_tokens=o[2].data_ptr())
+        size = S.beam_select_scratch_bytes(args)
+        work.append((args, cuda.empty(size, dtype=cuda.uint8, device="cuda"), size, cuda.cuda.Stream(), o, want, logits, scores))
+    cuda.cuda.synchronize()
+    for _ in range(20):
+        for args, scratch, size, stream, *_ in work:
+            S.beam_select(args, scratch.data_ptr(), size, stream.cuda_stream)
+    cuda.cuda.synchronize()
+    for *_, o, want, logits, scores in work:
+        assert all(np.array_equal(t.cpu().numpy(), w) for t, w in zip(o, want))

@@ -506,3 +506,36 @@ def test_wrong_length_hint_changes_nothing(cuda):
         want = reference(c, q, n, 4)
         for hint in (0, 1, 100, 900, 5000):
             near(attend(cuda, c, q, 4, rows, max_kv_len=hint), want)
+
+
+def test_two_calls_at_once(cuda):
+    """On two streams, with a scratch each: what each gives alone."""
+    work = []
+    for seed, (lengths, rows) in enumerate((([900, 33, 1500], None), ([700, 40], [300, 40]))):
+        c = Q8Cache(cuda, lengths, 2, 64, 16, seed=30 + seed)
+        q = queries(cuda, len(lengths) if rows is None else sum(rows), 8, 64, seed)
+        want = attend(cuda, c, q, 8, rows).clone()
+        out = cuda.zeros_like(want)
+        batch = c.batch(rows)
+        args = S.PagedAttentionArgs(q=q.data_ptr(), out=out.data_ptr(), ldq=512, ldo=512, num_heads=8)
+        size = S.paged_attention_scratch_bytes(c.pages, batch, args)
+        scratch = cuda.empty(size + 16, dtype=cuda.uint8, device="cuda")
+        work.append((c, batch, args, scratch, size, cuda.cuda.Stream(), out, want, q))
+    cuda.cuda.synchronize()
+    for _ in range(20):
+        for c, batch, args, scratch, size, stream, out, want, q in work:
+            S.paged_attention(c.pages, batch, args, scratch.data_ptr(), size, stream.cuda_stream)
+    cuda.cuda.synchronize()
+    for *_, out, want, q in work:
+        assert cuda.equal(out, want)
+
+
+@pytest.mark.parametrize("shape", [(9, 3, 64), (8, 1, 128)])
+def test_long_prompts(cuda, shape):
+    """Several row blocks and key tiles, both streams of a block, blocks that end in either."""
+    heads, kvh, hd = shape
+    lengths, rows = [700, 129, 260], [650, 129, 3]
+    c = Q8Cache(cuda, lengths, kvh, hd, 16, seed=40, spread=0.2)
+    q = 2 * queries(cuda, sum(rows), heads, hd, 3)
+    for window, sinks in ((0, 0), (300, 5)):
+        near(attend(cuda, c, q, heads, rows, window, sinks), reference(c, q, rows, heads, window, sinks))
