@@ -666,12 +666,17 @@ __device__ __forceinline__ void cp_async4_zfill(unsigned dst, const void *src, u
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(bytes));
 }
 
+// CTAs an SM holds: by registers, and by shared memory, of which a tile takes half
+// where head_dim is at most 64.  (64 x 2049, 9 / 3 heads of 64: three CTAs with four
+// stages each and one or two splits 22.4 and 21.2 us, four with two stages and two
+// or three 19.2.)
+__host__ __device__ constexpr int q8_ctas_per_sm(int lanes_per_row) { return lanes_per_row == 8 ? 3 : 4; }
+
 template <int LPR, int NG>
-__global__ void __launch_bounds__(PD_THREADS, 3) paged_decode_q8_kernel(KvView kv, BatchView b, PagedAttnView a, DecodePlan plan) {
+__global__ void __launch_bounds__(PD_THREADS, q8_ctas_per_sm(LPR)) paged_decode_q8_kernel(KvView kv, BatchView b, PagedAttnView a, DecodePlan plan) {
     constexpr int G = 4 * NG, TK = 32;        // heads of a CTA, keys of a tile
     constexpr int ROW = LPR * 16, RPP = 32 / LPR, PASSES = TK / RPP, TILE = TK * ROW;
-    constexpr int STAGES = LPR == 8 ? 2 : 4;  // the same bytes in either case
-    static_assert(STAGES * TILE == PD_STAGES * PD_TILE, "shared memory");
+    constexpr int STAGES = PD_STAGES;
     using Range = WeightRange<KV_F16>;
     extern __shared__ __align__(128) unsigned char pd_smem[];
     __shared__ unsigned s_valid[PD_WARPS][STAGES];
@@ -945,10 +950,10 @@ constexpr size_t PD_SMEM = (size_t)PD_WARPS * PD_STAGES * 2 * PD_TILE;
 
 template <typename K>
 void go(K *kernel, SmemOptIn &opt, const KvView &kv, const BatchView &b, const PagedAttnView &a, const DecodePlan &plan,
-        cudaStream_t s) {
+        cudaStream_t s, size_t smem = PD_SMEM) {
     const unsigned grid = (unsigned)((uint64_t)b.num_seqs * kv.kv_heads * plan.head_groups * plan.splits);
-    opt(kernel, (int)PD_SMEM);
-    launch_kernel(kernel, dim3(grid), dim3(PD_THREADS), PD_SMEM, s, false, kv, b, a, plan);
+    opt(kernel, (int)smem);
+    launch_kernel(kernel, dim3(grid), dim3(PD_THREADS), smem, s, false, kv, b, a, plan);
 }
 template <int TYPE, int LPR>
 void go_mma(const KvView &kv, const BatchView &b, const PagedAttnView &a, const DecodePlan &plan, cudaStream_t s) {
@@ -959,9 +964,9 @@ template <int LPR>
 void go_q8(const KvView &kv, const BatchView &b, const PagedAttnView &a, const DecodePlan &plan, cudaStream_t s) {
     static SmemOptIn one, two;
     if (plan.heads <= 4)
-        go(paged_decode_q8_kernel<LPR, 1>, one, kv, b, a, plan, s);
+        go(paged_decode_q8_kernel<LPR, 1>, one, kv, b, a, plan, s, PD_SMEM * LPR / 8);
     else
-        go(paged_decode_q8_kernel<LPR, 2>, two, kv, b, a, plan, s);
+        go(paged_decode_q8_kernel<LPR, 2>, two, kv, b, a, plan, s, PD_SMEM * LPR / 8);
 }
 template <int LPR, int G>
 void go_fma(const KvView &kv, const BatchView &b, const PagedAttnView &a, const DecodePlan &plan, cudaStream_t s) {
@@ -1004,20 +1009,22 @@ DecodePlan plan_paged_decode(const KvView &kv, const BatchView &b, const PagedAt
     // splits 289, 257, 226, 228, 241 us; 128 windows of 1028 keys f16, 1024
     // units: 1, 2, 3 splits 115, 120, 124 us.
     constexpr uint64_t SMS = 148, WAVE = 215 << 10, JOIN = 170 << 10;
-    const uint64_t slots = SMS * (uint64_t)(kv.type == KV_F32 ? ctas_per_sm(p.heads) : 3);
-    const uint64_t key_bytes = 2ull * (kv.type == KV_Q8 ? kv.hd + 4 : kv.hd * (kv.type == KV_F32 ? 4 : 2));
+    const bool q8 = kv.type == KV_Q8;
+    const uint64_t slots = SMS * (uint64_t)(kv.type == KV_F32 ? ctas_per_sm(p.heads) : q8 ? q8_ctas_per_sm(kv.hd <= 64 ? 4 : 8) : 3);
+    const uint64_t key_bytes = 2ull * (q8 ? kv.hd + 4 : kv.hd * (kv.type == KV_F32 ? 4 : 2));
+    const uint64_t key_cost = q8 ? key_bytes * 3 / 2 : key_bytes;  // (a byte of theirs takes more instructions)
     uint64_t best = UINT64_MAX;
     // lengths below the bound may be unlike: with at most 1 MB a CTA the last end
     // together, 0.5 MB of 8-bit pages (64 sequences of 500 to 8192: 2, 3, 4, 6, 8 splits
     // 125, 115, 113, 112, 114 us)
-    const uint64_t fewest = std::min<uint64_t>(64, std::max<uint64_t>(1, (most * key_bytes) >> (kv.type == KV_Q8 ? 19 : 20)));
+    const uint64_t fewest = std::min<uint64_t>(64, std::max<uint64_t>(1, (most * key_bytes) >> (q8 ? 19 : 20)));
     for (uint64_t s = fewest; s <= 64; s++) {
         const uint64_t chunk = ((most + s - 1) / s + 15) / 16 * 16;
         const uint64_t ctas = units * s;
         // (past eight waves the count seldom wins, and the scratch has its bound)
         if (s > fewest && (chunk < 64 || ctas > 8 * slots)) break;
         const uint64_t waves = (ctas + slots - 1) / slots, deep = (ctas + SMS - 1) / SMS;
-        const uint64_t cost = deep * chunk * key_bytes + waves * WAVE + (s > 1 ? JOIN : 0);
+        const uint64_t cost = deep * chunk * key_cost + waves * WAVE + (s > 1 ? JOIN : 0);
         if (best != UINT64_MAX && cost + cost / 32 >= best) continue;
         best = cost;
         p.chunk = (int)std::min<uint64_t>(chunk, INT32_MAX);
