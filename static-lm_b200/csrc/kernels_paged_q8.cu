@@ -15,8 +15,12 @@
 // head side by side, as two streams of 128: warps 0-3 run the softmax of stream 0,
 // a thread a row, warps 4-7 that of stream 1, warp 8 issues the MMAs of both,
 // warps 9-11 bring keys and values.  The streams wait for nothing of each other,
-// so one's arithmetic runs under the other's waits, and every key that is
-// converted serves both.
+// so one's arithmetic runs under the other's waits (w.v of its last tile and q.k
+// of its next, 1000 of a tile's 3550 cycles at head_dim 64), and every key that is
+// converted serves both.  8 x 4096 rows of 9 / 3 heads of 64: 541 us (286 TFLOP/s, two
+// products for each; f16 pages 649); 16 chunks of up to 512 behind up to 8192, 32 / 8
+// heads of 128: 765 us (335).  Instructions bound it: about 14 a score and row, half
+// the cycles issue one; at head_dim 128 also the copying warps, busy throughout.
 #include "kernels.h"
 #include "paged_tc.cuh"
 
@@ -598,7 +602,7 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
                 *reinterpret_cast<uint4 *>(dst + sw16_off(row, 2 * c, KT)) = make_uint4(b0.x, b0.y, b1.x, b1.y);
                 *reinterpret_cast<uint4 *>(dst + sw16_off(row, 2 * c + 1, KT)) = make_uint4(b2.x, b2.y, b3.x, b3.y);
             }
-            // (the MMA warp orders these stores before its own accesses)
+            fence_async_smem();
             mbar_arrive(&sh->full[s]);
         };
         At next = find(look(0));

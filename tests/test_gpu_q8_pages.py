@@ -539,3 +539,65 @@ def test_long_prompts(cuda, shape):
     q = 2 * queries(cuda, sum(rows), heads, hd, 3)
     for window, sinks in ((0, 0), (300, 5)):
         near(attend(cuda, c, q, heads, rows, window, sinks), reference(c, q, rows, heads, window, sinks))
+
+
+def peaked(torch, lengths, hd, gap, sink, spread, seed):
+    """Keys of scores near 0 but for key `sink`, `gap` above them, with value 0."""
+    c = Q8Cache(torch, lengths, 2, hd, 16, seed=seed)
+    k, k_scale = c.parts(c.k)
+    v, _ = c.parts(c.v)
+    k[..., 0] = 0
+    k_scale.mul_(spread)
+    v.abs_()
+    for s, n in enumerate(lengths):
+        if sink < n:
+            at = int(c.table[s, sink // 16]), slice(None), sink % 16
+            k[at], v[at] = 0, 0
+            k[at[0], :, at[2], 0] = 127
+            k_scale[at] = gap * hd ** 0.5 / 8 / 127
+    return c
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("gap", [10, 14, 17, 20])
+@pytest.mark.parametrize("rows", [None, [70, 60]])
+@pytest.mark.parametrize("sink,spread", [(0, 0.0), (37, 0.1)])
+def test_values_of_small_weights(cuda, hd, gap, rows, sink, spread):
+    """As with f16 pages (see its tolerance), with two more roundings, the scales', and
+    weights that are halved at most by a value's scale relative to a power of two."""
+    lengths = [2000, 60]
+    c = peaked(cuda, lengths, hd, gap, sink, spread, seed=gap)
+    n = [1, 1] if rows is None else rows
+    q = queries(cuda, sum(n), 8, hd, gap)
+    q.view(-1, 8, hd)[..., 0] = 8
+    got = attend(cuda, c, q, 8, rows).double().cpu().numpy()
+    want = reference(c, q, n, 8)
+    tol = (gap + 1) * (14 + 2 * hd / 16 / 3) * U + 2.0 ** (gap * np.log2(np.e) - 45)
+    off, size = np.linalg.norm(got - want, axis=1), np.linalg.norm(want, axis=1)
+    assert (off <= tol * size).all(), (off / size).max() / tol
+    assert (np.abs(got - want).max(1) <= 4 * tol * np.abs(want).max(1)).all()
+
+
+@pytest.mark.parametrize("factor", [1e5, 1e7, 1e9, 1e15, 1e25])
+@pytest.mark.parametrize("rows", [None, [150]])
+def test_scores_of_any_size(cuda, factor, rows):
+    """So far apart that one key takes the whole weight: the output is its value."""
+    c = Q8Cache(cuda, [150], 2, 64, 16, seed=31)
+    n = [1] if rows is None else rows
+    q = queries(cuda, sum(n), 4, 64, 12) * factor
+    near(attend(cuda, c, q, 4, rows), reference(c, q, n, 4))
+
+
+@pytest.mark.parametrize("rows", [None, [40]])
+@pytest.mark.parametrize("length", [50, 1500])
+def test_scores_near_the_lowest_f32(cuda, rows, length):
+    """-2.2e38, times log2(e) -3.2e38: finite, and the same for every key, whose values are averaged."""
+    c = Q8Cache(cuda, [length], 2, 64, 16, seed=32)
+    k, scale = c.parts(c.k)
+    k.zero_()
+    k[..., 0] = -127
+    scale.fill_(2.2e19 / 127)
+    n = [1] if rows is None else rows
+    q = cuda.zeros(sum(n), 4 * 64, device="cuda")
+    q.view(-1, 4, 64)[..., 0] = 1e19
+    near(attend(cuda, c, q, 4, rows, scale=1.0), reference(c, q, n, 4, scale=1.0))
