@@ -1,6 +1,7 @@
 // kernels_paged.cu -- the paged key/value cache: new keys and values into
 // their pages with the per-head RMSNorm and the position rotation applied on
 // the way.
+#include "async.cuh"
 #include "kernels.h"
 
 namespace slm {
@@ -49,7 +50,8 @@ __device__ __forceinline__ void turn(float &p, float &q, float c, float s) {
 //   12 x 4 + 4 + 4 of 32, bf16 pages   34.8  30.6  28.2  28.7
 // Three are best or within 5 % everywhere: 4.5 to 5.7 TB/s.  Single rows are one
 // launch's time.  8-bit pages (amax and two quotients a vector on top: issue, not
-// memory, bounds them): one, two, three 62.3, 48.1, 50.3 us for the first.
+// memory, bounds them): one, two, three 61.8, 48.0, 50.0 us for the first (without
+// the quotients 46.8).
 template <int TYPE>
 constexpr int AP_VECS = TYPE == KV_Q8 ? 2 : 3;
 
@@ -61,6 +63,11 @@ constexpr int AP_VECS = TYPE == KV_Q8 ? 2 : 3;
 struct Q8Row {
     float scale, up;
 };
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ Q8Row q8_row(unsigned top) {
     Q8Row r;
     r.scale = r.up = 0.f;
@@ -86,6 +93,10 @@ __device__ __forceinline__ unsigned q8_pack(const float (&x)[4], float up) {
 template <int TYPE, int LPV>
 __global__ void __launch_bounds__(AP_THREADS, 4) paged_append_kernel(KvView kv, BatchView b, AppendView a) {
     using T = typename KvElem<TYPE>::T;
+    if constexpr (TYPE == KV_Q8) {
+        pdl_wait();
+        pdl_release();
+    }
     const int l = threadIdx.x % LPV, hd = kv.hd;
     const int per_row = a.num_heads + 2 * kv.kv_heads, parts = (per_row + AP_VECS<TYPE> - 1) / AP_VECS<TYPE>;
     const unsigned item = blockIdx.x * (AP_THREADS / LPV) + threadIdx.x / LPV;  // below 2^32: the host's check
@@ -178,16 +189,14 @@ __global__ void __launch_bounds__(AP_THREADS, 4) paged_append_kernel(KvView kv, 
             }
         }
     }
-    unsigned top[AP_VECS<TYPE>];  // of the vector's magnitudes, as bits, which order as they do
+    float top[AP_VECS<TYPE>];  // the vector's largest magnitude, NaN where it holds one
     if constexpr (TYPE == KV_Q8) {
 #pragma unroll
         for (int n = 0; n < AP_VECS<TYPE>; n++) {
-            top[n] = 0;
+            top[n] = max3_abs(max3_abs(max3_abs(x[n][0], x[n][1], x[n][2]), x[n][3], y[n][0]),
+                              max3_abs(y[n][1], y[n][2], y[n][3]), 0.f);
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                top[n] = max(top[n], max(__float_as_uint(fabsf(x[n][j])), __float_as_uint(fabsf(y[n][j]))));
-#pragma unroll
-            for (int o = LPV / 2; o > 0; o >>= 1) top[n] = max(top[n], __shfl_xor_sync(0xffffffffu, top[n], o));
+            for (int o = LPV / 2; o > 0; o >>= 1) top[n] = max3_abs(top[n], __shfl_xor_sync(0xffffffffu, top[n], o), 0.f);
         }
     }
     if (!live) return;
@@ -214,9 +223,14 @@ __global__ void __launch_bounds__(AP_THREADS, 4) paged_append_kernel(KvView kv, 
             const long long above = (long long)(vec - (key ? k0 : v0)) * kv.page_size;  // rows of the heads before
             T *pool = reinterpret_cast<T *>(key ? kv.k : kv.v) + slot + above * hd;
             if constexpr (TYPE == KV_Q8) {
-                const Q8Row r = q8_row(top[n]);
-                *reinterpret_cast<unsigned *>(pool + i0) = q8_pack(x[n], r.up);
-                *reinterpret_cast<unsigned *>(pool + i1) = q8_pack(y[n], r.up);
+                const Q8Row r = q8_row(__float_as_uint(top[n]));
+                const unsigned lo = q8_pack(x[n], r.up), hi = q8_pack(y[n], r.up);
+                if (i1 == i0 + 4) {
+                    *reinterpret_cast<uint2 *>(pool + i0) = make_uint2(lo, hi);
+                } else {
+                    *reinterpret_cast<unsigned *>(pool + i0) = lo;
+                    *reinterpret_cast<unsigned *>(pool + i1) = hi;
+                }
                 if (l == 0)
                     *reinterpret_cast<float *>(reinterpret_cast<char *>(key ? kv.k : kv.v) + scale + above * 4) = r.scale;
             } else {
@@ -232,7 +246,7 @@ void append_typed(const KvView &kv, const BatchView &b, const AppendView &a, cud
     const uint64_t items = (uint64_t)b.num_rows * (unsigned)((a.num_heads + 2 * kv.kv_heads + AP_VECS<TYPE> - 1) / AP_VECS<TYPE>);
     auto go = [&](auto kernel, int lpv) {
         const uint64_t per = AP_THREADS / lpv;
-        kernel<<<(unsigned)((items + per - 1) / per), AP_THREADS, 0, s>>>(kv, b, a);
+        launch_kernel(kernel, dim3((unsigned)((items + per - 1) / per)), dim3(AP_THREADS), 0, s, TYPE == KV_Q8, kv, b, a);
     };
     if (kv.hd <= 32)
         go(paged_append_kernel<TYPE, 4>, 4);
@@ -257,9 +271,10 @@ __device__ __forceinline__ void read8(const void *pool, long long at, long long 
     } else if constexpr (TYPE == KV_Q8) {
         const uint2 u = *reinterpret_cast<const uint2 *>(reinterpret_cast<const char *>(pool) + at);
         const float f = scale_get(pool, scale);
+        const unsigned w[2] = {u.x ^ 0x80808080u, u.y ^ 0x80808080u};
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-            x[j] = __fmul_rn((float)(int8_t)((j < 4 ? u.x : u.y) >> (8 * (j & 3))), f);
+        for (int j = 0; j < 8; j++)  // 2^23 + b + 128 is b + 128 under the exponent of 2^23
+            x[j] = __fmul_rn(__fsub_rn(__uint_as_float(__byte_perm(w[j >> 2], 0x4b000000u, 0x7440 | (j & 3))), 8388736.0f), f);
     } else {
         const uint4 u = *reinterpret_cast<const uint4 *>(reinterpret_cast<const char *>(pool) + 2 * at);
         const unsigned w[4] = {u.x, u.y, u.z, u.w};
@@ -299,6 +314,8 @@ __device__ __forceinline__ void write8(void *out, size_t at, const float (&x)[8]
 
 template <int TYPE, int OUT>
 __global__ void __launch_bounds__(RD_THREADS) paged_read_kernel(KvView kv, BatchView b, ReadView a, int lanes_log2) {
+    pdl_wait();
+    pdl_release();
     const unsigned item = (blockIdx.x * (unsigned)RD_THREADS + threadIdx.x) >> lanes_log2;  // below 2^32: the host's check
     const int l = threadIdx.x & ((1 << lanes_log2) - 1);
     const unsigned row = item / (unsigned)kv.kv_heads, head = item - row * (unsigned)kv.kv_heads;
@@ -324,11 +341,11 @@ void read_typed(const KvView &kv, const BatchView &b, const ReadView &a, cudaStr
     const uint64_t threads = ((uint64_t)b.num_rows * kv.kv_heads) << log2;
     const unsigned grid = (unsigned)((threads + RD_THREADS - 1) / RD_THREADS);
     if (a.type == KV_F32)
-        paged_read_kernel<TYPE, KV_F32><<<grid, RD_THREADS, 0, s>>>(kv, b, a, log2);
+        launch_kernel(paged_read_kernel<TYPE, KV_F32>, dim3(grid), dim3(RD_THREADS), 0, s, true, kv, b, a, log2);
     else if (a.type == KV_F16)
-        paged_read_kernel<TYPE, KV_F16><<<grid, RD_THREADS, 0, s>>>(kv, b, a, log2);
+        launch_kernel(paged_read_kernel<TYPE, KV_F16>, dim3(grid), dim3(RD_THREADS), 0, s, true, kv, b, a, log2);
     else
-        paged_read_kernel<TYPE, KV_BF16><<<grid, RD_THREADS, 0, s>>>(kv, b, a, log2);
+        launch_kernel(paged_read_kernel<TYPE, KV_BF16>, dim3(grid), dim3(RD_THREADS), 0, s, true, kv, b, a, log2);
 }
 
 // Sequences that go on from others: CTA (i, y) makes sequence i's row of the
@@ -340,6 +357,8 @@ constexpr int FK_THREADS = 128, FK_WARPS = FK_THREADS / 32, FK_PER = 2;
 
 __global__ void __launch_bounds__(FK_THREADS) paged_fork_kernel(ForkPools pools, KvView kv, ForkView a, int layers, int per_cta,
                                                                 int el) {
+    pdl_wait();
+    pdl_release();
     const int i = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int p = a.parent[i];
     if (p >= a.num_seqs) {
@@ -432,8 +451,8 @@ void launch_paged_read(const KvView &kv, const BatchView &b, const ReadView &a, 
 void launch_paged_fork(const ForkPools &pools, const KvView &kv, const ForkView &a, int layers, cudaStream_t s) {
     // a (layer, K or V) for each warp; fewer, longer CTAs where there are many
     const int el = kv.type == KV_F32 ? 4 : kv.type == KV_Q8 ? 1 : 2, per_cta = FK_PER;
-    paged_fork_kernel<<<dim3((unsigned)a.num_new, (unsigned)((layers + per_cta - 1) / per_cta)), FK_THREADS, 0, s>>>(
-        pools, kv, a, layers, per_cta, el);
+    launch_kernel(paged_fork_kernel, dim3((unsigned)a.num_new, (unsigned)((layers + per_cta - 1) / per_cta)), dim3(FK_THREADS), 0, s,
+                  true, pools, kv, a, layers, per_cta, el);
 }
 
 void launch_paged_append(const KvView &kv, const BatchView &b, const AppendView &a, cudaStream_t s) {

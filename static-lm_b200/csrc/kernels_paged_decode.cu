@@ -683,6 +683,7 @@ __global__ void __launch_bounds__(PD_THREADS, q8_ctas_per_sm(LPR)) paged_decode_
     __shared__ float s_scale[PD_WARPS][STAGES][2][TK];  // of a tile's keys and values
     __shared__ float s_m[PD_WARPS][G], s_l[PD_WARPS][G];
 
+    pdl_wait();
     pdl_release();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     DecodeWork work;
@@ -953,7 +954,9 @@ void go(K *kernel, SmemOptIn &opt, const KvView &kv, const BatchView &b, const P
         cudaStream_t s, size_t smem = PD_SMEM) {
     const unsigned grid = (unsigned)((uint64_t)b.num_seqs * kv.kv_heads * plan.head_groups * plan.splits);
     opt(kernel, (int)smem);
-    launch_kernel(kernel, dim3(grid), dim3(PD_THREADS), smem, s, false, kv, b, a, plan);
+    // (8-bit pages: its CTAs come while the kernel before ends, and wait.  64 x 2049
+    // 19.1 to 17.6 us, one sequence of 8192 13.1 to 11.6)
+    launch_kernel(kernel, dim3(grid), dim3(PD_THREADS), smem, s, kv.type == KV_Q8, kv, b, a, plan);
 }
 template <int TYPE, int LPR>
 void go_mma(const KvView &kv, const BatchView &b, const PagedAttnView &a, const DecodePlan &plan, cudaStream_t s) {
