@@ -183,19 +183,42 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
             const unsigned t_s = t_lane + (unsigned)(x * KT), t_w = t_lane + (unsigned)(Cfg::T_W + x * KT), t_o = t_lane + (unsigned)(Cfg::T_O + x * HDP);
             float sl2;
             {  // the row of q in two parts, scaled so that its largest element is near 2^15
-                const float *src = a.q + (size_t)row * a.ldq + (size_t)(row_ok ? h : head * group) * hd;
-                const bool vec = (((uintptr_t)a.q | (a.ldq * 4)) & 15) == 0;
-                float f[HDP];  // (the row's sums are not yet in the registers)
-#pragma unroll
-                for (int d = 0; d < HDP; d += 4) {
-                    if (row_ok && d < hd && vec) {
-                        const float4 t = *reinterpret_cast<const float4 *>(src + d);
-                        f[d] = t.x, f[d + 1] = t.y, f[d + 2] = t.z, f[d + 3] = t.w;
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; i++) f[d + i] = row_ok && d < hd ? src[d + i] : 0.f;
+                // It comes through the stream's shared memory, whole rows at a time, 16-byte chunk
+                // c of row r at chunk c ^ (r & 7).  (Every thread its own row: 4400 to 9000
+                // cycles of a CTA, since each load met 32 lines.)
+                constexpr int LPR = HDP / 4, RPP = 32 / LPR;  // lanes a row, rows a pass
+                unsigned char *const s_f = pq_smem + x * Cfg::STREAM + (warp & 3) * 32 * HDP * 4;
+                const long long my_at = row_ok ? (long long)((size_t)row * a.ldq + (size_t)h * hd) : -1;
+                if ((((uintptr_t)a.q | (a.ldq * 4)) & 15) == 0) {
+#pragma unroll 4
+                    for (int i = 0; i < 32; i += RPP) {
+                        const int rr = i + lane / LPR, c = lane % LPR;
+                        const long long at = __shfl_sync(0xffffffffu, my_at, rr);
+                        const bool in = at >= 0 && c * 4 < hd;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_addr(s_f + (rr * LPR + (c ^ (rr & 7))) * 16)),
+                                     "l"(a.q + (in ? at + c * 4 : 0)), "r"(in ? 16u : 0u));
+                    }
+                } else {
+#pragma unroll 4
+                    for (int e = lane; e < 32 * HDP; e += 32) {
+                        const int rr = e / HDP, d = e % HDP;
+                        const long long at = __shfl_sync(0xffffffffu, my_at, rr);
+                        const bool in = at >= 0 && d < hd;
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(
+                                         smem_addr(s_f + (rr * LPR + ((d >> 2) ^ (rr & 7))) * 16 + (d & 3) * 4)),
+                                     "l"(a.q + (in ? at + d : 0)), "r"(in ? 4u : 0u));
                     }
                 }
+                cp_async_commit();
+                cp_async_wait<0>();
+                __syncwarp();
+                float f[HDP];  // (the row's sums are not yet in the registers)
+#pragma unroll
+                for (int c = 0; c < LPR; c++) {
+                    const float4 t = *reinterpret_cast<const float4 *>(s_f + (lane * LPR + (c ^ (lane & 7))) * 16);
+                    f[4 * c] = t.x, f[4 * c + 1] = t.y, f[4 * c + 2] = t.z, f[4 * c + 3] = t.w;
+                }
+                if constexpr (!Cfg::Q_TMEM) named_bar_sync(2 + x, 128);  // the parts go over other warps' rows
                 unsigned top = 0;  // the bits of non-negative floats order as they do
 #pragma unroll
                 for (int d = 0; d < HDP; d++) top = max(top, __float_as_uint(fabsf(f[d])));
@@ -378,7 +401,7 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
                                         : split_up ? (long long)((((size_t)row * a.num_heads + h) * plan.splits + split) * hd)
                                                    : (long long)((size_t)row * a.ldo + (size_t)h * hd);
                 float *const to_base = (split_up ? plan.part_o : a.out) + c * 4;
-#pragma unroll 4
+#pragma unroll 2
                 for (int i = 0; i < 32; i += RPP) {
                     const int rr = i + lane / LPR;
                     const long long at = __shfl_sync(0xffffffffu, my_at, rr);
