@@ -17,9 +17,9 @@
 // warps 9-11 bring keys and values.  The streams wait for nothing of each other,
 // so one's arithmetic runs under the other's waits (w.v of its last tile and q.k
 // of its next, 1000 of a tile's 3550 cycles at head_dim 64), and every key that is
-// converted serves both.  8 x 4096 rows of 9 / 3 heads of 64: 541 us (286 TFLOP/s, two
+// converted serves both.  8 x 4096 rows of 9 / 3 heads of 64: 530 us (292 TFLOP/s, two
 // products for each; f16 pages 649); 16 chunks of up to 512 behind up to 8192, 32 / 8
-// heads of 128: 765 us (335).  Instructions bound it: about 14 a score and row, half
+// heads of 128: 742 us (345).  Instructions bound it: about 14 a score and row, half
 // the cycles issue one; at head_dim 128 also the copying warps, busy throughout.
 #include "kernels.h"
 #include "paged_tc.cuh"
@@ -35,7 +35,8 @@ struct Q8Cfg {
     static constexpr int KT = 64;             // keys per tile: a thread holds a tile's scores in registers
     // Of which it works on 16 at a time, in a loop: code that is unrolled further leaves
     // the instruction cache.  (8 x 4096 rows of 9 / 3 heads of 64 and chunks of 32 / 8 of
-    // 128: 16 keys 541 and 765 us, 32 541 and 818, all 64 660 and 1073.)
+    // 128, before q came by whole rows: 16 keys 541 and 765 us, 32 541 and 818, all 64 660
+    // and 1073; now 530 and 742.)
     static constexpr int KC = 16;
     static constexpr bool Q_TMEM = HDP == 64;  // q's parts in TMEM (from shared memory an MMA of 64 columns takes 48 cycles, not 32)
     static constexpr int PRODUCERS = 96, THREADS = 384;
