@@ -276,7 +276,7 @@ __device__ __forceinline__ uint64_t ordered64(double v) {
 __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(BeamView a, BeamPlan plan, int staged) {
     extern __shared__ double s_lse[];  // [beams]: log sum exp; NaN for a row without candidates
     // staged: entries of all lists, where they are in shared memory
-    __shared__ uint64_t s_head[2][BJ_WARPS];
+    __shared__ uint64_t s_head[2][BJ_WARPS], s_key[2][BJ_WARPS];
     __shared__ int s_list[2][BJ_WARPS];
     double *const s_score = s_lse + a.beams;
     uint64_t *const s_keys = reinterpret_cast<uint64_t *>(s_score + a.beams), *const s_cand = s_keys + staged;
@@ -312,16 +312,15 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(BeamView a, BeamP
     for (int i = tid; i < staged; i += blockDim.x) s_keys[i] = keys[i];
     __syncthreads();
     // the candidate at a list's head, 0 for none
-    auto head = [&](int list, int &tok) -> uint64_t {
+    auto head = [&](int list, uint64_t &key) -> uint64_t {
         const int beam = list / plan.parts, at = s_next[list];
         const double lse = s_lse[beam];
         if (lse != lse || at >= K) return 0;
         if (a.ended && a.ended[row0 + beam] != 0) {
-            tok = a.end_token;
+            key = beam_key(0.f, a.end_token);
             return list % plan.parts == 0 && at == 0 ? ordered64(s_score[beam]) : 0;
         }
-        const uint64_t key = keys[(size_t)list * K + at];
-        tok = key_token(key);
+        key = keys[(size_t)list * K + at];
         return key ? ordered64(s_score[beam] + ((double)key_logit(key) - lse)) : 0;
     };
     auto put = [&](int k, uint64_t win, int list, int token) {
@@ -330,6 +329,18 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(BeamView a, BeamP
         a.out_scores[to] = win ? (float)__longlong_as_double((long long)u) : -INFINITY;
         a.out_rows[to] = win ? row0 + list / plan.parts : -1;
         a.out_tokens[to] = win ? token : -1;
+    };
+    // Of equal sums that of the lower row is first, then that of its larger logit and lower
+    // token: the larger key, which may be in any of the row's lists.
+    auto first = [&](bool &mine, int list, uint64_t key) {
+        const unsigned those = __ballot_sync(0xffffffffu, mine);
+        if (those & (those - 1)) {
+            const unsigned beam = (unsigned)(list / plan.parts);
+            const unsigned lowest = __reduce_min_sync(0xffffffffu, mine ? beam : 0xffffffffu);
+            mine = mine && beam == lowest;
+            const uint64_t largest = warp_max64(mine ? key : 0);
+            mine = mine && key == largest;
+        }
     };
     if (staged) {
         // every entry's sum at once; then a warp with up to four lists a lane picks,
@@ -357,16 +368,33 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(BeamView a, BeamP
             for (int u = 1; u < 4; u++)
                 if (h[u] > best) best = h[u], from = u;
             const uint64_t win = warp_max64(best);
-            const unsigned list = __reduce_min_sync(0xffffffffu, best == win && win ? (unsigned)(lane + 32 * from) : 0x7fffffffu);
             if (win == 0) {
                 if (lane == 0) put(k, 0, 0, 0);
-            } else if (list == (unsigned)(lane + 32 * from)) {
+                continue;
+            }
+            bool mine = best == win, twice = false;
+#pragma unroll
+            for (int u = 1; u < 4; u++) twice = twice || (h[u] == win && from < u);
+            const unsigned those = __ballot_sync(0xffffffffu, mine), more = __ballot_sync(0xffffffffu, twice);
+            if ((those & (those - 1)) | more) {
+                uint64_t key = 0;
+                int beam = -1;
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    if (h[u] != win) continue;
+                    const int list = lane + 32 * u, its = list / plan.parts;
+                    const uint64_t its_key = s_keys[list * K + at[u]];
+                    if (beam < 0 || (its == beam && its_key > key)) beam = its, key = its_key, from = u;
+                }
+                first(mine, lane + 32 * from, key);
+            }
+            if (mine) {
 #pragma unroll
                 for (int u = 0; u < 4; u++)
                     if (from == u) {
-                        const int i = (int)list * K + at[u];
-                        const bool ended = a.ended && a.ended[row0 + (int)list / plan.parts] != 0;
-                        put(k, win, (int)list, ended ? a.end_token : key_token(s_keys[i]));
+                        const int list = lane + 32 * u, i = list * K + at[u];
+                        const bool ended = a.ended && a.ended[row0 + list / plan.parts] != 0;
+                        put(k, win, list, ended ? a.end_token : key_token(s_keys[i]));
                         h[u] = ++at[u] < K ? s_cand[i + 1] : 0;
                     }
             }
@@ -374,31 +402,35 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(BeamView a, BeamP
         return;
     }
     const int pickers = (int)blockDim.x;
-    uint64_t best = 0;
-    int from = 0, tok = 0;
+    uint64_t best = 0, its = 0;  // a sum and its key
+    int from = 0;
     auto refresh = [&]() {
         best = 0;
         for (int i = tid; i < lists; i += pickers) {
-            int t;
-            const uint64_t h = head(i, t);
-            if (h > best) best = h, from = i, tok = t;
+            uint64_t key;
+            const uint64_t h = head(i, key);
+            if (h > best || (h == best && h && i / plan.parts == from / plan.parts && key > its)) best = h, from = i, its = key;
         }
     };
     refresh();
     for (int k = 0; k < K; k++) {
         uint64_t win = warp_max64(best);
-        int which = (int)__reduce_min_sync(0xffffffffu, best == win && win ? (unsigned)from : 0x7fffffffu);
-        if (lane == 0) s_head[k & 1][warp] = win, s_list[k & 1][warp] = which;
+        bool mine = best == win && win;
+        first(mine, from, its);
+        if (mine || (win == 0 && lane == 0)) s_head[k & 1][warp] = win, s_list[k & 1][warp] = from, s_key[k & 1][warp] = its;
         __syncthreads();
+        int which = 0x7fffffff;
+        uint64_t key = 0;
+        win = 0;
         for (int i = 0; i < warps; i++) {
-            const uint64_t h = s_head[k & 1][i];
-            const int li = s_list[k & 1][i];
-            if (h > win || (h == win && li < which)) win = h, which = li;
+            const uint64_t h = s_head[k & 1][i], hk = s_key[k & 1][i];
+            const int li = s_list[k & 1][i], d = li / plan.parts - which / plan.parts;
+            if (h > win || (h == win && h && (d < 0 || (d == 0 && hk > key)))) win = h, which = li, key = hk;
         }
         if (win == 0) {
             if (tid == 0) put(k, 0, 0, 0);
         } else if (best == win && from == which) {
-            put(k, win, which, tok);
+            put(k, win, which, key_token(key));
             s_next[which]++;
             refresh();
         }

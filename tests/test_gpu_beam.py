@@ -137,6 +137,21 @@ def test_ties_between_rows_go_to_the_lower_row(cuda):
     assert got[1].tolist() == [[0, 1, 2, 0, 1, 2, 0], [3, 4, 5, 3, 4, 5, 3]]
 
 
+@pytest.mark.parametrize("groups,beams,vocab,out", [(1, 1, 131072, 40), (1, 2, 49152, 8), (2, 64, 20000, 8), (1, 200, 9000, 33)])
+def test_sums_that_are_equal_go_by_row_and_logit(cuda, groups, beams, vocab, out):
+    """Scores beside which no log probability shows: every sum of a row is equal, wherever its tokens lie."""
+    torch = cuda
+    rng = np.random.default_rng(21)
+    x = rng.standard_normal((groups * beams, vocab)).astype(np.float32)
+    for row in x[::beams]:  # a group's first row has fewer tokens
+        row[np.argsort(-row)[out // 2:]] = -np.inf
+    scores = np.full(groups * beams, -1e20, np.float32)
+    want = select_reference(x, scores, beams, out)
+    got = select(torch, torch.tensor(x, device="cuda"), torch.tensor(scores, device="cuda"), beams, out)
+    assert np.array_equal(got[1], want[1]) and np.array_equal(got[2], want[2])
+    assert np.array_equal(got[0], want[0].astype(np.float32))
+
+
 def test_beams_that_ended_or_are_not_used(cuda):
     beams, vocab = 4, 5000
     wide, scores = inputs(cuda, 4, beams, vocab, 0, 11)
