@@ -426,7 +426,8 @@ int slm_paged_read(const slm_kv_pages *pages, const slm_paged_batch *batch, cons
  * page in the tables; a page whose slots two sequences would fill must not be
  * in two rows of page_table.  The outputs are apart from the inputs.
  * pages[0..num_layers-1] are layers with pages of one shape, indexed by one
- * table; pages[0].status takes the flags.  At most 65536 new sequences. */
+ * table; pages[0].status takes the flags.  At most 65536 new sequences, and
+ * pages below 32 GB. */
 typedef struct {
     const int32_t *parent;     /* [num_new] */
     const int32_t *kv_len;     /* [num_seqs] */

@@ -817,6 +817,10 @@ SLM_EXPORT int slm_sample_argmax(const float *logits, uint64_t n, int32_t *out, 
 namespace {
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+template <typename... P>
+bool aligned4(const P *...p) {
+    return ((0 | ... | (uintptr_t)p) & 3) == 0;
+}
 
 // Elements from one page to the next; an 8-bit page's, bytes, end with its scales.
 uint64_t page_elements(int32_t dtype, uint64_t kv_heads, uint64_t page_size, uint64_t head_dim) {
@@ -1083,6 +1087,11 @@ SLM_EXPORT int slm_paged_fork(const slm_kv_pages *pages, uint32_t num_layers, co
         return fail(SLM_ERR_SHAPE, "page table covers too many positions");
     if (!args->parent || !args->kv_len || !args->page_table || !args->kv_len_out || !args->page_table_out)
         return fail(SLM_ERR_INVALID_ARG, "null device pointer");
+    if (!aligned4(args->parent, args->kv_len, args->page_table, args->spare, args->kv_len_out, args->page_table_out, args->taken))
+        return fail(SLM_ERR_INVALID_ARG, "misaligned device pointer");
+    // (pieces of 16 bytes are counted in 32 bits)
+    if (page_elements(pages->dtype, kv.kv_heads, kv.page_size, kv.hd) * (kv.type == KV_F32 ? 4 : kv.type == KV_Q8 ? 1 : 2) >= 1ull << 35)
+        return fail(SLM_ERR_SHAPE, "pages too large");
     if (args->page_table_out == args->page_table) return fail(SLM_ERR_OVERLAP, "page_table_out is page_table");
     if (args->kv_len_out == args->kv_len) return fail(SLM_ERR_OVERLAP, "kv_len_out is kv_len");
     ForkView a{};
@@ -1148,6 +1157,8 @@ SLM_EXPORT int slm_beam_select(const slm_beam_select_args *args, void *scratch, 
     if (a.groups == 0) return SLM_OK;
     if (!a.logits || !a.scores || !a.out_scores || !a.out_rows || !a.out_tokens)
         return fail(SLM_ERR_INVALID_ARG, "null device pointer");
+    if (!aligned4(a.logits, a.scores, a.ended, a.out_scores, a.out_rows, a.out_tokens))
+        return fail(SLM_ERR_INVALID_ARG, "misaligned device pointer");
     if (a.out_rows == a.out_tokens) return fail(SLM_ERR_OVERLAP, "out_rows is out_tokens");
     if (a.out_scores == a.scores && a.num_out != a.beams)
         return fail(SLM_ERR_OVERLAP, "out_scores is scores, of another number a group");

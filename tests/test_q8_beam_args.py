@@ -83,6 +83,22 @@ def test_layers_have_one_shape(change):
     assert code(lambda: S.paged_fork([q8(), q8(**change)], fork_args())) == SHAPE
 
 
+@pytest.mark.parametrize("name", ["parent", "kv_len", "page_table", "spare", "kv_len_out", "page_table_out", "taken"])
+def test_fork_pointers_are_aligned(name):
+    assert code(lambda: S.paged_fork([q8()], fork_args(**{name: A + 2}))) == INVALID
+
+
+@pytest.mark.parametrize("name", ["logits", "scores", "ended", "out_scores", "out_rows", "out_tokens"])
+def test_beam_pointers_are_aligned(name):
+    assert code(lambda: S.beam_select(beam_args(**{name: A + 2}), A, 1 << 40)) == INVALID
+
+
+def test_fork_pages_have_a_largest_size():
+    # (one layer's keys of a page: 32 GB and more)
+    for change in (dict(dtype=S.KV_F32, page_size=1 << 19, num_kv_heads=128, head_dim=128), dict(page_size=1 << 20, num_kv_heads=256, head_dim=128)):
+        assert code(lambda: S.paged_fork([q8(num_pages=1, page_stride=0, **change)], fork_args(table_stride=8))) == SHAPE
+
+
 def test_no_layers_and_no_sequences():
     assert code(lambda: S.paged_fork([], fork_args())) == INVALID
     S.paged_fork([q8()], fork_args(num_new=0))
