@@ -405,8 +405,9 @@ __global__ void __launch_bounds__(FK_THREADS) paged_fork_kernel(ForkPools pools,
         if (tid == 0 && a.taken) a.taken[i] = wants && spare >= 0;
     }
     if (!copies || spare < 0) return;
-    const unsigned chunks = used * (unsigned)(kv.hd * el) / 16u;  // of a KV head's used slots
-    const unsigned all = chunks * (unsigned)kv.kv_heads, gap = (unsigned)kv.page_size * (unsigned)(kv.hd * el) / 16u - chunks;
+    // pieces of 16 bytes, a slot's (a whole number) first: a page has fewer than 2^31, though 2^35 bytes
+    const unsigned piece = (unsigned)(kv.hd * el) / 16u, chunks = used * piece;  // of a KV head's used slots
+    const unsigned all = chunks * (unsigned)kv.kv_heads, gap = (unsigned)kv.page_size * piece - chunks;
     const uint64_t from = (uint64_t)source * kv.page_stride * el, to = (uint64_t)spare * kv.page_stride * el;
     const int end = min(layers, (int)(blockIdx.y + 1) * per_cta) * 2;
     for (int x = blockIdx.y * per_cta * 2 + warp; x < end; x += FK_WARPS) {
