@@ -812,6 +812,10 @@ __global__ void __launch_bounds__(PD_THREADS, q8_ctas_per_sm(LPR)) paged_decode_
         const unsigned bits = __float_as_uint(fabsf(vs[lane]));
         const int e = min(max((int)(__reduce_max_sync(0xffffffffu, bits < 0x7f800000u ? bits : 0u) >> 23) - 126, -125), 126);
         const float v_up = __uint_as_float((unsigned)(127 - e) << 23), v_down = __uint_as_float((unsigned)(127 + e) << 23);
+        if (__any_sync(0xffffffffu, q8_large_key(ks[lane]))) {
+#pragma unroll
+            for (int n = 0; n < NG; n++) l[n] = __uint_as_float(0x7fc00000u);
+        }
         float x[NG][TK / 8];  // keys g + 8 i
         bool move = false;
 #pragma unroll

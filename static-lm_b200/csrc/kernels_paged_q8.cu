@@ -414,8 +414,8 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
                     else
                         dst[0] = y.x, dst[1] = y.y, dst[2] = y.z, dst[3] = y.w;
                 }
-                // rows that met a scale that is not finite, or scores so large, once the
-                // warp's first results are written
+                // rows that met a scale that is not finite or a large key's, or scores so
+                // large, once the warp's first results are written
                 __syncwarp();
                 unsigned redo = __ballot_sync(0xffffffffu, row_ok && !finite);
                 while (redo) {
@@ -646,7 +646,8 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
             if (warp < 11) {
                 // 2^e above the tile's largest scale of a value that is finite
                 const int e = min(max((int)(max(sh->top[0], sh->top[1]) >> 23) - 126, -125), 126);
-                sh->scale[j & 3][0][p] = next.k_scale;
+                // (NaN: the rows that see the key are redone)
+                sh->scale[j & 3][0][p] = q8_large_key(next.k_scale) ? __uint_as_float(0x7fc00000u) : next.k_scale;
                 sh->scale[j & 3][1][p] = __fmul_rn(next.v_scale, __uint_as_float((unsigned)(127 - e) << 23));
                 if (p == 0) sh->down[j & 7] = __uint_as_float((unsigned)(127 + e) << 23);
             }

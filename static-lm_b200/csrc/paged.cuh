@@ -283,12 +283,22 @@ struct KvElem<KV_Q8> {
     static __device__ __forceinline__ float get(const int8_t *p) { return (float)*p; }
 };
 
+// The 8-bit kernels sum bytes times q 2^e, whose largest element is below 2^15, and
+// take 2^-e back after the key's scale: |sum| < 2^15 127 128 < 2^29, so that the
+// product with a scale below 2^98 is finite, while with a larger one it may pass f32
+// where the score itself does not.  Rows that see such a key are redone.
+constexpr unsigned Q8_KEY_LIMIT = (unsigned)(127 + 98) << 23;
+__device__ __forceinline__ bool q8_large_key(float scale) {
+    return __float_as_uint(fabsf(scale)) - Q8_KEY_LIMIT < 0x7f800000u - Q8_KEY_LIMIT;
+}
+
 // One row and query head over the keys [lo, hi) of a list, of which it sees
 // those below sink_end and those in [from, to), on the CUDA cores by one warp:
 // 32 keys at a time, a key per lane for the scores, head_dim over the lanes
 // for the values.  The tensor-core kernels redo so what came out not finite:
 // 0 x NaN of a key in the tile that a row does not see reaches it there, and
-// the parts of an infinity are not its parts.
+// the parts of an infinity are not its parts.  (Scores of 8-bit keys in 64 bits
+// until their last factor: neither the sum nor the scale is near their ends.)
 struct RowState {
     float m, l, acc[4];
 };
@@ -314,14 +324,17 @@ __device__ __noinline__ RowState attend_row(const KvView &kv, const BatchView &b
             if (page >= 0) {
                 off = row_offset(kv, page, head, slot);
                 const T *k = reinterpret_cast<const T *>(kv.k) + off;
-                float dot = 0.f;
-                for (int d = 0; d < hd; d++) dot = __fmaf_rn(q[d], KvElem<TYPE>::get(k + d), dot);
                 if constexpr (TYPE == KV_Q8) {
+                    double dot = 0.0;
+                    for (int d = 0; d < hd; d++) dot = fma((double)q[d], (double)KvElem<TYPE>::get(k + d), dot);
                     const long long at = scale_offset(kv, page, head, slot);
-                    dot = __fmul_rn(dot, scale_get(kv.k, at));
+                    x = (float)(dot * (double)scale_get(kv.k, at) * (double)sl2);
                     v_scale = scale_get(kv.v, at);
+                } else {
+                    float dot = 0.f;
+                    for (int d = 0; d < hd; d++) dot = __fmaf_rn(q[d], KvElem<TYPE>::get(k + d), dot);
+                    x = __fmul_rn(dot, sl2);
                 }
-                x = __fmul_rn(dot, sl2);
             }
         }
         float top = x;

@@ -1,0 +1,86 @@
+"""Attention over 8-bit pages where scales or scores lie far apart, against the 64-bit reference.
+
+Tolerances (u = 2^-24): a score x (in powers of two) is rounded to f32 and its
+difference to the reference of its row again, so a weight is off by at most
+(2 |x| u + 2^-22) ln 2 of itself, and the output, of values of one sign, by twice the
+largest of these.  Elsewhere as in test_gpu_paged.
+"""
+import numpy as np
+import pytest
+
+from test_gpu_paged import NORM_TOL, U, attend, queries, reference
+from test_gpu_q8_pages import Q8Cache
+
+pytestmark = pytest.mark.gpu
+
+
+def negative(torch, lengths, kvh, hd, magnitude, seed):
+    """Keys of elements -magnitude, values above zero."""
+    c = Q8Cache(torch, lengths, kvh, hd, 16, seed=seed)
+    k, scale = c.parts(c.k)
+    k.fill_(-127)
+    scale.fill_(magnitude / 127)
+    c.parts(c.v)[0].abs_()
+    return c
+
+
+def seen_values(c):
+    """[position][KV head][head_dim] of the first sequence's values."""
+    j = np.arange(int(c.lengths[0]))
+    return c.host(c.v)[c.table[0, j // c.page], :, j % c.page]
+
+
+def fine_rows(got, want, tol):
+    got = got.double().cpu().numpy()
+    assert np.isfinite(got).all()
+    off, size = np.linalg.norm(got - want, axis=1), np.linalg.norm(want, axis=1)
+    assert (off <= tol * np.maximum(size, 1e-30)).all(), (off / np.maximum(size, 1e-30)).max()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("size,magnitude", [(1.0, 1e33), (1.0, 1e35), (1e-20, 1e36), (1e6, 1e30)])
+@pytest.mark.parametrize("rows,length", [(None, 50), (None, 2000), ([40], 50), ([300], 2000)])
+def test_scores_far_below_zero(cuda, hd, size, magnitude, rows, length):
+    """Every score finite, and the same for every key: the values are averaged."""
+    c = negative(cuda, [length], 2, hd, magnitude, 3)
+    n = [1] if rows is None else rows
+    q = queries(cuda, sum(n), 4, hd, 7).abs() * size
+    got = attend(cuda, c, q, 4, rows)
+    # (not by the scores in 64 bits: sums of the same products in another order differ by more than the weights bear)
+    v = seen_values(c)
+    want = np.stack([np.repeat(v[:length - n[0] + 1 + i].mean(0), 2, 0).reshape(-1) for i in range(n[0])])
+    # (sums of up to 2000 values of one sign in f32, over at least 32 lanes)
+    fine_rows(got, want, NORM_TOL)
+    assert int(c.status) == 0
+
+
+@pytest.mark.parametrize("rows", [None, [60]])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (20, 3)])
+def test_the_nearest_of_scores_far_below_zero(cuda, rows, window, sinks):
+    """One key's score lies above the others', all of them finite and far below zero."""
+    c = negative(cuda, [90], 2, 64, 1e35, 4)
+    c.parts(c.k)[1][int(c.table[0, 80 // 16]), :, 80 % 16] = 5e34 / 127
+    c.parts(c.k)[1][int(c.table[0, 40 // 16]), :, 40 % 16] = 9e34 / 127
+    n = [1] if rows is None else rows
+    q = queries(cuda, sum(n), 4, 64, 7).abs()
+    got, v, want = attend(cuda, c, q, 4, rows, window, sinks), seen_values(c), []
+    for p in range(90 - n[0], 90):
+        seen = [j for j in range(p + 1) if not window or p - j < window or j < sinks]
+        best = [80] if 80 in seen else [40] if 40 in seen else seen
+        want.append(np.repeat(v[best].mean(0), 2, 0).reshape(-1))
+    fine_rows(got, np.stack(want), NORM_TOL)
+
+
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("heads", [4, 12])
+@pytest.mark.parametrize("rows", [None, [200]])
+def test_tiny_queries_and_huge_keys(cuda, rows, heads, sign):
+    """Scores of 30 to 36 of either sign from elements of 1e-32 and 1e33."""
+    c = negative(cuda, [200], 2, 64, 0.0, 5)
+    g = cuda.Generator().manual_seed(2)
+    k, scale = c.parts(c.k)
+    k.fill_(127 * sign)
+    scale.copy_((30 + 6 * cuda.rand(scale.shape, generator=g)) / (64 * 127 * 0.125) * 1e32)
+    n = [1] if rows is None else rows
+    q = cuda.full((sum(n), heads * 64), 1e-32, device="cuda")
+    fine_rows(attend(cuda, c, q, heads, rows), reference(c, q, n, heads), 2 * (2 * 36 * np.log2(np.e) * U + 2.0 ** -22) * np.log(2))
