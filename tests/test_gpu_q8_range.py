@@ -84,3 +84,35 @@ def test_tiny_queries_and_huge_keys(cuda, rows, heads, sign):
     n = [1] if rows is None else rows
     q = cuda.full((sum(n), heads * 64), 1e-32, device="cuda")
     fine_rows(attend(cuda, c, q, heads, rows), reference(c, q, n, heads), 2 * (2 * 36 * np.log2(np.e) * U + 2.0 ** -22) * np.log(2))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("ratio", [2.0 ** 10, 2.0 ** 20, 2.0 ** 36, 2.0 ** 60, 2.0 ** 120])
+@pytest.mark.parametrize("length,window,sinks", [(100, 0, 0), (300, 25, 0), (300, 25, 4), (1500, 0, 0)])
+def test_large_values_that_a_row_does_not_see(cuda, hd, ratio, length, window, sinks):
+    """Values `ratio` times the others', later than a row or behind its window, in the
+    tiles of what it sees: each row is held to its own size."""
+    c = Q8Cache(cuda, [length], 2, hd, 16, seed=8)
+    c.parts(c.v)[0].abs_()
+    scale = c.parts(c.v)[1]
+    for at in (70, length - 31):
+        scale[int(c.table[0, at // 16]), :, at % 16] *= ratio
+    q = queries(cuda, length, 4, hd, 9)
+    got, want = attend(cuda, c, q, 4, [length], window, sinks), reference(c, q, [length], 4, window, sinks)
+    fine_rows(got, want, NORM_TOL)
+    # the last row alone, as one of many
+    one = attend(cuda, c, q[-1:], 4, None, window, sinks)
+    fine_rows(one, want[-1:], NORM_TOL)
+
+
+@pytest.mark.parametrize("rows", [[100], [40, 3]])
+def test_rows_of_zeros_beside_large_values(cuda, rows):
+    """Scales of 0 are nothing that a larger one could hide."""
+    c = Q8Cache(cuda, [100, 60][:len(rows)], 2, 64, 16, seed=9)
+    scale = c.parts(c.v)[1]
+    for s, n in enumerate(c.lengths):
+        for at in range(0, int(n), 3):
+            scale[int(c.table[s, at // 16]), :, at % 16] = 0
+        scale[int(c.table[s, (int(n) - 1) // 16]), :, (int(n) - 1) % 16] = 1e20
+    q = queries(cuda, sum(rows), 4, 64, 10)
+    fine_rows(attend(cuda, c, q, 4, rows), reference(c, q, rows, 4), NORM_TOL)
