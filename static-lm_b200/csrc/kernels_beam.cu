@@ -173,7 +173,9 @@ __global__ void __launch_bounds__(BS_THREADS, 8) beam_part_kernel(BeamView a, Be
             if (lane == 0 && bound > -INFINITY) atomicMax(&s_least, (unsigned long long)(beam_key(bound, 0) | 0xffffffffu) - 0xffffffffull - 1);
             __syncthreads();
         }
-        see(*(volatile unsigned long long *)&s_least);
+        // (as lane 0 read it: other warps write it meanwhile, and the lanes go on together only
+        // where low is the same in all of them)
+        see(__shfl_sync(0xffffffffu, *(volatile unsigned long long *)&s_least, 0));
         if (top > m) {
             s = __fmul_rn(s, exp2_approx(__fmul_rn(__fsub_rn(m, top), 1.44269504088896340736f)));
             m = top;
