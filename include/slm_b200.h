@@ -453,8 +453,9 @@ int slm_paged_fork(const slm_kv_pages *pages, uint32_t num_layers, const slm_pag
  * in slm_sample_argmax, and count nothing in the softmax; logits of -infinity
  * are never proposed; a row that holds +infinity proposes nothing.  Places for
  * which there is no candidate are (-infinity, -1, -1).
- * The exponentials are f32, their sums over a row's parts and the candidates'
- * sums 64 bits, rounded once.  1 to 256 beams, num_out 1 to 64, vocab at most
+ * The exponentials are f32, summed 16 at a time; the sums of these and the
+ * candidates' are 64 bits, rounded once.  A row's log sum exp is so within 1e-6,
+ * by less than that another in calls of other sizes.  1 to 256 beams, num_out 1 to 64, vocab at most
  * 2^30, 2^24 rows.  out_scores may be scores where num_out = beams; the outputs
  * are apart otherwise.  `scratch` as for slm_paged_attention. */
 typedef struct {

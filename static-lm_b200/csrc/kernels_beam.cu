@@ -119,7 +119,8 @@ __global__ void __launch_bounds__(BS_THREADS, 8) beam_part_kernel(BeamView a, Be
     if (threadIdx.x < BS_WARPS) s_place[threadIdx.x] = 0;
     if (threadIdx.x == 0) s_least = 0;
     __syncthreads();
-    float m = -INFINITY, s = 0.f;
+    float m = -INFINITY;
+    double s = 0.0;           // this lane's sum of exp(x - m): in f32 its error grows with the row's length
     uint64_t low = 0;         // the threshold as this warp last saw it; 0: none
     float least = -FLT_MAX;   // its logit (-infinity is no candidate)
     auto see = [&](uint64_t key) {
@@ -177,17 +178,21 @@ __global__ void __launch_bounds__(BS_THREADS, 8) beam_part_kernel(BeamView a, Be
         // where low is the same in all of them)
         see(__shfl_sync(0xffffffffu, *(volatile unsigned long long *)&s_least, 0));
         if (top > m) {
-            s = __fmul_rn(s, exp2_approx(__fmul_rn(__fsub_rn(m, top), 1.44269504088896340736f)));
+            s *= (double)exp2_approx(__fmul_rn(__fsub_rn(m, top), 1.44269504088896340736f));
             m = top;
         }
         if (m > -INFINITY) {
-            float s0 = 0.f, s1 = 0.f;
+            const uint64_t minus_m = pack2(-m, -m), log2e = pack2(1.44269504088896340736f, 1.44269504088896340736f);
+            uint64_t sums = 0;
 #pragma unroll
             for (int i = 0; i < BS_PER; i += 2) {
-                s0 = __fadd_rn(s0, exp2_approx(__fmul_rn(__fsub_rn(v[i], m), 1.44269504088896340736f)));
-                s1 = __fadd_rn(s1, exp2_approx(__fmul_rn(__fsub_rn(v[i + 1], m), 1.44269504088896340736f)));
+                float e0, e1;
+                unpack2(mul2(add2(pack2(v[i], v[i + 1]), minus_m), log2e), e0, e1);
+                sums = add2(sums, pack2(exp2_approx(e0), exp2_approx(e1)));
             }
-            s = __fadd_rn(s, __fadd_rn(s0, s1));
+            float s0, s1;
+            unpack2(sums, s0, s1);
+            s += (double)__fadd_rn(s0, s1);
         }
         if (!__any_sync(0xffffffffu, top >= least)) continue;
         unsigned pass = 0;  // of this lane's
@@ -242,7 +247,7 @@ __global__ void __launch_bounds__(BS_THREADS, 8) beam_part_kernel(BeamView a, Be
     float all = m;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
-    double sum = m > -INFINITY ? (double)__fmul_rn(s, exp2_approx(__fmul_rn(__fsub_rn(m, all), 1.44269504088896340736f))) : 0.0;
+    double sum = m > -INFINITY ? s * (double)exp2_approx(__fmul_rn(__fsub_rn(m, all), 1.44269504088896340736f)) : 0.0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) s_m[warp] = all, s_s[warp] = sum;
