@@ -454,10 +454,11 @@ int slm_paged_fork(const slm_kv_pages *pages, uint32_t num_layers, const slm_pag
  * are never proposed; a row that holds +infinity proposes nothing.  Places for
  * which there is no candidate are (-infinity, -1, -1).
  * The exponentials are f32, summed 16 at a time; the sums of these and the
- * candidates' are 64 bits, rounded once.  A row's log sum exp is so within 1e-6,
- * by less than that another in calls of other sizes.  1 to 256 beams, num_out 1 to 64, vocab at most
- * 2^30, 2^24 rows.  out_scores may be scores where num_out = beams; the outputs
- * are apart otherwise.  `scratch` as for slm_paged_attention. */
+ * candidates' are 64 bits, rounded once.  A row's log sum exp is within 4e-6, by
+ * 1e-7 as a rule, and may differ by as much with the number of rows in the call.
+ * 1 to 256 beams, num_out 1 to 64, vocab at most 2^30, 2^24 rows.  out_scores may
+ * be scores where num_out = beams; the outputs are apart otherwise.  `scratch` as
+ * for slm_paged_attention. */
 typedef struct {
     const float *logits; /* rows of vocab, ld floats apart */
     uint64_t ld;
