@@ -59,7 +59,15 @@ class BeamSearch:
         return s.logits[:n]
 
     def run(self, prompts, n_out):
-        """[prompt][beam] of (score, tokens), best first."""
+        """[prompt][beam] of (score, tokens), best first; every page is given back, also by a search that fails."""
+        s = self.s
+        free, requests = list(s.free), list(s.requests)
+        try:
+            return self._run(prompts, n_out)
+        finally:
+            s.free, s.requests = free, requests
+
+    def _run(self, prompts, n_out):
         s, beams = self.s, self.beams
         groups, n = len(prompts), len(prompts) * self.beams
         if n > s.max_rows:
@@ -106,8 +114,6 @@ class BeamSearch:
             s._forward(np.maximum(toks, 0), batch)
             logits.copy_(self._logits(n))
             S.paged_check(s.pages[0], stream)
-        s.free = sorted(set(s.free) | set(self._held(tables[0])) | set(self._held(tables[1])) | {p for r in made for p in r.pages.values()},
-                        reverse=True)
         result = []
         for g in range(groups):
             found = [(float(scores[i]), [int(t) for t in history[i]]) for i in range(g * beams, (g + 1) * beams) if scores[i] > -np.inf]
