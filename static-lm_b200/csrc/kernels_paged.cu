@@ -293,7 +293,7 @@ template <int OUT>
 __device__ __forceinline__ void write8(void *out, size_t at, const float (&x)[8], bool vec) {
     using T = typename KvElem<OUT>::T;
     T *p = reinterpret_cast<T *>(out) + at;
-    T y[8];
+    alignas(16) T y[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         if constexpr (OUT == KV_F32)
