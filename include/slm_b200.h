@@ -360,8 +360,8 @@ int slm_paged_append(const slm_kv_pages *pages, const slm_paged_batch *batch,
  * What is in slots a row does not see (stale, infinite, NaN) does not reach
  * it.  Sums and the softmax are f32; with f16 pages weights below 2^-23 of a
  * row's largest are held to 2^-46 of it, with 8-bit pages to 2^-45 times the
- * largest scale of the values next to theirs (32 or 64 keys), 2^-30 where the row
- * sees only some of these.  out is apart from q.
+ * largest scale of the values next to theirs (32 or 64 keys), and rows of which
+ * that could leave less than f32's accuracy are done anew.  out is apart from q.
  * `scratch` holds slm_paged_attention_scratch_bytes bytes, 16-byte aligned,
  * contents of no account before and after; calls that may overlap on the GPU
  * need scratches of their own.  Sums are in an order that does not change from

@@ -776,6 +776,7 @@ __global__ void __launch_bounds__(PD_THREADS, q8_ctas_per_sm(LPR)) paged_decode_
         }
     };
 
+    unsigned most = 0, large = 0xffffffffu;  // the values' largest scale, and this lane's keys' least q8_above_limit
     float m[NG], l[NG];
     float acc[NG][LPR][2];  // elements 16 c + 2 g + {0, 1} of the output of head t4
 #pragma unroll
@@ -810,12 +811,11 @@ __global__ void __launch_bounds__(PD_THREADS, q8_ctas_per_sm(LPR)) paged_decode_
         const float *ks = s_scale[warp][stage][0], *vs = s_scale[warp][stage][1];
         // 2^e above the tile's largest scale of a value that is finite
         const unsigned bits = __float_as_uint(fabsf(vs[lane]));
-        const int e = min(max((int)(__reduce_max_sync(0xffffffffu, bits < 0x7f800000u ? bits : 0u) >> 23) - 126, -125), 126);
+        const unsigned top = __reduce_max_sync(0xffffffffu, bits < 0x7f800000u ? bits : 0u);
+        const int e = min(max((int)(top >> 23) - 126, -125), 126);
         const float v_up = __uint_as_float((unsigned)(127 - e) << 23), v_down = __uint_as_float((unsigned)(127 + e) << 23);
-        if (__any_sync(0xffffffffu, q8_large_key(ks[lane]))) {
-#pragma unroll
-            for (int n = 0; n < NG; n++) l[n] = __uint_as_float(0x7fc00000u);
-        }
+        most = max(most, top);
+        large = min(large, q8_above_limit(ks[lane]));
         float x[NG][TK / 8];  // keys g + 8 i
         bool move = false;
 #pragma unroll
@@ -918,7 +918,8 @@ __global__ void __launch_bounds__(PD_THREADS, q8_ctas_per_sm(LPR)) paged_decode_
     __syncthreads();  // every ring is free: the warps' results go there
 
     float *s_o = reinterpret_cast<float *>(pd_smem);  // [warp][head][hd]
-    bool finite = true;
+    bool finite = !q8_large_key(large);
+    const float least = most != 0 ? __fmul_rn(__uint_as_float(most & 0x7f800000u), 2.0f * Q8_RESULT_LEAST) : 0.f;
 #pragma unroll
     for (int n = 0; n < NG; n++) {
         const int h = n * 4 + t4;
@@ -926,12 +927,16 @@ __global__ void __launch_bounds__(PD_THREADS, q8_ctas_per_sm(LPR)) paged_decode_
         for (int o = 4; o < 32; o <<= 1) l[n] = __fadd_rn(l[n], __shfl_xor_sync(0xffffffffu, l[n], o));
         if (g == 0) s_m[warp][h] = m[n], s_l[warp][h] = l[n];
         bool fine = fabsf(l[n]) < INFINITY;
+        float largest = 0.f;
 #pragma unroll
         for (int d = 0; d < LPR; d++) {
+            if (d * 16 < kv.hd) largest = fmaxf(largest, fmaxf(fabsf(acc[n][d][0]), fabsf(acc[n][d][1])));
             if (d * 16 < kv.hd)
                 *reinterpret_cast<float2 *>(s_o + (warp * G + h) * kv.hd + d * 16 + 2 * g) = make_float2(acc[n][d][0], acc[n][d][1]);
             fine = fine && fabsf(acc[n][d][0]) < INFINITY && fabsf(acc[n][d][1]) < INFINITY;
         }
+        const unsigned show = __ballot_sync(0xffffffffu, largest >= least) & 0x11111111u << t4;
+        fine = fine && (l[n] == 0.f || show != 0);
         finite = finite && (fine || h >= work.ng);
     }
     if (__syncthreads_or(!finite)) {

@@ -7,8 +7,8 @@
 // value's by its column of weights.  q 2^e = q0 + q1 / 2^12 and the weights are
 // two f16 parts each, 2 products for q.k and for w.v, as for f16 pages.  A value's
 // scale enters the weights relative to a power of two at or above its tile's
-// largest, which the f32 sums take back; a row that sees only far smaller ones of
-// the tile is redone.  No chain of MMAs is longer than one
+// largest, which the f32 sums take back; a row whose sums come out far smaller (see
+// Q8_RESULT_LEAST) is redone.  No chain of MMAs is longer than one
 // key tile (the tensor core cuts each sum towards zero): every tile's w.v
 // starts from zero and is added to the row's sums in registers.
 //
@@ -63,8 +63,8 @@ struct Q8Shared {
     alignas(16) float scale[4][2][64];  // of the keys and values of the newest 4 tiles
     unsigned valid[8][2];     // held keys of the newest 8 tiles
     float down[8];            // what their values' scales are relative to
-    unsigned top[2], low[2];  // of a warp's values' scales, the largest and the smallest that is not 0
-    bool wide;                // a tile of which a row may see a part has them PQ_SPREAD apart
+    unsigned top[2];
+    float most;               // the largest of all tiles' down
     unsigned taddr;
     int abort;
     // the CTA's work
@@ -97,35 +97,6 @@ __device__ __forceinline__ uint2 bytes_f16(unsigned w) {
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r.x) : "r"(lo), "r"(0x64806480u));
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r.y) : "r"(hi), "r"(0x64806480u));
     return r;
-}
-
-// Whether a row sees, of a tile, only values with scales far below those of others.
-// Parts of weights end at 2^-36, and a row's largest weight is 2^9 or more: with scales
-// above 2^-16 of the tile's power of two (2^-15 of its largest) weights are held to
-// 2^-37 2^-9 2^16 = 2^-30 of the largest weight times the largest scale that the row
-// sees, 64 of them to 2^-24.  Others are redone.  Only the tiles that an end of what the
-// row sees cuts are looked at, and only where the copying warps met such scales (asked
-// of every masked tile as it came, 8 x 4096 rows took 540 us, chunks 755).
-constexpr int PQ_SPREAD = 16;
-template <int KT>
-__device__ __noinline__ bool q8_dwarfed(const KvView &kv, const BatchView &b, int seq, int head, SeenKeys keys, int lo, int hi,
-                                        int from, int sink_end, int to) {
-    for (int e = 0; e < 3; e++) {
-        const int edge = e == 0 ? sink_end : e == 1 ? from : to;
-        if (edge <= lo || edge >= hi || (edge - lo) % KT == 0) continue;
-        const int i0 = edge - (edge - lo) % KT, i1 = min(i0 + KT, hi);
-        float all = 0.f, most = 0.f;  // of the tile, and of what the row sees of it
-        for (int i = i0; i < i1; i++) {
-            unsigned slot;
-            const int page = key_page(kv, b, seq, (unsigned)keys.key(i), slot);
-            const float s = page < 0 ? 0.f : fabsf(scale_get(kv.v, scale_offset(kv, page, head, slot)));
-            if (!(s < INFINITY)) continue;
-            all = fmaxf(all, s);
-            if (i < to && (i < sink_end || i >= from)) most = fmaxf(most, s);
-        }
-        if (most > 0.f && most < __fmul_rn(all, 2.0f / (1 << PQ_SPREAD))) return true;
-    }
-    return false;
 }
 
 template <int HDP>
@@ -168,7 +139,7 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
         }
         mbar_init(&sh->drain, 1);
         sh->abort = 0;
-        sh->wide = false;
+        sh->most = 0.f;
         mbar_fence_init();
     }
     const int seq = sh->seq, row0 = sh->row0, rows = sh->rows, tile = sh->tile;
@@ -412,6 +383,7 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
                 // every product of the stream is complete: the results go through its
                 // shared memory, 16-byte chunk c of row r at chunk c ^ (r & 7), to whole rows
                 float4 *s_o = reinterpret_cast<float4 *>(pq_smem + x * Cfg::STREAM + (warp & 3) * 32 * HDP * 4);
+                float largest = 0.f;
 #pragma unroll
                 for (int i = 0; i < HDP; i += 4) {
                     float y[4];
@@ -420,10 +392,11 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
 #pragma unroll
                     for (int u = 0; u < 4; u++) {
                         y[u] = __fmul_rn(y[u], inv);
-                        if (i < hd) finite = finite && fabsf(y[u]) < INFINITY;
+                        if (i < hd) finite = finite && fabsf(y[u]) < INFINITY, largest = fmaxf(largest, fabsf(y[u]));
                     }
                     s_o[lane * (HDP / 4) + ((i / 4) ^ (lane & 7))] = make_float4(y[0], y[1], y[2], y[3]);
                 }
+                finite = finite && largest >= __fmul_rn(__fmul_rn(sh->most, Q8_RESULT_LEAST), l == 0.f ? 0.f : inv);
                 if (split_up && row_ok)
                     plan.part_ml[((size_t)row * a.num_heads + h) * plan.splits + split] = make_float2(m, l);
                 __syncwarp();
@@ -447,9 +420,8 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
                         dst[0] = y.x, dst[1] = y.y, dst[2] = y.z, dst[3] = y.w;
                 }
                 // rows that met a scale that is not finite or a large key's, scores so large, or
-                // values far below their neighbours', once the warp's first results are written
+                // values beside which their own do not show, once the warp's first results are written
                 __syncwarp();
-                if (sh->wide && row_ok && finite) finite = !q8_dwarfed<KT>(kv, b, seq, head, keys, lo, hi, from, sink_end, to);
                 unsigned redo = __ballot_sync(0xffffffffu, row_ok && !finite);
                 while (redo) {
                     const int who = __ffs(redo) - 1;
@@ -662,15 +634,10 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
             fence_async_smem();
             mbar_arrive(&sh->full[s]);
         };
-        // list positions from edge0 on and those below edge1 may be seen by some of the block's rows alone
-        const int first = pos0 + tok0, last = pos0 + tok1;
-        const int edge0 = first < 0 ? 0 : first - keys.low + keys.sinks + 1;
-        const int edge1 = a.window == 0 || last < 0 || (unsigned)last < a.window ? 0 : last - (int)a.window + 1 - keys.low + keys.sinks;
         At next = find(look(0));
         Id ahead = look(1);
         for (int j = 0; j < ntile && ok; j++) {
             // tile j's offsets and scales for all, its copies on their way, then the next tile's look-ups
-            const bool cut = lo + (j + 1) * KT > edge0 || lo + j * KT < edge1;
             if (warp < 11) {
                 const int w = warp - 9;
                 sh->off[p] = next.row;
@@ -678,18 +645,21 @@ __global__ void __launch_bounds__(Q8Cfg<HDP>::THREADS, 1) paged_rows_q8_kernel(K
                 const unsigned bits_v = __float_as_uint(fabsf(next.v_scale));
                 const unsigned top = __reduce_max_sync(0xffffffffu, bits_v < 0x7f800000u ? bits_v : 0u);
                 if (lane == 0) sh->valid[j & 7][w] = held, sh->top[w] = top;
-                if (cut) sh->low[w] = __reduce_min_sync(0xffffffffu, bits_v != 0 ? bits_v : 0x7f800000u);
             }
             named_bar_sync(1, Cfg::PRODUCERS);
             copy(j);
             if (warp < 11) {
                 // 2^e above the tile's largest scale of a value that is finite
-                const int e = min(max((int)(max(sh->top[0], sh->top[1]) >> 23) - 126, -125), 126);
+                const unsigned top = max(sh->top[0], sh->top[1]);
+                const int e = min(max((int)(top >> 23) - 126, -125), 126);
                 // (NaN: the rows that see the key are redone)
-                sh->scale[j & 3][0][p] = q8_large_key(next.k_scale) ? __uint_as_float(0x7fc00000u) : next.k_scale;
+                sh->scale[j & 3][0][p] = q8_large_key(q8_above_limit(next.k_scale)) ? __uint_as_float(0x7fc00000u) : next.k_scale;
                 sh->scale[j & 3][1][p] = __fmul_rn(next.v_scale, __uint_as_float((unsigned)(127 - e) << 23));
-                if (p == 0) sh->down[j & 7] = __uint_as_float((unsigned)(127 + e) << 23);
-                if (cut && p == 0 && (int)(min(sh->low[0], sh->low[1]) >> 23) - 127 < e - PQ_SPREAD) sh->wide = true;
+                if (p == 0) {
+                    const float down = top != 0 ? __uint_as_float((unsigned)(127 + e) << 23) : 0.f;
+                    sh->down[j & 7] = down;
+                    sh->most = fmaxf(sh->most, down);
+                }
             }
             next = find(ahead);
             ahead = look(j + 2);

@@ -288,9 +288,17 @@ struct KvElem<KV_Q8> {
 // product with a scale below 2^98 is finite, while with a larger one it may pass f32
 // where the score itself does not.  Rows that see such a key are redone.
 constexpr unsigned Q8_KEY_LIMIT = (unsigned)(127 + 98) << 23;
-__device__ __forceinline__ bool q8_large_key(float scale) {
-    return __float_as_uint(fabsf(scale)) - Q8_KEY_LIMIT < 0x7f800000u - Q8_KEY_LIMIT;
-}
+__device__ __forceinline__ unsigned q8_above_limit(float scale) { return __float_as_uint(fabsf(scale)) - Q8_KEY_LIMIT; }
+__device__ __forceinline__ bool q8_large_key(unsigned above_limit) { return above_limit < 0x7f800000u - Q8_KEY_LIMIT; }
+
+// Their weights, times a value's scale relative to a power of two at or above its
+// tile's largest, are two f16 parts, off by up to 2^-37, and times bytes by 2^-30 a key.
+// Scales beside them that a row does not see, or sees with next to no weight, so take
+// bits of its own; a row whose sums of n keys all come out below 2^-5 of the largest
+// power of two (where a row's largest weight is 2^9 or more: its result is below 2^-21
+// of the largest value) is redone.  What is left is off by n 2^-25 at most, sqrt(n) 2^-27
+// as a rule.
+constexpr float Q8_RESULT_LEAST = 1.0f / 32;
 
 // One row and query head over the keys [lo, hi) of a list, of which it sees
 // those below sink_end and those in [from, to), on the CUDA cores by one warp:

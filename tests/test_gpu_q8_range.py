@@ -116,3 +116,45 @@ def test_rows_of_zeros_beside_large_values(cuda, rows):
         scale[int(c.table[s, (int(n) - 1) // 16]), :, (int(n) - 1) % 16] = 1e20
     q = queries(cuda, sum(rows), 4, 64, 10)
     fine_rows(attend(cuda, c, q, 4, rows), reference(c, q, rows, 4), NORM_TOL)
+
+
+@pytest.mark.parametrize("hd", [48, 64, 128])
+@pytest.mark.parametrize("ratio", [2.0 ** 12, 2.0 ** 30, 2.0 ** 45, 2.0 ** 60])
+@pytest.mark.parametrize("rows,heads", [(None, 4), (None, 12), ([90], 4)])
+@pytest.mark.parametrize("length", [100, 1500])
+def test_large_values_of_no_weight(cuda, hd, ratio, rows, heads, length):
+    """Values `ratio` times the others', of keys that every row sees with a weight of
+    e^-40 or less: beside them in their tiles, and with up to 2^60 e^-40 = 5 of the others' size in all."""
+    c = Q8Cache(cuda, [length], 2, hd, 16, seed=11)
+    c.parts(c.v)[0].abs_()
+    k, k_scale = c.parts(c.k)
+    k[..., 0] = 0
+    v_scale = c.parts(c.v)[1]
+    for at in range(0, length - 90 if rows else length, 45):
+        to = int(c.table[0, at // 16]), slice(None), at % 16
+        k[to] = 0
+        k[to[0], :, to[2], 0] = -127
+        k_scale[to] = 40 * hd ** 0.5 / 8 / 127
+        v_scale[to] *= ratio
+    n = [1] if rows is None else rows
+    q = queries(cuda, sum(n), heads, hd, 9)
+    q.view(-1, heads, hd)[..., 0] = 8
+    got, want = attend(cuda, c, q, heads, rows), reference(c, q, n, heads)
+    # (scores to 40 log2(e) = 58, of both signs)
+    fine_rows(got, want, 2 * (2 * 58 * U + 2.0 ** -22) * np.log(2))
+
+
+@pytest.mark.parametrize("spread", [2.0, 4.0, 8.0])
+@pytest.mark.parametrize("rows", [None, [120, 7, 33]])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (30, 4)])
+def test_values_of_all_sizes(cuda, spread, rows, window, sinks):
+    """Scales that are spread by e^(8 N): each row and head is held to its own size."""
+    c = Q8Cache(cuda, [150, 64, 700], 2, 64, 16, seed=13)
+    g = cuda.Generator().manual_seed(6)
+    scale = c.parts(c.v)[1]
+    scale.mul_(cuda.exp(spread * cuda.randn(scale.shape, generator=g)).cuda())
+    c.parts(c.v)[0].abs_()
+    n = [1, 1, 1] if rows is None else rows
+    q = queries(cuda, sum(n), 6, 64, 12)
+    got, want = attend(cuda, c, q, 6, rows, window, sinks), reference(c, q, n, 6, window, sinks)
+    fine_rows(got.reshape(-1, 64), want.reshape(-1, 64), NORM_TOL)
