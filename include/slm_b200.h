@@ -331,7 +331,8 @@ typedef struct {
  * every sequence or before position 0 stores nothing and gets a zero q_out;
  * so does one past the rope table (SLM_PAGED_BAD_POSITION).  A page id that
  * is not a page of the pool stores nothing (SLM_PAGED_BAD_PAGE).  Two rows at
- * one slot of one page leave either's values.  Pairs without a norm into f32
+ * one slot of one page leave either's elements, in 8-bit pages either's bytes and
+ * either's scale, which may belong to different rows.  Pairs without a norm into f32
  * pages give the bits of slm_apply_rope_cached.  Into 8-bit pages a row of k or
  * v of a head goes as q = x*(127/max|x|) rounded to the nearest, ties to even,
  * and scale = max|x|/127; one whose values are all below 2^-100 in size as zeros,

@@ -44,20 +44,21 @@ __device__ __forceinline__ bool row_lives(const BeamView &a, int row) {
 
 // CTA (row, part); its warps take chunks of 512 logits in turn, each through its
 // own ring of cp.async stages.  A chunk costs a maximum, an exp and a vote unless a
-// logit reaches the CTA's threshold, a number that num_out of its logits are known
-// to reach: those that do go one by one into the warp's best so far, a list over
-// its lanes, rank r in lane r (and r - 32), by a count of the ranks above and a
-// shift.  The threshold is first a bound from the first chunks, by the lanes' own
-// largest; then the least of num_out slots in shared memory, the least of which
-// every logit that passes replaces (where two warps replace the same one the
-// smaller is lost there, and the threshold only lower than it could be); or the
-// last place of a warp's full list.  Where more than a few of a chunk reach it
-// (rising logits), the chunk's own bound comes first: at most 16 num_out are not
-// below that.  No warp waits for another but after the first chunk and before the
-// lists are merged.
-// 256 rows of 131072 (134 MB, 20 us), both launches: one list a CTA, with a barrier
-// a chunk, 85 us; a list a warp without a common threshold 63; with the least of
-// the warps' own places as the threshold, loads to registers, 55.
+// logit passes the CTA's threshold, a key that num_out of its logits are known to lie
+// above: those that do go one by one into the warp's best so far, a list over its
+// lanes, rank r in lane r (and r - 32), by a count of the ranks above and a shift.
+// The threshold is first a bound from the warps' first chunks, by the lanes' own
+// largest: num_out of one chunk reach it.  From then on each warp publishes its
+// ceil(num_out / 4)-th best (s_place): the four warps hold num_out between them that
+// are no lower than the least of the four, which goes into s_least by an atomic
+// maximum, as does the last place of a warp's own full list.  Both only rise, so one
+// that is read late is a lower threshold that holds too.  Where more than a few of
+// a chunk pass (rising logits), the chunk's own bound comes first: at most 16
+// num_out are not below that.  No warp waits for another but after the first chunk
+// and before the lists are merged.
+// 256 rows of 131072 (134 MB, 20.5 us), both launches, 44.3 us; one list a CTA, with a
+// barrier a chunk, 85; a list a warp without a common threshold 63; loads to registers
+// instead of the rings 55.
 template <bool VEC, bool TWO>
 __global__ void __launch_bounds__(BS_THREADS, 8) beam_part_kernel(BeamView a, BeamPlan plan) {
     extern __shared__ __align__(16) float s_ring[];  // [warp][stage][512]
@@ -478,7 +479,7 @@ void launch_beam_select(const BeamView &a, const BeamPlan &plan, cudaStream_t s)
     auto go = [&](auto *kernel, SmemOptIn &opt) {
         constexpr int bytes = BS_WARPS * BS_STAGES * BS_CHUNK * 4;
         opt(kernel, bytes);
-        // (its CTAs come while the kernel before ends, and wait: 46.1 to 44.3 us, 12.4 to 10.6)
+        // (its CTAs come while the kernel before ends, and wait: 46.7 to 44.3 us, 12.3 to 10.0)
         launch_kernel(kernel, grid, block, bytes, s, true, a, plan);
     };
     static SmemOptIn opt[4];
@@ -487,7 +488,7 @@ void launch_beam_select(const BeamView &a, const BeamPlan &plan, cudaStream_t s)
     else
         a.vec ? go(beam_part_kernel<true, true>, opt[2]) : go(beam_part_kernel<false, true>, opt[3]);
     const int lists = a.beams * plan.parts, warps = std::min(std::max((lists + 31) / 32, a.beams), BJ_WARPS);
-    // (at most 4 KB of sums, 32 KB of lists and a byte for each of 32768)
+    // (at most 4 KB of sums, 32 KB of lists and a byte for each of 32 * 148: rows are cut into no more parts in all)
     const int staged = lists <= 128 && lists * a.num_out <= 2048 ? lists * a.num_out : 0;
     launch_kernel(beam_join_kernel, dim3((unsigned)a.groups), dim3((unsigned)warps * 32), (size_t)a.beams * 16 + staged * 16 + lists,
                   s, true, a, plan, staged);

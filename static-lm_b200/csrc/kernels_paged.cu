@@ -258,8 +258,9 @@ void append_typed(const KvView &kv, const BatchView &b, const AppendView &a, cud
 
 // Rows of the cache as they were appended: a group of lanes (a power of two, 8
 // elements each) takes the K and the V of one KV head of a row.  (8 x 4096 rows of 3
-// heads of 64, 8-bit to f16: 15.2 us, 3.3 TB/s with the launch; two, three, four
-// heads a group, for which the row's place is found once, 19.2, 17.4, 21.4.)
+// heads of 64, 8-bit to f16, 38.5 MB: 15.2 us with the launch, 2.5 TB/s; two, three, four
+// heads a group, for which the row's place is found once, 19.2, 17.4, 21.4.  What it
+// waits for is a chain: the row's sequence, its page's id, the row.)
 constexpr int RD_THREADS = 256;
 
 template <int TYPE>
@@ -450,7 +451,7 @@ void launch_paged_read(const KvView &kv, const BatchView &b, const ReadView &a, 
 }
 
 void launch_paged_fork(const ForkPools &pools, const KvView &kv, const ForkView &a, int layers, cudaStream_t s) {
-    // a (layer, K or V) for each warp; fewer, longer CTAs where there are many
+    // two layers a CTA: a (layer, K or V) for each of its warps
     const int el = kv.type == KV_F32 ? 4 : kv.type == KV_Q8 ? 1 : 2, per_cta = FK_PER;
     launch_kernel(paged_fork_kernel, dim3((unsigned)a.num_new, (unsigned)((layers + per_cta - 1) / per_cta)), dim3(FK_THREADS), 0, s,
                   true, pools, kv, a, layers, per_cta, el);

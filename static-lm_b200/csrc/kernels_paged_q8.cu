@@ -20,8 +20,10 @@
 // of its next, 1000 of a tile's 3550 cycles at head_dim 64), and every key that is
 // converted serves both.  8 x 4096 rows of 9 / 3 heads of 64: 530 us (292 TFLOP/s, two
 // products for each; f16 pages 649); 16 chunks of up to 512 behind up to 8192, 32 / 8
-// heads of 128: 742 us (345).  Instructions bound it: about 14 a score and row, half
-// the cycles issue one; at head_dim 128 also the copying warps, busy throughout.
+// heads of 128: 742 us (345).  Neither issue (52 and 48 % of the cycles, about 14
+// instructions a score and row) nor the tensor pipe (28 and 39 %) is full: a stream's
+// warps wait for their own products, and the other stream's two warps an SM quarter
+// cover a part of that; at head_dim 128 the copying warps are busy throughout, too.
 #include "kernels.h"
 #include "paged_tc.cuh"
 
